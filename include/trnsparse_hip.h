@@ -36,6 +36,7 @@ extern "C" {
 #define TSP_F32 0
 #define TSP_F64 1
 #define TSP_BF16 2
+#define TSP_F16 3 /* the attention operators over strided operands */
 
 /* ---- index type codes (CSR) ------------------------------------------ */
 #define TSP_I32 0
@@ -594,6 +595,63 @@ int tsp_csr_transpose(const void* values, int dtype, const int64_t* col_indices,
                       int64_t nnz, int64_t* out_row_ptrs, int64_t* out_col,
                       void* out_values, void* workspace,
                       int64_t workspace_bytes, void* stream);
+
+/* ====================================================================
+ * Attention over strided operands: cross attention and attention over a
+ * prefix that a batch shares.
+ *
+ * Operands are (batch, heads, rows, head_dim) views with unit stride over
+ * head_dim; `*_strides` points to three int64 in host memory: the strides
+ * in elements of the batch, head and row dimensions. Pointers and strides
+ * are whole 16-byte pieces, head_dim is at most 128 and a whole number of
+ * them (8 elements of 16 bits, 4 of 32), row strides are at least head_dim
+ * and below 16 MiB (TSP_EINVAL / TSP_EUNSUPPORTED otherwise). dtype is
+ * TSP_F32, TSP_BF16 or TSP_F16, the same for all operands; sums, maxima and
+ * partial results are fp32. heads is a multiple of kv_heads; query head h
+ * reads key head h / (heads / kv_heads). scale is positive.
+ * `key_lengths` / `lengths` (batch,) of `index_type`, or NULL for all keys:
+ * values are taken into [0, keys]; K and V rows behind them are not read.
+ * A row without a key to see is zero.
+ *
+ * tsp_cross_attn_fwd: O[b,h,i] = sum_j softmax_j(scale Q[b,h,i].K[b,hk,j])
+ *   V[b,hk,j] over j < key_lengths[b]; lse (batch, heads, queries) fp32 or
+ *   NULL receives log sum_j exp(scale Q.K_j) (-inf for a row without keys).
+ *   Two calls that may run at the same time need workspaces of their own.
+ * No counterpart in the reference, whose attention is one sequence's over
+ * itself (trnsparse/ops.py:549-625).
+ * ==================================================================== */
+int64_t tsp_cross_attn_workspace_size(int dtype, int64_t batch, int64_t heads,
+                                      int64_t kv_heads, int64_t queries,
+                                      int64_t keys, int64_t head_dim);
+int tsp_cross_attn_fwd(const void* Q, const int64_t* q_strides, const void* K,
+                       const int64_t* k_strides, const void* V,
+                       const int64_t* v_strides, int dtype, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t queries,
+                       int64_t keys, int64_t head_dim, const void* key_lengths,
+                       int index_type, double scale, void* O,
+                       const int64_t* o_strides, float* lse, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* tsp_prefix_attn_fwd: the same with two sets of keys in one softmax: the
+ *   prefix (PK, PV (kv_heads, prefix, head_dim); the batch entry of their
+ *   strides is ignored), which every batch entry sees whole, and each batch
+ *   entry's own K, V (batch, kv_heads, keys, head_dim), of which lengths[b]
+ *   rows hold its tokens, the `queries` new ones last: query i sees own keys
+ *   j < lengths[b] - (queries - 1 - i). */
+int64_t tsp_prefix_attn_workspace_size(int dtype, int64_t batch, int64_t heads,
+                                       int64_t kv_heads, int64_t queries,
+                                       int64_t prefix, int64_t keys,
+                                       int64_t head_dim);
+int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
+                        const void* PK, const int64_t* pk_strides,
+                        const void* PV, const int64_t* pv_strides,
+                        const void* K, const int64_t* k_strides, const void* V,
+                        const int64_t* v_strides, int dtype, int64_t batch,
+                        int64_t heads, int64_t kv_heads, int64_t queries,
+                        int64_t prefix, int64_t keys, int64_t head_dim,
+                        const void* lengths, int index_type, double scale,
+                        void* O, const int64_t* o_strides, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,9 +17,11 @@ from .iterative import chebyshev_bsr, chebyshev_coeffs, richardson_bsr
 from .ops import (
     block_sparse_attention_tiled,
     bsr_spmm,
+    cross_attention,
     nnz_per_row,
     screened_mask,
     screened_spmm,
+    shared_prefix_attention,
     sparse_add,
     sparse_scale,
     sparse_transpose,
@@ -42,6 +44,8 @@ __all__ = [
     "screened_spmm",
     "screened_mask",
     "block_sparse_attention_tiled",
+    "cross_attention",
+    "shared_prefix_attention",
     "sparse_add",
     "sparse_scale",
     "sparse_transpose",

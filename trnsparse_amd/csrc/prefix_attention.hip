@@ -1,0 +1,105 @@
+// Attention of new tokens over a prefix that all sequences of a batch share and
+// each sequence's own keys behind it (serving):
+//   O[b, h, i] = sum_j p_j V_j over the prefix keys of key head hk = h / group
+//   and b's own keys j < lengths[b] - (Sq - 1 - i), p = softmax_j(scale Q . K_j)
+// No counterpart in the reference, whose attention is one sequence's over
+// itself (trnsparse/ops.py:549-625).
+//
+// The rows of all sequences that read one key head form one unit for the
+// prefix, so it is read once for the batch; every sequence's own keys are a
+// unit of their own. Both parts are ranges of the same softmax and are joined
+// by their log-sum-exps (xattn_fwd.h).
+#include "xattn_fwd.h"
+
+namespace tsp {
+namespace xat {
+int check_sizes(const char* who, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D);
+
+namespace {
+struct PrefixPlan {
+  Plan shared, own;
+  int nsplit;
+};
+PrefixPlan prefix_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t P, int64_t S) {
+  const int64_t G = Hq / Hkv;
+  PrefixPlan p{};
+  if (P > 0) p.shared = fwd_plan(Hkv, B * G * Sq, P);
+  if (S > 0) p.own = fwd_plan(B * Hkv, G * Sq, S);
+  p.nsplit = p.shared.nsplit + p.own.nsplit;
+  return p;
+}
+}  // namespace
+}  // namespace xat
+}  // namespace tsp
+
+using namespace tsp;
+
+extern "C" int64_t tsp_prefix_attn_workspace_size(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t P,
+                                                  int64_t S, int64_t D) {
+  if (xat::check_sizes("tsp_prefix_attn_workspace_size", dtype, B, Hq, Hkv, Sq, P > S ? P : S, D)) return -1;
+  if (P < 0 || S < 0) return fail(TSP_EINVAL, "tsp_prefix_attn_workspace_size: negative length"), -1;
+  if (B * Hq * Sq == 0) return 0;
+  return xat::prefix_plan(B, Hq, Hkv, Sq, P, S).nsplit * B * Hq * Sq * (D + 1) * 4;
+}
+
+extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void* PK, const int64_t* pks, const void* PV,
+                                   const int64_t* pvs, const void* K, const int64_t* ks, const void* V,
+                                   const int64_t* vs, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
+                                   int64_t P, int64_t S, int64_t D, const void* lengths, int index_type, double scale,
+                                   void* O, const int64_t* os, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "tsp_prefix_attn_fwd";
+  const hipStream_t st = (hipStream_t)stream;
+  if (P < 0 || S < 0) return fail(TSP_EINVAL, "%s: negative length", who);
+  int rc = xat::check_sizes(who, dtype, B, Hq, Hkv, Sq, P > S ? P : S, D);
+  if (rc) return rc;
+  if (B * Hq * Sq == 0) return TSP_OK;
+  if ((rc = xat::check_operand(who, "Q", Q, qs, Sq, D, dtype))) return rc;
+  if ((rc = xat::check_operand(who, "O", O, os, Sq, D, dtype))) return rc;
+  if (P > 0) {
+    if ((rc = xat::check_operand(who, "prefix K", PK, pks, P, D, dtype))) return rc;
+    if ((rc = xat::check_operand(who, "prefix V", PV, pvs, P, D, dtype))) return rc;
+  }
+  if (S > 0) {
+    if ((rc = xat::check_operand(who, "K", K, ks, S, D, dtype))) return rc;
+    if ((rc = xat::check_operand(who, "V", V, vs, S, D, dtype))) return rc;
+  }
+  if (!(scale > 0) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
+  if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
+  const xat::PrefixPlan p = xat::prefix_plan(B, Hq, Hkv, Sq, P, S);
+  const int64_t rows = B * Hq * Sq, need = p.nsplit * rows * (D + 1) * 4;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
+  xat::FwdArgs a{};
+  a.Q = xat::operand(Q, qs, dtype);
+  const xat::Operand o = xat::operand(O, os, dtype);
+  a.O = (char*)O;
+  a.ob = o.b, a.oh = o.h, a.os = o.s;
+  a.prows = rows;
+  a.part = (float*)workspace;
+  a.plse = a.part + p.nsplit * rows * D;
+  a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.D = (int)D;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  if (P > 0) {
+    xat::FwdArgs s = a;
+    s.K = xat::operand(PK, pks, dtype);
+    s.V = xat::operand(PV, pvs, dtype);
+    s.units_b = 1;
+    s.R = (int)(B * Hq / Hkv * Sq);
+    s.L = P;
+    if ((rc = xat::launch_fwd(dtype, p.shared, s, st))) return rc;
+  }
+  if (S > 0) {
+    xat::FwdArgs s = a;
+    s.K = xat::operand(K, ks, dtype);
+    s.V = xat::operand(V, vs, dtype);
+    s.lengths = lengths;
+    s.len64 = index_type == TSP_I64;
+    s.units_b = (int)B;
+    s.R = (int)(Hq / Hkv * Sq);
+    s.L = S;
+    s.causal = Sq > 1;
+    s.split0 = p.shared.nsplit;
+    if ((rc = xat::launch_fwd(dtype, p.own, s, st))) return rc;
+  }
+  const xat::CombineArgs c{a.part, a.plse, rows, p.nsplit, a.D, (int)Hq, a.Sq, a.O, a.ob, a.oh, a.os, nullptr};
+  return xat::launch_combine(dtype, c, st);
+}

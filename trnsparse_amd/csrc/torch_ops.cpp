@@ -498,6 +498,136 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> bsa_bwd_meta(
   return {at::empty_like(Q), at::empty_like(Q), at::empty_like(Q)};
 }
 
+// ------------------------------------- attention over strided operands
+
+int attn_dtype(at::ScalarType t, const char* who) {
+  TORCH_CHECK(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, who, ": dtype ", t, " not supported");
+  return t == at::kFloat ? TSP_F32 : t == at::kHalf ? TSP_F16 : TSP_BF16;
+}
+
+// head_dim as the kernels take it: whole 16-byte pieces
+int64_t piece_dim(const at::Tensor& t) {
+  const int64_t ce = 16 / t.element_size();
+  return (t.size(-1) + ce - 1) / ce * ce;
+}
+
+// A (batch, heads, rows, head_dim) operand as the kernels take it: t itself
+// where its strides and address are whole 16-byte pieces and its rows lie
+// apart, else a contiguous copy (head_dim padded with zeros).
+at::Tensor attn_operand(const at::Tensor& t) {
+  const int64_t ce = 16 / t.element_size(), D = t.size(3), Dp = piece_dim(t);
+  if (D != Dp) return at::constant_pad_nd(t, {0, Dp - D}).contiguous();
+  bool ok = (t.stride(3) == 1 || D == 1) && (uintptr_t)t.data_ptr() % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % ce == 0);
+  ok = ok && (t.size(2) <= 1 || (t.stride(2) >= D && t.stride(2) * t.element_size() < (1 << 24)));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+struct Strides {
+  int64_t s[3];
+  explicit Strides(const at::Tensor& t) {
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) <= 1 ? (i == 2 ? t.size(3) : 0) : t.stride(i);
+  }
+};
+
+// A result of the operand's shape with head_dim Dp, in the operand's order of
+// heads and rows.
+at::Tensor attn_like(const at::Tensor& t, int64_t Dp) {
+  const int64_t B = t.size(0), H = t.size(1), S = t.size(2);
+  if (H > 1 && S > 1 && t.stride(2) > t.stride(1)) return at::empty({B, S, H, Dp}, t.options()).transpose(1, 2);
+  return at::empty({B, H, S, Dp}, t.options());
+}
+at::Tensor attn_trim(const at::Tensor& t, int64_t D) { return t.size(3) == D ? t : t.narrow(3, 0, D).contiguous(); }
+
+void need_4d(const at::Tensor& t, const at::Tensor& Q, const char* who, const char* name) {
+  TORCH_CHECK(t.device() == Q.device(), who, ": ", name, " is on ", t.device(), ", expected ", Q.device());
+  TORCH_CHECK(t.dim() == 4, who, ": ", name, " must be (batch, heads, rows, head_dim)");
+  need_dtype(t, Q.scalar_type(), who, name);
+  TORCH_CHECK(t.size(3) == Q.size(3), who, ": head_dim of ", name, " is ", t.size(3), ", expected ", Q.size(3));
+}
+
+const void* lengths_ptr(const c10::optional<at::Tensor>& t, int64_t B, const at::Tensor& Q, const char* who, int& code) {
+  code = TSP_I64;
+  if (!t.has_value()) return nullptr;
+  need(*t, Q, "lengths");
+  code = index_code(t->scalar_type());
+  TORCH_CHECK(t->dim() == 1 && t->numel() == B, who, ": lengths must be (batch,)");
+  return t->data_ptr();
+}
+
+at::Tensor workspace_of(int64_t bytes, const at::Tensor& like, const char* who) {
+  TORCH_CHECK(bytes >= 0, who, " failed: ", tsp_last_error());
+  return at::empty({bytes > 0 ? bytes : 16}, like.options().dtype(at::kByte));
+}
+
+void cross_shapes(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V, const char* who) {
+  need_4d(Q, Q, who, "Q");
+  need_4d(K, Q, who, "K");
+  need_4d(V, Q, who, "V");
+  TORCH_CHECK(K.sizes() == V.sizes() && K.size(0) == Q.size(0), who, ": K and V must be one shape, with Q's batch");
+  TORCH_CHECK(K.size(1) > 0 && Q.size(1) % K.size(1) == 0, who, ": ", Q.size(1), " query heads do not divide over ",
+              K.size(1), " key heads");
+}
+
+std::tuple<at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& Q_, const at::Tensor& K_, const at::Tensor& V_,
+                                                  const c10::optional<at::Tensor>& key_lengths, double scale,
+                                                  bool return_lse) {
+  const char* who = "cross_attn_fwd";
+  cross_shapes(Q_, K_, V_, who);
+  const int code = attn_dtype(Q_.scalar_type(), who);
+  const auto Q = attn_operand(Q_), K = attn_operand(K_), V = attn_operand(V_);
+  const int64_t B = Q.size(0), Hq = Q.size(1), Sq = Q.size(2), D = Q.size(3), Hk = K.size(1), L = K.size(2);
+  int icode;
+  const void* lens = lengths_ptr(key_lengths, B, Q, who, icode);
+  auto O = attn_like(Q_, D);
+  auto lse = at::empty(return_lse ? at::IntArrayRef({B, Hq, Sq}) : at::IntArrayRef({0}), Q.options().dtype(at::kFloat));
+  const int64_t wsb = tsp_cross_attn_workspace_size(code, B, Hq, Hk, Sq, L, D);
+  auto ws = workspace_of(wsb, Q, who);
+  check(tsp_cross_attn_fwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, code, B,
+                           Hq, Hk, Sq, L, D, lens, icode, scale, O.data_ptr(), Strides(O).s,
+                           return_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), wsb, stream_of(Q)),
+        "tsp_cross_attn_fwd");
+  return {attn_trim(O, Q_.size(3)), lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> cross_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&,
+                                                       const c10::optional<at::Tensor>&, double, bool return_lse) {
+  auto lo = Q.options().dtype(at::kFloat);
+  auto lse = return_lse ? at::empty({Q.size(0), Q.size(1), Q.size(2)}, lo) : at::empty({0}, lo);
+  return {Q.size(3) == piece_dim(Q) ? attn_like(Q, Q.size(3)) : at::empty(Q.sizes(), Q.options()), lse};
+}
+
+at::Tensor prefix_attn_fwd(const at::Tensor& Q_, const at::Tensor& PK_, const at::Tensor& PV_, const at::Tensor& K_,
+                           const at::Tensor& V_, const c10::optional<at::Tensor>& lengths, double scale) {
+  const char* who = "prefix_attn_fwd";
+  cross_shapes(Q_, K_, V_, who);
+  TORCH_CHECK(PK_.dim() == 3 && PK_.sizes() == PV_.sizes() && PK_.size(0) == K_.size(1), who,
+              ": the prefix must be (kv_heads, prefix, head_dim) like K's heads");
+  const int code = attn_dtype(Q_.scalar_type(), who);
+  const auto pk4 = PK_.unsqueeze(0), pv4 = PV_.unsqueeze(0);
+  need_4d(pk4, Q_, who, "prefix K");
+  need_4d(pv4, Q_, who, "prefix V");
+  const auto Q = attn_operand(Q_), K = attn_operand(K_), V = attn_operand(V_), PK = attn_operand(pk4),
+             PV = attn_operand(pv4);
+  const int64_t B = Q.size(0), Hq = Q.size(1), Sq = Q.size(2), D = Q.size(3), Hk = K.size(1), S = K.size(2);
+  const int64_t P = PK.size(2);
+  int icode;
+  const void* lens = lengths_ptr(lengths, B, Q, who, icode);
+  auto O = attn_like(Q_, D);
+  const int64_t wsb = tsp_prefix_attn_workspace_size(code, B, Hq, Hk, Sq, P, S, D);
+  auto ws = workspace_of(wsb, Q, who);
+  check(tsp_prefix_attn_fwd(Q.data_ptr(), Strides(Q).s, PK.data_ptr(), Strides(PK).s, PV.data_ptr(), Strides(PV).s,
+                            K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, code, B, Hq, Hk, Sq, P, S, D, lens,
+                            icode, scale, O.data_ptr(), Strides(O).s, ws.data_ptr(), wsb, stream_of(Q)),
+        "tsp_prefix_attn_fwd");
+  return attn_trim(O, Q_.size(3));
+}
+
+at::Tensor prefix_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                const at::Tensor&, const c10::optional<at::Tensor>&, double) {
+  return Q.size(3) == piece_dim(Q) ? attn_like(Q, Q.size(3)) : at::empty(Q.sizes(), Q.options());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(trnsparse_hip, m) {
@@ -523,6 +653,10 @@ TORCH_LIBRARY(trnsparse_hip, m) {
   m.def("bsa_bwd(Tensor Q, Tensor K, Tensor V, Tensor O, Tensor dO, Tensor block_row_ptrs, Tensor block_col_indices, "
         "Tensor col_ptrs, Tensor col_block_rows, int n_block_cols, int block_size, float scale, Tensor row_max, "
         "Tensor row_denom, Tensor plan, int n_items, int n_splits, int n_partials) -> (Tensor, Tensor, Tensor)");
+  m.def("cross_attn_fwd(Tensor Q, Tensor K, Tensor V, Tensor? key_lengths, float scale, bool return_lse) -> "
+        "(Tensor, Tensor)");
+  m.def("prefix_attn_fwd(Tensor Q, Tensor prefix_K, Tensor prefix_V, Tensor K, Tensor V, Tensor? lengths, "
+        "float scale) -> Tensor");
 }
 
 // the "CUDA" dispatch key is the GPU key of PyTorch-ROCm
@@ -538,6 +672,8 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
   m.impl("screened_spmm_backward", &screened_spmm_backward);
   m.impl("bsa_fwd", &bsa_fwd);
   m.impl("bsa_bwd", &bsa_bwd);
+  m.impl("cross_attn_fwd", &cross_attn_fwd);
+  m.impl("prefix_attn_fwd", &prefix_attn_fwd);
 }
 
 TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
@@ -552,4 +688,6 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
   m.impl("screened_spmm_backward", &screened_spmm_backward_meta);
   m.impl("bsa_fwd", &bsa_fwd_meta);
   m.impl("bsa_bwd", &bsa_bwd_meta);
+  m.impl("cross_attn_fwd", &cross_attn_fwd_meta);
+  m.impl("prefix_attn_fwd", &prefix_attn_fwd_meta);
 }

@@ -1,0 +1,289 @@
+// Forward kernels of dense attention over strided operands: grouped key heads,
+// a length for each batch entry, keys split over workgroups when there are few
+// rows. Instantiated by cross_attention.hip and prefix_attention.hip.
+//
+// A unit is one (batch entry, key head) pair, or one key head alone where all
+// batch entries share their keys; its rows are the (batch entry, query head of
+// the group, query) triples that read those keys, so one pass over the keys
+// serves them all.
+//   wide    128 rows to a workgroup, a wavefront to 32 of them; stages of keys
+//           shared by the four wavefronts through an LDS ring of two
+//   narrow  up to 32 rows to a workgroup: every wavefront has all of them and
+//           takes every NW-th stage of 32 keys through a ring of its own, with
+//           no workgroup barrier until the wavefronts' results are joined
+// Either takes one of `nsplit` ranges of `chunk` keys. With one range it writes
+// the rows' results; with more it writes each range's own normalised result
+// and log-sum-exp in fp32, which combine_kernel joins in range order.
+#pragma once
+
+#include "tile_item.h"
+#include "xattn_tiles.h"
+
+namespace tsp {
+namespace xat {
+
+struct Operand {
+  const char* p;
+  int64_t b, h, s;  // strides in bytes: batch entry, head, row
+};
+
+struct FwdArgs {
+  Operand Q, K, V;
+  char* O;
+  int64_t ob, oh, os;   // strides of O in bytes
+  float* lse;           // (batch, heads, queries) natural log-sum-exp, or null
+  float *part, *plse;   // partial results and log-sum-exps (base 2) of [split][row]; null with one range
+  int64_t prows;        // rows of a partial result: batch * heads * queries
+  const void* lengths;  // valid keys of each batch entry (null: all)
+  int len64;            // lengths are int64 (else int32)
+  int units_b;          // batch entries with keys of their own (1: shared)
+  int Hkv, G, Sq, R, D; // R: rows of a unit
+  int64_t L;            // keys
+  int causal;           // query i sees keys below length - (Sq - 1 - i)
+  int tiles, nsplit, split0;
+  int64_t chunk;
+  float scale_log2;
+};
+
+struct RowId {
+  int64_t b, head, orow;
+  int i;
+};
+__device__ inline RowId row_id(const FwdArgs& a, int64_t ub, int64_t hk, int r) {
+  const uint32_t per = (uint32_t)(a.G * a.Sq), bb = (uint32_t)r / per, rem = (uint32_t)r - bb * per;
+  const uint32_t g = rem / (uint32_t)a.Sq;
+  RowId x;
+  x.i = (int)(rem - g * (uint32_t)a.Sq);
+  x.b = ub + bb;
+  x.head = hk * a.G + g;
+  x.orow = (x.b * a.Hkv * a.G + x.head) * a.Sq + x.i;
+  return x;
+}
+__device__ inline int64_t unit_length(const FwdArgs& a, int64_t ub) {
+  if (!a.lengths) return a.L;
+  const int64_t n = a.len64 ? ((const int64_t*)a.lengths)[ub] : (int64_t)((const int32_t*)a.lengths)[ub];
+  return n < 0 ? 0 : n > a.L ? a.L : n;
+}
+
+// Results of one row (four values at d): final, or one range's part.
+template <typename T>
+struct RowOut {
+  char* o;
+  float* p;
+  __device__ inline RowOut(const FwdArgs& a, const RowId& id, int split) {
+    o = a.O + id.b * a.ob + id.head * a.oh + id.i * a.os;
+    p = a.part ? a.part + ((int64_t)(a.split0 + split) * a.prows + id.orow) * a.D : nullptr;
+  }
+  __device__ inline void put(int d, f32x4 v) const {
+    if (p)
+      *(f32x4*)(p + d) = v;
+    else
+      T::store4(o + d * T::ESZ, v);
+  }
+};
+__device__ inline void put_lse(const FwdArgs& a, const RowId& id, int split, float lse2) {
+  if (a.part)
+    a.plse[(int64_t)(a.split0 + split) * a.prows + id.orow] = lse2;
+  else if (a.lse)
+    a.lse[id.orow] = lse2 * 0.69314718055994531f;
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(256, 2) void fwd_wide(const FwdArgs a) {
+  constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  int64_t unit, item;
+  if (!head_item(blockIdx.x, (int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+  const int tile = (int)(item % a.tiles), split = (int)(item / a.tiles);
+  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
+  const int r = tile * 128 + w * 32 + l32;
+  const bool live = r < a.R;
+  const RowId id = row_id(a, ub, hk, live ? r : 0);
+
+  typename T::Rows q;
+  T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
+
+  const int64_t n = unit_length(a, ub);
+  const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
+  const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;  // keys of this row
+  const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, HK) : 0;
+  const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
+  const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
+  Stager<T, HK, 4> ks, vs;
+  ks.init(w, lane, a.K.s, a.D);
+  vs.init(w, lane, a.V.s, a.D);
+  const typename T::Lane ln = T::lane_of(lane);
+  const uint32_t lds0 = dma::lds_addr(lds);
+  auto issue = [&](int s) {
+    const uint32_t st = lds0 + (s & 1) * STAGE;
+    ks.issue(Kp, k0 + (int64_t)s * HK, k1, a.K.s, a.D, st, w);
+    vs.issue(Vp, k0 + (int64_t)s * HK, k1, a.V.s, a.D, st + HBYTES, w);
+  };
+  RowState<T> x;
+  x.clear();
+  if (nst > 0) issue(0);
+  for (int s = 0; s < nst; ++s) {
+    dma::wait_vm<0>();
+    dma::barrier();
+    if (s + 1 < nst) issue(s + 1);
+    const int64_t at = k0 + (int64_t)s * HK;
+    const uint32_t st = lds0 + (s & 1) * STAGE;
+    softmax_stage<T, NT>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,
+                         (sees < k1 ? sees : k1) - at);
+  }
+  const float l = halves_sum(x.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  if (!live) return;
+  const RowOut<T> out(a, id, split);
+  T::quads(x.acc, h, [&](int d, f32x4 v) {
+    if (d < a.D) out.put(d, v * inv);
+  });
+  if (h == 0) put_lse(a, id, split, x.m + __builtin_amdgcn_logf(l));
+}
+
+template <typename T, int NW, int NST>
+__global__ __launch_bounds__(64 * NW, 1) void fwd_narrow(const FwdArgs a) {
+  constexpr int HBYTES = 32 * T::ROWB, STAGE = 2 * HBYTES, XLD = T::DP + 4;
+  constexpr int RING = NW * NST * STAGE, XB = NW * 32 * (XLD + 2) * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[RING > XB ? RING : XB];
+  int64_t unit, item;
+  if (!head_item(blockIdx.x, a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+  const int split = (int)item;
+  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
+  const bool live = l32 < a.R;
+  const RowId id = row_id(a, ub, hk, live ? l32 : 0);
+
+  const int64_t n = unit_length(a, ub);
+  const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
+  const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;
+  const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, 32) : 0, mine = nst > w ? (nst - w + NW - 1) / NW : 0;
+  const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
+  const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
+  Stager<T, 32, 1> ks, vs;
+  ks.init(0, lane, a.K.s, a.D);
+  vs.init(0, lane, a.V.s, a.D);
+  constexpr int NI = 2 * Stager<T, 32, 1>::NI;  // loads of a stage
+  const typename T::Lane ln = T::lane_of(lane);
+  const uint32_t ring = dma::lds_addr(lds) + w * NST * STAGE;
+  auto key = [&](int s) { return k0 + 32 * ((int64_t)s * NW + w); };
+  auto issue = [&](int s) {
+    const uint32_t st = ring + (s % NST) * STAGE;
+    ks.issue(Kp, key(s), k1, a.K.s, a.D, st, 0);
+    vs.issue(Vp, key(s), k1, a.V.s, a.D, st + HBYTES, 0);
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if (s < mine) issue(s);
+  typename T::Rows q;
+  T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
+  RowState<T> x;
+  x.clear();
+  for (int s = 0; s < mine; ++s) {
+    // the slot of stage s - 1 is free once this wavefront's reads of it returned
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (s + NST - 1 < mine) {
+      issue(s + NST - 1);
+      dma::wait_vm<(NST - 1) * NI>();
+    } else {
+      dma::wait_vm<0>();
+    }
+    asm volatile("" ::: "memory");
+    const uint32_t st = ring + (s % NST) * STAGE;
+    const int64_t at = key(s);
+    softmax_stage<T, 1>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + 32 > k1,
+                        (sees < k1 ? sees : k1) - at);
+  }
+  // ---- join the wavefronts: m, l, acc of each row through LDS
+  const float l = halves_sum(x.l);
+  float* xo = (float*)lds;
+  float* xm = xo + NW * 32 * XLD;
+  float* xl = xm + NW * 32;
+  __syncthreads();
+  if (live) {
+    T::quads(x.acc, h, [&](int d, f32x4 v) { *(f32x4*)(xo + (w * 32 + l32) * XLD + d) = v; });
+    if (h == 0) {
+      xm[w * 32 + l32] = x.m;
+      xl[w * 32 + l32] = l;
+    }
+  }
+  __syncthreads();
+  constexpr int QPR = T::DP / 4;  // quads of a row
+  for (int e = tid; e < a.R * QPR; e += 64 * NW) {
+    const int row = e / QPR, d = 4 * (e % QPR);
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NW; ++j) m = fmaxf(m, xm[j * 32 + row]);
+    float total = 0.f;
+    f32x4 sum = f32x4{};
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      const float lj = xl[j * 32 + row];
+      // (a wavefront without keys for the row has m = -inf, l = 0; a NaN score leaves NaN in l)
+      const float f = xm[j * 32 + row] == -INFINITY ? (lj == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(xm[j * 32 + row] - m);
+      total += f * lj;
+      sum += *(const f32x4*)(xo + (j * 32 + row) * XLD + d) * f;
+    }
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+    const RowId rid = row_id(a, ub, hk, row);
+    if (d < a.D) RowOut<T>(a, rid, split).put(d, sum * inv);
+    if (d == 0) put_lse(a, rid, split, m + __builtin_amdgcn_logf(total));
+  }
+}
+
+// The ranges' results of every row in one: weights 2^(lse_j - max lse). Rows
+// that no range has keys for are zero with a log-sum-exp of -inf. 32 lanes to a
+// row, four values each.
+struct CombineArgs {
+  const float *part, *plse;
+  int64_t prows;
+  int nsplit, D, heads, Sq;
+  char* O;
+  int64_t ob, oh, os;
+  float* lse;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int d = 4 * (threadIdx.x & 31);
+  if (row >= a.prows) return;
+  float m = -INFINITY;
+  for (int j = 0; j < a.nsplit; ++j) m = fmaxf(m, a.plse[j * a.prows + row]);
+  float total = 0.f;
+  f32x4 sum = f32x4{};
+  for (int j = 0; j < a.nsplit; ++j) {
+    const float lse = a.plse[j * a.prows + row];
+    if (lse == -INFINITY) continue;  // (its part is not read; a NaN goes on)
+    const float f = __builtin_amdgcn_exp2f(lse - m);
+    total += f;
+    if (d < a.D) sum += *(const f32x4*)(a.part + (j * a.prows + row) * a.D + d) * f;
+  }
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  const int64_t i = row % a.Sq, bh = row / a.Sq;
+  if (d < a.D) T::store4(a.O + bh / a.heads * a.ob + bh % a.heads * a.oh + i * a.os + d * T::ESZ, sum * inv);
+  if (d == 0 && a.lse) a.lse[row] = (m + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
+}
+
+// ------------------------------------------------------------------- host
+
+// How one set of keys is gone over: narrow or wide, row tiles, key ranges.
+struct Plan {
+  bool narrow;
+  int tiles, nsplit;
+  int64_t chunk;
+};
+Plan fwd_plan(int64_t units, int64_t rows, int64_t keys);
+int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st);
+int launch_combine(int dtype, const CombineArgs& a, hipStream_t st);
+
+// Checks of one strided operand; 0 or a status with a message.
+int check_operand(const char* who, const char* name, const void* p, const int64_t* strides, int64_t rows, int64_t D,
+                  int dtype);
+inline int esize(int dtype) { return dtype == TSP_F32 ? 4 : 2; }
+inline Operand operand(const void* p, const int64_t* strides, int dtype) {
+  const int e = esize(dtype);
+  return Operand{(const char*)p, strides[0] * e, strides[1] * e, strides[2] * e};
+}
+
+}  // namespace xat
+}  // namespace tsp

@@ -16,7 +16,7 @@ import torch
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent.parent / "libtrnsparse_hip.so"
 
-TSP_F32, TSP_F64, TSP_BF16 = 0, 1, 2
+TSP_F32, TSP_F64, TSP_BF16, TSP_F16 = 0, 1, 2, 3
 TSP_I32, TSP_I64 = 0, 1
 
 _DTYPE_CODE = {torch.float32: TSP_F32, torch.float64: TSP_F64, torch.bfloat16: TSP_BF16}
@@ -98,6 +98,12 @@ SIGNATURES: dict[str, tuple] = {
         [_P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _DBL, _P, _P, _P, _P, _P,
          _P, _I64, _I64, _I64, _P, _P],
     ),
+    "tsp_cross_attn_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "tsp_cross_attn_fwd": (_INT, [_P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _INT, _DBL, _P,
+                                  _P, _P, _P, _I64, _P]),
+    "tsp_prefix_attn_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "tsp_prefix_attn_fwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64,
+                                   _I64, _P, _INT, _DBL, _P, _P, _P, _I64, _P]),
 }
 
 _lib = None

@@ -925,3 +925,33 @@ def hip_block_sparse_attention_backward(Q, K, V, O, dO, mask_bsr, scale: float, 
         dQ, dK, dV = _lib.ops().bsa_bwd(q, k, v, o, do, rp, ci, cp, crow, nbc, b, float(scale), rm, rd, plan, n_items,
                                         n_splits, n_partials)
     return tuple(g.reshape(*lead, S, D).to(orig) for g in (dQ, dK, dV))
+
+
+# ------------------------------------------- attention between sequences
+
+
+def _lengths_on(t, dev: torch.device):
+    return None if t is None else t.to(dev).contiguous()
+
+
+@_library_call
+def hip_cross_attention(Q, K, V, key_lengths, scale: float):
+    """cross_attention on the HIP kernels (operands on the host are copied
+    over, the result returned on Q's device)."""
+    orig = Q.device
+    dev = _target_device(Q, K, V)
+    with torch.cuda.device(dev):
+        Q, K, V = (t.to(dev) for t in (Q, K, V))
+        lens = _lengths_on(key_lengths, dev)
+        return _lib.ops().cross_attn_fwd(Q, K, V, lens, float(scale), False)[0].to(orig)
+
+
+@_library_call
+def hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale: float):
+    """shared_prefix_attention on the HIP kernels."""
+    orig = Q.device
+    dev = _target_device(Q, K, V)
+    with torch.cuda.device(dev), torch.no_grad():
+        Q, prefix_K, prefix_V, K, V = (t.to(dev) for t in (Q, prefix_K, prefix_V, K, V))
+        lens = _lengths_on(lengths, dev)
+        return _lib.ops().prefix_attn_fwd(Q, prefix_K, prefix_V, K, V, lens, float(scale)).to(orig)

@@ -496,3 +496,157 @@ def block_sparse_attention_tiled(
 
         return hip_block_sparse_attention(Q, K, V, mask_bsr, scale)
     return _attn_pytorch_batched(Q, K, V, mask_bsr, scale)
+
+
+# ------------------------------------------- attention between sequences
+#
+# Operators that a decoder layer has next to block_sparse_attention_tiled: no
+# counterpart in the reference.
+
+
+def _check_heads(who: str, Q, K, V, lengths, scale: float) -> None:
+    """Shapes and types of (batch, heads, rows, head_dim) operands; on both backends."""
+    for name, t in (("Q", Q), ("K", K), ("V", V)):
+        if t.dim() != 4:
+            raise RuntimeError(f"{who}: {name} must be (batch, heads, rows, head_dim), got shape {tuple(t.shape)}")
+    if K.shape != V.shape or K.shape[0] != Q.shape[0] or K.shape[3] != Q.shape[3]:
+        raise RuntimeError(f"{who}: Q {tuple(Q.shape)}, K {tuple(K.shape)} and V {tuple(V.shape)} do not belong together")
+    if K.shape[1] == 0 or Q.shape[1] % K.shape[1]:
+        raise RuntimeError(f"{who}: {Q.shape[1]} query heads do not divide over {K.shape[1]} key heads")
+    if not (Q.dtype == K.dtype == V.dtype) or not Q.is_floating_point():
+        raise RuntimeError(f"{who}: Q, K, V must have one floating dtype, got {Q.dtype}, {K.dtype}, {V.dtype}")
+    if not 1 <= Q.shape[3] <= 128:
+        raise RuntimeError(f"{who}: head_dim {Q.shape[3]} is not in 1 .. 128")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise RuntimeError(f"{who}: scale must be positive, got {scale}")
+    if lengths is not None:
+        if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != (Q.shape[0],):
+            raise RuntimeError(f"{who}: lengths must be ({Q.shape[0]},) of int32 or int64, got {tuple(lengths.shape)} of "
+                               f"{lengths.dtype}")
+
+
+def _masked_softmax(S: torch.Tensor) -> torch.Tensor:
+    """Softmax over the last dimension; a row of -inf alone gives zeros."""
+    m = S.amax(-1, keepdim=True).detach()
+    P = torch.exp(S - torch.where(m == float("-inf"), torch.zeros_like(m), m))
+    total = P.sum(-1, keepdim=True)
+    return P / torch.where(total == 0, torch.ones_like(total), total)
+
+
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t.float() if t.dtype in (torch.bfloat16, torch.float16) else t
+
+
+def _attn_parts_pytorch(Q, parts, scale):
+    """Grouped-head attention over several sets of keys in one softmax. Each
+    part is (K, V, seen): K, V (batch, kv_heads, keys, head_dim) and seen a
+    mask broadcast to (batch, 1, queries, keys) or None. What no query sees is
+    zeroed first: masked rows may hold anything."""
+    B, H, N, D = Q.shape
+    Hk = parts[0][0].shape[1]
+    G = H // Hk
+    q = _wide(Q).reshape(B, Hk, G * N, D)
+    scores, values = [], []
+    for K, V, seen in parts:
+        k, v = _wide(K), _wide(V)
+        if seen is not None:
+            some = seen.any(2).unsqueeze(-1)  # (batch, 1, keys, 1)
+            k, v = torch.where(some, k, torch.zeros_like(k)), torch.where(some, v, torch.zeros_like(v))
+        s = (q @ k.transpose(2, 3)) * scale
+        if seen is not None:
+            s = s.view(B, H, N, -1).masked_fill(~seen, float("-inf")).view(B, Hk, G * N, -1)
+        scores.append(s)
+        values.append(v)
+    if sum(s.shape[-1] for s in scores) == 0:
+        return Q * 0
+    P = _masked_softmax(torch.cat(scores, -1))
+    O = P.new_zeros(B, Hk, G * N, D)
+    at = 0
+    for s, v in zip(scores, values):
+        O = O + P[..., at : at + s.shape[-1]] @ v
+        at += s.shape[-1]
+    return O.reshape(B, H, N, D).to(Q.dtype)
+
+
+def cross_attention(
+    Q: torch.Tensor,
+    K: torch.Tensor,
+    V: torch.Tensor,
+    key_lengths: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Softmax attention of one sequence's queries over another's keys.
+
+    Q (batch, heads, queries, head_dim); K, V (batch, kv_heads, keys,
+    head_dim) of any other length, heads a multiple of kv_heads: query head h
+    reads key head h // (heads // kv_heads). `key_lengths` (batch,) int32 or
+    int64 gives each sample's number of valid keys (values are taken into
+    [0, keys]); what stands in K and V behind them is not read, and its
+    gradient is zero. A sample without keys gives zeros. `scale` defaults to
+    head_dim**-0.5 and is positive; head_dim is at most 128.
+
+    float32, bfloat16 and float16 on the HIP backend, accumulated in float32.
+    Operands may be strided views (heads of a projection's output); the result
+    has Q's order of heads and rows. Differentiable in Q, K and V.
+    """
+    if scale is None:
+        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
+    _check_heads("cross_attention", Q, K, V, key_lengths, scale)
+    if _use_hip():
+        from .hip.dispatch import hip_cross_attention
+
+        return hip_cross_attention(Q, K, V, key_lengths, scale)
+    seen = None
+    if key_lengths is not None:
+        at = torch.arange(K.shape[2], device=Q.device)
+        seen = (at < key_lengths.to(Q.device).view(-1, 1, 1, 1)).expand(-1, 1, Q.shape[2], -1)
+        if Q.shape[2] == 0:
+            return Q * 1
+    return _attn_parts_pytorch(Q, [(K, V, seen)], scale)
+
+
+def shared_prefix_attention(
+    Q: torch.Tensor,
+    prefix_K: torch.Tensor,
+    prefix_V: torch.Tensor,
+    K: torch.Tensor,
+    V: torch.Tensor,
+    lengths: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Attention of new tokens over a prefix that the whole batch shares and
+    each sequence's own tokens behind it (serving: no gradients).
+
+    Q (batch, heads, queries, head_dim), the new tokens: one, or a few in
+    order. prefix_K, prefix_V (kv_heads, prefix, head_dim), read once for the
+    batch. K, V (batch, kv_heads, keys, head_dim), each sequence's cache, whose
+    first lengths[b] rows hold its own tokens, the new ones last (None: all
+    rows; values are taken into [0, keys]); rows behind them are not read.
+    Query i sees the prefix and own tokens j < lengths[b] - (queries - 1 - i);
+    a query that sees nothing gives zeros. Types, heads, scale, strides and the
+    result's order as in `cross_attention`.
+    """
+    who = "shared_prefix_attention"
+    if scale is None:
+        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
+    _check_heads(who, Q, K, V, lengths, scale)
+    want = (K.shape[1], K.shape[3])
+    if prefix_K.dim() != 3 or prefix_K.shape != prefix_V.shape or (prefix_K.shape[0], prefix_K.shape[2]) != want:
+        raise RuntimeError(f"{who}: prefix_K {tuple(prefix_K.shape)} and prefix_V {tuple(prefix_V.shape)} must be "
+                           f"({want[0]}, prefix, {want[1]})")
+    if not (prefix_K.dtype == prefix_V.dtype == Q.dtype):
+        raise RuntimeError(f"{who}: the prefix must have Q's dtype {Q.dtype}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (Q, prefix_K, prefix_V, K, V)):
+        raise RuntimeError(f"{who} has no gradients: call it under torch.no_grad()")
+    if _use_hip():
+        from .hip.dispatch import hip_shared_prefix_attention
+
+        return hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale)
+    B, _, N, _ = Q.shape
+    if Q.numel() == 0:
+        return Q * 1
+    n = K.shape[2] if lengths is None else lengths.to(Q.device).clamp(0, K.shape[2]).view(-1, 1)
+    last = n - N + 1 + torch.arange(N, device=Q.device)  # own keys each query sees
+    seen = torch.arange(K.shape[2], device=Q.device) < last.expand(B, N).view(B, 1, N, 1)
+    shared = (prefix_K.expand(B, -1, -1, -1), prefix_V.expand(B, -1, -1, -1), None)
+    return _attn_parts_pytorch(Q, [shared, (K, V, seen)], scale)
