@@ -653,6 +653,57 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
                         void* O, const int64_t* o_strides, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/* ====================================================================
+ * RMS norm of query and key heads and their rotation by position.
+ *
+ * For every head vector x of Q (batch, q_heads, tokens, head_dim) and K
+ * (batch, k_heads, tokens, head_dim), with its side's weight w (head_dim,)
+ * and its token's position t:
+ *   r = 1 / sqrt(mean_d x_d^2 + eps),  n_d = x_d r w_d,
+ *   (y_a, y_b) = (n_a cos p - n_b sin p, n_b cos p + n_a sin p),
+ *   p = t inv_freq[j], for the pairs (a, b) = (j, j + rot / 2) or, with
+ *   interleaved, (2 j, 2 j + 1), j < rot / 2; y_d = n_d for d >= rot.
+ * Strides as in tsp_cross_attn_fwd (any, in elements; unit stride over
+ * head_dim); dtype TSP_F32, TSP_BF16 or TSP_F16; weights of weight_dtype:
+ * dtype or TSP_F32. positions of index_type at pos_batch_stride *
+ * b + pos_token_stride * i. inv_freq (rot / 2,) fp64; the angles are formed
+ * in 64 bits. head_dim is even and at most 256, rot even and at most
+ * head_dim. No counterpart in the reference, whose attention takes Q and K
+ * as they are (trnsparse/ops.py:549-625).
+ *
+ * tsp_qk_norm_rope_bwd: from the gradients of both results, those of Q, K
+ *   and, where dq_weight / dk_weight are not NULL, of the weights (in
+ *   weight_dtype). workspace (read only with a weight gradient):
+ *   tsp_qk_norm_rope_bwd_workspace_size bytes.
+ * ==================================================================== */
+int tsp_qk_norm_rope_fwd(const void* Q, const int64_t* q_strides, const void* K,
+                         const int64_t* k_strides, int dtype, int64_t batch,
+                         int64_t q_heads, int64_t k_heads, int64_t tokens,
+                         int64_t head_dim, const void* q_weight,
+                         const void* k_weight, int weight_dtype,
+                         const void* positions, int index_type,
+                         int64_t pos_batch_stride, int64_t pos_token_stride,
+                         const double* inv_freq, int64_t rot, int interleaved,
+                         double eps, void* Q_out, const int64_t* qo_strides,
+                         void* K_out, const int64_t* ko_strides, void* stream);
+int64_t tsp_qk_norm_rope_bwd_workspace_size(int64_t batch, int64_t tokens,
+                                            int64_t head_dim);
+int tsp_qk_norm_rope_bwd(const void* Q, const int64_t* q_strides, const void* K,
+                         const int64_t* k_strides, int dtype, int64_t batch,
+                         int64_t q_heads, int64_t k_heads, int64_t tokens,
+                         int64_t head_dim, const void* q_weight,
+                         const void* k_weight, int weight_dtype,
+                         const void* positions, int index_type,
+                         int64_t pos_batch_stride, int64_t pos_token_stride,
+                         const double* inv_freq, int64_t rot, int interleaved,
+                         double eps, const void* grad_Q,
+                         const int64_t* gq_strides, const void* grad_K,
+                         const int64_t* gk_strides, void* dQ,
+                         const int64_t* dq_strides, void* dK,
+                         const int64_t* dk_strides, void* dq_weight,
+                         void* dk_weight, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -69,3 +69,38 @@ def lengths_seen(lengths, N, L, causal=False):
     if causal:
         n = n - (N - 1 - torch.arange(N)).view(1, N, 1)
     return (torch.arange(L) < n).expand(-1, N, -1)
+
+
+def norm_rope(x, w, positions, inv_freq, eps, interleaved, dy=None):
+    """x (B, H, S, D), w (D,), positions (S,) or (B, S). Returns a dict in
+    float64: y; ay = |n_a| + |n_b| of each element's pair (its error scale);
+    with dy also dx, dw, and the scales adx = r (|w dn| + |x| r^2 / D sum |x w
+    dn|), adw = sum_rows |dn x r|, |dn| being |dy_a| + |dy_b|.
+    """
+    x, w = x.detach().double().cpu(), w.detach().double().cpu()
+    B, H, S, D = x.shape
+    pos = positions.cpu().double().expand(B, S)
+    f = inv_freq.detach().double().cpu()
+    half = f.numel()
+    idx = torch.arange(half)
+    a, b = (2 * idx, 2 * idx + 1) if interleaved else (idx, idx + half)
+    cos, sin = (fn(pos[:, None, :, None] * f) for fn in (torch.cos, torch.sin))
+    r = ((x * x).mean(-1, keepdim=True) + eps) ** -0.5
+    n = x * r * w
+
+    def turn(t, sgn):
+        y, ab = t.clone(), t.abs()
+        y[..., a] = t[..., a] * cos - sgn * t[..., b] * sin
+        y[..., b] = t[..., b] * cos + sgn * t[..., a] * sin
+        ab[..., a] = ab[..., b] = t[..., a].abs() + t[..., b].abs()
+        return y, ab
+
+    out = {}
+    out["y"], out["ay"] = turn(n, 1.0)
+    if dy is not None:
+        dn, adn = turn(dy.detach().double().cpu(), -1.0)
+        out["dw"] = (dn * x * r).sum((0, 1, 2))
+        out["adw"] = (adn * (x * r).abs()).sum((0, 1, 2))
+        out["dx"] = r * (w * dn) - x * r**3 * (x * w * dn).mean(-1, keepdim=True)
+        out["adx"] = r * ((w * adn).abs() + x.abs() * r**2 * (x * w * adn).abs().mean(-1, keepdim=True))
+    return out

@@ -63,6 +63,33 @@ def test_shared_prefix_attention(pytorch_backend, N):
         torch.testing.assert_close(O, r["O"], rtol=1e-12, atol=1e-12)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rot", [8, 4, 0])
+def test_qk_norm_rope(pytorch_backend, interleaved, rot):
+    """Against the formula, its gradients and differences."""
+    g = torch.Generator().manual_seed(2)
+    Q, K = (torch.randn(2, h, 3, 8, dtype=F64, generator=g).requires_grad_() for h in (3, 2))
+    wq, wk = (torch.randn(8, dtype=F64, generator=g).requires_grad_() for _ in range(2))
+    f = ts.rope_frequencies(rot, 100.0)
+    for pos in (torch.tensor([0, 5, 70000]), torch.tensor([[1, 2, 3], [9, -4, 0]], dtype=torch.int32)):
+        fn = lambda *t: ts.qk_norm_rope(*t, pos, f, 1e-3, interleaved)  # noqa: E731
+        outs = fn(Q, K, wq, wk)
+        dys = [torch.randn(o.shape, dtype=F64, generator=g) for o in outs]
+        dQ, dK, dwq, dwk = torch.autograd.grad(outs, (Q, K, wq, wk), dys)
+        for x, w, o, dy, dx, dw in ((Q, wq, outs[0], dys[0], dQ, dwq), (K, wk, outs[1], dys[1], dK, dwk)):
+            r = layer.norm_rope(x, w, pos, f, 1e-3, interleaved, dy)
+            for got, want in ((o, r["y"]), (dx, r["dx"]), (dw, r["dw"])):
+                torch.testing.assert_close(got, want, rtol=1e-11, atol=1e-11)
+        assert torch.autograd.gradcheck(fn, (Q, K, wq, wk))
+
+
+def test_rope_frequencies():
+    f = ts.rope_frequencies(64, 500.0)
+    assert f.dtype == F64 and f.shape == (32,) and f[0] == 1 and abs(f[16] - 500.0**-0.5) < 1e-15
+    with pytest.raises(RuntimeError):
+        ts.rope_frequencies(7)
+
+
 def refusals():
     Q, K, V = heads(2, 4, 2, 3, 5, 8)
     p = K[0]
@@ -76,6 +103,20 @@ def refusals():
         (s, (Q, p[:1], p[:1], K, V)), (s, (Q, p, p[:, :2], K, V)), (s, (Q, p[..., :4], p[..., :4], K, V)),
         (s, (Q, K, V, K, V)), (s, (Q, p.float(), p.float(), K, V)), (s, (Q.clone().requires_grad_(), p, p, K, V)),
         (s, (Q, p, p, K, V, torch.tensor([1, 2, 3]))),
+    ] + rope_refusals()
+
+
+def rope_refusals():
+    Q, K, _ = heads(2, 4, 2, 3, 3, 8)
+    w, pos, f, n = torch.ones(8, dtype=F64), torch.arange(3), ts.rope_frequencies(8), ts.qk_norm_rope
+    odd, big = (torch.zeros(1, 1, 3, d, dtype=F64) for d in (7, 258))
+    return [
+        (n, (Q[0], K[0], w, w, pos, f)), (n, (Q, K[:, :, :2], w, w, pos, f)), (n, (Q, K.float(), w, w, pos, f)),
+        (n, (Q, K, w[:4], w, pos, f)), (n, (Q, K, w, w.float(), pos, f)), (n, (Q.half(), K.half(), w, w, pos, f)),
+        (n, (odd, odd, w[:7], w[:7], pos, f[:2])), (n, (big, big, torch.ones(258), torch.ones(258), pos, f)),
+        (n, (Q, K, w, w, pos, ts.rope_frequencies(10))), (n, (Q, K, w, w, pos, f.view(2, 2))), (n, (Q, K, w, w, pos, pos)),
+        (n, (Q, K, w, w, pos.float(), f)), (n, (Q, K, w, w, pos[:2], f)), (n, (Q, K, w, w, pos.view(1, 3), f)),
+        (n, (Q, K, w, w, pos, f, -1.0)), (n, (Q, K, w, w, pos, f, float("nan"))),
     ]
 
 

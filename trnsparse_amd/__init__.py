@@ -19,6 +19,8 @@ from .ops import (
     bsr_spmm,
     cross_attention,
     nnz_per_row,
+    qk_norm_rope,
+    rope_frequencies,
     screened_mask,
     screened_spmm,
     shared_prefix_attention,
@@ -46,6 +48,8 @@ __all__ = [
     "block_sparse_attention_tiled",
     "cross_attention",
     "shared_prefix_attention",
+    "qk_norm_rope",
+    "rope_frequencies",
     "sparse_add",
     "sparse_scale",
     "sparse_transpose",

@@ -1,0 +1,483 @@
+// RMS norm of query and key heads and the rotation by their tokens' positions,
+// in one pass, for gfx950. For a head vector x of D elements, weight w and the
+// token's position t:
+//   r = 1 / sqrt(mean_d x_d^2 + eps),  n_d = x_d r w_d
+//   (y_a, y_b) = (n_a cos p - n_b sin p, n_b cos p + n_a sin p),  p = t f_j
+// for the pair (a, b) of every frequency f_j, j < rot / 2: (j, j + rot / 2), or
+// (2 j, 2 j + 1) interleaved; elements from rot on are not rotated. Backward:
+// dn is dy rotated back, dw = sum_rows dn x r and
+//   dx_d = r (w_d dn_d) - x_d r^3 / D sum_e x_e w_e dn_e.
+// No counterpart in the reference, whose attention takes Q and K as they are
+// (trnsparse/ops.py:549-625).
+//
+// Bound by memory: x in and y out once (backward: x and dy in, dx out). A row
+// is held by a group of lanes, each with two chunks of CE elements that hold
+// whole pairs (chunk t of either half, or two chunks in a row), so rotation
+// needs no other lane and the sums a few shuffles. A wavefront's groups take
+// consecutive heads of one token: they lie together in a projection's output,
+// and the angles are formed once for all of them. Angles are products in 64
+// bits, reduced to half turns there: a position of 10^6 would leave an fp32
+// product no correct digit after the point. Sums, norms and weight gradients
+// are fp32; a result is rounded once.
+//
+// Weight gradients: every workgroup sums its tokens' rows in registers and
+// writes one part; wgrad_kernel adds the parts in a fixed order, so results do
+// not change from run to run.
+#include "common.h"
+
+namespace {
+
+template <typename E, int CE>
+struct alignas(sizeof(E) * CE) Chunk {
+  E v[CE];
+};
+
+__device__ inline float widen(float x) { return x; }
+__device__ inline float widen(__bf16 x) { return (float)x; }
+__device__ inline float widen(_Float16 x) { return (float)x; }
+
+struct Rows {
+  const char* p;
+  int64_t b, h, s;  // strides in bytes
+};
+struct Side {  // the query or the key heads
+  Rows x, y, g;   // x; y (forward: written) or dx (backward: written); dy
+  const void* w;
+  int H;
+};
+struct Args {
+  Side side[2];
+  const void* pos;
+  int64_t pos_b, pos_s;  // strides in elements
+  int pos64, w32;        // positions are int64; weights are fp32 (else the rows' type)
+  const double* freq;
+  int S, D, rot, interleaved, need_w;
+  int64_t tokens;
+  int parts;   // forward: wavefronts to a token
+  float eps;
+  float* wpart;  // (workgroups, 2, D)
+};
+
+// Where the two chunks of lane t's pair of chunks start, and the first of their
+// frequencies (-1: not rotated).
+struct Place {
+  int a, b, j;
+  bool on;
+};
+template <int CE>
+__device__ inline Place place(const Args& g, int t) {
+  Place p;
+  p.on = 2 * CE * t < g.D;
+  const int half = g.rot / 2;
+  if (g.interleaved) {
+    p.a = 2 * CE * t;
+    p.b = p.a + CE;
+    p.j = p.a < g.rot ? p.a / 2 : -1;
+  } else if (CE * t < half) {
+    p.a = CE * t;
+    p.b = half + CE * t;
+    p.j = CE * t;
+  } else {
+    p.a = g.rot + 2 * (CE * t - half);
+    p.b = p.a + CE;
+    p.j = -1;
+  }
+  return p;
+}
+
+template <int CE>
+struct Angles {
+  float c[CE], s[CE];
+  __device__ inline void set(const Args& g, const Place& p, int64_t b, int64_t i) {
+    const int64_t at = b * g.pos_b + i * g.pos_s;
+    const double t = g.pos64 ? (double)((const int64_t*)g.pos)[at] : (double)((const int32_t*)g.pos)[at];
+#pragma unroll
+    for (int e = 0; e < CE; ++e) {
+      c[e] = 1.f;
+      s[e] = 0.f;
+      if (p.on && p.j >= 0 && p.j + e < g.rot / 2) {
+        // less whole turns, 2 pi in two parts: right to 2^-50 at any angle
+        double angle = t * g.freq[p.j + e];
+        const double turns = __builtin_rint(angle * 0.15915494309189535);
+        angle = __builtin_fma(-turns, 6.283185307179586477, angle);
+        angle = __builtin_fma(-turns, 2.449293598294706414e-16, angle);
+        sincospif((float)(angle * 0.31830988618379067154), &s[e], &c[e]);
+      }
+    }
+  }
+  // forward (dir = 1) or back (dir = -1), of the chunk pair x[0 .. 2 CE)
+  __device__ inline void turn(float* x, bool interleaved, float dir) const {
+    auto pair = [&](float& a, float& b, int e) {
+      const float sn = dir * s[e], na = a * c[e] - b * sn, nb = b * c[e] + a * sn;
+      a = na;
+      b = nb;
+    };
+    if (interleaved) {
+      if constexpr (CE == 1) {
+        pair(x[0], x[1], 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < CE; ++e) pair(x[2 * e], x[2 * e + 1], e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < CE; ++e) pair(x[e], x[CE + e], e);
+    }
+  }
+};
+
+template <typename E, int CE>
+__device__ inline void load2(float* x, const char* row, const Place& p) {
+  if (p.on) {
+    const Chunk<E, CE> a = *(const Chunk<E, CE>*)(row + p.a * sizeof(E)), b = *(const Chunk<E, CE>*)(row + p.b * sizeof(E));
+#pragma unroll
+    for (int e = 0; e < CE; ++e) {
+      x[e] = widen(a.v[e]);
+      x[CE + e] = widen(b.v[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2 * CE; ++e) x[e] = 0.f;
+  }
+}
+template <typename E, int CE>
+__device__ inline void store2(char* row, const float* x, const Place& p) {
+  if (!p.on) return;
+  Chunk<E, CE> a, b;
+#pragma unroll
+  for (int e = 0; e < CE; ++e) {
+    a.v[e] = (E)x[e];
+    b.v[e] = (E)x[CE + e];
+  }
+  *(Chunk<E, CE>*)(row + p.a * sizeof(E)) = a;
+  *(Chunk<E, CE>*)(row + p.b * sizeof(E)) = b;
+}
+template <typename E, int CE>
+__device__ inline void load_weight(float* w, const void* p0, bool w32, const Place& p) {
+#pragma unroll
+  for (int e = 0; e < 2 * CE; ++e) {
+    const int d = (e < CE ? p.a : p.b - CE) + e;
+    w[e] = !p.on ? 0.f : w32 ? ((const float*)p0)[d] : widen(((const E*)p0)[d]);
+  }
+}
+__device__ inline float lanes_sum(float v, int G) {
+  for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// J chunk pairs to a lane, G lanes to a row.
+template <typename E, int CE, int J, int G>
+__global__ __launch_bounds__(256) void norm_rope_fwd(const Args g) {
+  constexpr int GW = 64 / G;  // rows a wavefront takes at once
+  const int lane = threadIdx.x & 63, t0 = lane % G, grp = lane / G;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t tok = item / g.parts;
+  const int part = (int)(item - tok * g.parts);
+  if (tok >= g.tokens) return;
+  const int64_t b = tok / g.S, i = tok - b * g.S;
+  Place p[J];
+  Angles<CE> ang[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    p[j] = place<CE>(g, t0 + j * G);
+    ang[j].set(g, p[j], b, i);
+  }
+#pragma unroll
+  for (int sd = 0; sd < 2; ++sd) {
+    const Side& s = g.side[sd];
+    float w[J][2 * CE];
+#pragma unroll
+    for (int j = 0; j < J; ++j) load_weight<E, CE>(w[j], s.w, g.w32, p[j]);
+    for (int hd = part * GW + grp; hd < s.H; hd += GW * g.parts) {
+      const char* row = s.x.p + b * s.x.b + hd * s.x.h + i * s.x.s;
+      float x[J][2 * CE], ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        load2<E, CE>(x[j], row, p[j]);
+#pragma unroll
+        for (int e = 0; e < 2 * CE; ++e) ss += x[j][e] * x[j][e];
+      }
+      const float r = __builtin_amdgcn_rsqf(lanes_sum(ss, G) / (float)g.D + g.eps);
+      char* out = (char*)s.y.p + b * s.y.b + hd * s.y.h + i * s.y.s;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2 * CE; ++e) x[j][e] *= r * w[j][e];
+        ang[j].turn(x[j], g.interleaved, 1.f);
+        store2<E, CE>(out, x[j], p[j]);
+      }
+    }
+  }
+}
+
+template <typename E, int CE, int J, int G>
+__global__ __launch_bounds__(256) void norm_rope_bwd(const Args g) {
+  constexpr int GW = 64 / G;
+  __shared__ float sum[4][2][256];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, t0 = lane % G, grp = lane / G;
+  Place p[J];
+  float w[2][J][2 * CE], dw[2][J][2 * CE];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    p[j] = place<CE>(g, t0 + j * G);
+#pragma unroll
+    for (int sd = 0; sd < 2; ++sd) {
+      load_weight<E, CE>(w[sd][j], g.side[sd].w, g.w32, p[j]);
+#pragma unroll
+      for (int e = 0; e < 2 * CE; ++e) dw[sd][j][e] = 0.f;
+    }
+  }
+  const float invD = 1.f / (float)g.D;
+  for (int64_t tok = (int64_t)blockIdx.x * 4 + wv; tok < g.tokens; tok += (int64_t)gridDim.x * 4) {
+    const int64_t b = tok / g.S, i = tok - b * g.S;
+    Angles<CE> ang[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) ang[j].set(g, p[j], b, i);
+#pragma unroll
+    for (int sd = 0; sd < 2; ++sd) {
+      const Side& s = g.side[sd];
+      for (int hd = grp; hd < s.H; hd += GW) {
+        const char* row = s.x.p + b * s.x.b + hd * s.x.h + i * s.x.s;
+        const char* grow = s.g.p + b * s.g.b + hd * s.g.h + i * s.g.s;
+        float x[J][2 * CE], d[J][2 * CE], ss = 0.f, sw = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          load2<E, CE>(x[j], row, p[j]);
+          load2<E, CE>(d[j], grow, p[j]);
+          ang[j].turn(d[j], g.interleaved, -1.f);
+#pragma unroll
+          for (int e = 0; e < 2 * CE; ++e) {
+            ss += x[j][e] * x[j][e];
+            sw += x[j][e] * (w[sd][j][e] * d[j][e]);
+          }
+        }
+        const float r = __builtin_amdgcn_rsqf(lanes_sum(ss, G) * invD + g.eps);
+        const float c = r * r * r * invD * lanes_sum(sw, G);
+        char* out = (char*)s.y.p + b * s.y.b + hd * s.y.h + i * s.y.s;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+          for (int e = 0; e < 2 * CE; ++e) {
+            dw[sd][j][e] += d[j][e] * (x[j][e] * r);
+            x[j][e] = r * (w[sd][j][e] * d[j][e]) - x[j][e] * c;
+          }
+          store2<E, CE>(out, x[j], p[j]);
+        }
+      }
+    }
+  }
+  if (!g.need_w) return;
+  // ---- the wavefront's groups, then the four wavefronts, in a fixed order
+#pragma unroll
+  for (int sd = 0; sd < 2; ++sd)
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 2 * CE; ++e) {
+        float v = dw[sd][j][e];
+        for (int o = G; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+        if (grp == 0 && p[j].on) sum[wv][sd][(e < CE ? p[j].a : p[j].b - CE) + e] = v;
+      }
+  __syncthreads();
+  for (int k = threadIdx.x; k < 2 * g.D; k += 256) {
+    const int sd = k / g.D, d = k - sd * g.D;
+    g.wpart[(int64_t)blockIdx.x * 2 * g.D + k] = (sum[0][sd][d] + sum[1][sd][d]) + (sum[2][sd][d] + sum[3][sd][d]);
+  }
+}
+
+// dw of 32 columns of (2, D): 32 threads to a column, then their sums in order.
+template <typename E>
+__global__ __launch_bounds__(1024) void wgrad_kernel(const float* __restrict__ part, int n, int D, int w32, void* dwq,
+                                                     void* dwk) {
+  __shared__ float sum[32][33];
+  const int c = threadIdx.x & 31, rg = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
+  float v = 0.f;
+  if (col < 2 * D)
+    for (int k = rg; k < n; k += 32) v += part[(int64_t)k * 2 * D + col];
+  sum[rg][c] = v;
+  __syncthreads();
+  if (rg != 0 || col >= 2 * D) return;
+  float t = 0.f;
+  for (int k = 0; k < 32; ++k) t += sum[k][c];
+  void* out = col < D ? dwq : dwk;
+  const int d = col < D ? col : col - D;
+  if (!out) return;
+  if (w32)
+    ((float*)out)[d] = t;
+  else
+    ((E*)out)[d] = (E)t;
+}
+
+constexpr int MAX_WGS = 512;  // parts of a weight gradient
+
+int bwd_wgs(int64_t tokens) {
+  const int64_t n = tsp::ceil_div(tokens, 4);
+  return (int)(n < 1 ? 1 : n < MAX_WGS ? n : MAX_WGS);
+}
+
+template <typename E, int CE, int J, int G>
+int launch(const Args& a, bool back, hipStream_t st) {
+  const int64_t grid = back ? bwd_wgs(a.tokens) : tsp::ceil_div(a.tokens * a.parts, 4);
+  if (grid > INT32_MAX) return tsp::fail(TSP_EUNSUPPORTED, "qk_norm_rope: too many tokens");
+  if (back)
+    hipLaunchKernelGGL((norm_rope_bwd<E, CE, J, G>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((norm_rope_fwd<E, CE, J, G>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  return tsp::check_launch("norm_rope launch");
+}
+template <typename E, int CE>
+int launch_ce(Args a, bool back, hipStream_t st) {
+  const int lanes = (a.D + 2 * CE - 1) / (2 * CE);
+  // wavefronts to a token: all its heads at once while the chip is not full
+  const int G = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
+  const int most = (int)tsp::ceil_div(a.side[0].H > a.side[1].H ? a.side[0].H : a.side[1].H, 64 / G);
+  const int64_t want = tsp::ceil_div(4096, a.tokens > 0 ? a.tokens : 1);
+  a.parts = (int)(want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most);
+  if (lanes <= 4) return launch<E, CE, 1, 4>(a, back, st);
+  if (lanes <= 8) return launch<E, CE, 1, 8>(a, back, st);
+  if (CE == 8 || lanes <= 16) return launch<E, CE, 1, 16>(a, back, st);
+  if constexpr (CE <= 4)
+    if (CE == 4 || lanes <= 32) return launch<E, CE, 1, 32>(a, back, st);
+  if constexpr (CE <= 2)
+    if (CE == 2 || lanes <= 64) return launch<E, CE, 1, 64>(a, back, st);
+  if constexpr (CE == 1) return launch<E, CE, 2, 64>(a, back, st);
+  return TSP_EUNSUPPORTED;  // not reached: head_dim is at most 256
+}
+
+// The widest chunk that the pairing, the addresses and the strides allow.
+template <typename E>
+int launch_e(const Args& a, bool back, hipStream_t st) {
+  uint64_t all = 0;
+  for (const Side& s : a.side)
+    if (s.H > 0)
+      for (const Rows* r : {&s.x, &s.y, &s.g}) all |= (uint64_t)(uintptr_t)r->p | r->b | r->h | r->s;
+  auto fits = [&](int ce) {
+    return a.D % (2 * ce) == 0 && (a.interleaved || a.rot / 2 % ce == 0) && all % (ce * sizeof(E)) == 0;
+  };
+  if constexpr (sizeof(E) == 2)
+    if (fits(8)) return launch_ce<E, 8>(a, back, st);
+  if (fits(4)) return launch_ce<E, 4>(a, back, st);
+  if (fits(2)) return launch_ce<E, 2>(a, back, st);
+  return launch_ce<E, 1>(a, back, st);
+}
+
+int run(int dtype, const Args& a, bool back, hipStream_t st) {
+  if (dtype == TSP_F32) return launch_e<float>(a, back, st);
+  if (dtype == TSP_BF16) return launch_e<__bf16>(a, back, st);
+  return launch_e<_Float16>(a, back, st);
+}
+
+Rows rows(const void* p, const int64_t* s, int e) {
+  if (!p || !s) return Rows{nullptr, 0, 0, 0};
+  return Rows{(const char*)p, s[0] * e, s[1] * e, s[2] * e};
+}
+
+int fill(const char* who, Args& a, int dtype, int64_t B, int64_t Hq, int64_t Hk, int64_t S, int64_t D, const void* wq,
+         const void* wk, int wdtype, const void* pos, int index_type, int64_t pos_b, int64_t pos_s, const double* freq,
+         int64_t rot, int interleaved, double eps) {
+  if (dtype != TSP_F32 && dtype != TSP_BF16 && dtype != TSP_F16)
+    return tsp::fail(TSP_EUNSUPPORTED, "%s: dtype %d not supported", who, dtype);
+  if (wdtype != dtype && wdtype != TSP_F32)
+    return tsp::fail(TSP_EUNSUPPORTED, "%s: weights must have the rows' type or fp32", who);
+  if (B < 0 || Hq < 0 || Hk < 0 || S < 0 || D < 2 || rot < 0 || rot > D || D % 2 || rot % 2)
+    return tsp::fail(TSP_EINVAL, "%s: bad sizes batch %lld heads %lld, %lld tokens %lld head_dim %lld rotated %lld", who,
+                     (long long)B, (long long)Hq, (long long)Hk, (long long)S, (long long)D, (long long)rot);
+  if (D > 256) return tsp::fail(TSP_EUNSUPPORTED, "%s: head_dim %lld is over 256", who, (long long)D);
+  if (S > INT32_MAX || Hq > INT32_MAX || Hk > INT32_MAX || B * S > (int64_t(1) << 32))
+    return tsp::fail(TSP_EUNSUPPORTED, "%s: too many rows", who);
+  if (index_type != TSP_I32 && index_type != TSP_I64) return tsp::fail(TSP_EINVAL, "%s: bad index type", who);
+  if (!(eps >= 0)) return tsp::fail(TSP_EINVAL, "%s: eps must not be negative", who);
+  if (B * S * (Hq + Hk) > 0 && (!pos || !wq || !wk || (rot > 0 && !freq)))
+    return tsp::fail(TSP_EINVAL, "%s: null operand", who);
+  a.side[0].w = wq;
+  a.side[1].w = wk;
+  a.side[0].H = (int)Hq;
+  a.side[1].H = (int)Hk;
+  a.pos = pos;
+  a.pos_b = pos_b;
+  a.pos_s = pos_s;
+  a.pos64 = index_type == TSP_I64;
+  a.w32 = wdtype == TSP_F32;
+  a.freq = freq;
+  a.S = (int)S;
+  a.D = (int)D;
+  a.rot = (int)rot;
+  a.interleaved = interleaved != 0;
+  a.tokens = B * S;
+  a.eps = (float)eps;
+  return TSP_OK;
+}
+
+int need(const char* who, const char* name, int64_t heads, const void* p, const int64_t* s) {
+  return heads > 0 && (!p || !s) ? tsp::fail(TSP_EINVAL, "%s: null %s", who, name) : TSP_OK;
+}
+
+}  // namespace
+
+extern "C" int tsp_qk_norm_rope_fwd(const void* Q, const int64_t* qs, const void* K, const int64_t* ks, int dtype,
+                                    int64_t B, int64_t Hq, int64_t Hk, int64_t S, int64_t D, const void* wq,
+                                    const void* wk, int wdtype, const void* pos, int index_type, int64_t pos_b,
+                                    int64_t pos_s, const double* freq, int64_t rot, int interleaved, double eps, void* Qo,
+                                    const int64_t* qos, void* Ko, const int64_t* kos, void* stream) {
+  const char* who = "tsp_qk_norm_rope_fwd";
+  Args a{};
+  int rc = fill(who, a, dtype, B, Hq, Hk, S, D, wq, wk, wdtype, pos, index_type, pos_b, pos_s, freq, rot, interleaved, eps);
+  if (rc) return rc;
+  if (a.tokens * (Hq + Hk) == 0) return TSP_OK;
+  if ((rc = need(who, "Q", Hq, Q, qs)) || (rc = need(who, "K", Hk, K, ks)) || (rc = need(who, "Q result", Hq, Qo, qos)) ||
+      (rc = need(who, "K result", Hk, Ko, kos)))
+    return rc;
+  const int e = dtype == TSP_F32 ? 4 : 2;
+  a.side[0].x = rows(Q, qs, e);
+  a.side[1].x = rows(K, ks, e);
+  a.side[0].y = rows(Qo, qos, e);
+  a.side[1].y = rows(Ko, kos, e);
+  return run(dtype, a, false, (hipStream_t)stream);
+}
+
+extern "C" int64_t tsp_qk_norm_rope_bwd_workspace_size(int64_t B, int64_t S, int64_t D) {
+  if (B < 0 || S < 0 || D < 2 || D > 256 || B * S > (int64_t(1) << 32)) return -1;
+  return (int64_t)bwd_wgs(B * S) * 2 * D * 4;
+}
+
+extern "C" int tsp_qk_norm_rope_bwd(const void* Q, const int64_t* qs, const void* K, const int64_t* ks, int dtype,
+                                    int64_t B, int64_t Hq, int64_t Hk, int64_t S, int64_t D, const void* wq,
+                                    const void* wk, int wdtype, const void* pos, int index_type, int64_t pos_b,
+                                    int64_t pos_s, const double* freq, int64_t rot, int interleaved, double eps,
+                                    const void* gQ, const int64_t* gqs, const void* gK, const int64_t* gks, void* dQ,
+                                    const int64_t* dqs, void* dK, const int64_t* dks, void* dwq, void* dwk,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "tsp_qk_norm_rope_bwd";
+  Args a{};
+  int rc = fill(who, a, dtype, B, Hq, Hk, S, D, wq, wk, wdtype, pos, index_type, pos_b, pos_s, freq, rot, interleaved, eps);
+  if (rc) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  const int ew = wdtype == TSP_F32 ? 4 : 2, e = dtype == TSP_F32 ? 4 : 2;
+  if (a.tokens * (Hq + Hk) == 0) {  // no row: the weights' gradients are zero
+    for (void* w : {dwq, dwk})
+      if (w && (rc = tsp::zero_fill(w, D * ew, st))) return rc;
+    return TSP_OK;
+  }
+  if ((rc = need(who, "Q", Hq, Q, qs)) || (rc = need(who, "K", Hk, K, ks)) || (rc = need(who, "grad of Q", Hq, gQ, gqs)) ||
+      (rc = need(who, "grad of K", Hk, gK, gks)) || (rc = need(who, "dQ", Hq, dQ, dqs)) ||
+      (rc = need(who, "dK", Hk, dK, dks)))
+    return rc;
+  a.need_w = dwq || dwk;
+  if (a.need_w && (!workspace || workspace_bytes < tsp_qk_norm_rope_bwd_workspace_size(B, S, D)))
+    return tsp::fail(TSP_EINVAL, "%s: workspace too small", who);
+  a.side[0].x = rows(Q, qs, e);
+  a.side[1].x = rows(K, ks, e);
+  a.side[0].g = rows(gQ, gqs, e);
+  a.side[1].g = rows(gK, gks, e);
+  a.side[0].y = rows(dQ, dqs, e);
+  a.side[1].y = rows(dK, dks, e);
+  a.wpart = (float*)workspace;
+  if ((rc = run(dtype, a, true, st)) || !a.need_w) return rc;
+  const dim3 grid((unsigned)tsp::ceil_div(2 * D, 32)), block(1024);
+  const int n = bwd_wgs(a.tokens), w32 = wdtype == TSP_F32;
+  if (dtype == TSP_BF16)
+    hipLaunchKernelGGL((wgrad_kernel<__bf16>), grid, block, 0, st, a.wpart, n, (int)D, w32, dwq, dwk);
+  else
+    hipLaunchKernelGGL((wgrad_kernel<_Float16>), grid, block, 0, st, a.wpart, n, (int)D, w32, dwq, dwk);
+  return tsp::check_launch("wgrad launch");
+}

@@ -628,6 +628,97 @@ at::Tensor prefix_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at
   return Q.size(3) == piece_dim(Q) ? attn_like(Q, Q.size(3)) : at::empty(Q.sizes(), Q.options());
 }
 
+// --------------------------------- norm and rotation of query and key heads
+
+// t with unit stride over head_dim (a contiguous copy where it has another)
+at::Tensor unit_rows(const at::Tensor& t) {
+  return t.stride(3) == 1 || t.size(3) == 1 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+struct RopeArgs {
+  int code, wcode, icode;
+  int64_t pos_b, pos_s, rot;
+  RopeArgs(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& pos,
+           const at::Tensor& freq, const char* who) {
+    need_4d(Q, Q, who, "Q");
+    need_4d(K, Q, who, "K");
+    code = attn_dtype(Q.scalar_type(), who);
+    const int64_t B = Q.size(0), S = Q.size(2), D = Q.size(3);
+    TORCH_CHECK(K.size(0) == B && K.size(2) == S, who, ": K must have Q's batch and tokens");
+    for (auto* w : {&wq, &wk}) {
+      need(*w, Q, "weight");
+      TORCH_CHECK(w->dim() == 1 && w->numel() == D, who, ": weights must be (head_dim,)");
+      TORCH_CHECK(w->scalar_type() == wq.scalar_type() &&
+                      (w->scalar_type() == Q.scalar_type() || w->scalar_type() == at::kFloat),
+                  who, ": weights must both have Q's dtype or both be float32");
+    }
+    wcode = attn_dtype(wq.scalar_type(), who);
+    TORCH_CHECK(pos.device() == Q.device(), who, ": positions are on ", pos.device(), ", expected ", Q.device());
+    icode = index_code(pos.scalar_type());
+    TORCH_CHECK((pos.dim() == 1 && pos.size(0) == S) || (pos.dim() == 2 && pos.size(0) == B && pos.size(1) == S), who,
+                ": positions must be (tokens,) or (batch, tokens)");
+    pos_b = pos.dim() == 2 ? pos.stride(0) : 0;
+    pos_s = pos.stride(pos.dim() - 1);
+    need(freq, Q, "inv_freq");
+    need_dtype(freq, at::kDouble, who, "inv_freq");
+    TORCH_CHECK(freq.dim() == 1, who, ": inv_freq must be (rot / 2,)");
+    rot = 2 * freq.numel();
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& Q_, const at::Tensor& K_, const at::Tensor& wq,
+                                                    const at::Tensor& wk, const at::Tensor& pos, const at::Tensor& freq,
+                                                    double eps, bool interleaved) {
+  const RopeArgs r(Q_, K_, wq, wk, pos, freq, "qk_norm_rope_fwd");
+  const auto Q = unit_rows(Q_), K = unit_rows(K_);
+  auto Qo = at::empty(Q.sizes(), Q.options()), Ko = at::empty(K.sizes(), K.options());
+  check(tsp_qk_norm_rope_fwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, r.code, Q.size(0), Q.size(1),
+                             K.size(1), Q.size(2), Q.size(3), wq.data_ptr(), wk.data_ptr(), r.wcode, pos.data_ptr(),
+                             r.icode, r.pos_b, r.pos_s, freq.data_ptr<double>(), r.rot, interleaved, eps, Qo.data_ptr(),
+                             Strides(Qo).s, Ko.data_ptr(), Strides(Ko).s, stream_of(Q)),
+        "tsp_qk_norm_rope_fwd");
+  return {Qo, Ko};
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd_meta(const at::Tensor& Q, const at::Tensor& K, const at::Tensor&,
+                                                         const at::Tensor&, const at::Tensor&, const at::Tensor&, double,
+                                                         bool) {
+  return {at::empty(Q.sizes(), Q.options()), at::empty(K.sizes(), K.options())};
+}
+
+// a weight gradient that is not asked for comes back empty
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
+    const at::Tensor& Q_, const at::Tensor& K_, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& pos,
+    const at::Tensor& freq, double eps, bool interleaved, const at::Tensor& gQ_, const at::Tensor& gK_,
+    bool need_weights) {
+  const char* who = "qk_norm_rope_bwd";
+  const RopeArgs r(Q_, K_, wq, wk, pos, freq, who);
+  need_4d(gQ_, Q_, who, "grad_Q");
+  need_4d(gK_, Q_, who, "grad_K");
+  TORCH_CHECK(gQ_.sizes() == Q_.sizes() && gK_.sizes() == K_.sizes(), who, ": gradients must have the results' shapes");
+  const auto Q = unit_rows(Q_), K = unit_rows(K_), gQ = unit_rows(gQ_), gK = unit_rows(gK_);
+  auto dQ = attn_like(Q_, Q.size(3)), dK = attn_like(K_, K.size(3));
+  auto dwq = need_weights ? at::empty_like(wq) : at::empty({0}, wq.options());
+  auto dwk = need_weights ? at::empty_like(wk) : at::empty({0}, wk.options());
+  const int64_t wsb = tsp_qk_norm_rope_bwd_workspace_size(Q.size(0), Q.size(2), Q.size(3));
+  auto ws = workspace_of(need_weights ? std::max<int64_t>(wsb, 0) : 0, Q, who);
+  check(tsp_qk_norm_rope_bwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, r.code, Q.size(0), Q.size(1),
+                             K.size(1), Q.size(2), Q.size(3), wq.data_ptr(), wk.data_ptr(), r.wcode, pos.data_ptr(),
+                             r.icode, r.pos_b, r.pos_s, freq.data_ptr<double>(), r.rot, interleaved, eps, gQ.data_ptr(),
+                             Strides(gQ).s, gK.data_ptr(), Strides(gK).s, dQ.data_ptr(), Strides(dQ).s, dK.data_ptr(),
+                             Strides(dK).s, need_weights ? dwq.data_ptr() : nullptr,
+                             need_weights ? dwk.data_ptr() : nullptr, ws.data_ptr(), wsb, stream_of(Q)),
+        "tsp_qk_norm_rope_bwd");
+  return {dQ, dK, dwq, dwk};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd_meta(
+    const at::Tensor& Q, const at::Tensor& K, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor&,
+    const at::Tensor&, double, bool, const at::Tensor&, const at::Tensor&, bool need_weights) {
+  return {attn_like(Q, Q.size(3)), attn_like(K, K.size(3)), need_weights ? at::empty_like(wq) : at::empty({0}, wq.options()),
+          need_weights ? at::empty_like(wk) : at::empty({0}, wk.options())};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(trnsparse_hip, m) {
@@ -657,6 +748,11 @@ TORCH_LIBRARY(trnsparse_hip, m) {
         "(Tensor, Tensor)");
   m.def("prefix_attn_fwd(Tensor Q, Tensor prefix_K, Tensor prefix_V, Tensor K, Tensor V, Tensor? lengths, "
         "float scale) -> Tensor");
+  m.def("qk_norm_rope_fwd(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
+        "float eps, bool interleaved) -> (Tensor, Tensor)");
+  m.def("qk_norm_rope_bwd(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
+        "float eps, bool interleaved, Tensor grad_Q, Tensor grad_K, bool need_weights) -> (Tensor, Tensor, Tensor, "
+        "Tensor)");
 }
 
 // the "CUDA" dispatch key is the GPU key of PyTorch-ROCm
@@ -674,6 +770,8 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
   m.impl("bsa_bwd", &bsa_bwd);
   m.impl("cross_attn_fwd", &cross_attn_fwd);
   m.impl("prefix_attn_fwd", &prefix_attn_fwd);
+  m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
 }
 
 TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
@@ -690,4 +788,6 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
   m.impl("bsa_bwd", &bsa_bwd_meta);
   m.impl("cross_attn_fwd", &cross_attn_fwd_meta);
   m.impl("prefix_attn_fwd", &prefix_attn_fwd_meta);
+  m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd_meta);
+  m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_meta);
 }

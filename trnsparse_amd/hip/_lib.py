@@ -104,6 +104,11 @@ SIGNATURES: dict[str, tuple] = {
     "tsp_prefix_attn_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "tsp_prefix_attn_fwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64,
                                    _I64, _P, _INT, _DBL, _P, _P, _P, _I64, _P]),
+    "tsp_qk_norm_rope_fwd": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _INT, _P, _INT, _I64,
+                                    _I64, _P, _I64, _INT, _DBL, _P, _P, _P, _P, _P]),
+    "tsp_qk_norm_rope_bwd_workspace_size": (_I64, [_I64, _I64, _I64]),
+    "tsp_qk_norm_rope_bwd": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _INT, _P, _INT, _I64,
+                                    _I64, _P, _I64, _INT, _DBL, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
 }
 
 _lib = None

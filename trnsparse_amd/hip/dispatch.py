@@ -955,3 +955,43 @@ def hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale: flo
         Q, prefix_K, prefix_V, K, V = (t.to(dev) for t in (Q, prefix_K, prefix_V, K, V))
         lens = _lengths_on(lengths, dev)
         return _lib.ops().prefix_attn_fwd(Q, prefix_K, prefix_V, K, V, lens, float(scale)).to(orig)
+
+
+# ------------------------------- norm and rotation of query and key heads
+
+
+class _QKNormRopeFunction(torch.autograd.Function):
+    """Autograd wrapper of the norm and rotation: keeps Q, K and the weights,
+    forms the norms and angles again in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved):
+        ctx.save_for_backward(Q, K, q_weight, k_weight, positions, inv_freq)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return _lib.ops().qk_norm_rope_fwd(Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gQ, gK):
+        Q, K, wq, wk, pos, freq = ctx.saved_tensors
+        with torch.cuda.device(Q.device):
+            need_w = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+            dQ, dK, dwq, dwk = _lib.ops().qk_norm_rope_bwd(Q, K, wq, wk, pos, freq, ctx.eps, ctx.interleaved, gQ, gK, need_w)
+        return dQ, dK, (dwq if need_w else None), (dwk if need_w else None), None, None, None, None
+
+
+@_library_call
+def hip_qk_norm_rope(Q, K, q_weight, k_weight, positions, inv_freq, eps: float, interleaved: bool):
+    """qk_norm_rope on the HIP kernels."""
+    orig = Q.device
+    dev = _target_device(Q, K)
+    with torch.cuda.device(dev):
+        Q, K = Q.to(dev), K.to(dev)
+        wq, wk = q_weight.to(dev).contiguous(), k_weight.to(dev).contiguous()
+        pos, freq = positions.to(dev), inv_freq.detach().to(dev, torch.float64).contiguous()
+        args = (Q, K, wq, wk, pos, freq, float(eps), bool(interleaved))
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (Q, K, wq, wk)):
+            out = _QKNormRopeFunction.apply(*args)
+        else:
+            out = _lib.ops().qk_norm_rope_fwd(*args)
+    return out[0].to(orig), out[1].to(orig)

@@ -650,3 +650,81 @@ def shared_prefix_attention(
     seen = torch.arange(K.shape[2], device=Q.device) < last.expand(B, N).view(B, 1, N, 1)
     shared = (prefix_K.expand(B, -1, -1, -1), prefix_V.expand(B, -1, -1, -1), None)
     return _attn_parts_pytorch(Q, [shared, (K, V, seen)], scale)
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, device=None) -> torch.Tensor:
+    """The angles per position of `qk_norm_rope`: theta**(-2 j / rot_dim) for
+    j < rot_dim / 2, in float64."""
+    if rot_dim < 0 or rot_dim % 2:
+        raise RuntimeError(f"rope_frequencies: rot_dim {rot_dim} must be even")
+    j = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device)
+    return float(theta) ** (-j / max(rot_dim, 1))
+
+
+def _rope_join(a, b, rest, interleaved):
+    pairs = torch.stack([a, b], -1).flatten(-2) if interleaved else torch.cat([a, b], -1)
+    return torch.cat([pairs, rest], -1)
+
+
+def _norm_rope_pytorch(x, w, cos, sin, rot, eps, interleaved):
+    X, W = _wide(x), _wide(w)
+    n = X * torch.rsqrt((X * X).mean(-1, keepdim=True) + eps) * W
+    if interleaved:
+        a, b = n[..., 0:rot:2], n[..., 1:rot:2]
+    else:
+        a, b = n[..., : rot // 2], n[..., rot // 2 : rot]
+    cos, sin = cos.to(n.dtype), sin.to(n.dtype)
+    return _rope_join(a * cos - b * sin, b * cos + a * sin, n[..., rot:], interleaved).to(x.dtype)
+
+
+def qk_norm_rope(
+    Q: torch.Tensor,
+    K: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head and its rotation by its token's
+    position: what goes into an attention's Q and K, in one pass over both.
+
+    Q (batch, heads, tokens, head_dim) and K (batch, kv_heads, tokens,
+    head_dim), strided views allowed; the results are contiguous, as
+    `block_sparse_attention_tiled` takes them. Every head vector is divided by
+    sqrt(mean square + eps) and multiplied by q_weight / k_weight (head_dim,),
+    in Q's dtype or float32. Its first rot = 2 * len(inv_freq) elements are
+    then rotated in pairs, (j, j + rot / 2) or with `interleaved` (2 j, 2 j +
+    1), by the angle positions * inv_freq[j] formed in float64
+    (`rope_frequencies`); the rest stay. positions (tokens,) or (batch, tokens)
+    are int32 or int64.
+
+    float32, bfloat16 and float16 on the HIP backend, head_dim even and at most
+    256. Differentiable in Q, K and the weights.
+    """
+    who = "qk_norm_rope"
+    if Q.dim() != 4 or K.dim() != 4 or (K.shape[0], K.shape[2], K.shape[3]) != (Q.shape[0], Q.shape[2], Q.shape[3]):
+        raise RuntimeError(f"{who}: Q {tuple(Q.shape)} and K {tuple(K.shape)} must be (batch, heads, tokens, head_dim)")
+    B, _, S, D = Q.shape
+    if Q.dtype != K.dtype or not Q.is_floating_point():
+        raise RuntimeError(f"{who}: Q and K must have one floating dtype, got {Q.dtype} and {K.dtype}")
+    if q_weight.shape != (D,) or k_weight.shape != (D,) or q_weight.dtype != k_weight.dtype:
+        raise RuntimeError(f"{who}: weights must be ({D},) of one dtype")
+    if q_weight.dtype not in (Q.dtype, torch.float32):
+        raise RuntimeError(f"{who}: weights must be {Q.dtype} or torch.float32, got {q_weight.dtype}")
+    if D % 2 or not 2 <= D <= 256:
+        raise RuntimeError(f"{who}: head_dim {D} must be even and at most 256")
+    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or 2 * inv_freq.numel() > D:
+        raise RuntimeError(f"{who}: inv_freq must be up to {D // 2} floating values")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((S,), (B, S)):
+        raise RuntimeError(f"{who}: positions must be ({S},) or ({B}, {S}) of int32 or int64")
+    if not eps >= 0:
+        raise RuntimeError(f"{who}: eps must not be negative")
+    if _use_hip():
+        from .hip.dispatch import hip_qk_norm_rope
+
+        return hip_qk_norm_rope(Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    angle = (positions.to(Q.device).double().unsqueeze(-1) * inv_freq.to(Q.device).double()).expand(B, S, -1).unsqueeze(1)
+    cos, sin, rot = angle.cos(), angle.sin(), 2 * inv_freq.numel()
+    return tuple(_norm_rope_pytorch(x, w, cos, sin, rot, eps, interleaved) for x, w in ((Q, q_weight), (K, k_weight)))
