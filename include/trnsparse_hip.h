@@ -632,7 +632,30 @@ int tsp_cross_attn_fwd(const void* Q, const int64_t* q_strides, const void* K,
                        const int64_t* o_strides, float* lse, void* workspace,
                        int64_t workspace_bytes, void* stream);
 
-/* tsp_prefix_attn_fwd: the same with two sets of keys in one softmax: the
+/* tsp_cross_attn_bwd: from the forward's O and lse and the gradient dO,
+ *   D_i = dO_i . O_i,  P_ij = exp(scale Q_i.K_j - lse_i),
+ *   dS_ij = P_ij (dO_i.V_j - D_i),  dQ_i = scale sum_j dS_ij K_j,
+ *   dK_j = scale sum dS_ij Q_i,  dV_j = sum P_ij dO_i over the queries of the
+ *   key head's group; dK and dV are zero behind key_lengths. Every element is
+ *   written. dK and dV both NULL: only dQ is formed. Strides as above. */
+int64_t tsp_cross_attn_bwd_workspace_size(int dtype, int64_t batch,
+                                          int64_t heads, int64_t kv_heads,
+                                          int64_t queries, int64_t keys,
+                                          int64_t head_dim);
+int tsp_cross_attn_bwd(const void* Q, const int64_t* q_strides, const void* K,
+                       const int64_t* k_strides, const void* V,
+                       const int64_t* v_strides, const void* O,
+                       const int64_t* o_strides, const void* dO,
+                       const int64_t* do_strides, const float* lse, int dtype,
+                       int64_t batch, int64_t heads, int64_t kv_heads,
+                       int64_t queries, int64_t keys, int64_t head_dim,
+                       const void* key_lengths, int index_type, double scale,
+                       void* dQ, const int64_t* dq_strides, void* dK,
+                       const int64_t* dk_strides, void* dV,
+                       const int64_t* dv_strides, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* tsp_prefix_attn_fwd: cross attention with two sets of keys in one softmax: the
  *   prefix (PK, PV (kv_heads, prefix, head_dim); the batch entry of their
  *   strides is ignored), which every batch entry sees whole, and each batch
  *   entry's own K, V (batch, kv_heads, keys, head_dim), of which lengths[b]

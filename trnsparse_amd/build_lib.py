@@ -38,10 +38,10 @@ CFLAGS = [
 ]
 
 
-# Per-source extra flags. attention_bwd.hip: MFMA results in VGPRs (the
+# Per-source extra flags. The attention backwards: MFMA results in VGPRs (the
 # softmax-gradient VALU reads the S / dP tiles straight from the MFMA
 # destination; the default AGPR form costs a register move per element).
-EXTRA = {"attention_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for src in ("attention_bwd.hip", "cross_attention_bwd.hip")}
 
 
 def _sources() -> list[pathlib.Path]:

@@ -1,0 +1,394 @@
+// Cross attention backward for gfx950, from the forward's output O and its
+// rows' log-sum-exps (cross_attention.hip). Per batch entry, query head and its
+// key head, over keys j < key_lengths[b]:
+//   D_i   = sum_d dO_id O_id
+//   P_ij  = exp(scale Q_i . K_j - lse_i),  dS_ij = P_ij (dO_i . V_j - D_i)
+//   dQ_i  = scale sum_j dS_ij K_j
+//   dK_j  = scale sum_{g, i} dS_ij Q_i,  dV_j = sum_{g, i} P_ij dO_i
+// with the sums of dK and dV over the query heads g of the key head's group.
+// No counterpart in the reference, whose attention is one sequence's over
+// itself (trnsparse/ops.py:360-473).
+//
+//   row_pass     128 rows of a unit to a workgroup (rows and units as in
+//                xattn_fwd.h), a wavefront to 32 with their Q and dO in
+//                registers; K and V stages stream through LDS. Leaves each
+//                row's log2(e) lse and D for the column pass.
+//   column_pass  128 keys of a unit to a workgroup, a wavefront to 32 with
+//                their K and V in registers; the Q and dO rows of all heads of
+//                the group stream through LDS with their rows' two numbers.
+// S and dO V^T are formed in both passes (7 products instead of 5) so that
+// neither adds across workgroups: results do not depend on any order of
+// arrival. Where a pass has few workgroups its inner axis is split, each part
+// writes fp32 and sum_parts adds them in order.
+#include "xattn_fwd.h"
+
+namespace tsp {
+namespace xat {
+
+int check_sizes(const char* who, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D);
+
+namespace {
+
+struct BwdArgs {
+  FwdArgs f;           // Q, K, V, lengths and sizes; tiles, nsplit, chunk of the row pass
+  Operand O, dO;
+  Operand dQ, dK, dV;  // written
+  const float* lse;
+  float *stat;         // (2, rows): log2(e) lse, D
+  float *qpart;        // (nsplit, rows, D), null with one range
+  float *kpart;        // (ksplit, 2, batch * kv_heads * keys, D), null with one range
+  int ktiles, ksplit, per;  // column pass: key tiles, ranges of `per` stages
+  float scale;
+};
+
+// (fp32 at 128: Q, dO and dQ alone take 192 registers of a lane)
+template <typename T, int NT>
+__global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const BwdArgs b) {
+  const FwdArgs& a = b.f;
+  constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  int64_t unit, item;
+  if (!head_item(blockIdx.x, (int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+  const int tile = (int)(item % a.tiles), split = (int)(item / a.tiles);
+  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
+  const int r = tile * 128 + w * 32 + l32;
+  const bool live = r < a.R;
+  const RowId id = row_id(a, ub, hk, live ? r : 0);
+  auto row_of = [&](const Operand& x) { return x.p + id.b * x.b + id.head * x.h + id.i * x.s; };
+
+  const int64_t n = unit_length(a, ub);
+  const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
+  const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, HK) : 0;
+  const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
+  const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
+  Stager<T, HK, 4> ks, vs;
+  ks.init(w, lane, a.K.s, a.D);
+  vs.init(w, lane, a.V.s, a.D);
+  const typename T::Lane ln = T::lane_of(lane);
+  const uint32_t lds0 = dma::lds_addr(lds);
+  auto issue = [&](int s) {
+    const uint32_t st = lds0 + (s & 1) * STAGE;
+    ks.issue(Kp, k0 + (int64_t)s * HK, k1, a.K.s, a.D, st, w);
+    vs.issue(Vp, k0 + (int64_t)s * HK, k1, a.V.s, a.D, st + HBYTES, w);
+  };
+  if (nst > 0) issue(0);
+  typename T::Rows q, g;
+  T::load(q, row_of(a.Q), live, a.D, h);
+  T::load(g, row_of(b.dO), live, a.D, h);
+  float Dr, rq;
+  {
+    typename T::Rows o;
+    T::load(o, row_of(b.O), live, a.D, h);
+    Dr = halves_sum(T::dot(g, o));
+    rq = live ? b.lse[id.orow] * LOG2E : 0.f;
+    if (live && split == 0 && h == 0) {
+      b.stat[id.orow] = rq;
+      b.stat[a.prows + id.orow] = Dr;
+    }
+  }
+  f32x16 acc[T::NU];
+#pragma unroll
+  for (int u = 0; u < T::NU; ++u) acc[u] = f32x16{};
+  for (int s = 0; s < nst; ++s) {
+    dma::wait_vm<0>();
+    dma::barrier();
+    if (s + 1 < nst) issue(s + 1);
+    const int keys = (int)(k1 - k0 - (int64_t)s * HK < HK ? k1 - k0 - (int64_t)s * HK : HK);
+    const uint32_t st = lds0 + (s & 1) * STAGE;
+    f32x16 sc[NT], dp[NT];
+    T::template scores<NT>(sc, st, ln, q);
+    T::template scores<NT>(dp, st + HBYTES, ln, g);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        sc[t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v], a.scale_log2, -rq)) * (dp[t][v] - Dr);
+    if (keys < HK) {  // staged rows past the last key are zero, but their P is not
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (32 * t + 8 * (v >> 2) + 4 * h + (v & 3) >= keys) sc[t][v] = 0.f;
+    }
+    typename T::template Prob<NT> p;
+    T::template pack<NT>(p, sc);
+    T::template outer<NT>(acc, st, ln, p);
+  }
+  if (!live) return;
+  char* out = (char*)row_of(b.dQ);
+  float* part = b.qpart ? b.qpart + ((int64_t)split * a.prows + id.orow) * a.D : nullptr;
+  T::quads(acc, h, [&](int d, f32x4 v) {
+    if (d >= a.D) return;
+    if (part)
+      *(f32x4*)(part + d) = v * b.scale;
+    else
+      T::store4(out + d * T::ESZ, v * b.scale);
+  });
+}
+
+template <typename T, int NQ>
+__global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const BwdArgs b) {
+  const FwdArgs& a = b.f;
+  constexpr int HQ = 32 * NQ, HBYTES = HQ * T::ROWB, STAGE = 2 * HBYTES + 1024;  // Q, dO, two numbers of each row
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  int64_t unit, item;
+  if (!head_item(blockIdx.x, (int64_t)b.ktiles * b.ksplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+  const int tile = (int)(item % b.ktiles), split = (int)(item / b.ktiles);
+  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
+  const int64_t n = unit_length(a, ub);
+  const int64_t key = (int64_t)tile * 128 + w * 32 + l32;
+
+  const int spg = (int)ceil_div(a.Sq, HQ), total = a.G * spg;  // stages of a head, of the group
+  const int s0 = split * b.per, s1 = s0 + b.per < total ? s0 + b.per : total;
+  const int nst = (int64_t)tile * 128 < n && s1 > s0 ? s1 - s0 : 0;
+  Stager<T, HQ, 4> qs, gs;
+  qs.init(w, lane, a.Q.s, a.D);
+  gs.init(w, lane, b.dO.s, a.D);
+  const typename T::Lane ln = T::lane_of(lane);
+  const uint32_t lds0 = dma::lds_addr(lds);
+  auto issue = [&](int s) {
+    const int g = (s0 + s) / spg, i0 = ((s0 + s) - g * spg) * HQ;
+    const int64_t head = hk * a.G + g;
+    const uint32_t st = lds0 + (s & 1) * STAGE;
+    qs.issue(a.Q.p + ub * a.Q.b + head * a.Q.h, i0, a.Sq, a.Q.s, a.D, st, w);
+    gs.issue(b.dO.p + ub * b.dO.b + head * b.dO.h, i0, a.Sq, b.dO.s, a.D, st + HBYTES, w);
+    if (w < 2) {  // rows past the last one: both numbers zero, so P = 1 meets dO = 0 and dS = 0
+      const float* x = b.stat + w * a.prows + (ub * a.Hkv * a.G + head) * a.Sq + i0;
+      const int left = a.Sq - i0;
+      dma::buffer4(dma::make_rsrc(x, 4u * (left < HQ ? left : HQ)), 4u * lane, st + 2 * HBYTES + w * 256);
+    }
+  };
+  if (nst > 0) issue(0);
+  typename T::Rows k, v;
+  T::load(k, a.K.p + ub * a.K.b + hk * a.K.h + key * a.K.s, key < n, a.D, h);
+  T::load(v, a.V.p + ub * a.V.b + hk * a.V.h + key * a.V.s, key < n, a.D, h);
+  f32x16 dk[T::NU], dv[T::NU];
+#pragma unroll
+  for (int u = 0; u < T::NU; ++u) dk[u] = dv[u] = f32x16{};
+  for (int s = 0; s < nst; ++s) {
+    dma::wait_vm<0>();
+    dma::barrier();
+    if (s + 1 < nst) issue(s + 1);
+    const uint32_t st = lds0 + (s & 1) * STAGE;
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      const uint32_t at = st + 32 * t * T::ROWB;
+      f32x16 sc[1], dp[1];
+      T::template scores<1>(sc, at, ln, k);
+      T::template scores<1>(dp, at + HBYTES, ln, v);
+      typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t x = st + 2 * HBYTES + 4 * (32 * t + 8 * c + 4 * h);
+        const f32x4 rq = *(const lds_f32x4*)(uintptr_t)x, Dr = *(const lds_f32x4*)(uintptr_t)(x + 256);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][4 * c + e], a.scale_log2, -rq[e]));
+          sc[0][4 * c + e] = p;
+          dp[0][4 * c + e] = p * (dp[0][4 * c + e] - Dr[e]);
+        }
+      }
+      typename T::template Prob<1> P, dS;
+      T::template pack<1>(P, sc);
+      T::template pack<1>(dS, dp);
+      T::template outer<1>(dv, at + HBYTES, ln, P);
+      T::template outer<1>(dk, at, ln, dS);
+    }
+  }
+  if (key >= a.L) return;
+  const bool in = key < n;
+  char* ok = (char*)b.dK.p + ub * b.dK.b + hk * b.dK.h + key * b.dK.s;
+  char* ov = (char*)b.dV.p + ub * b.dV.b + hk * b.dV.h + key * b.dV.s;
+  const int64_t krows = (int64_t)a.units_b * a.Hkv * a.L, row = unit * a.L + key;
+  float* pk = b.kpart ? b.kpart + ((int64_t)split * 2 * krows + row) * a.D : nullptr;
+  auto put = [&](const f32x16* acc, char* o, float* p, float f) {
+    T::quads(acc, h, [&](int d, f32x4 x) {
+      if (d >= a.D) return;
+      const f32x4 y = in ? x * f : f32x4{};
+      if (p)
+        *(f32x4*)(p + d) = y;
+      else
+        T::store4(o + d * T::ESZ, y);
+    });
+  };
+  put(dk, ok, pk, b.scale);
+  put(dv, ov, pk ? pk + krows * a.D : nullptr, 1.f);
+}
+
+// Sums of the parts of `rows` rows in order, rounded once: 32 lanes to a row.
+struct SumArgs {
+  const float* part;
+  int64_t rows, stride;  // floats between parts
+  int nsplit, D, heads;
+  int64_t S;
+  Operand out;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void sum_parts(const SumArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int d = 4 * (threadIdx.x & 31);
+  if (row >= a.rows || d >= a.D) return;
+  f32x4 sum = f32x4{};
+  for (int j = 0; j < a.nsplit; ++j) sum += *(const f32x4*)(a.part + j * a.stride + row * a.D + d);
+  const int64_t i = row % a.S, bh = row / a.S;
+  T::store4((char*)a.out.p + bh / a.heads * a.out.b + bh % a.heads * a.out.h + i * a.out.s + d * T::ESZ, sum);
+}
+
+struct BwdPlan {
+  int tiles, nsplit, ktiles, ksplit, per;
+  int64_t chunk;
+  int64_t stat, qpart, kpart;  // bytes
+};
+BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D) {
+  BwdPlan p{};
+  const int64_t G = Hq / Hkv, units = B * Hkv, stage = dtype == TSP_F32 ? 32 : 64, want = 512;
+  p.tiles = (int)ceil_div(G * Sq, 128);
+  int64_t n = units * p.tiles >= want / 2 ? 1 : ceil_div(want, units * p.tiles);
+  const int64_t kst = ceil_div(L > 0 ? L : 1, stage);  // stages of keys
+  if (n > kst / 2) n = kst / 2 > 1 ? kst / 2 : 1;
+  p.chunk = ceil_div(kst, n) * stage;
+  p.nsplit = (int)ceil_div(L > 0 ? L : 1, p.chunk);
+  p.ktiles = (int)ceil_div(L, 128);
+  const int64_t total = G * ceil_div(Sq, stage), wgs = units * p.ktiles;
+  n = wgs == 0 || wgs >= want / 2 ? 1 : ceil_div(want, wgs);
+  if (n > total / 2) n = total / 2 > 1 ? total / 2 : 1;
+  p.per = (int)ceil_div(total, n);
+  p.ksplit = (int)ceil_div(total, p.per > 0 ? p.per : 1);
+  if (p.ksplit < 1) p.ksplit = 1;
+  const int64_t rows = B * Hq * Sq, up = 255;
+  p.stat = (2 * rows * 4 + up) & ~up;
+  p.qpart = p.nsplit > 1 ? (p.nsplit * rows * D * 4 + up) & ~up : 0;
+  p.kpart = p.ksplit > 1 ? p.ksplit * 2 * units * L * D * 4 : 0;
+  return p;
+}
+
+template <typename T>
+int run_t(const BwdPlan& p, const BwdArgs& b, hipStream_t st) {
+  const FwdArgs& a = b.f;
+  const int64_t units = (int64_t)a.units_b * a.Hkv;
+  constexpr int N = T::ESZ == 2 ? 2 : 1;
+  const int64_t g1 = head_grid((int64_t)p.tiles * p.nsplit, units), g2 = b.dK.p ? head_grid((int64_t)p.ktiles * p.ksplit, units) : 0;
+  if (g1 > INT32_MAX || g2 > INT32_MAX) return fail(TSP_EUNSUPPORTED, "tsp_cross_attn_bwd: too large a grid");
+  int rc;
+  hipLaunchKernelGGL((row_pass<T, N>), dim3((unsigned)g1), dim3(256), 0, st, b);
+  if ((rc = check_launch("row_pass launch"))) return rc;
+  if (g2 > 0) {
+    hipLaunchKernelGGL((column_pass<T, N>), dim3((unsigned)g2), dim3(256), 0, st, b);
+    if ((rc = check_launch("column_pass launch"))) return rc;
+  }
+  auto sum = [&](const float* part, int64_t rows, int64_t stride, int n, int heads, int64_t S, const Operand& out) {
+    const SumArgs s{part, rows, stride, n, a.D, heads, S, out};
+    hipLaunchKernelGGL((sum_parts<T>), dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, s);
+    return check_launch("sum_parts launch");
+  };
+  const int64_t krows = units * a.L;
+  if (p.nsplit > 1 && (rc = sum(b.qpart, a.prows, a.prows * a.D, p.nsplit, a.Hkv * a.G, a.Sq, b.dQ))) return rc;
+  if (p.ksplit > 1 && g2 > 0) {
+    if ((rc = sum(b.kpart, krows, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dK))) return rc;
+    if ((rc = sum(b.kpart + krows * a.D, krows, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dV))) return rc;
+  }
+  return TSP_OK;
+}
+
+// zeros in a strided result
+struct ZeroArgs {
+  Operand out;
+  int64_t rows, S;
+  int heads, bytes;  // of a row
+};
+__global__ __launch_bounds__(256) void zero_rows(const ZeroArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const int64_t i = row % a.S, bh = row / a.S;
+  char* p = (char*)a.out.p + bh / a.heads * a.out.b + bh % a.heads * a.out.h + i * a.out.s;
+  for (int d = 16 * (threadIdx.x & 31); d < a.bytes; d += 512) *(u32x4*)(p + d) = u32x4{};
+}
+
+}  // namespace
+}  // namespace xat
+}  // namespace tsp
+
+using namespace tsp;
+
+extern "C" int64_t tsp_cross_attn_bwd_workspace_size(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq,
+                                                     int64_t L, int64_t D) {
+  if (xat::check_sizes("tsp_cross_attn_bwd_workspace_size", dtype, B, Hq, Hkv, Sq, L, D)) return -1;
+  if (B * Hq * Sq == 0) return 0;
+  const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D);
+  return p.stat + p.qpart + p.kpart;
+}
+
+extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* K, const int64_t* ks, const void* V,
+                                  const int64_t* vs, const void* O, const int64_t* os, const void* dO,
+                                  const int64_t* gs, const float* lse, int dtype, int64_t B, int64_t Hq, int64_t Hkv,
+                                  int64_t Sq, int64_t L, int64_t D, const void* key_lengths, int index_type,
+                                  double scale, void* dQ, const int64_t* dqs, void* dK, const int64_t* dks, void* dV,
+                                  const int64_t* dvs, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "tsp_cross_attn_bwd";
+  const hipStream_t st = (hipStream_t)stream;
+  int rc = xat::check_sizes(who, dtype, B, Hq, Hkv, Sq, L, D);
+  if (rc) return rc;
+  if (!(scale > 0) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
+  if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
+  const bool rows = B * Hq * Sq > 0, keys = B * L > 0, cols = keys && (dK || dV);
+  if (cols)
+    if ((rc = xat::check_operand(who, "dK", dK, dks, L, D, dtype)) ||
+        (rc = xat::check_operand(who, "dV", dV, dvs, L, D, dtype)))
+      return rc;
+  if (!rows) {  // no query: the keys' gradients are zero
+    if (!cols) return TSP_OK;
+    const int64_t n = B * Hkv * L;
+    for (const xat::Operand& o : {xat::operand(dK, dks, dtype), xat::operand(dV, dvs, dtype)}) {
+      const xat::ZeroArgs z{o, n, L, (int)Hkv, (int)(D * xat::esize(dtype))};
+      if (ceil_div(n, 8) > INT32_MAX) return fail(TSP_EUNSUPPORTED, "%s: too many rows", who);
+      hipLaunchKernelGGL(xat::zero_rows, dim3((unsigned)ceil_div(n, 8)), dim3(256), 0, st, z);
+      if ((rc = check_launch("zero_rows launch"))) return rc;
+    }
+    return TSP_OK;
+  }
+  if ((rc = xat::check_operand(who, "Q", Q, qs, Sq, D, dtype)) || (rc = xat::check_operand(who, "O", O, os, Sq, D, dtype)) ||
+      (rc = xat::check_operand(who, "dO", dO, gs, Sq, D, dtype)) ||
+      (rc = xat::check_operand(who, "dQ", dQ, dqs, Sq, D, dtype)))
+    return rc;
+  if (keys)
+    if ((rc = xat::check_operand(who, "K", K, ks, L, D, dtype)) || (rc = xat::check_operand(who, "V", V, vs, L, D, dtype)))
+      return rc;
+  if (!lse) return fail(TSP_EINVAL, "%s: null lse", who);
+  const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D);
+  if (!workspace || workspace_bytes < p.stat + p.qpart + p.kpart)
+    return fail(TSP_EINVAL, "%s: workspace too small", who);
+  if (ceil_div(B * Hq * Sq, 8) > INT32_MAX || ceil_div(B * Hkv * L, 8) > INT32_MAX)
+    return fail(TSP_EUNSUPPORTED, "%s: too many rows", who);
+  const int64_t none[3] = {0, 0, 0};
+  xat::BwdArgs b{};
+  xat::FwdArgs& a = b.f;
+  a.Q = xat::operand(Q, qs, dtype);
+  a.K = xat::operand(K, keys ? ks : none, dtype);
+  a.V = xat::operand(V, keys ? vs : none, dtype);
+  b.O = xat::operand(O, os, dtype);
+  b.dO = xat::operand(dO, gs, dtype);
+  b.dQ = xat::operand(dQ, dqs, dtype);
+  b.dK = xat::operand(dK, cols ? dks : none, dtype);
+  b.dV = xat::operand(dV, cols ? dvs : none, dtype);
+  b.lse = lse;
+  b.stat = (float*)workspace;
+  if (p.qpart) b.qpart = (float*)((char*)workspace + p.stat);
+  if (p.kpart) b.kpart = (float*)((char*)workspace + p.stat + p.qpart);
+  b.ktiles = p.ktiles, b.ksplit = p.ksplit, b.per = p.per;
+  b.scale = (float)scale;
+  a.prows = B * Hq * Sq;
+  a.lengths = key_lengths;
+  a.len64 = index_type == TSP_I64;
+  a.units_b = (int)B;
+  a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
+  a.L = L;
+  a.tiles = p.tiles, a.nsplit = p.nsplit, a.chunk = p.chunk;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  const bool w = D > 64;
+  using namespace xat;
+  if (dtype == TSP_BF16) return w ? run_t<Tile16<__bf16, 128>>(p, b, st) : run_t<Tile16<__bf16, 64>>(p, b, st);
+  if (dtype == TSP_F16) return w ? run_t<Tile16<_Float16, 128>>(p, b, st) : run_t<Tile16<_Float16, 64>>(p, b, st);
+  return w ? run_t<Tile32<128>>(p, b, st) : run_t<Tile32<64>>(p, b, st);
+}

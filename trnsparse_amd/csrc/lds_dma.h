@@ -55,6 +55,13 @@ __device__ inline void buffer16(i32x4 rsrc, uint32_t voff, uint32_t lds) {
                : "memory", "m0");
 }
 
+// 4 bytes per lane at byte offset voff of the buffer: lane l writes M0 + 4 l (256 bytes per wave instruction).
+__device__ inline void buffer4(i32x4 rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc),
+               "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory", "m0");
+}
+
 // Low 32 bits of *p, waited for in place (all earlier loads included): the
 // compiler does not see this load either, so it never adds a wait for it on
 // the streaming path.

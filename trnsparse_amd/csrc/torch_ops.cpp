@@ -597,6 +597,53 @@ std::tuple<at::Tensor, at::Tensor> cross_attn_fwd_meta(const at::Tensor& Q, cons
   return {Q.size(3) == piece_dim(Q) ? attn_like(Q, Q.size(3)) : at::empty(Q.sizes(), Q.options()), lse};
 }
 
+// dK and dV come back empty when they are not asked for
+std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(const at::Tensor& Q_, const at::Tensor& K_,
+                                                              const at::Tensor& V_, const at::Tensor& O_,
+                                                              const at::Tensor& dO_, const at::Tensor& lse,
+                                                              const c10::optional<at::Tensor>& key_lengths, double scale,
+                                                              bool need_kv) {
+  const char* who = "cross_attn_bwd";
+  cross_shapes(Q_, K_, V_, who);
+  need_4d(O_, Q_, who, "O");
+  need_4d(dO_, Q_, who, "grad_out");
+  TORCH_CHECK(O_.sizes() == Q_.sizes() && dO_.sizes() == Q_.sizes(), who, ": O and grad_out must have Q's shape");
+  const int code = attn_dtype(Q_.scalar_type(), who);
+  const auto Q = attn_operand(Q_), K = attn_operand(K_), V = attn_operand(V_), O = attn_operand(O_),
+             dO = attn_operand(dO_);
+  const int64_t B = Q.size(0), Hq = Q.size(1), Sq = Q.size(2), D = Q.size(3), Hk = K.size(1), L = K.size(2);
+  need(lse, Q, "lse");
+  need_dtype(lse, at::kFloat, who, "lse");
+  need_numel(lse, B * Hq * Sq, who, "lse");
+  int icode;
+  const void* lens = lengths_ptr(key_lengths, B, Q, who, icode);
+  auto dQ = attn_like(Q_, D);
+  auto dK = need_kv ? attn_like(K_, D) : at::empty({0, 0, 0, D}, K.options());
+  auto dV = need_kv ? attn_like(V_, D) : at::empty({0, 0, 0, D}, V.options());
+  const int64_t wsb = tsp_cross_attn_bwd_workspace_size(code, B, Hq, Hk, Sq, L, D);
+  auto ws = workspace_of(wsb, Q, who);
+  check(tsp_cross_attn_bwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s,
+                           O.data_ptr(), Strides(O).s, dO.data_ptr(), Strides(dO).s, lse.data_ptr<float>(), code, B, Hq,
+                           Hk, Sq, L, D, lens, icode, scale, dQ.data_ptr(), Strides(dQ).s,
+                           need_kv ? dK.data_ptr() : nullptr, Strides(dK).s, need_kv ? dV.data_ptr() : nullptr,
+                           Strides(dV).s, ws.data_ptr(), wsb, stream_of(Q)),
+        "tsp_cross_attn_bwd");
+  const int64_t d = Q_.size(3);
+  return {attn_trim(dQ, d), attn_trim(dK, d), attn_trim(dV, d)};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd_meta(const at::Tensor& Q, const at::Tensor& K,
+                                                                   const at::Tensor& V, const at::Tensor&,
+                                                                   const at::Tensor&, const at::Tensor&,
+                                                                   const c10::optional<at::Tensor>&, double,
+                                                                   bool need_kv) {
+  auto like = [&](const at::Tensor& t, bool need) {
+    if (!need) return at::empty({0, 0, 0, t.size(3)}, t.options());
+    return t.size(3) == piece_dim(t) ? attn_like(t, t.size(3)) : at::empty(t.sizes(), t.options());
+  };
+  return {like(Q, true), like(K, need_kv), like(V, need_kv)};
+}
+
 at::Tensor prefix_attn_fwd(const at::Tensor& Q_, const at::Tensor& PK_, const at::Tensor& PV_, const at::Tensor& K_,
                            const at::Tensor& V_, const c10::optional<at::Tensor>& lengths, double scale) {
   const char* who = "prefix_attn_fwd";
@@ -746,6 +793,8 @@ TORCH_LIBRARY(trnsparse_hip, m) {
         "Tensor row_denom, Tensor plan, int n_items, int n_splits, int n_partials) -> (Tensor, Tensor, Tensor)");
   m.def("cross_attn_fwd(Tensor Q, Tensor K, Tensor V, Tensor? key_lengths, float scale, bool return_lse) -> "
         "(Tensor, Tensor)");
+  m.def("cross_attn_bwd(Tensor Q, Tensor K, Tensor V, Tensor O, Tensor grad_out, Tensor lse, Tensor? key_lengths, "
+        "float scale, bool need_kv) -> (Tensor, Tensor, Tensor)");
   m.def("prefix_attn_fwd(Tensor Q, Tensor prefix_K, Tensor prefix_V, Tensor K, Tensor V, Tensor? lengths, "
         "float scale) -> Tensor");
   m.def("qk_norm_rope_fwd(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
@@ -769,6 +818,7 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
   m.impl("bsa_fwd", &bsa_fwd);
   m.impl("bsa_bwd", &bsa_bwd);
   m.impl("cross_attn_fwd", &cross_attn_fwd);
+  m.impl("cross_attn_bwd", &cross_attn_bwd);
   m.impl("prefix_attn_fwd", &prefix_attn_fwd);
   m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
@@ -787,6 +837,7 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
   m.impl("bsa_fwd", &bsa_fwd_meta);
   m.impl("bsa_bwd", &bsa_bwd_meta);
   m.impl("cross_attn_fwd", &cross_attn_fwd_meta);
+  m.impl("cross_attn_bwd", &cross_attn_bwd_meta);
   m.impl("prefix_attn_fwd", &prefix_attn_fwd_meta);
   m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd_meta);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_meta);

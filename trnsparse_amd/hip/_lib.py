@@ -101,6 +101,9 @@ SIGNATURES: dict[str, tuple] = {
     "tsp_cross_attn_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64, _I64]),
     "tsp_cross_attn_fwd": (_INT, [_P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _INT, _DBL, _P,
                                   _P, _P, _P, _I64, _P]),
+    "tsp_cross_attn_bwd_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "tsp_cross_attn_bwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64,
+                                  _P, _INT, _DBL, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "tsp_prefix_attn_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "tsp_prefix_attn_fwd": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64,
                                    _I64, _P, _INT, _DBL, _P, _P, _P, _I64, _P]),

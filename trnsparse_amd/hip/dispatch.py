@@ -934,6 +934,27 @@ def _lengths_on(t, dev: torch.device):
     return None if t is None else t.to(dev).contiguous()
 
 
+class _CrossAttentionFunction(torch.autograd.Function):
+    """Autograd wrapper of cross attention: keeps Q, K, V, the result and its
+    rows' log-sum-exps."""
+
+    @staticmethod
+    def forward(ctx, Q, K, V, key_lengths, scale):
+        out, lse = _lib.ops().cross_attn_fwd(Q, K, V, key_lengths, scale, True)
+        ctx.save_for_backward(Q, K, V, out, lse, key_lengths)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dO):
+        Q, K, V, O, lse, key_lengths = ctx.saved_tensors
+        need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        with torch.cuda.device(Q.device):
+            dQ, dK, dV = _lib.ops().cross_attn_bwd(Q, K, V, O, dO, lse, key_lengths, ctx.scale, need_kv)
+        return dQ, (dK if need_kv else None), (dV if need_kv else None), None, None
+
+
 @_library_call
 def hip_cross_attention(Q, K, V, key_lengths, scale: float):
     """cross_attention on the HIP kernels (operands on the host are copied
@@ -943,6 +964,8 @@ def hip_cross_attention(Q, K, V, key_lengths, scale: float):
     with torch.cuda.device(dev):
         Q, K, V = (t.to(dev) for t in (Q, K, V))
         lens = _lengths_on(key_lengths, dev)
+        if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
+            return _CrossAttentionFunction.apply(Q, K, V, lens, float(scale)).to(orig)
         return _lib.ops().cross_attn_fwd(Q, K, V, lens, float(scale), False)[0].to(orig)
 
 
