@@ -15,7 +15,9 @@
 // keeps the planning and caching (row orders, CSR windows and column plans,
 // the attention backward's column plan) and the autograd wrappers.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -555,10 +557,14 @@ const void* lengths_ptr(const c10::optional<at::Tensor>& t, int64_t B, const at:
   return t->data_ptr();
 }
 
-at::Tensor workspace_of(int64_t bytes, const at::Tensor& like, const char* who) {
-  TORCH_CHECK(bytes >= 0, who, " failed: ", tsp_last_error());
-  return at::empty({bytes > 0 ? bytes : 16}, like.options().dtype(at::kByte));
-}
+struct Workspace {
+  at::Tensor t;  // none when no byte is needed
+  Workspace(int64_t bytes, const at::Tensor& like, const char* who) {
+    TORCH_CHECK(bytes >= 0, who, " failed: ", tsp_last_error());
+    if (bytes > 0) t = at::empty({bytes}, like.options().dtype(at::kByte));
+  }
+  void* ptr() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
 
 void cross_shapes(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V, const char* who) {
   need_4d(Q, Q, who, "Q");
@@ -569,10 +575,11 @@ void cross_shapes(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
               K.size(1), " key heads");
 }
 
-std::tuple<at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& Q_, const at::Tensor& K_, const at::Tensor& V_,
-                                                  const c10::optional<at::Tensor>& key_lengths, double scale,
-                                                  bool return_lse) {
+// the result, and with `lse` its rows' log-sum-exps
+at::Tensor cross_forward(const at::Tensor& Q_, const at::Tensor& K_, const at::Tensor& V_,
+                         const c10::optional<at::Tensor>& key_lengths, double scale, at::Tensor* lse) {
   const char* who = "cross_attn_fwd";
+  const c10::DeviceGuard guard(Q_.device());
   cross_shapes(Q_, K_, V_, who);
   const int code = attn_dtype(Q_.scalar_type(), who);
   const auto Q = attn_operand(Q_), K = attn_operand(K_), V = attn_operand(V_);
@@ -580,14 +587,23 @@ std::tuple<at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& Q_, const at
   int icode;
   const void* lens = lengths_ptr(key_lengths, B, Q, who, icode);
   auto O = attn_like(Q_, D);
-  auto lse = at::empty(return_lse ? at::IntArrayRef({B, Hq, Sq}) : at::IntArrayRef({0}), Q.options().dtype(at::kFloat));
+  if (lse) *lse = at::empty({B, Hq, Sq}, Q.options().dtype(at::kFloat));
   const int64_t wsb = tsp_cross_attn_workspace_size(code, B, Hq, Hk, Sq, L, D);
-  auto ws = workspace_of(wsb, Q, who);
+  const Workspace ws(wsb, Q, who);
   check(tsp_cross_attn_fwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, code, B,
                            Hq, Hk, Sq, L, D, lens, icode, scale, O.data_ptr(), Strides(O).s,
-                           return_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), wsb, stream_of(Q)),
+                           lse ? lse->data_ptr<float>() : nullptr, ws.ptr(), wsb, stream_of(Q)),
         "tsp_cross_attn_fwd");
-  return {attn_trim(O, Q_.size(3)), lse};
+  return attn_trim(O, Q_.size(3));
+}
+
+std::tuple<at::Tensor, at::Tensor> cross_attn_fwd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
+                                                  const c10::optional<at::Tensor>& key_lengths, double scale,
+                                                  bool return_lse) {
+  at::Tensor lse;
+  auto O = cross_forward(Q, K, V, key_lengths, scale, return_lse ? &lse : nullptr);
+  if (!return_lse) lse = at::empty({0}, Q.options().dtype(at::kFloat));
+  return {O, lse};
 }
 
 std::tuple<at::Tensor, at::Tensor> cross_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&,
@@ -604,6 +620,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(const at::Tensor& 
                                                               const c10::optional<at::Tensor>& key_lengths, double scale,
                                                               bool need_kv) {
   const char* who = "cross_attn_bwd";
+  const c10::DeviceGuard guard(Q_.device());
   cross_shapes(Q_, K_, V_, who);
   need_4d(O_, Q_, who, "O");
   need_4d(dO_, Q_, who, "grad_out");
@@ -621,12 +638,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd(const at::Tensor& 
   auto dK = need_kv ? attn_like(K_, D) : at::empty({0, 0, 0, D}, K.options());
   auto dV = need_kv ? attn_like(V_, D) : at::empty({0, 0, 0, D}, V.options());
   const int64_t wsb = tsp_cross_attn_bwd_workspace_size(code, B, Hq, Hk, Sq, L, D);
-  auto ws = workspace_of(wsb, Q, who);
+  const Workspace ws(wsb, Q, who);
   check(tsp_cross_attn_bwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s,
                            O.data_ptr(), Strides(O).s, dO.data_ptr(), Strides(dO).s, lse.data_ptr<float>(), code, B, Hq,
                            Hk, Sq, L, D, lens, icode, scale, dQ.data_ptr(), Strides(dQ).s,
                            need_kv ? dK.data_ptr() : nullptr, Strides(dK).s, need_kv ? dV.data_ptr() : nullptr,
-                           Strides(dV).s, ws.data_ptr(), wsb, stream_of(Q)),
+                           Strides(dV).s, ws.ptr(), wsb, stream_of(Q)),
         "tsp_cross_attn_bwd");
   const int64_t d = Q_.size(3);
   return {attn_trim(dQ, d), attn_trim(dK, d), attn_trim(dV, d)};
@@ -647,6 +664,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cross_attn_bwd_meta(const at::Ten
 at::Tensor prefix_attn_fwd(const at::Tensor& Q_, const at::Tensor& PK_, const at::Tensor& PV_, const at::Tensor& K_,
                            const at::Tensor& V_, const c10::optional<at::Tensor>& lengths, double scale) {
   const char* who = "prefix_attn_fwd";
+  const c10::DeviceGuard guard(Q_.device());
   cross_shapes(Q_, K_, V_, who);
   TORCH_CHECK(PK_.dim() == 3 && PK_.sizes() == PV_.sizes() && PK_.size(0) == K_.size(1), who,
               ": the prefix must be (kv_heads, prefix, head_dim) like K's heads");
@@ -662,10 +680,10 @@ at::Tensor prefix_attn_fwd(const at::Tensor& Q_, const at::Tensor& PK_, const at
   const void* lens = lengths_ptr(lengths, B, Q, who, icode);
   auto O = attn_like(Q_, D);
   const int64_t wsb = tsp_prefix_attn_workspace_size(code, B, Hq, Hk, Sq, P, S, D);
-  auto ws = workspace_of(wsb, Q, who);
+  const Workspace ws(wsb, Q, who);
   check(tsp_prefix_attn_fwd(Q.data_ptr(), Strides(Q).s, PK.data_ptr(), Strides(PK).s, PV.data_ptr(), Strides(PV).s,
                             K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, code, B, Hq, Hk, Sq, P, S, D, lens,
-                            icode, scale, O.data_ptr(), Strides(O).s, ws.data_ptr(), wsb, stream_of(Q)),
+                            icode, scale, O.data_ptr(), Strides(O).s, ws.ptr(), wsb, stream_of(Q)),
         "tsp_prefix_attn_fwd");
   return attn_trim(O, Q_.size(3));
 }
@@ -716,6 +734,7 @@ struct RopeArgs {
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& Q_, const at::Tensor& K_, const at::Tensor& wq,
                                                     const at::Tensor& wk, const at::Tensor& pos, const at::Tensor& freq,
                                                     double eps, bool interleaved) {
+  const c10::DeviceGuard guard(Q_.device());
   const RopeArgs r(Q_, K_, wq, wk, pos, freq, "qk_norm_rope_fwd");
   const auto Q = unit_rows(Q_), K = unit_rows(K_);
   auto Qo = at::empty(Q.sizes(), Q.options()), Ko = at::empty(K.sizes(), K.options());
@@ -739,6 +758,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
     const at::Tensor& freq, double eps, bool interleaved, const at::Tensor& gQ_, const at::Tensor& gK_,
     bool need_weights) {
   const char* who = "qk_norm_rope_bwd";
+  const c10::DeviceGuard guard(Q_.device());
   const RopeArgs r(Q_, K_, wq, wk, pos, freq, who);
   need_4d(gQ_, Q_, who, "grad_Q");
   need_4d(gK_, Q_, who, "grad_K");
@@ -748,13 +768,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
   auto dwq = need_weights ? at::empty_like(wq) : at::empty({0}, wq.options());
   auto dwk = need_weights ? at::empty_like(wk) : at::empty({0}, wk.options());
   const int64_t wsb = tsp_qk_norm_rope_bwd_workspace_size(Q.size(0), Q.size(2), Q.size(3));
-  auto ws = workspace_of(need_weights ? std::max<int64_t>(wsb, 0) : 0, Q, who);
+  const Workspace ws(need_weights ? wsb : 0, Q, who);
   check(tsp_qk_norm_rope_bwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), Strides(K).s, r.code, Q.size(0), Q.size(1),
                              K.size(1), Q.size(2), Q.size(3), wq.data_ptr(), wk.data_ptr(), r.wcode, pos.data_ptr(),
                              r.icode, r.pos_b, r.pos_s, freq.data_ptr<double>(), r.rot, interleaved, eps, gQ.data_ptr(),
                              Strides(gQ).s, gK.data_ptr(), Strides(gK).s, dQ.data_ptr(), Strides(dQ).s, dK.data_ptr(),
                              Strides(dK).s, need_weights ? dwq.data_ptr() : nullptr,
-                             need_weights ? dwk.data_ptr() : nullptr, ws.data_ptr(), wsb, stream_of(Q)),
+                             need_weights ? dwk.data_ptr() : nullptr, ws.ptr(), wsb, stream_of(Q)),
         "tsp_qk_norm_rope_bwd");
   return {dQ, dK, dwq, dwk};
 }
@@ -764,6 +784,110 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd_meta
     const at::Tensor&, double, bool, const at::Tensor&, const at::Tensor&, bool need_weights) {
   return {attn_like(Q, Q.size(3)), attn_like(K, K.size(3)), need_weights ? at::empty_like(wq) : at::empty({0}, wq.options()),
           need_weights ? at::empty_like(wk) : at::empty({0}, wk.options())};
+}
+
+// ----------------------------------------------- operators with gradients
+//
+// cross_attention and qk_norm_rope carry their gradients themselves, in C++: a
+// small training step is bound by the host (forward and backward of 333 tokens
+// took 140 us through a Python autograd function, 27 of them kernels).
+
+namespace ag = torch::autograd;
+
+// The registered operator `name`, of f's type: below autograd the calls go
+// through the dispatcher, so that tracing reaches the Meta implementations.
+template <typename F>
+auto op_of(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  return std::any_of(ts.begin(), ts.end(), [](const at::Tensor* t) { return t->requires_grad(); });
+}
+
+void first_order(const char* who) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), who, " has no second derivatives: backward with create_graph=False");
+}
+
+at::Tensor cross_attention(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
+                           const c10::optional<at::Tensor>& key_lengths, double scale) {
+  return cross_forward(Q, K, V, key_lengths, scale, nullptr);
+}
+
+at::Tensor cross_attention_meta(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
+                                const c10::optional<at::Tensor>& key_lengths, double scale) {
+  return std::get<0>(cross_attn_fwd_meta(Q, K, V, key_lengths, scale, false));
+}
+
+struct CrossAttention : public ag::Function<CrossAttention> {
+  static at::Tensor forward(ag::AutogradContext* ctx, const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
+                            const c10::optional<at::Tensor>& key_lengths, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = op_of("trnsparse_hip::cross_attn_fwd", &cross_attn_fwd);
+    auto [O, lse] = op.call(Q, K, V, key_lengths, scale, true);
+    ctx->save_for_backward({Q, K, V, O, lse, key_lengths.has_value() ? *key_lengths : at::Tensor()});
+    ctx->saved_data["scale"] = scale;
+    return O;
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, const ag::variable_list& grads) {
+    first_order("cross_attention");
+    const auto s = ctx->get_saved_variables();
+    const bool need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    static const auto op = op_of("trnsparse_hip::cross_attn_bwd", &cross_attn_bwd);
+    auto [dQ, dK, dV] = op.call(s[0], s[1], s[2], s[3], grads[0], s[4],
+                                s[5].defined() ? c10::optional<at::Tensor>(s[5]) : c10::nullopt,
+                                ctx->saved_data["scale"].toDouble(), need_kv);
+    if (!need_kv) dK = dV = at::Tensor();
+    return {dQ, dK, dV, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor cross_attention_autograd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
+                                    const c10::optional<at::Tensor>& key_lengths, double scale) {
+  if (wants_grad({&Q, &K, &V})) return CrossAttention::apply(Q, K, V, key_lengths, scale);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static const auto op = op_of("trnsparse_hip::cross_attention", &cross_attention);
+  return op.call(Q, K, V, key_lengths, scale);
+}
+
+struct QKNormRope : public ag::Function<QKNormRope> {
+  static ag::variable_list forward(ag::AutogradContext* ctx, const at::Tensor& Q, const at::Tensor& K,
+                                   const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& pos,
+                                   const at::Tensor& freq, double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = op_of("trnsparse_hip::qk_norm_rope_fwd", &qk_norm_rope_fwd);
+    auto [q, k] = op.call(Q, K, wq, wk, pos, freq, eps, interleaved);
+    ctx->save_for_backward({Q, K, wq, wk, pos, freq});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {q, k};
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, const ag::variable_list& grads) {
+    first_order("qk_norm_rope");
+    const auto s = ctx->get_saved_variables();
+    const bool need_w = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
+    auto grad = [&](int i) {  // a result that was not used
+      return grads[i].defined() ? grads[i] : at::zeros(s[i].sizes(), s[i].options());
+    };
+    static const auto op = op_of("trnsparse_hip::qk_norm_rope_bwd", &qk_norm_rope_bwd);
+    auto [dQ, dK, dwq, dwk] = op.call(s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble(),
+                                      ctx->saved_data["interleaved"].toBool(), grad(0), grad(1), need_w);
+    if (!need_w) dwq = dwk = at::Tensor();
+    return {dQ, dK, dwq, dwk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& wq,
+                                                         const at::Tensor& wk, const at::Tensor& pos,
+                                                         const at::Tensor& freq, double eps, bool interleaved) {
+  if (wants_grad({&Q, &K, &wq, &wk})) {
+    auto r = QKNormRope::apply(Q, K, wq, wk, pos, freq, eps, interleaved);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  static const auto op = op_of("trnsparse_hip::qk_norm_rope", &qk_norm_rope_fwd);
+  return op.call(Q, K, wq, wk, pos, freq, eps, interleaved);
 }
 
 }  // namespace
@@ -802,6 +926,9 @@ TORCH_LIBRARY(trnsparse_hip, m) {
   m.def("qk_norm_rope_bwd(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
         "float eps, bool interleaved, Tensor grad_Q, Tensor grad_K, bool need_weights) -> (Tensor, Tensor, Tensor, "
         "Tensor)");
+  m.def("cross_attention(Tensor Q, Tensor K, Tensor V, Tensor? key_lengths, float scale) -> Tensor");
+  m.def("qk_norm_rope(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
+        "float eps, bool interleaved) -> (Tensor, Tensor)");
 }
 
 // the "CUDA" dispatch key is the GPU key of PyTorch-ROCm
@@ -822,6 +949,13 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
   m.impl("prefix_attn_fwd", &prefix_attn_fwd);
   m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+  m.impl("cross_attention", &cross_attention);
+  m.impl("qk_norm_rope", &qk_norm_rope_fwd);
+}
+
+TORCH_LIBRARY_IMPL(trnsparse_hip, AutogradCUDA, m) {
+  m.impl("cross_attention", &cross_attention_autograd);
+  m.impl("qk_norm_rope", &qk_norm_rope_autograd);
 }
 
 TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
@@ -841,4 +975,6 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
   m.impl("prefix_attn_fwd", &prefix_attn_fwd_meta);
   m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd_meta);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_meta);
+  m.impl("cross_attention", &cross_attention_meta);
+  m.impl("qk_norm_rope", &qk_norm_rope_fwd_meta);
 }

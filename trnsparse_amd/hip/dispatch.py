@@ -928,93 +928,48 @@ def hip_block_sparse_attention_backward(Q, K, V, O, dO, mask_bsr, scale: float, 
 
 
 # ------------------------------------------- attention between sequences
+#
+# These operators take strided operands as they are and carry their gradients
+# in the operator library (csrc/torch_ops.cpp), which also selects the
+# operands' device: what is left here is to bring operands together.
 
 
-def _lengths_on(t, dev: torch.device):
-    return None if t is None else t.to(dev).contiguous()
-
-
-class _CrossAttentionFunction(torch.autograd.Function):
-    """Autograd wrapper of cross attention: keeps Q, K, V, the result and its
-    rows' log-sum-exps."""
-
-    @staticmethod
-    def forward(ctx, Q, K, V, key_lengths, scale):
-        out, lse = _lib.ops().cross_attn_fwd(Q, K, V, key_lengths, scale, True)
-        ctx.save_for_backward(Q, K, V, out, lse, key_lengths)
-        ctx.scale = scale
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dO):
-        Q, K, V, O, lse, key_lengths = ctx.saved_tensors
-        need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        with torch.cuda.device(Q.device):
-            dQ, dK, dV = _lib.ops().cross_attn_bwd(Q, K, V, O, dO, lse, key_lengths, ctx.scale, need_kv)
-        return dQ, (dK if need_kv else None), (dV if need_kv else None), None, None
+def _together(first, *rest):
+    """The operands on one GPU: as they are when they share first's, else
+    copied to the first GPU among them (None stays)."""
+    dev = first.device
+    if dev.type == "cuda" and all(t is None or t.device == dev for t in rest):
+        return (first, *rest)
+    dev = _target_device(first, *rest)
+    return tuple(None if t is None else t.to(dev) for t in (first, *rest))
 
 
 @_library_call
 def hip_cross_attention(Q, K, V, key_lengths, scale: float):
     """cross_attention on the HIP kernels (operands on the host are copied
     over, the result returned on Q's device)."""
-    orig = Q.device
-    dev = _target_device(Q, K, V)
-    with torch.cuda.device(dev):
-        Q, K, V = (t.to(dev) for t in (Q, K, V))
-        lens = _lengths_on(key_lengths, dev)
-        if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
-            return _CrossAttentionFunction.apply(Q, K, V, lens, float(scale)).to(orig)
-        return _lib.ops().cross_attn_fwd(Q, K, V, lens, float(scale), False)[0].to(orig)
+    q, k, v, lens = _together(Q, K, V, key_lengths)
+    if lens is not None and not lens.is_contiguous():
+        lens = lens.contiguous()
+    out = _lib.ops().cross_attention(q, k, v, lens, scale)
+    return out if q is Q else out.to(Q.device)
 
 
 @_library_call
 def hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale: float):
     """shared_prefix_attention on the HIP kernels."""
-    orig = Q.device
-    dev = _target_device(Q, K, V)
-    with torch.cuda.device(dev), torch.no_grad():
-        Q, prefix_K, prefix_V, K, V = (t.to(dev) for t in (Q, prefix_K, prefix_V, K, V))
-        lens = _lengths_on(lengths, dev)
-        return _lib.ops().prefix_attn_fwd(Q, prefix_K, prefix_V, K, V, lens, float(scale)).to(orig)
-
-
-# ------------------------------- norm and rotation of query and key heads
-
-
-class _QKNormRopeFunction(torch.autograd.Function):
-    """Autograd wrapper of the norm and rotation: keeps Q, K and the weights,
-    forms the norms and angles again in the backward pass."""
-
-    @staticmethod
-    def forward(ctx, Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved):
-        ctx.save_for_backward(Q, K, q_weight, k_weight, positions, inv_freq)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return _lib.ops().qk_norm_rope_fwd(Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gQ, gK):
-        Q, K, wq, wk, pos, freq = ctx.saved_tensors
-        with torch.cuda.device(Q.device):
-            need_w = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-            dQ, dK, dwq, dwk = _lib.ops().qk_norm_rope_bwd(Q, K, wq, wk, pos, freq, ctx.eps, ctx.interleaved, gQ, gK, need_w)
-        return dQ, dK, (dwq if need_w else None), (dwk if need_w else None), None, None, None, None
+    q, pk, pv, k, v, lens = _together(Q, prefix_K, prefix_V, K, V, lengths)
+    if lens is not None and not lens.is_contiguous():
+        lens = lens.contiguous()
+    out = _lib.ops().prefix_attn_fwd(q, pk, pv, k, v, lens, scale)
+    return out if q is Q else out.to(Q.device)
 
 
 @_library_call
 def hip_qk_norm_rope(Q, K, q_weight, k_weight, positions, inv_freq, eps: float, interleaved: bool):
     """qk_norm_rope on the HIP kernels."""
-    orig = Q.device
-    dev = _target_device(Q, K)
-    with torch.cuda.device(dev):
-        Q, K = Q.to(dev), K.to(dev)
-        wq, wk = q_weight.to(dev).contiguous(), k_weight.to(dev).contiguous()
-        pos, freq = positions.to(dev), inv_freq.detach().to(dev, torch.float64).contiguous()
-        args = (Q, K, wq, wk, pos, freq, float(eps), bool(interleaved))
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (Q, K, wq, wk)):
-            out = _QKNormRopeFunction.apply(*args)
-        else:
-            out = _lib.ops().qk_norm_rope_fwd(*args)
-    return out[0].to(orig), out[1].to(orig)
+    q, k, wq, wk, pos, freq = _together(Q, K, q_weight, k_weight, positions, inv_freq)
+    if freq.dtype != torch.float64 or not freq.is_contiguous():
+        freq = freq.detach().double().contiguous()
+    out = _lib.ops().qk_norm_rope(q, k, wq.contiguous(), wk.contiguous(), pos, freq, eps, interleaved)
+    return out if q is Q else tuple(t.to(Q.device) for t in out)

@@ -506,22 +506,22 @@ def block_sparse_attention_tiled(
 
 def _check_heads(who: str, Q, K, V, lengths, scale: float) -> None:
     """Shapes and types of (batch, heads, rows, head_dim) operands; on both backends."""
-    for name, t in (("Q", Q), ("K", K), ("V", V)):
-        if t.dim() != 4:
-            raise RuntimeError(f"{who}: {name} must be (batch, heads, rows, head_dim), got shape {tuple(t.shape)}")
-    if K.shape != V.shape or K.shape[0] != Q.shape[0] or K.shape[3] != Q.shape[3]:
-        raise RuntimeError(f"{who}: Q {tuple(Q.shape)}, K {tuple(K.shape)} and V {tuple(V.shape)} do not belong together")
-    if K.shape[1] == 0 or Q.shape[1] % K.shape[1]:
-        raise RuntimeError(f"{who}: {Q.shape[1]} query heads do not divide over {K.shape[1]} key heads")
-    if not (Q.dtype == K.dtype == V.dtype) or not Q.is_floating_point():
-        raise RuntimeError(f"{who}: Q, K, V must have one floating dtype, got {Q.dtype}, {K.dtype}, {V.dtype}")
-    if not 1 <= Q.shape[3] <= 128:
-        raise RuntimeError(f"{who}: head_dim {Q.shape[3]} is not in 1 .. 128")
-    if not (scale > 0 and math.isfinite(scale)):
+    q, k, v, dt = Q.shape, K.shape, V.shape, Q.dtype
+    if not (len(q) == len(k) == len(v) == 4):
+        raise RuntimeError(f"{who}: Q, K, V must be (batch, heads, rows, head_dim), got {tuple(q)}, {tuple(k)}, {tuple(v)}")
+    if k != v or k[0] != q[0] or k[3] != q[3]:
+        raise RuntimeError(f"{who}: Q {tuple(q)}, K {tuple(k)} and V {tuple(v)} do not belong together")
+    if k[1] == 0 or q[1] % k[1]:
+        raise RuntimeError(f"{who}: {q[1]} query heads do not divide over {k[1]} key heads")
+    if K.dtype != dt or V.dtype != dt or not dt.is_floating_point:
+        raise RuntimeError(f"{who}: Q, K, V must have one floating dtype, got {dt}, {K.dtype}, {V.dtype}")
+    if not 1 <= q[3] <= 128:
+        raise RuntimeError(f"{who}: head_dim {q[3]} is not in 1 .. 128")
+    if not 0 < scale < math.inf:
         raise RuntimeError(f"{who}: scale must be positive, got {scale}")
     if lengths is not None:
-        if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != (Q.shape[0],):
-            raise RuntimeError(f"{who}: lengths must be ({Q.shape[0]},) of int32 or int64, got {tuple(lengths.shape)} of "
+        if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != q[:1]:
+            raise RuntimeError(f"{who}: lengths must be ({q[0]},) of int32 or int64, got {tuple(lengths.shape)} of "
                                f"{lengths.dtype}")
 
 
@@ -590,7 +590,7 @@ def cross_attention(
     has Q's order of heads and rows. Differentiable in Q, K and V.
     """
     if scale is None:
-        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
+        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0  # (such shapes are refused below)
     _check_heads("cross_attention", Q, K, V, key_lengths, scale)
     if _use_hip():
         from .hip.dispatch import hip_cross_attention
@@ -628,7 +628,7 @@ def shared_prefix_attention(
     """
     who = "shared_prefix_attention"
     if scale is None:
-        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0
+        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0  # (such shapes are refused below)
     _check_heads(who, Q, K, V, lengths, scale)
     want = (K.shape[1], K.shape[3])
     if prefix_K.dim() != 3 or prefix_K.shape != prefix_V.shape or (prefix_K.shape[0], prefix_K.shape[2]) != want:
