@@ -22,13 +22,13 @@ int check_operand(const char* who, const char* name, const void* p, const int64_
   return TSP_OK;
 }
 
-Plan fwd_plan(int64_t units, int64_t rows, int64_t keys) {
+Plan fwd_plan(int64_t units, int64_t rows, int64_t keys, int64_t want) {
   Plan p;
   p.narrow = rows <= 32;
   p.tiles = p.narrow ? 1 : (int)ceil_div(rows, 128);
-  // Ranges of keys: enough workgroups for the chip (256 CUs, two wide
-  // workgroups to each), none shorter than a few stages.
-  const int64_t wgs = units * p.tiles, want = p.narrow ? 1024 : 512, least = 256;
+  // Ranges of keys: `want` workgroups where the units alone are fewer than half
+  // of them, none shorter than 256 keys.
+  const int64_t wgs = units * p.tiles, least = 256;
   int64_t n = wgs >= want / 2 ? 1 : ceil_div(want, wgs);
   if (n > ceil_div(keys, least)) n = ceil_div(keys, least);
   if (n < 1) n = 1;
@@ -37,29 +37,53 @@ Plan fwd_plan(int64_t units, int64_t rows, int64_t keys) {
   return p;
 }
 
-template <typename T>
-static int launch_t(const Plan& p, const FwdArgs& a, hipStream_t st) {
-  const int64_t grid = head_grid((int64_t)p.tiles * p.nsplit, (int64_t)a.units_b * a.Hkv);
-  if (grid > INT32_MAX) return fail(TSP_EUNSUPPORTED, "attention: too large a grid");
-  constexpr int stage = 2 * 32 * T::ROWB;  // 8, 16 or 32 KiB
-  if (p.narrow) {
-    constexpr int NW = stage > 16384 ? 2 : 4;
-    hipLaunchKernelGGL((fwd_narrow<T, NW, 2>), dim3((unsigned)grid), dim3(64 * NW), 0, st, a);
-    return check_launch("fwd_narrow launch");
-  }
-  constexpr int NT = T::ESZ == 2 ? 2 : 1;
-  hipLaunchKernelGGL((fwd_wide<T, NT>), dim3((unsigned)grid), dim3(256), 0, st, a);
-  return check_launch("fwd_wide launch");
+// 512 workgroups are the chip's, two to a CU; ragged lengths leave some idle.
+static Plan cross_plan(int64_t units, int64_t rows, int64_t keys) {
+  return fwd_plan(units, rows, keys, rows <= 32 ? 1024 : 512);
 }
 
-int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st) {
+static void set_plan(FwdArgs& a, const Plan& p) {
   a.tiles = p.tiles;
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
-  const bool w = a.D > 64;
-  if (dtype == TSP_BF16) return w ? launch_t<Tile16<__bf16, 128>>(p, a, st) : launch_t<Tile16<__bf16, 64>>(p, a, st);
-  if (dtype == TSP_F16) return w ? launch_t<Tile16<_Float16, 128>>(p, a, st) : launch_t<Tile16<_Float16, 64>>(p, a, st);
-  return w ? launch_t<Tile32<128>>(p, a, st) : launch_t<Tile32<64>>(p, a, st);
+}
+static int64_t grid_of(const FwdArgs& a) {
+  return head_grid((int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv);
+}
+
+// f.operator()<Tile>() for the operands' type and head_dim
+template <typename F>
+static int with_tile(int dtype, int D, F&& f) {
+  if (dtype == TSP_BF16) return D > 64 ? f(Tile16<__bf16, 128>{}) : f(Tile16<__bf16, 64>{});
+  if (dtype == TSP_F16) return D > 64 ? f(Tile16<_Float16, 128>{}) : f(Tile16<_Float16, 64>{});
+  return D > 64 ? f(Tile32<128>{}) : f(Tile32<64>{});
+}
+
+int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st) {
+  set_plan(a, p);
+  const int64_t grid = grid_of(a);
+  if (grid > INT32_MAX) return fail(TSP_EUNSUPPORTED, "attention: too large a grid");
+  return with_tile(dtype, a.D, [&](auto tile) {
+    typedef decltype(tile) T;
+    if (p.narrow)
+      hipLaunchKernelGGL((fwd_narrow<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((fwd_wide<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    return check_launch("attention launch");
+  });
+}
+
+int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st) {
+  set_plan(a, pa);
+  set_plan(b, pb);
+  const int64_t ga = grid_of(a), gb = grid_of(b);
+  if (ga + gb > INT32_MAX) return fail(TSP_EUNSUPPORTED, "attention: too large a grid");
+  return with_tile(dtype, a.D, [&](auto tile) {
+    typedef decltype(tile) T;
+    hipLaunchKernelGGL((fwd_two<T>), dim3((unsigned)(ga + gb)), dim3(256), 0, st, a, b, (uint32_t)ga, !pa.narrow,
+                       !pb.narrow);
+    return check_launch("attention launch");
+  });
 }
 
 int launch_combine(int dtype, const CombineArgs& a, hipStream_t st) {
@@ -99,7 +123,7 @@ extern "C" int64_t tsp_cross_attn_workspace_size(int dtype, int64_t B, int64_t H
                                                  int64_t D) {
   if (xat::check_sizes("tsp_cross_attn_workspace_size", dtype, B, Hq, Hkv, Sq, L, D)) return -1;
   if (B * Hq * Sq == 0) return 0;
-  const xat::Plan p = xat::fwd_plan(B * Hkv, Hq / Hkv * Sq, L);
+  const xat::Plan p = xat::cross_plan(B * Hkv, Hq / Hkv * Sq, L);
   return p.nsplit > 1 ? p.nsplit * B * Hq * Sq * (D + 1) * 4 : 0;
 }
 
@@ -123,7 +147,7 @@ extern "C" int tsp_cross_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const int64_t need = tsp_cross_attn_workspace_size(dtype, B, Hq, Hkv, Sq, L, D);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   const int64_t none[3] = {0, 0, 0};
-  const xat::Plan p = xat::fwd_plan(B * Hkv, Hq / Hkv * Sq, L);
+  const xat::Plan p = xat::cross_plan(B * Hkv, Hq / Hkv * Sq, L);
   xat::FwdArgs a{};
   a.Q = xat::operand(Q, qs, dtype);
   a.K = xat::operand(K, L > 0 ? ks : none, dtype);

@@ -23,8 +23,8 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t P, int64_t S) {
   const int64_t G = Hq / Hkv;
   PrefixPlan p{};
-  if (P > 0) p.shared = fwd_plan(Hkv, B * G * Sq, P);
-  if (S > 0) p.own = fwd_plan(B * Hkv, G * Sq, S);
+  if (P > 0) p.shared = fwd_plan(Hkv, B * G * Sq, P, 128);
+  if (S > 0) p.own = fwd_plan(B * Hkv, G * Sq, S, 512);
   p.nsplit = p.shared.nsplit + p.own.nsplit;
   return p;
 }
@@ -78,28 +78,32 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
   a.plse = a.part + p.nsplit * rows * D;
   a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.D = (int)D;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
+  xat::FwdArgs sh = a, own = a;
   if (P > 0) {
-    xat::FwdArgs s = a;
-    s.K = xat::operand(PK, pks, dtype);
-    s.V = xat::operand(PV, pvs, dtype);
-    s.units_b = 1;
-    s.R = (int)(B * Hq / Hkv * Sq);
-    s.L = P;
-    if ((rc = xat::launch_fwd(dtype, p.shared, s, st))) return rc;
+    sh.K = xat::operand(PK, pks, dtype);
+    sh.V = xat::operand(PV, pvs, dtype);
+    sh.units_b = 1;
+    sh.R = (int)(B * Hq / Hkv * Sq);
+    sh.L = P;
   }
   if (S > 0) {
-    xat::FwdArgs s = a;
-    s.K = xat::operand(K, ks, dtype);
-    s.V = xat::operand(V, vs, dtype);
-    s.lengths = lengths;
-    s.len64 = index_type == TSP_I64;
-    s.units_b = (int)B;
-    s.R = (int)(Hq / Hkv * Sq);
-    s.L = S;
-    s.causal = Sq > 1;
-    s.split0 = p.shared.nsplit;
-    if ((rc = xat::launch_fwd(dtype, p.own, s, st))) return rc;
+    own.K = xat::operand(K, ks, dtype);
+    own.V = xat::operand(V, vs, dtype);
+    own.lengths = lengths;
+    own.len64 = index_type == TSP_I64;
+    own.units_b = (int)B;
+    own.R = (int)(Hq / Hkv * Sq);
+    own.L = S;
+    own.causal = Sq > 1;
+    own.split0 = p.shared.nsplit;
   }
+  if (P > 0 && S > 0)
+    rc = xat::launch_fwd_two(dtype, p.shared, sh, p.own, own, st);
+  else if (P > 0)
+    rc = xat::launch_fwd(dtype, p.shared, sh, st);
+  else if (S > 0)
+    rc = xat::launch_fwd(dtype, p.own, own, st);
+  if (rc) return rc;
   const xat::CombineArgs c{a.part, a.plse, rows, p.nsplit, a.D, (int)Hq, a.Sq, a.O, a.ob, a.oh, a.os, nullptr};
   return xat::launch_combine(dtype, c, st);
 }

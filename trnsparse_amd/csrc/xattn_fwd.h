@@ -9,8 +9,8 @@
 //   wide    128 rows to a workgroup, a wavefront to 32 of them; stages of keys
 //           shared by the four wavefronts through an LDS ring of two
 //   narrow  up to 32 rows to a workgroup: every wavefront has all of them and
-//           takes every NW-th stage of 32 keys through a ring of its own, with
-//           no workgroup barrier until the wavefronts' results are joined
+//           takes every fourth stage of 32 keys through LDS of its own, with no
+//           workgroup barrier until the wavefronts' results are joined
 // Either takes one of `nsplit` ranges of `chunk` keys. With one range it writes
 // the rows' results; with more it writes each range's own normalised result
 // and log-sum-exp in fp32, which combine_kernel joins in range order.
@@ -88,147 +88,201 @@ __device__ inline void put_lse(const FwdArgs& a, const RowId& id, int split, flo
     a.lse[id.orow] = lse2 * 0.69314718055994531f;
 }
 
-template <typename T, int NT>
-__global__ __launch_bounds__(256, 2) void fwd_wide(const FwdArgs a) {
-  constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
-  int64_t unit, item;
-  if (!head_item(blockIdx.x, (int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-  const int tile = (int)(item % a.tiles), split = (int)(item / a.tiles);
-  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
-  const int r = tile * 128 + w * 32 + l32;
-  const bool live = r < a.R;
-  const RowId id = row_id(a, ub, hk, live ? r : 0);
-
-  typename T::Rows q;
-  T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
-
-  const int64_t n = unit_length(a, ub);
-  const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
-  const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;  // keys of this row
-  const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, HK) : 0;
-  const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
-  const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
-  Stager<T, HK, 4> ks, vs;
-  ks.init(w, lane, a.K.s, a.D);
-  vs.init(w, lane, a.V.s, a.D);
-  const typename T::Lane ln = T::lane_of(lane);
-  const uint32_t lds0 = dma::lds_addr(lds);
-  auto issue = [&](int s) {
-    const uint32_t st = lds0 + (s & 1) * STAGE;
-    ks.issue(Kp, k0 + (int64_t)s * HK, k1, a.K.s, a.D, st, w);
-    vs.issue(Vp, k0 + (int64_t)s * HK, k1, a.V.s, a.D, st + HBYTES, w);
-  };
-  RowState<T> x;
-  x.clear();
-  if (nst > 0) issue(0);
-  for (int s = 0; s < nst; ++s) {
-    dma::wait_vm<0>();
-    dma::barrier();
-    if (s + 1 < nst) issue(s + 1);
-    const int64_t at = k0 + (int64_t)s * HK;
-    const uint32_t st = lds0 + (s & 1) * STAGE;
-    softmax_stage<T, NT>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,
-                         (sees < k1 ? sees : k1) - at);
-  }
-  const float l = halves_sum(x.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  if (!live) return;
-  const RowOut<T> out(a, id, split);
-  T::quads(x.acc, h, [&](int d, f32x4 v) {
-    if (d < a.D) out.put(d, v * inv);
-  });
-  if (h == 0) put_lse(a, id, split, x.m + __builtin_amdgcn_logf(l));
+// Keys of a row within the range that ends at k1, from key `at` of a stage.
+__device__ inline int keys_from(int64_t sees, int64_t k1, int64_t at) {
+  const int64_t n = (sees < k1 ? sees : k1) - at;
+  return n < 0 ? 0 : n > 64 ? 64 : (int)n;
 }
 
-template <typename T, int NW, int NST>
-__global__ __launch_bounds__(64 * NW, 1) void fwd_narrow(const FwdArgs a) {
-  constexpr int HBYTES = 32 * T::ROWB, STAGE = 2 * HBYTES, XLD = T::DP + 4;
-  constexpr int RING = NW * NST * STAGE, XB = NW * 32 * (XLD + 2) * 4;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[RING > XB ? RING : XB];
-  int64_t unit, item;
-  if (!head_item(blockIdx.x, a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-  const int split = (int)item;
-  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
-  const bool live = l32 < a.R;
-  const RowId id = row_id(a, ub, hk, live ? l32 : 0);
+template <typename T, int NT>
+struct Wide {
+  static constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES, LDS = 2 * STAGE;
+  static __device__ inline void run(const FwdArgs& a, uint32_t block, uint8_t* lds) {
+    int64_t unit, item;
+    if (!head_item(block, (int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+    const int tile = (int)(item % a.tiles), split = (int)(item / a.tiles);
+    const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int r = tile * 128 + w * 32 + (lane & 31);
+    const bool live = r < a.R;
+    const RowId id = row_id(a, ub, hk, live ? r : 0);
 
-  const int64_t n = unit_length(a, ub);
-  const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
-  const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;
-  const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, 32) : 0, mine = nst > w ? (nst - w + NW - 1) / NW : 0;
-  const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
-  const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
-  Stager<T, 32, 1> ks, vs;
-  ks.init(0, lane, a.K.s, a.D);
-  vs.init(0, lane, a.V.s, a.D);
-  constexpr int NI = 2 * Stager<T, 32, 1>::NI;  // loads of a stage
-  const typename T::Lane ln = T::lane_of(lane);
-  const uint32_t ring = dma::lds_addr(lds) + w * NST * STAGE;
-  auto key = [&](int s) { return k0 + 32 * ((int64_t)s * NW + w); };
-  auto issue = [&](int s) {
-    const uint32_t st = ring + (s % NST) * STAGE;
-    ks.issue(Kp, key(s), k1, a.K.s, a.D, st, 0);
-    vs.issue(Vp, key(s), k1, a.V.s, a.D, st + HBYTES, 0);
-  };
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
-    if (s < mine) issue(s);
-  typename T::Rows q;
-  T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
-  RowState<T> x;
-  x.clear();
-  for (int s = 0; s < mine; ++s) {
-    // the slot of stage s - 1 is free once this wavefront's reads of it returned
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (s + NST - 1 < mine) {
-      issue(s + NST - 1);
-      dma::wait_vm<(NST - 1) * NI>();
-    } else {
+    typename T::Rows q;
+    T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
+
+    const int64_t n = unit_length(a, ub);
+    const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
+    const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;  // keys of this row
+    const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, HK) : 0;
+    const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
+    const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
+    Stager<T, HK, 4> ks, vs;
+    ks.init(w, lane, a.K.s, a.D);
+    vs.init(w, lane, a.V.s, a.D);
+    const typename T::Lane ln = T::lane_of(lane);
+    const uint32_t lds0 = dma::lds_addr(lds);
+    auto issue = [&](int s) {
+      const uint32_t st = lds0 + (s & 1) * STAGE;
+      ks.issue(Kp, k0 + (int64_t)s * HK, k1, a.K.s, a.D, st, w);
+      vs.issue(Vp, k0 + (int64_t)s * HK, k1, a.V.s, a.D, st + HBYTES, w);
+    };
+    RowState<T> x;
+    x.clear();
+    if (nst > 0) issue(0);
+    for (int s = 0; s < nst; ++s) {
       dma::wait_vm<0>();
+      dma::barrier();
+      if (s + 1 < nst) issue(s + 1);
+      const int64_t at = k0 + (int64_t)s * HK;
+      const uint32_t st = lds0 + (s & 1) * STAGE;
+      softmax_stage<T, NT>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,
+                           keys_from(sees, k1, at), [] {});
     }
-    asm volatile("" ::: "memory");
-    const uint32_t st = ring + (s % NST) * STAGE;
-    const int64_t at = key(s);
-    softmax_stage<T, 1>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + 32 > k1,
-                        (sees < k1 ? sees : k1) - at);
+    const float l = halves_sum(x.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (!live) return;
+    const RowOut<T> out(a, id, split);
+    T::quads(x.acc, h, [&](int d, f32x4 v) {
+      if (d < a.D) out.put(d, v * inv);
+    });
+    if (h == 0) put_lse(a, id, split, x.m + __builtin_amdgcn_logf(l));
   }
-  // ---- join the wavefronts: m, l, acc of each row through LDS
-  const float l = halves_sum(x.l);
-  float* xo = (float*)lds;
-  float* xm = xo + NW * 32 * XLD;
-  float* xl = xm + NW * 32;
-  __syncthreads();
-  if (live) {
-    T::quads(x.acc, h, [&](int d, f32x4 v) { *(f32x4*)(xo + (w * 32 + l32) * XLD + d) = v; });
-    if (h == 0) {
-      xm[w * 32 + l32] = x.m;
-      xl[w * 32 + l32] = l;
+};
+
+// Four wavefronts, each with a stage of K and one of V of its own: the next
+// stage's K is loaded while this one's softmax and V are worked on, its V while
+// the next scores are. Half the LDS of a ring of two, so that two workgroups
+// share a CU (16 bit; 128 wide fp32 has one): one streams while the other
+// starts or joins its wavefronts (16 sequences of up to 1500 keys, 8 heads of
+// 128: rings of two with one workgroup to a CU 21.7 us).
+template <typename T>
+struct Narrow {
+  static constexpr int NW = 4, HBYTES = 32 * T::ROWB, XLD = T::DP + 4;
+  static constexpr int RING = NW * 2 * HBYTES, XB = NW * 32 * (XLD + 2) * 4, LDS = RING > XB ? RING : XB;
+  typedef Stager<T, 32, 1> St;
+
+  static __device__ inline void run(const FwdArgs& a, uint32_t block, uint8_t* lds) {
+    int64_t unit, item;
+    if (!head_item(block, a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+    const int split = (int)item;
+    const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int l32 = lane & 31;
+    const bool live = l32 < a.R;
+    const RowId id = row_id(a, ub, hk, live ? l32 : 0);
+
+    const int64_t n = unit_length(a, ub);
+    const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
+    const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;
+    const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, 32) : 0, mine = nst > w ? (nst - w + NW - 1) / NW : 0;
+    const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
+    const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
+    St ks, vs;
+    ks.init(0, lane, a.K.s, a.D);
+    vs.init(0, lane, a.V.s, a.D);
+    const uint32_t kst = dma::lds_addr(lds) + w * 2 * HBYTES, vst = kst + HBYTES;
+    auto key = [&](int s) { return k0 + 32 * ((int64_t)s * NW + w); };
+    if (mine > 0) {
+      ks.issue(Kp, key(0), k1, a.K.s, a.D, kst, 0);
+      vs.issue(Vp, key(0), k1, a.V.s, a.D, vst, 0);
     }
+    typename T::Rows q;
+    T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
+    const typename T::Lane ln = T::lane_of(lane);
+    RowState<T> x;
+    x.clear();
+    for (int s = 0; s < mine; ++s) {
+      const bool more = s + 1 < mine;
+      const int64_t at = key(s);
+      dma::wait_vm<St::NI>();  // K is there once only V's loads are out
+      fence();
+      softmax_stage<T, 1>(x, q, kst, vst, ln, h, a.scale_log2, a.causal || at + 32 > k1, keys_from(sees, k1, at), [&] {
+        drained();  // this wavefront's reads of K have returned: its place is free
+        if (more) {
+          ks.issue(Kp, key(s + 1), k1, a.K.s, a.D, kst, 0);
+          dma::wait_vm<St::NI>();
+        } else {
+          dma::wait_vm<0>();
+        }
+        fence();
+      });
+      drained();
+      if (more) vs.issue(Vp, key(s + 1), k1, a.V.s, a.D, vst, 0);
+    }
+    join(a, ub, hk, split, x, lds, w, h, l32, live);
   }
-  __syncthreads();
-  constexpr int QPR = T::DP / 4;  // quads of a row
-  for (int e = tid; e < a.R * QPR; e += 64 * NW) {
-    const int row = e / QPR, d = 4 * (e % QPR);
-    float m = -INFINITY;
+
+  static __device__ inline void fence() { asm volatile("" ::: "memory"); }
+  static __device__ inline void drained() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+  // m, l, acc of each row over the wavefronts, through LDS
+  static __device__ inline void join(const FwdArgs& a, int64_t ub, int64_t hk, int split, const RowState<T>& x, uint8_t* lds,
+                                     int w, int h, int l32, bool live) {
+    const float l = halves_sum(x.l);
+    float* xo = (float*)lds;
+    float* xm = xo + NW * 32 * XLD;
+    float* xl = xm + NW * 32;
+    __syncthreads();
+    if (live) {
+      T::quads(x.acc, h, [&](int d, f32x4 v) { *(f32x4*)(xo + (w * 32 + l32) * XLD + d) = v; });
+      if (h == 0) {
+        xm[w * 32 + l32] = x.m;
+        xl[w * 32 + l32] = l;
+      }
+    }
+    __syncthreads();
+    constexpr int QPR = T::DP / 4;  // quads of a row
+    for (int e = threadIdx.x; e < a.R * QPR; e += 64 * NW) {
+      const int row = e / QPR, d = 4 * (e % QPR);
+      float m = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NW; ++j) m = fmaxf(m, xm[j * 32 + row]);
-    float total = 0.f;
-    f32x4 sum = f32x4{};
+      for (int j = 0; j < NW; ++j) m = fmaxf(m, xm[j * 32 + row]);
+      float total = 0.f;
+      f32x4 sum = f32x4{};
 #pragma unroll
-    for (int j = 0; j < NW; ++j) {
-      const float lj = xl[j * 32 + row];
-      // (a wavefront without keys for the row has m = -inf, l = 0; a NaN score leaves NaN in l)
-      const float f = xm[j * 32 + row] == -INFINITY ? (lj == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(xm[j * 32 + row] - m);
-      total += f * lj;
-      sum += *(const f32x4*)(xo + (j * 32 + row) * XLD + d) * f;
+      for (int j = 0; j < NW; ++j) {
+        const float lj = xl[j * 32 + row], mj = xm[j * 32 + row];
+        // (a wavefront without keys for the row has m = -inf, l = 0; a NaN score leaves NaN in l)
+        const float f = mj == -INFINITY ? (lj == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mj - m);
+        total += f * lj;
+        sum += *(const f32x4*)(xo + (j * 32 + row) * XLD + d) * f;
+      }
+      const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+      const RowId rid = row_id(a, ub, hk, row);
+      if (d < a.D) RowOut<T>(a, rid, split).put(d, sum * inv);
+      if (d == 0) put_lse(a, rid, split, m + __builtin_amdgcn_logf(total));
     }
-    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-    const RowId rid = row_id(a, ub, hk, row);
-    if (d < a.D) RowOut<T>(a, rid, split).put(d, sum * inv);
-    if (d == 0) put_lse(a, rid, split, m + __builtin_amdgcn_logf(total));
   }
+};
+
+template <typename T>
+struct Kernels {
+  typedef Wide<T, T::ESZ == 2 ? 2 : 1> W;
+  typedef Narrow<T> N;
+  static constexpr int PER_CU = N::LDS <= 80 * 1024 ? 2 : 1;
+};
+template <typename T>
+__global__ __launch_bounds__(256, 2) void fwd_wide(const FwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Kernels<T>::W::LDS];
+  Kernels<T>::W::run(a, blockIdx.x, lds);
+}
+template <typename T>
+__global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_narrow(const FwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Kernels<T>::N::LDS];
+  Kernels<T>::N::run(a, blockIdx.x, lds);
+}
+// Two sets of keys in one launch: the first `grid0` workgroups take the first.
+template <typename T>
+__global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_two(const FwdArgs a, const FwdArgs b, uint32_t grid0,
+                                                                   bool wide_a, bool wide_b) {
+  typedef Kernels<T> K;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[K::W::LDS > K::N::LDS ? K::W::LDS : K::N::LDS];
+  const bool first = blockIdx.x < grid0;
+  const FwdArgs& x = first ? a : b;
+  const uint32_t block = first ? blockIdx.x : blockIdx.x - grid0;
+  if (first ? wide_a : wide_b)
+    K::W::run(x, block, lds);
+  else
+    K::N::run(x, block, lds);
 }
 
 // The ranges' results of every row in one: weights 2^(lse_j - max lse). Rows
@@ -245,18 +299,33 @@ struct CombineArgs {
 template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int d = 4 * (threadIdx.x & 31);
+  const int lane = threadIdx.x & 31, d = 4 * lane;
   if (row >= a.prows) return;
-  float m = -INFINITY;
-  for (int j = 0; j < a.nsplit; ++j) m = fmaxf(m, a.plse[j * a.prows + row]);
-  float total = 0.f;
+  // 32 ranges at a time, one to a lane: their weights against the largest so
+  // far; then their parts, read without waiting for one another
+  float m = -INFINITY, total = 0.f;
   f32x4 sum = f32x4{};
-  for (int j = 0; j < a.nsplit; ++j) {
-    const float lse = a.plse[j * a.prows + row];
-    if (lse == -INFINITY) continue;  // (its part is not read; a NaN goes on)
-    const float f = __builtin_amdgcn_exp2f(lse - m);
-    total += f;
-    if (d < a.D) sum += *(const f32x4*)(a.part + (j * a.prows + row) * a.D + d) * f;
+  for (int j0 = 0; j0 < a.nsplit; j0 += 32) {
+    const float lse = j0 + lane < a.nsplit ? a.plse[(j0 + lane) * a.prows + row] : -INFINITY;
+    float mx = lse;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    const float mn = fmaxf(m, mx);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    total *= f;
+    sum *= f;
+    // (a range without keys weighs nothing; a NaN goes on)
+    const float wgt = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - mn);
+    const int n = a.nsplit - j0 < 32 ? a.nsplit - j0 : 32;
+    const float* p = a.part + (j0 * a.prows + row) * a.D + (d < a.D ? d : 0);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const float wj = __shfl(wgt, (threadIdx.x & 32) + j, 64);
+      const f32x4 v = *(const f32x4*)(p + j * a.prows * a.D);
+      total += wj;
+      sum += wj == 0.f ? f32x4{} : v * wj;
+    }
   }
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
   const int64_t i = row % a.Sq, bh = row / a.Sq;
@@ -272,8 +341,9 @@ struct Plan {
   int tiles, nsplit;
   int64_t chunk;
 };
-Plan fwd_plan(int64_t units, int64_t rows, int64_t keys);
+Plan fwd_plan(int64_t units, int64_t rows, int64_t keys, int64_t want);
 int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st);
+int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st);
 int launch_combine(int dtype, const CombineArgs& a, hipStream_t st);
 
 // Checks of one strided operand; 0 or a status with a message.

@@ -263,11 +263,14 @@ struct RowState {
     l = 0.f;
   }
 };
-template <typename T, int NT>
+// `between` runs once the scores have left the K stage, before V is read.
+template <typename T, int NT, typename F>
 __device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, uint32_t kst, uint32_t vst,
-                                     const typename T::Lane& ln, int h, float scale_log2, bool check, int64_t keys) {
+                                     const typename T::Lane& ln, int h, float scale_log2, bool check, int keys,
+                                     F&& between) {
   f32x16 s[NT];
   T::template scores<NT>(s, kst, ln, q);
+  between();
   if (check) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
