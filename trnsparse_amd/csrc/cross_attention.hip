@@ -22,24 +22,27 @@ int check_operand(const char* who, const char* name, const void* p, const int64_
   return TSP_OK;
 }
 
-Plan fwd_plan(int64_t units, int64_t rows, int64_t keys, int64_t want) {
+Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want) {
   Plan p;
   p.narrow = rows <= 32;
   p.tiles = p.narrow ? 1 : (int)ceil_div(rows, 128);
-  // Ranges of keys: `want` workgroups where the units alone are fewer than half
-  // of them, none shorter than 256 keys.
-  const int64_t wgs = units * p.tiles, least = 256;
-  int64_t n = wgs >= want / 2 ? 1 : ceil_div(want, wgs);
+  // Ranges of keys where the units and tiles are fewer than half of `want`
+  // workgroups; none shorter than `least` keys, which is where a range costs as
+  // much as the launch that joins the ranges. Narrow bf16 of 128, 300 / 1500 /
+  // 4000 / 16000 keys of 32 units: 7.4 / 13.2 / 21.8 / 59 us, with 256 at
+  // least 9.6 / 13.6 / 23.8 / 59; of 128 units 8.4 / 26 / 56 / 192, with one
+  // range 8.4 / 25 / 55 / 197. In fp32 a stage of 32 keys is 3.4 us of matrix
+  // instructions and a CU holds one workgroup: shorter ranges, fewer of them.
+  const bool f32 = dtype == TSP_F32;
+  const int64_t want = p.narrow ? (f32 ? 256 : 512) : wide_want, least = p.narrow ? (f32 ? 128 : 512) : (f32 ? 64 : 256);
+  const int64_t wgs = units * p.tiles, step = p.narrow ? 128 : 64;
+  int64_t n = wgs >= (p.narrow && f32 ? want : want / 2) ? 1 : ceil_div(want, wgs);
   if (n > ceil_div(keys, least)) n = ceil_div(keys, least);
+  if (n > 32) n = 32;  // (8 heads on one key head, 16000 keys in fp32: 125 ranges 51 us, 32 36)
   if (n < 1) n = 1;
-  p.chunk = ceil_div(ceil_div(keys > 0 ? keys : 1, n), 128) * 128;
+  p.chunk = ceil_div(ceil_div(keys > 0 ? keys : 1, n), step) * step;
   p.nsplit = (int)(keys > 0 ? ceil_div(keys, p.chunk) : 1);
   return p;
-}
-
-// 512 workgroups are the chip's, two to a CU; ragged lengths leave some idle.
-static Plan cross_plan(int64_t units, int64_t rows, int64_t keys) {
-  return fwd_plan(units, rows, keys, rows <= 32 ? 1024 : 512);
 }
 
 static void set_plan(FwdArgs& a, const Plan& p) {
@@ -123,7 +126,7 @@ extern "C" int64_t tsp_cross_attn_workspace_size(int dtype, int64_t B, int64_t H
                                                  int64_t D) {
   if (xat::check_sizes("tsp_cross_attn_workspace_size", dtype, B, Hq, Hkv, Sq, L, D)) return -1;
   if (B * Hq * Sq == 0) return 0;
-  const xat::Plan p = xat::cross_plan(B * Hkv, Hq / Hkv * Sq, L);
+  const xat::Plan p = xat::fwd_plan(dtype, B * Hkv, Hq / Hkv * Sq, L, 512);
   return p.nsplit > 1 ? p.nsplit * B * Hq * Sq * (D + 1) * 4 : 0;
 }
 
@@ -147,7 +150,7 @@ extern "C" int tsp_cross_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const int64_t need = tsp_cross_attn_workspace_size(dtype, B, Hq, Hkv, Sq, L, D);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   const int64_t none[3] = {0, 0, 0};
-  const xat::Plan p = xat::cross_plan(B * Hkv, Hq / Hkv * Sq, L);
+  const xat::Plan p = xat::fwd_plan(dtype, B * Hkv, Hq / Hkv * Sq, L, 512);
   xat::FwdArgs a{};
   a.Q = xat::operand(Q, qs, dtype);
   a.K = xat::operand(K, L > 0 ? ks : none, dtype);

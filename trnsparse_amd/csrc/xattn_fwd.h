@@ -341,7 +341,7 @@ struct Plan {
   int tiles, nsplit;
   int64_t chunk;
 };
-Plan fwd_plan(int64_t units, int64_t rows, int64_t keys, int64_t want);
+Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want);
 int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st);
 int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st);
 int launch_combine(int dtype, const CombineArgs& a, hipStream_t st);
