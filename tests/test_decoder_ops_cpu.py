@@ -90,39 +90,45 @@ def test_rope_frequencies():
         ts.rope_frequencies(7)
 
 
-def refusals():
-    Q, K, V = heads(2, 4, 2, 3, 5, 8)
-    p = K[0]
-    x, s = ts.cross_attention, ts.shared_prefix_attention
+def refusals(dt=F64, other=torch.float32, dev="cpu"):
+    Q, K, V = (t.to(dev) for t in heads(2, 4, 2, 3, 5, 8, dt))
+    p, i = K[0], lambda *v: torch.tensor(v, device=dev)
+    x, s, n = ts.cross_attention, ts.shared_prefix_attention, ts.qk_norm_rope
+    wide = [torch.zeros(1, 1, 2, 129, dtype=dt, device=dev) for _ in range(3)]
+    R = V[:, :, :3]  # Q's tokens
+    w, pos, f = torch.ones(8, dtype=dt, device=dev), torch.arange(3, device=dev), ts.rope_frequencies(8, device=dev)
+    odd, big = (torch.zeros(1, 1, 3, d, dtype=dt, device=dev) for d in (7, 258))
+    ones, narrow = torch.ones(258, dtype=dt, device=dev), w.to(torch.bfloat16)
     return [
         (x, (Q[0], K, V)), (x, (Q, K, V[:, :, :4])), (x, (Q[:1], K, V)), (x, (Q[..., :4], K, V)), (x, (Q[:, :3], K, V)),
-        (x, (Q, K[:, :0], V[:, :0])), (x, (Q.float(), K, V)), (x, (Q.int(), K.int(), V.int())),
+        (x, (Q, K[:, :0], V[:, :0])), (x, (Q.to(other), K, V)), (x, (Q.int(), K.int(), V.int())),
         (x, (Q, K, V, None, 0.0)), (x, (Q, K, V, None, -1.0)), (x, (Q, K, V, None, float("nan"))),
-        (x, (Q, K, V, torch.tensor([1]))), (x, (Q, K, V, torch.tensor([1.0, 2.0]))), (x, (Q, K, V, torch.ones(2, 1).int())),
-        (x, tuple(torch.zeros(1, 1, 2, 129, dtype=F64) for _ in range(3))), (x, (Q[..., :0], K[..., :0], V[..., :0])),
+        (x, (Q, K, V, None, float("inf"))), (x, (Q, K, V, i(1))), (x, (Q, K, V, i(1.0, 2.0))),
+        (x, (Q, K, V, i(1, 1).int().view(2, 1))), (x, tuple(wide)), (x, (Q[..., :0], K[..., :0], V[..., :0])),
         (s, (Q, p[:1], p[:1], K, V)), (s, (Q, p, p[:, :2], K, V)), (s, (Q, p[..., :4], p[..., :4], K, V)),
-        (s, (Q, K, V, K, V)), (s, (Q, p.float(), p.float(), K, V)), (s, (Q.clone().requires_grad_(), p, p, K, V)),
-        (s, (Q, p, p, K, V, torch.tensor([1, 2, 3]))),
-    ] + rope_refusals()
-
-
-def rope_refusals():
-    Q, K, _ = heads(2, 4, 2, 3, 3, 8)
-    w, pos, f, n = torch.ones(8, dtype=F64), torch.arange(3), ts.rope_frequencies(8), ts.qk_norm_rope
-    odd, big = (torch.zeros(1, 1, 3, d, dtype=F64) for d in (7, 258))
-    return [
-        (n, (Q[0], K[0], w, w, pos, f)), (n, (Q, K[:, :, :2], w, w, pos, f)), (n, (Q, K.float(), w, w, pos, f)),
-        (n, (Q, K, w[:4], w, pos, f)), (n, (Q, K, w, w.float(), pos, f)), (n, (Q.half(), K.half(), w, w, pos, f)),
-        (n, (odd, odd, w[:7], w[:7], pos, f[:2])), (n, (big, big, torch.ones(258), torch.ones(258), pos, f)),
-        (n, (Q, K, w, w, pos, ts.rope_frequencies(10))), (n, (Q, K, w, w, pos, f.view(2, 2))), (n, (Q, K, w, w, pos, pos)),
-        (n, (Q, K, w, w, pos.float(), f)), (n, (Q, K, w, w, pos[:2], f)), (n, (Q, K, w, w, pos.view(1, 3), f)),
-        (n, (Q, K, w, w, pos, f, -1.0)), (n, (Q, K, w, w, pos, f, float("nan"))),
+        (s, (Q, K, V, K, V)), (s, (Q, p.to(other), p.to(other), K, V)), (s, (Q.clone().requires_grad_(), p, p, K, V)),
+        (s, (Q, p, p, K, V, i(1, 2, 3))), (s, (Q, p, p, K, V, None, 0.0)),
+        (n, (Q[0], R[0], w, w, pos, f)), (n, (Q, R[:, :, :2], w, w, pos, f)), (n, (Q, R.to(other), w, w, pos, f)),
+        (n, (Q, R, w[:4], w, pos, f)), (n, (Q, R, w, narrow, pos, f)), (n, (Q, R, narrow, narrow, pos, f)),
+        (n, (odd, odd, w[:7], w[:7], pos, f[:2])), (n, (big, big, ones, ones, pos, f)),
+        (n, (Q, R, w, w, pos, ts.rope_frequencies(10, device=dev))), (n, (Q, R, w, w, pos, f.view(2, 2))),
+        (n, (Q, R, w, w, pos, pos)), (n, (Q, R, w, w, pos.float(), f)), (n, (Q, R, w, w, pos[:2], f)),
+        (n, (Q, R, w, w, pos.view(1, 3), f)), (n, (Q, R, w, w, pos, f, -1.0)), (n, (Q, R, w, w, pos, f, float("nan"))),
     ]
 
 
 @pytest.mark.parametrize("i", range(len(refusals())))
 def test_refusals(pytorch_backend, i):
     f, args = refusals()[i]
+    with pytest.raises(RuntimeError):
+        f(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(refusals())))
+def test_refusals_on_the_gpu(hip_backend, i):
+    """The HIP operators refuse the same calls, on the host."""
+    f, args = refusals(torch.float32, torch.float16, "cuda")[i]
     with pytest.raises(RuntimeError):
         f(*args)
 

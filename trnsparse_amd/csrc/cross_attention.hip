@@ -76,6 +76,17 @@ int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st) {
   });
 }
 
+int launch_fwd_joint(int dtype, FwdArgs a, const FwdArgs& first, hipStream_t st) {
+  a.tiles = a.nsplit = 1;
+  const int64_t grid = grid_of(a);
+  if (grid > INT32_MAX) return fail(TSP_EUNSUPPORTED, "attention: too large a grid");
+  return with_tile(dtype, a.D, [&](auto tile) {
+    typedef decltype(tile) T;
+    hipLaunchKernelGGL((fwd_joint<T>), dim3((unsigned)grid), dim3(256), 0, st, a, first);
+    return check_launch("attention launch");
+  });
+}
+
 int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st) {
   set_plan(a, pa);
   set_plan(b, pb);

@@ -217,21 +217,28 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
   put(dv, ov, pk ? pk + krows * a.D : nullptr, 1.f);
 }
 
-// Sums of the parts of `rows` rows in order, rounded once: 32 lanes to a row.
+// Sums of the parts of each result's rows in order, rounded once: 32 lanes to a
+// row; blockIdx.y is the result (dQ, dK, dV; no rows where there is one part).
 struct SumArgs {
   const float* part;
   int64_t rows, stride;  // floats between parts
-  int nsplit, D, heads;
+  int nsplit, heads;
   int64_t S;
   Operand out;
 };
+struct SumsArgs {
+  SumArgs of[3];
+  int D;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void sum_parts(const SumArgs a) {
+__global__ __launch_bounds__(256) void sum_parts(const SumsArgs all) {
+  const SumArgs& a = all.of[blockIdx.y];
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int d = 4 * (threadIdx.x & 31);
-  if (row >= a.rows || d >= a.D) return;
+  if (row >= a.rows || d >= all.D) return;
   f32x4 sum = f32x4{};
-  for (int j = 0; j < a.nsplit; ++j) sum += *(const f32x4*)(a.part + j * a.stride + row * a.D + d);
+#pragma unroll 4
+  for (int j = 0; j < a.nsplit; ++j) sum += *(const f32x4*)(a.part + j * a.stride + row * all.D + d);
   const int64_t i = row % a.S, bh = row / a.S;
   T::store4((char*)a.out.p + bh / a.heads * a.out.b + bh % a.heads * a.out.h + i * a.out.s + d * T::ESZ, sum);
 }
@@ -278,18 +285,16 @@ int run_t(const BwdPlan& p, const BwdArgs& b, hipStream_t st) {
     hipLaunchKernelGGL((column_pass<T, N>), dim3((unsigned)g2), dim3(256), 0, st, b);
     if ((rc = check_launch("column_pass launch"))) return rc;
   }
-  auto sum = [&](const float* part, int64_t rows, int64_t stride, int n, int heads, int64_t S, const Operand& out) {
-    const SumArgs s{part, rows, stride, n, a.D, heads, S, out};
-    hipLaunchKernelGGL((sum_parts<T>), dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, st, s);
-    return check_launch("sum_parts launch");
-  };
-  const int64_t krows = units * a.L;
-  if (p.nsplit > 1 && (rc = sum(b.qpart, a.prows, a.prows * a.D, p.nsplit, a.Hkv * a.G, a.Sq, b.dQ))) return rc;
-  if (p.ksplit > 1 && g2 > 0) {
-    if ((rc = sum(b.kpart, krows, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dK))) return rc;
-    if ((rc = sum(b.kpart + krows * a.D, krows, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dV))) return rc;
-  }
-  return TSP_OK;
+  const int64_t krows = units * a.L, qsum = p.nsplit > 1 ? a.prows : 0, ksum = p.ksplit > 1 && g2 > 0 ? krows : 0;
+  const int64_t most = qsum > ksum ? qsum : ksum;
+  if (most == 0) return TSP_OK;
+  SumsArgs s{};
+  s.D = a.D;
+  s.of[0] = SumArgs{b.qpart, qsum, a.prows * a.D, p.nsplit, a.Hkv * a.G, a.Sq, b.dQ};
+  s.of[1] = SumArgs{b.kpart, ksum, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dK};
+  s.of[2] = SumArgs{b.kpart + krows * a.D, ksum, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dV};
+  hipLaunchKernelGGL((sum_parts<T>), dim3((unsigned)ceil_div(most, 8), 3), dim3(256), 0, st, s);
+  return check_launch("sum_parts launch");
 }
 
 // zeros in a strided result

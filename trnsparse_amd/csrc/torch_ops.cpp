@@ -570,7 +570,9 @@ void cross_shapes(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
   need_4d(Q, Q, who, "Q");
   need_4d(K, Q, who, "K");
   need_4d(V, Q, who, "V");
-  TORCH_CHECK(K.sizes() == V.sizes() && K.size(0) == Q.size(0), who, ": K and V must be one shape, with Q's batch");
+  TORCH_CHECK(K.sizes() == V.sizes() && K.size(0) == Q.size(0), who, ": Q ", Q.sizes(), ", K ", K.sizes(), " and V ",
+              V.sizes(), " do not belong together");
+  TORCH_CHECK(Q.size(3) >= 1 && Q.size(3) <= 128, who, ": head_dim ", Q.size(3), " is not in 1 .. 128");
   TORCH_CHECK(K.size(1) > 0 && Q.size(1) % K.size(1) == 0, who, ": ", Q.size(1), " query heads do not divide over ",
               K.size(1), " key heads");
 }
@@ -666,8 +668,8 @@ at::Tensor prefix_attn_fwd(const at::Tensor& Q_, const at::Tensor& PK_, const at
   const char* who = "prefix_attn_fwd";
   const c10::DeviceGuard guard(Q_.device());
   cross_shapes(Q_, K_, V_, who);
-  TORCH_CHECK(PK_.dim() == 3 && PK_.sizes() == PV_.sizes() && PK_.size(0) == K_.size(1), who,
-              ": the prefix must be (kv_heads, prefix, head_dim) like K's heads");
+  TORCH_CHECK(PK_.dim() == 3 && PK_.sizes() == PV_.sizes() && PK_.size(0) == K_.size(1), who, ": prefix_K ",
+              PK_.sizes(), " and prefix_V ", PV_.sizes(), " must be (kv_heads, prefix, head_dim)");
   const int code = attn_dtype(Q_.scalar_type(), who);
   const auto pk4 = PK_.unsqueeze(0), pv4 = PV_.unsqueeze(0);
   need_4d(pk4, Q_, who, "prefix K");

@@ -211,6 +211,75 @@ struct Narrow {
     join(a, ub, hk, split, x, lds, w, h, l32, live);
   }
 
+  // One range over two sets of keys, the first shared by the batch: for sets so
+  // short that joining two results would cost more than reading the first again.
+  static __device__ inline void run_joint(const FwdArgs& a, const FwdArgs& first, uint32_t block, uint8_t* lds) {
+    int64_t unit, item;
+    if (!head_item(block, 1, (int64_t)a.units_b * a.Hkv, unit, item)) return;
+    const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int l32 = lane & 31;
+    const bool live = l32 < a.R;
+    const RowId id = row_id(a, ub, hk, live ? l32 : 0);
+
+    const int64_t P = first.L, n = unit_length(a, ub), sees = a.causal ? n - (a.Sq - 1 - id.i) : n;
+    const int np = (int)ceil_div(P, 32), nst = np + (int)ceil_div(n, 32), mine = nst > w ? (nst - w + NW - 1) / NW : 0;
+    const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
+    const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
+    const char* Kf = first.K.p + hk * first.K.h;
+    const char* Vf = first.V.p + hk * first.V.h;
+    St ks, vs, kf, vf;
+    ks.init(0, lane, a.K.s, a.D);
+    vs.init(0, lane, a.V.s, a.D);
+    kf.init(0, lane, first.K.s, a.D);
+    vf.init(0, lane, first.V.s, a.D);
+    const uint32_t kst = dma::lds_addr(lds) + w * 2 * HBYTES, vst = kst + HBYTES;
+    auto stage = [&](int s) { return s * NW + w; };
+    auto issue_k = [&](int s) {
+      const int t = stage(s);
+      if (t < np)
+        kf.issue(Kf, 32 * (int64_t)t, P, first.K.s, a.D, kst, 0);
+      else
+        ks.issue(Kp, 32 * (int64_t)(t - np), n, a.K.s, a.D, kst, 0);
+    };
+    auto issue_v = [&](int s) {
+      const int t = stage(s);
+      if (t < np)
+        vf.issue(Vf, 32 * (int64_t)t, P, first.V.s, a.D, vst, 0);
+      else
+        vs.issue(Vp, 32 * (int64_t)(t - np), n, a.V.s, a.D, vst, 0);
+    };
+    if (mine > 0) {
+      issue_k(0);
+      issue_v(0);
+    }
+    typename T::Rows q;
+    T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
+    const typename T::Lane ln = T::lane_of(lane);
+    RowState<T> x;
+    x.clear();
+    for (int s = 0; s < mine; ++s) {
+      const bool more = s + 1 < mine, own = stage(s) >= np;
+      const int64_t at = 32 * (int64_t)(own ? stage(s) - np : stage(s)), end = own ? n : P;
+      dma::wait_vm<St::NI>();
+      fence();
+      softmax_stage<T, 1>(x, q, kst, vst, ln, h, a.scale_log2, (own && a.causal) || at + 32 > end,
+                          keys_from(own ? sees : P, end, at), [&] {
+                            drained();
+                            if (more) {
+                              issue_k(s + 1);
+                              dma::wait_vm<St::NI>();
+                            } else {
+                              dma::wait_vm<0>();
+                            }
+                            fence();
+                          });
+      drained();
+      if (more) issue_v(s + 1);
+    }
+    join(a, ub, hk, 0, x, lds, w, h, l32, live);
+  }
+
   static __device__ inline void fence() { asm volatile("" ::: "memory"); }
   static __device__ inline void drained() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
@@ -269,6 +338,11 @@ template <typename T>
 __global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_narrow(const FwdArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[Kernels<T>::N::LDS];
   Kernels<T>::N::run(a, blockIdx.x, lds);
+}
+template <typename T>
+__global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_joint(const FwdArgs a, const FwdArgs first) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Kernels<T>::N::LDS];
+  Kernels<T>::N::run_joint(a, first, blockIdx.x, lds);
 }
 // Two sets of keys in one launch: the first `grid0` workgroups take the first.
 template <typename T>
@@ -343,6 +417,7 @@ struct Plan {
 };
 Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want);
 int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st);
+int launch_fwd_joint(int dtype, FwdArgs a, const FwdArgs& first, hipStream_t st);
 int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st);
 int launch_combine(int dtype, const CombineArgs& a, hipStream_t st);
 

@@ -504,8 +504,14 @@ def block_sparse_attention_tiled(
 # counterpart in the reference.
 
 
+def _default_scale(Q: torch.Tensor) -> float:
+    d = Q.shape[-1] if Q.dim() else 0
+    return d**-0.5 if d else 1.0  # (an empty head_dim is refused)
+
+
 def _check_heads(who: str, Q, K, V, lengths, scale: float) -> None:
-    """Shapes and types of (batch, heads, rows, head_dim) operands; on both backends."""
+    """Shapes and types of (batch, heads, rows, head_dim) operands. The HIP
+    operators refuse the same calls themselves (csrc/torch_ops.cpp)."""
     q, k, v, dt = Q.shape, K.shape, V.shape, Q.dtype
     if not (len(q) == len(k) == len(v) == 4):
         raise RuntimeError(f"{who}: Q, K, V must be (batch, heads, rows, head_dim), got {tuple(q)}, {tuple(k)}, {tuple(v)}")
@@ -590,12 +596,12 @@ def cross_attention(
     has Q's order of heads and rows. Differentiable in Q, K and V.
     """
     if scale is None:
-        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0  # (such shapes are refused below)
-    _check_heads("cross_attention", Q, K, V, key_lengths, scale)
+        scale = _default_scale(Q)
     if _use_hip():
         from .hip.dispatch import hip_cross_attention
 
         return hip_cross_attention(Q, K, V, key_lengths, scale)
+    _check_heads("cross_attention", Q, K, V, key_lengths, scale)
     seen = None
     if key_lengths is not None:
         at = torch.arange(K.shape[2], device=Q.device)
@@ -628,7 +634,13 @@ def shared_prefix_attention(
     """
     who = "shared_prefix_attention"
     if scale is None:
-        scale = Q.shape[-1] ** -0.5 if Q.dim() and Q.shape[-1] else 1.0  # (such shapes are refused below)
+        scale = _default_scale(Q)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (Q, prefix_K, prefix_V, K, V)):
+        raise RuntimeError(f"{who} has no gradients: call it under torch.no_grad()")
+    if _use_hip():
+        from .hip.dispatch import hip_shared_prefix_attention
+
+        return hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale)
     _check_heads(who, Q, K, V, lengths, scale)
     want = (K.shape[1], K.shape[3])
     if prefix_K.dim() != 3 or prefix_K.shape != prefix_V.shape or (prefix_K.shape[0], prefix_K.shape[2]) != want:
@@ -636,12 +648,6 @@ def shared_prefix_attention(
                            f"({want[0]}, prefix, {want[1]})")
     if not (prefix_K.dtype == prefix_V.dtype == Q.dtype):
         raise RuntimeError(f"{who}: the prefix must have Q's dtype {Q.dtype}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (Q, prefix_K, prefix_V, K, V)):
-        raise RuntimeError(f"{who} has no gradients: call it under torch.no_grad()")
-    if _use_hip():
-        from .hip.dispatch import hip_shared_prefix_attention
-
-        return hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale)
     B, _, N, _ = Q.shape
     if Q.numel() == 0:
         return Q * 1
@@ -703,6 +709,10 @@ def qk_norm_rope(
     float32, bfloat16 and float16 on the HIP backend, head_dim even and at most
     256. Differentiable in Q, K and the weights.
     """
+    if _use_hip():
+        from .hip.dispatch import hip_qk_norm_rope
+
+        return hip_qk_norm_rope(Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved)
     who = "qk_norm_rope"
     if Q.dim() != 4 or K.dim() != 4 or (K.shape[0], K.shape[2], K.shape[3]) != (Q.shape[0], Q.shape[2], Q.shape[3]):
         raise RuntimeError(f"{who}: Q {tuple(Q.shape)} and K {tuple(K.shape)} must be (batch, heads, tokens, head_dim)")
@@ -721,10 +731,6 @@ def qk_norm_rope(
         raise RuntimeError(f"{who}: positions must be ({S},) or ({B}, {S}) of int32 or int64")
     if not eps >= 0:
         raise RuntimeError(f"{who}: eps must not be negative")
-    if _use_hip():
-        from .hip.dispatch import hip_qk_norm_rope
-
-        return hip_qk_norm_rope(Q, K, q_weight, k_weight, positions, inv_freq, eps, interleaved)
     angle = (positions.to(Q.device).double().unsqueeze(-1) * inv_freq.to(Q.device).double()).expand(B, S, -1).unsqueeze(1)
     cos, sin, rot = angle.cos(), angle.sin(), 2 * inv_freq.numel()
     return tuple(_norm_rope_pytorch(x, w, cos, sin, rot, eps, interleaved) for x, w in ((Q, q_weight), (K, k_weight)))
