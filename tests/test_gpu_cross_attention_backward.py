@@ -10,8 +10,9 @@ lse) with s off by (D + 4) e smax and lse by as much and (2 L + 64) e (sum and
 logarithm) and 4 e |lse|; dO V^T and D, sums of D products, D e of their
 scale, and again for their rounding when subtracted; the sums over L keys or
 R = G N rows, one e a term.
-fp16 gradients below its normal range are off by half a step, 2^-25, and so is
-each of dS's terms there: 2^-25 sum |K| (or |Q|) scale.
+fp16 gradients below its normal range are off by half a step, 2^-25, and so are
+the terms of P and dS there, which are formed with dO near 1: 2^-25 sum |K| (or
+|Q|) scale max |dO|.
 """
 
 from __future__ import annotations
@@ -49,6 +50,8 @@ def check_backward(Q, K, V, lengths=None, scale=None, dO=None, seed=50):
     low = 2.0**-25 if Q.dtype == HF else 0.0
     sumK = (K.double().cpu().nan_to_num(0, 0, 0).abs() * ok).sum(2, keepdim=True).repeat_interleave(G, 1) * sc
     sumQ = Q.double().cpu().abs().reshape(B, H // G, G * N, D).sum(2, keepdim=True) * sc
+    top = 2 * float(dO.abs().max())
+    sumK, sumQ = sumK * top, sumQ * top
     sumG = dO.double().cpu().abs().reshape(B, H // G, G * N, D).sum(2, keepdim=True)
     for got, like, k, terms, extra in zip(grads, (Q, K, V), ("Q", "K", "V"), (L, G * N, G * N), (sumK, sumQ, sumG)):
         assert got.shape == like.shape and got.dtype == like.dtype
@@ -160,3 +163,17 @@ def test_repeats_are_equal(hip_backend):
         grads = torch.autograd.grad(ts.cross_attention(Q, K, V), (Q, K, V), torch.ones_like(Q))
         first = first or grads
         assert all(torch.equal(a, b) for a, b in zip(first, grads))
+
+
+@pytest.mark.parametrize("size", [2.0**-16, 2.0**-8, 2.0**10])
+@pytest.mark.parametrize("N", [3, 200])
+def test_fp16_gradients_of_any_size(hip_backend, size, N):
+    """fp16 gradients far below 1 (an unscaled loss) and far above (a scaled
+    one): dS is formed with dO brought near 1, so what is lost is the rounding of
+    the results alone. Same bounds; rows of dO of different sizes in one tile."""
+    g = torch.Generator(device="cuda").manual_seed(60)
+    Q, K, V = make(2, 4, 2, N, 700, 64, HF, seed=10)
+    dO = size * torch.randn(2, 4, N, 64, device="cuda", generator=g)
+    dO = (dO * 2.0 ** -(torch.arange(N, device="cuda") % 5).view(N, 1)).to(HF)
+    check_backward(Q, K, V, dO=dO)
+    check_backward(Q, K, V, dO=torch.zeros_like(dO))

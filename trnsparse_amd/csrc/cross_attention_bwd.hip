@@ -35,6 +35,7 @@ struct BwdArgs {
   Operand dQ, dK, dV;  // written
   const float* lse;
   float *stat;         // (2, rows): log2(e) lse, D
+  float *gmax;         // fp16: (units, tiles, 4) largest |dO| of each wavefront's rows
   float *qpart;        // (nsplit, rows, D), null with one range
   float *kpart;        // (ksplit, 2, batch * kv_heads * keys, D), null with one range
   int ktiles, ksplit, per;  // column pass: key tiles, ranges of `per` stages
@@ -53,7 +54,7 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
   const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
   const int r = tile * 128 + w * 32 + l32;
-  const bool live = r < a.R;
+  const bool live = r < a.R, some = tile * 128 + w * 32 < a.R;
   const RowId id = row_id(a, ub, hk, live ? r : 0);
   auto row_of = [&](const Operand& x) { return x.p + id.b * x.b + id.head * x.h + id.i * x.s; };
 
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
   typename T::Rows q, g;
   T::load(q, row_of(a.Q), live, a.D, h);
   T::load(g, row_of(b.dO), live, a.D, h);
-  float Dr, rq;
+  float Dr, rq, out_scale = b.scale;
   {
     typename T::Rows o;
     T::load(o, row_of(b.O), live, a.D, h);
@@ -87,6 +88,19 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
       b.stat[a.prows + id.orow] = Dr;
     }
   }
+  if constexpr (T::SHORT_RANGE) {
+    // dS in fp16: with each row's dO near 1 it neither leaves fp16's range where
+    // the loss is scaled up nor loses its digits where gradients are small. A
+    // power of two, so nothing is rounded by it.
+    float mx = halves_max(T::largest(g));
+    const float c = unit_scale(mx);
+    T::scale(g, c);
+    Dr *= c;
+    out_scale = b.scale * unit_scale(c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    if (split == 0 && lane == 0) b.gmax[(unit * a.tiles + tile) * 4 + w] = mx;
+  }
   f32x16 acc[T::NU];
 #pragma unroll
   for (int u = 0; u < T::NU; ++u) acc[u] = f32x16{};
@@ -94,6 +108,7 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
     dma::wait_vm<0>();
     dma::barrier();
     if (s + 1 < nst) issue(s + 1);
+    if (!some) continue;
     const int keys = (int)(k1 - k0 - (int64_t)s * HK < HK ? k1 - k0 - (int64_t)s * HK : HK);
     const uint32_t st = lds0 + (s & 1) * STAGE;
     f32x16 sc[NT], dp[NT];
@@ -121,9 +136,9 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
   T::quads(acc, h, [&](int d, f32x4 v) {
     if (d >= a.D) return;
     if (part)
-      *(f32x4*)(part + d) = v * b.scale;
+      *(f32x4*)(part + d) = v * out_scale;
     else
-      T::store4(out + d * T::ESZ, v * b.scale);
+      T::store4(out + d * T::ESZ, v * out_scale);
   });
 }
 
@@ -139,6 +154,7 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
   const int64_t n = unit_length(a, ub);
   const int64_t key = (int64_t)tile * 128 + w * 32 + l32;
+  const bool some = (int64_t)tile * 128 + w * 32 < n;
 
   const int spg = (int)ceil_div(a.Sq, HQ), total = a.G * spg;  // stages of a head, of the group
   const int s0 = split * b.per, s1 = s0 + b.per < total ? s0 + b.per : total;
@@ -164,6 +180,15 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
   typename T::Rows k, v;
   T::load(k, a.K.p + ub * a.K.b + hk * a.K.h + key * a.K.s, key < n, a.D, h);
   T::load(v, a.V.p + ub * a.V.b + hk * a.V.h + key * a.V.s, key < n, a.D, h);
+  float c = 1.f;
+  if constexpr (T::SHORT_RANGE) {  // as in the row pass, one factor for the rows of the unit
+    float mx = 0.f;
+    for (int e = lane; e < a.tiles * 4; e += 64) mx = fmaxf(mx, b.gmax[unit * a.tiles * 4 + e]);
+    mx = halves_max(mx);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    c = unit_scale(mx);
+  }
   f32x16 dk[T::NU], dv[T::NU];
 #pragma unroll
   for (int u = 0; u < T::NU; ++u) dk[u] = dv[u] = f32x16{};
@@ -171,6 +196,7 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
     dma::wait_vm<0>();
     dma::barrier();
     if (s + 1 < nst) issue(s + 1);
+    if (!some) continue;
     const uint32_t st = lds0 + (s & 1) * STAGE;
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
@@ -180,14 +206,15 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
       T::template scores<1>(dp, at + HBYTES, ln, v);
       typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t x = st + 2 * HBYTES + 4 * (32 * t + 8 * c + 4 * h);
-        const f32x4 rq = *(const lds_f32x4*)(uintptr_t)x, Dr = *(const lds_f32x4*)(uintptr_t)(x + 256);
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t sa = st + 2 * HBYTES + 4 * (32 * t + 8 * x + 4 * h);
+        const f32x4 rq = *(const lds_f32x4*)(uintptr_t)sa, Dr = *(const lds_f32x4*)(uintptr_t)(sa + 256);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][4 * c + e], a.scale_log2, -rq[e]));
-          sc[0][4 * c + e] = p;
-          dp[0][4 * c + e] = p * (dp[0][4 * c + e] - Dr[e]);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][4 * x + e], a.scale_log2, -rq[e]));
+          sc[0][4 * x + e] = p;
+          const float ds = p * (dp[0][4 * x + e] - Dr[e]);
+          dp[0][4 * x + e] = T::SHORT_RANGE ? ds * c : ds;
         }
       }
       typename T::template Prob<1> P, dS;
@@ -213,7 +240,7 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
         T::store4(o + d * T::ESZ, y);
     });
   };
-  put(dk, ok, pk, b.scale);
+  put(dk, ok, pk, b.scale * unit_scale(c));
   put(dv, ov, pk ? pk + krows * a.D : nullptr, 1.f);
 }
 
@@ -246,7 +273,8 @@ __global__ __launch_bounds__(256) void sum_parts(const SumsArgs all) {
 struct BwdPlan {
   int tiles, nsplit, ktiles, ksplit, per;
   int64_t chunk;
-  int64_t stat, qpart, kpart;  // bytes
+  int64_t stat, gmax, qpart, kpart;  // bytes
+  int64_t bytes() const { return stat + gmax + qpart + kpart; }
 };
 BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D) {
   BwdPlan p{};
@@ -266,6 +294,7 @@ BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int6
   if (p.ksplit < 1) p.ksplit = 1;
   const int64_t rows = B * Hq * Sq, up = 255;
   p.stat = (2 * rows * 4 + up) & ~up;
+  p.gmax = dtype == TSP_F16 ? (units * p.tiles * 16 + up) & ~up : 0;
   p.qpart = p.nsplit > 1 ? (p.nsplit * rows * D * 4 + up) & ~up : 0;
   p.kpart = p.ksplit > 1 ? p.ksplit * 2 * units * L * D * 4 : 0;
   return p;
@@ -322,7 +351,7 @@ extern "C" int64_t tsp_cross_attn_bwd_workspace_size(int dtype, int64_t B, int64
   if (xat::check_sizes("tsp_cross_attn_bwd_workspace_size", dtype, B, Hq, Hkv, Sq, L, D)) return -1;
   if (B * Hq * Sq == 0) return 0;
   const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D);
-  return p.stat + p.qpart + p.kpart;
+  return p.bytes();
 }
 
 extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* K, const int64_t* ks, const void* V,
@@ -362,7 +391,7 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
       return rc;
   if (!lse) return fail(TSP_EINVAL, "%s: null lse", who);
   const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D);
-  if (!workspace || workspace_bytes < p.stat + p.qpart + p.kpart)
+  if (!workspace || workspace_bytes < p.bytes())
     return fail(TSP_EINVAL, "%s: workspace too small", who);
   if (ceil_div(B * Hq * Sq, 8) > INT32_MAX || ceil_div(B * Hkv * L, 8) > INT32_MAX)
     return fail(TSP_EUNSUPPORTED, "%s: too many rows", who);
@@ -379,8 +408,10 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   b.dV = xat::operand(dV, cols ? dvs : none, dtype);
   b.lse = lse;
   b.stat = (float*)workspace;
-  if (p.qpart) b.qpart = (float*)((char*)workspace + p.stat);
-  if (p.kpart) b.kpart = (float*)((char*)workspace + p.stat + p.qpart);
+  char* at = (char*)workspace + p.stat;
+  if (p.gmax) b.gmax = (float*)at;
+  if (p.qpart) b.qpart = (float*)(at + p.gmax);
+  if (p.kpart) b.kpart = (float*)(at + p.gmax + p.qpart);
   b.ktiles = p.ktiles, b.ksplit = p.ksplit, b.per = p.per;
   b.scale = (float)scale;
   a.prows = B * Hq * Sq;

@@ -104,7 +104,7 @@ struct Wide {
     const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int r = tile * 128 + w * 32 + (lane & 31);
-    const bool live = r < a.R;
+    const bool live = r < a.R, some = tile * 128 + w * 32 < a.R;  // this row, a row of the wavefront's
     const RowId id = row_id(a, ub, hk, live ? r : 0);
 
     typename T::Rows q;
@@ -133,6 +133,7 @@ struct Wide {
       dma::wait_vm<0>();
       dma::barrier();
       if (s + 1 < nst) issue(s + 1);
+      if (!some) continue;
       const int64_t at = k0 + (int64_t)s * HK;
       const uint32_t st = lds0 + (s & 1) * STAGE;
       softmax_stage<T, NT>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,

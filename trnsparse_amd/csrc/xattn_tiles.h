@@ -21,6 +21,8 @@
 #include "common.h"
 #include "lds_dma.h"
 
+#include <type_traits>
+
 namespace tsp {
 namespace xat {
 
@@ -49,6 +51,12 @@ __device__ inline float halves_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The power of two that brings x > 0 into [1, 2); 1 for zero, infinity and NaN.
+__device__ inline float unit_scale(float x) {
+  const uint32_t e = __float_as_uint(x) >> 23;
+  return e == 0 || e >= 254 ? 1.f : __uint_as_float((254u - e) << 23);
+}
+
 // ---------------------------------------------------------------- 16 bit
 template <typename E, int DP_>
 struct Tile16 {
@@ -56,6 +64,7 @@ struct Tile16 {
   typedef E vec8 __attribute__((ext_vector_type(8)));
   typedef E vec4 __attribute__((ext_vector_type(4)));
   static constexpr int DP = DP_, ESZ = 2, CE = 8;  // CE: elements of a 16-byte chunk
+  static constexpr bool SHORT_RANGE = std::is_same<E, _Float16>::value;  // of exponents: 2^-24 to 2^16
   static constexpr int ROWB = DP * 2, CPR = ROWB / 16, KS = DP / 16, NU = DP / 32;
   struct Rows {
     vec8 f[KS];
@@ -73,6 +82,21 @@ struct Tile16 {
 #pragma unroll
       for (int i = 0; i < 8; ++i) t += (float)a.f[s][i] * (float)b.f[s][i];
     return t;
+  }
+
+  static __device__ inline float largest(const Rows& a) {
+    float t = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf((float)a.f[s][i]));
+    return t;
+  }
+  static __device__ inline void scale(Rows& a, float c) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a.f[s][i] = (E)((float)a.f[s][i] * c);
   }
 
   // LDS addresses of one stage, formed once per stage
@@ -142,6 +166,7 @@ template <int DP_>
 struct Tile32 {
   typedef float elem;
   static constexpr int DP = DP_, ESZ = 4, CE = 4;
+  static constexpr bool SHORT_RANGE = false;
   static constexpr int ROWB = DP * 4, CPR = ROWB / 16, KT = DP / 8, NU = DP / 32;
   struct Rows {
     f32x4 f[KT];
