@@ -48,10 +48,10 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
   const FwdArgs& a = b.f;
   constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
-  int64_t unit, item;
-  if (!head_item(blockIdx.x, (int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-  const int tile = (int)(item % a.tiles), split = (int)(item / a.tiles);
-  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+  Item it;
+  if (!item_of(a, blockIdx.x, a.tiles, a.nsplit, it)) return;
+  const int tile = it.tile, split = it.split;
+  const int64_t unit = it.unit, ub = it.ub, hk = it.hk;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
   const int r = tile * 128 + w * 32 + l32;
   const bool live = r < a.R, some = tile * 128 + w * 32 < a.R;
@@ -147,10 +147,10 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
   const FwdArgs& a = b.f;
   constexpr int HQ = 32 * NQ, HBYTES = HQ * T::ROWB, STAGE = 2 * HBYTES + 1024;  // Q, dO, two numbers of each row
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
-  int64_t unit, item;
-  if (!head_item(blockIdx.x, (int64_t)b.ktiles * b.ksplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-  const int tile = (int)(item % b.ktiles), split = (int)(item / b.ktiles);
-  const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+  Item it;
+  if (!item_of(a, blockIdx.x, b.ktiles, b.ksplit, it)) return;
+  const int tile = it.tile, split = it.split;
+  const int64_t unit = it.unit, ub = it.ub, hk = it.hk;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
   const int64_t n = unit_length(a, ub);
   const int64_t key = (int64_t)tile * 128 + w * 32 + l32;
@@ -266,8 +266,10 @@ __global__ __launch_bounds__(256) void sum_parts(const SumsArgs all) {
   f32x4 sum = f32x4{};
 #pragma unroll 4
   for (int j = 0; j < a.nsplit; ++j) sum += *(const f32x4*)(a.part + j * a.stride + row * all.D + d);
-  const int64_t i = row % a.S, bh = row / a.S;
-  T::store4((char*)a.out.p + bh / a.heads * a.out.b + bh % a.heads * a.out.h + i * a.out.s + d * T::ESZ, sum);
+  int64_t bh, i, b, h;
+  split_row(row, a.S, bh, i);
+  split_row(bh, a.heads, b, h);
+  T::store4((char*)a.out.p + b * a.out.b + h * a.out.h + i * a.out.s + d * T::ESZ, sum);
 }
 
 struct BwdPlan {

@@ -45,6 +45,24 @@ struct FwdArgs {
   float scale_log2;
 };
 
+// What a workgroup takes: tile and range of a unit. The counts' product fits
+// int32 (checked by the host), so 32-bit divisions do.
+struct Item {
+  uint32_t unit, ub, hk;
+  int tile, split;
+};
+__device__ inline bool item_of(const FwdArgs& a, uint32_t block, int tiles, int nsplit, Item& x) {
+  int64_t unit, item;
+  if (!head_item(block, (int64_t)tiles * nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return false;
+  const uint32_t i = (uint32_t)item, u = (uint32_t)unit;
+  x.split = (int)(i / (uint32_t)tiles);
+  x.tile = (int)(i - (uint32_t)x.split * (uint32_t)tiles);
+  x.unit = u;
+  x.ub = u / (uint32_t)a.Hkv;
+  x.hk = u - x.ub * (uint32_t)a.Hkv;
+  return true;
+}
+
 struct RowId {
   int64_t b, head, orow;
   int i;
@@ -98,10 +116,10 @@ template <typename T, int NT>
 struct Wide {
   static constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES, LDS = 2 * STAGE;
   static __device__ inline void run(const FwdArgs& a, uint32_t block, uint8_t* lds) {
-    int64_t unit, item;
-    if (!head_item(block, (int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-    const int tile = (int)(item % a.tiles), split = (int)(item / a.tiles);
-    const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+    Item it;
+    if (!item_of(a, block, a.tiles, a.nsplit, it)) return;
+    const int tile = it.tile, split = it.split;
+    const int64_t ub = it.ub, hk = it.hk;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int r = tile * 128 + w * 32 + (lane & 31);
     const bool live = r < a.R, some = tile * 128 + w * 32 < a.R;  // this row, a row of the wavefront's
@@ -162,10 +180,10 @@ struct Narrow {
   typedef Stager<T, 32, 1> St;
 
   static __device__ inline void run(const FwdArgs& a, uint32_t block, uint8_t* lds) {
-    int64_t unit, item;
-    if (!head_item(block, a.nsplit, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-    const int split = (int)item;
-    const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+    Item it;
+    if (!item_of(a, block, 1, a.nsplit, it)) return;
+    const int split = it.split;
+    const int64_t ub = it.ub, hk = it.hk;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int l32 = lane & 31;
     const bool live = l32 < a.R;
@@ -215,9 +233,9 @@ struct Narrow {
   // One range over two sets of keys, the first shared by the batch: for sets so
   // short that joining two results would cost more than reading the first again.
   static __device__ inline void run_joint(const FwdArgs& a, const FwdArgs& first, uint32_t block, uint8_t* lds) {
-    int64_t unit, item;
-    if (!head_item(block, 1, (int64_t)a.units_b * a.Hkv, unit, item)) return;
-    const int64_t ub = unit / a.Hkv, hk = unit % a.Hkv;
+    Item it;
+    if (!item_of(a, block, 1, 1, it)) return;
+    const int64_t ub = it.ub, hk = it.hk;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int l32 = lane & 31;
     const bool live = l32 < a.R;
@@ -363,6 +381,17 @@ __global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_two(const FwdArgs
 // The ranges' results of every row in one: weights 2^(lse_j - max lse). Rows
 // that no range has keys for are zero with a log-sum-exp of -inf. 32 lanes to a
 // row, four values each.
+// row = bh * S + i
+__device__ inline void split_row(int64_t row, int64_t S, int64_t& bh, int64_t& i) {
+  if (((row | S) >> 32) == 0) {
+    const uint32_t q = (uint32_t)row / (uint32_t)S;
+    bh = q;
+    i = (uint32_t)row - q * (uint32_t)S;
+  } else {
+    bh = row / S;
+    i = row - bh * S;
+  }
+}
 struct CombineArgs {
   const float *part, *plse;
   int64_t prows;
@@ -403,8 +432,10 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
     }
   }
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-  const int64_t i = row % a.Sq, bh = row / a.Sq;
-  if (d < a.D) T::store4(a.O + bh / a.heads * a.ob + bh % a.heads * a.oh + i * a.os + d * T::ESZ, sum * inv);
+  int64_t bh, i, b, h;
+  split_row(row, a.Sq, bh, i);
+  split_row(bh, a.heads, b, h);
+  if (d < a.D) T::store4(a.O + b * a.ob + h * a.oh + i * a.os + d * T::ESZ, sum * inv);
   if (d == 0 && a.lse) a.lse[row] = (m + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
 }
 
