@@ -42,9 +42,10 @@ struct BwdArgs {
   float scale;
 };
 
+// FINE: P and dS as sums of two 16-bit numbers (see fine() below).
 // (fp32 at 128: Q, dO and dQ alone take 192 registers of a lane)
-template <typename T, int NT>
-__global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const BwdArgs b) {
+template <typename T, int NT, bool FINE>
+__global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(const BwdArgs b) {
   const FwdArgs& a = b.f;
   constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
@@ -61,6 +62,7 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
   const int64_t n = unit_length(a, ub);
   const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
   const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, HK) : 0;
+  const bool short_rows = FINE && a.nsplit == 1 && nst == 1;
   const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
   const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
   Stager<T, HK, 4> ks, vs;
@@ -85,9 +87,10 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
     rq = live ? b.lse[id.orow] * LOG2E : 0.f;
     if (live && split == 0 && h == 0) {
       b.stat[id.orow] = rq;
-      b.stat[a.prows + id.orow] = Dr;
+      if (!short_rows) b.stat[a.prows + id.orow] = Dr;
     }
   }
+  float back = 1.f;  // of dO's scale
   if constexpr (T::SHORT_RANGE) {
     // dS in fp16: with each row's dO near 1 it neither leaves fp16's range where
     // the loss is scaled up nor loses its digits where gradients are small. A
@@ -96,7 +99,8 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
     const float c = unit_scale(mx);
     T::scale(g, c);
     Dr *= c;
-    out_scale = b.scale * unit_scale(c);
+    back = unit_scale(c);
+    out_scale = b.scale * back;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
     if (split == 0 && lane == 0) b.gmax[(unit * a.tiles + tile) * 4 + w] = mx;
@@ -114,6 +118,21 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
     f32x16 sc[NT], dp[NT];
     T::template scores<NT>(sc, st, ln, q);
     T::template scores<NT>(dp, st + HBYTES, ln, g);
+    if (short_rows) {
+      // All of the row's keys are here: D = sum_j P_ij dP_ij, without the
+      // rounding of O, which of few keys is as large as dS (7 keys in bf16: dQ
+      // 1.6 times as far off as its own rounding, 1.4 this way).
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v], a.scale_log2, -rq));
+          if (32 * t + 8 * (v >> 2) + 4 * h + (v & 3) < keys) sum += p * dp[t][v];
+        }
+      Dr = halves_sum(sum);
+      if (live && h == 0) b.stat[a.prows + id.orow] = Dr * back;
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -126,9 +145,7 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
         for (int v = 0; v < 16; ++v)
           if (32 * t + 8 * (v >> 2) + 4 * h + (v & 3) >= keys) sc[t][v] = 0.f;
     }
-    typename T::template Prob<NT> p;
-    T::template pack<NT>(p, sc);
-    T::template outer<NT>(acc, st, ln, p);
+    T::template product<NT, FINE>(acc, st, ln, sc);
   }
   if (!live) return;
   char* out = (char*)row_of(b.dQ);
@@ -142,8 +159,8 @@ __global__ __launch_bounds__(256, T::ROWB > 256 ? 1 : 2) void row_pass(const Bwd
   });
 }
 
-template <typename T, int NQ>
-__global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const BwdArgs b) {
+template <typename T, int NQ, bool FINE>
+__global__ __launch_bounds__(256, T::ESZ == 4 || FINE ? 1 : 2) void column_pass(const BwdArgs b) {
   const FwdArgs& a = b.f;
   constexpr int HQ = 32 * NQ, HBYTES = HQ * T::ROWB, STAGE = 2 * HBYTES + 1024;  // Q, dO, two numbers of each row
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
@@ -217,11 +234,8 @@ __global__ __launch_bounds__(256, T::ESZ == 4 ? 1 : 2) void column_pass(const Bw
           dp[0][4 * x + e] = T::SHORT_RANGE ? ds * c : ds;
         }
       }
-      typename T::template Prob<1> P, dS;
-      T::template pack<1>(P, sc);
-      T::template pack<1>(dS, dp);
-      T::template outer<1>(dv, at + HBYTES, ln, P);
-      T::template outer<1>(dk, at, ln, dS);
+      T::template product<1, FINE>(dv, at + HBYTES, ln, sc);
+      T::template product<1, FINE>(dk, at, ln, dp);
     }
   }
   if (key >= a.L) return;
@@ -302,7 +316,16 @@ BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int6
   return p;
 }
 
-template <typename T>
+// P and dS rounded to 16 bits move a gradient as far as the rounding of its
+// result does: 1.41 times the error of that alone, of few rows or keys up to
+// 1.6. A sum of two 16-bit numbers leaves the result's own, for 4 products in
+// place of 3 in the row pass and 6 of 4 in the column pass. That is taken where
+// the matrix cores are not what a step waits for: 2 x 16 heads of 256 x 512 x
+// 128 45.9 us and 47.4 this way, 4 x 16 heads (2^30 products of the scores) 50.7
+// and 59.8, 4 x 32 heads of 4096 x 32 x 128 293.5 and 293.6.
+bool fine(int64_t rows, int64_t L, int64_t D) { return L <= 64 || rows * L <= (int64_t(1) << 29) / D; }
+
+template <typename T, bool FINE>
 int run_t(const BwdPlan& p, const BwdArgs& b, hipStream_t st) {
   const FwdArgs& a = b.f;
   const int64_t units = (int64_t)a.units_b * a.Hkv;
@@ -310,10 +333,10 @@ int run_t(const BwdPlan& p, const BwdArgs& b, hipStream_t st) {
   const int64_t g1 = head_grid((int64_t)p.tiles * p.nsplit, units), g2 = b.dK.p ? head_grid((int64_t)p.ktiles * p.ksplit, units) : 0;
   if (g1 > INT32_MAX || g2 > INT32_MAX) return fail(TSP_EUNSUPPORTED, "tsp_cross_attn_bwd: too large a grid");
   int rc;
-  hipLaunchKernelGGL((row_pass<T, N>), dim3((unsigned)g1), dim3(256), 0, st, b);
+  hipLaunchKernelGGL((row_pass<T, N, FINE>), dim3((unsigned)g1), dim3(256), 0, st, b);
   if ((rc = check_launch("row_pass launch"))) return rc;
   if (g2 > 0) {
-    hipLaunchKernelGGL((column_pass<T, N>), dim3((unsigned)g2), dim3(256), 0, st, b);
+    hipLaunchKernelGGL((column_pass<T, N, FINE>), dim3((unsigned)g2), dim3(256), 0, st, b);
     if ((rc = check_launch("column_pass launch"))) return rc;
   }
   const int64_t krows = units * a.L, qsum = p.nsplit > 1 ? a.prows : 0, ksum = p.ksplit > 1 && g2 > 0 ? krows : 0;
@@ -424,9 +447,13 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   a.L = L;
   a.tiles = p.tiles, a.nsplit = p.nsplit, a.chunk = p.chunk;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
-  const bool w = D > 64;
   using namespace xat;
-  if (dtype == TSP_BF16) return w ? run_t<Tile16<__bf16, 128>>(p, b, st) : run_t<Tile16<__bf16, 64>>(p, b, st);
-  if (dtype == TSP_F16) return w ? run_t<Tile16<_Float16, 128>>(p, b, st) : run_t<Tile16<_Float16, 64>>(p, b, st);
-  return w ? run_t<Tile32<128>>(p, b, st) : run_t<Tile32<64>>(p, b, st);
+  if (dtype == TSP_F32) return D > 64 ? run_t<Tile32<128>, false>(p, b, st) : run_t<Tile32<64>, false>(p, b, st);
+  auto run = [&](auto fn) {
+    constexpr bool F = decltype(fn)::value;
+    if (dtype == TSP_BF16)
+      return D > 64 ? run_t<Tile16<__bf16, 128>, F>(p, b, st) : run_t<Tile16<__bf16, 64>, F>(p, b, st);
+    return D > 64 ? run_t<Tile16<_Float16, 128>, F>(p, b, st) : run_t<Tile16<_Float16, 64>, F>(p, b, st);
+  };
+  return fine(a.prows, L, D) ? run(std::true_type{}) : run(std::false_type{});
 }

@@ -137,6 +137,14 @@ struct Tile16 {
         o.b[t][a] = __builtin_convertvector(x, vec8);
       }
   }
+  // p less what pack() kept of it
+  template <int NT>
+  static __device__ inline void rest(f32x16* p, const Prob<NT>& kept) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) p[t][v] -= (float)kept.b[t][v >> 3][v & 7];
+  }
   template <int NT>
   static __device__ inline void outer(f32x16* acc, uint32_t st, const Lane& ln, const Prob<NT>& p) {
     const uint32_t t0 = st + ln.t0, t1 = st + ln.t1;
@@ -148,6 +156,19 @@ struct Tile16 {
         for (int u = 0; u < NU; ++u)
           acc[u] = mfma16(__builtin_bit_cast(vec8, abw::lds_trp(t0, t1, u, (32 * t + 16 * a) * ROWB)), p.b[t][a],
                           acc[u]);
+  }
+  // acc += X^T p, with p in 16 bits or (TWICE) as the sum of two such numbers
+  template <int NT, bool TWICE>
+  static __device__ inline void product(f32x16* acc, uint32_t st, const Lane& ln, f32x16* p) {
+    Prob<NT> a;
+    pack<NT>(a, p);
+    outer<NT>(acc, st, ln, a);
+    if constexpr (TWICE) {
+      Prob<NT> b;
+      rest<NT>(p, a);
+      pack<NT>(b, p);
+      outer<NT>(acc, st, ln, b);
+    }
   }
   // f(d, four consecutive values at d) over the lane's part of its own row
   template <typename F>
@@ -229,6 +250,12 @@ struct Tile32 {
 #pragma unroll
         for (int u = 0; u < NU; ++u) acc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[u], p.b[t][s], acc[u], 0, 0, 0);
       }
+  }
+  template <int NT, bool>
+  static __device__ inline void product(f32x16* acc, uint32_t st, const Lane& ln, f32x16* p) {
+    Prob<NT> a;
+    pack<NT>(a, p);
+    outer<NT>(acc, st, ln, a);
   }
   template <typename F>
   static __device__ inline void quads(const f32x16* acc, int h, F&& f) {
