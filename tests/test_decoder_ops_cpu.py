@@ -25,6 +25,14 @@ def test_cross_attention(pytorch_backend, size):
     torch.testing.assert_close(ts.cross_attention(Q, K, V), r["O"], rtol=1e-12, atol=1e-12)
 
 
+def test_cross_attention_without_keys(pytorch_backend):
+    Q, K, V = heads(2, 2, 2, 3, 0, 8)
+    Q[0, 0, 0, 0] = float("inf")
+    Q.requires_grad_()
+    O = ts.cross_attention(Q, K, V)
+    assert (O == 0).all() and (torch.autograd.grad(O.sum(), Q)[0] == 0).all()
+
+
 def test_cross_attention_lengths(pytorch_backend):
     Q, K, V = heads(4, 4, 2, 3, 9, 8)
     lengths = torch.tensor([0, 1, 9, 20])
@@ -159,6 +167,8 @@ def test_c_abi_refusals():
     assert call(vs=st(64 * 64, 64, 0)) == -1  # rows on top of each other
     assert call(ks=st(0, 0, 1 << 24)) == -1  # rows 32 MiB apart
     assert call(scale=0.0) == -1 and call(scale=float("nan")) == -1 and call(it=5) == -1
+    assert call(scale=1e-40) == -1  # zero in fp32
+    assert call(H=2048, Hk=2048, N=1 << 20) == -2 and call(L=1 << 31) == -2 and call(B=1 << 31) == -2
     assert call(L=100000, ws=None) == -1 and b"workspace" in lib.tsp_last_error()
     assert call(L=100000, wsb=16) == -1
     assert call(B=0) == 0 and call(N=0) == 0  # nothing to do

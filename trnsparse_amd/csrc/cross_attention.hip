@@ -54,14 +54,6 @@ static int64_t grid_of(const FwdArgs& a) {
   return head_grid((int64_t)a.tiles * a.nsplit, (int64_t)a.units_b * a.Hkv);
 }
 
-// f.operator()<Tile>() for the operands' type and head_dim
-template <typename F>
-static int with_tile(int dtype, int D, F&& f) {
-  if (dtype == TSP_BF16) return D > 64 ? f(Tile16<__bf16, 128>{}) : f(Tile16<__bf16, 64>{});
-  if (dtype == TSP_F16) return D > 64 ? f(Tile16<_Float16, 128>{}) : f(Tile16<_Float16, 64>{});
-  return D > 64 ? f(Tile32<128>{}) : f(Tile32<64>{});
-}
-
 int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st) {
   set_plan(a, p);
   const int64_t grid = grid_of(a);
@@ -122,9 +114,10 @@ int check_sizes(const char* who, int dtype, int64_t B, int64_t Hq, int64_t Hkv, 
                 (long long)B, (long long)Hq, (long long)Hkv, (long long)Sq, (long long)L, (long long)D);
   if (D > 128 || D % (16 / esize(dtype)) != 0)
     return fail(TSP_EUNSUPPORTED, "%s: head_dim %lld (at most 128, whole 16-byte pieces)", who, (long long)D);
-  if (Sq > INT32_MAX || B * Hq > INT32_MAX || Hq * Sq > INT32_MAX || B * Hq * Sq > (int64_t(1) << 40) ||
-      L > (int64_t(1) << 40))
-    return fail(TSP_EUNSUPPORTED, "%s: too many rows", who);
+  // rows of a unit and keys are counted in 32 bits, tiles past the last included
+  const int64_t most = int64_t(1) << 30;
+  if (Sq > most || Hq > most || B > most || L > most || Hq * Sq > most || B * Hq > most || B * Hq * Sq > most * 256)
+    return fail(TSP_EUNSUPPORTED, "%s: too many rows or keys", who);
   return TSP_OK;
 }
 
@@ -156,7 +149,7 @@ extern "C" int tsp_cross_attn_fwd(const void* Q, const int64_t* qs, const void* 
     if ((rc = xat::check_operand(who, "K", K, ks, L, D, dtype))) return rc;
     if ((rc = xat::check_operand(who, "V", V, vs, L, D, dtype))) return rc;
   }
-  if (!(scale > 0) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
+  if (!(scale > 1e-30) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
   if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
   const int64_t need = tsp_cross_attn_workspace_size(dtype, B, Hq, Hkv, Sq, L, D);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);

@@ -389,7 +389,7 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   const hipStream_t st = (hipStream_t)stream;
   int rc = xat::check_sizes(who, dtype, B, Hq, Hkv, Sq, L, D);
   if (rc) return rc;
-  if (!(scale > 0) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
+  if (!(scale > 1e-30) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
   if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
   const bool rows = B * Hq * Sq > 0, keys = B * L > 0, cols = keys && (dK || dV);
   if (cols)
@@ -448,12 +448,11 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   a.tiles = p.tiles, a.nsplit = p.nsplit, a.chunk = p.chunk;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   using namespace xat;
-  if (dtype == TSP_F32) return D > 64 ? run_t<Tile32<128>, false>(p, b, st) : run_t<Tile32<64>, false>(p, b, st);
-  auto run = [&](auto fn) {
-    constexpr bool F = decltype(fn)::value;
-    if (dtype == TSP_BF16)
-      return D > 64 ? run_t<Tile16<__bf16, 128>, F>(p, b, st) : run_t<Tile16<__bf16, 64>, F>(p, b, st);
-    return D > 64 ? run_t<Tile16<_Float16, 128>, F>(p, b, st) : run_t<Tile16<_Float16, 64>, F>(p, b, st);
-  };
-  return fine(a.prows, L, D) ? run(std::true_type{}) : run(std::false_type{});
+  const bool two = fine(a.prows, L, D);
+  return with_tile(dtype, D, [&](auto tile) {
+    typedef decltype(tile) T;
+    if constexpr (T::ESZ == 2)
+      if (two) return run_t<T, true>(p, b, st);
+    return run_t<T, false>(p, b, st);
+  });
 }

@@ -62,6 +62,7 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
   int rc = xat::check_sizes(who, dtype, B, Hq, Hkv, Sq, P > S ? P : S, D);
   if (rc) return rc;
   if (B * Hq * Sq == 0) return TSP_OK;
+  if (B * Hq / Hkv * Sq > (int64_t(1) << 30)) return fail(TSP_EUNSUPPORTED, "%s: too many rows on a key head", who);
   if ((rc = xat::check_operand(who, "Q", Q, qs, Sq, D, dtype))) return rc;
   if ((rc = xat::check_operand(who, "O", O, os, Sq, D, dtype))) return rc;
   if (P > 0) {
@@ -72,7 +73,7 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
     if ((rc = xat::check_operand(who, "K", K, ks, S, D, dtype))) return rc;
     if ((rc = xat::check_operand(who, "V", V, vs, S, D, dtype))) return rc;
   }
-  if (!(scale > 0) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
+  if (!(scale > 1e-30) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
   if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
   const xat::PrefixPlan p = xat::prefix_plan(dtype, B, Hq, Hkv, Sq, P, S);
   const int64_t rows = B * Hq * Sq, need = p.nsplit * rows * (D + 1) * 4;

@@ -453,6 +453,16 @@ int launch_fwd_joint(int dtype, FwdArgs a, const FwdArgs& first, hipStream_t st)
 int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st);
 int launch_combine(int dtype, const CombineArgs& a, hipStream_t st);
 
+// f(tile) for the operands' type and head_dim.
+template <typename F>
+int with_tile(int dtype, int64_t D, F&& f) {
+  if (dtype == TSP_BF16)
+    return D > 96 ? f(Tile16<__bf16, 128>{}) : D > 64 ? f(Tile16<__bf16, 128, 96>{}) : f(Tile16<__bf16, 64>{});
+  if (dtype == TSP_F16)
+    return D > 96 ? f(Tile16<_Float16, 128>{}) : D > 64 ? f(Tile16<_Float16, 128, 96>{}) : f(Tile16<_Float16, 64>{});
+  return D > 96 ? f(Tile32<128>{}) : D > 64 ? f(Tile32<128, 96>{}) : f(Tile32<64>{});
+}
+
 // Checks of one strided operand; 0 or a status with a message.
 int check_operand(const char* who, const char* name, const void* p, const int64_t* strides, int64_t rows, int64_t D,
                   int dtype);

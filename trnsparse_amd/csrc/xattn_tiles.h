@@ -58,14 +58,16 @@ __device__ inline float unit_scale(float x) {
 }
 
 // ---------------------------------------------------------------- 16 bit
-template <typename E, int DP_>
+// DP: elements of a staged row; DC: elements that the products go over (the
+// ones behind are zero in every operand). head_dim 80 and 96 in rows of 128.
+template <typename E, int DP_, int DC = DP_>
 struct Tile16 {
   typedef E elem;
   typedef E vec8 __attribute__((ext_vector_type(8)));
   typedef E vec4 __attribute__((ext_vector_type(4)));
   static constexpr int DP = DP_, ESZ = 2, CE = 8;  // CE: elements of a 16-byte chunk
   static constexpr bool SHORT_RANGE = std::is_same<E, _Float16>::value;  // of exponents: 2^-24 to 2^16
-  static constexpr int ROWB = DP * 2, CPR = ROWB / 16, KS = DP / 16, NU = DP / 32;
+  static constexpr int ROWB = DP * 2, CPR = ROWB / 16, KS = DC / 16, NU = DC / 32;
   struct Rows {
     vec8 f[KS];
   };
@@ -183,12 +185,15 @@ struct Tile16 {
 };
 
 // ------------------------------------------------------------------ fp32
-template <int DP_>
+template <int DP_, int DC = DP_>
 struct Tile32 {
   typedef float elem;
   static constexpr int DP = DP_, ESZ = 4, CE = 4;
   static constexpr bool SHORT_RANGE = false;
-  static constexpr int ROWB = DP * 4, CPR = ROWB / 16, KT = DP / 8, NU = DP / 32;
+  static constexpr int ROWB = DP * 4, CPR = ROWB / 16, KT = DC / 8, NU = DC / 32;
+  // output rows: element r of subtile u is d = NU r + u, so that one read of NU
+  // floats feeds NU products; with three, d = 32 u + r and a read to each
+  static constexpr bool TOGETHER = NU != 3;
   struct Rows {
     f32x4 f[KT];
   };
@@ -208,14 +213,15 @@ struct Tile32 {
   }
   struct Lane {
     uint32_t row, kx;  // chunk reads
-    uint32_t h, col;   // row reads: 4 h rows down, byte NU * 4 * l32
+    uint32_t h, col;   // row reads: 4 h rows down, the lane's first byte
   };
   static __device__ inline Lane lane_of(int lane) {
     const int l32 = lane & 31, h = lane >> 5;
-    return Lane{(uint32_t)(l32 * ROWB), (uint32_t)((l32 & 15) ^ h), (uint32_t)h, (uint32_t)(NU * 4 * l32)};
+    return Lane{(uint32_t)(l32 * ROWB), (uint32_t)((l32 & 15) ^ h), (uint32_t)h, (uint32_t)((TOGETHER ? NU : 1) * 4 * l32)};
   }
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  typedef typename abf::VRow<NU>::type vrow;
+  typedef typename abf::VRow<TOGETHER ? NU : 4>::type vrow;
+  typedef __attribute__((address_space(3))) float lds_float;
   typedef __attribute__((address_space(3))) vrow lds_vrow;
   template <int NT>
   static __device__ inline void scores(f32x16* c, uint32_t st, const Lane& ln, const Rows& y) {
@@ -245,8 +251,16 @@ struct Tile32 {
 #pragma unroll
       for (int s = 0; s < 16; ++s) {
         const uint32_t r = 8 * (s >> 2) + 4 * ln.h + (s & 3);  // row % 16 decides the slot, 32 t does not
-        const vrow a = *(const lds_vrow*)(uintptr_t)(st + (32 * t + r) * ROWB +
-                                                     ((((ln.col >> 4) ^ (r & 15)) << 4) | (ln.col & 15)));
+        vrow a;
+        if constexpr (TOGETHER) {
+          a = *(const lds_vrow*)(uintptr_t)(st + (32 * t + r) * ROWB +
+                                            ((((ln.col >> 4) ^ (r & 15)) << 4) | (ln.col & 15)));
+        } else {
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+            a[u] = *(const lds_float*)(uintptr_t)(st + (32 * t + r) * ROWB +
+                                                  (((8 * u + (ln.col >> 4)) ^ (r & 15)) << 4 | (ln.col & 15)));
+        }
 #pragma unroll
         for (int u = 0; u < NU; ++u) acc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[u], p.b[t][s], acc[u], 0, 0, 0);
       }
@@ -265,8 +279,9 @@ struct Tile32 {
       for (int k = 0; k < NU; ++k) {
         f32x4 t;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = acc[(4 * k + e) % NU][4 * a + (4 * k + e) / NU];
-        f(NU * (8 * a + 4 * h) + 4 * k, t);
+        for (int e = 0; e < 4; ++e)
+          t[e] = TOGETHER ? acc[(4 * k + e) % NU][4 * a + (4 * k + e) / NU] : acc[k][4 * a + e];
+        f(TOGETHER ? NU * (8 * a + 4 * h) + 4 * k : 32 * k + 8 * a + 4 * h, t);
       }
   }
   static __device__ inline void store4(char* p, f32x4 v) { *(f32x4*)p = v; }

@@ -564,7 +564,7 @@ def _attn_parts_pytorch(Q, parts, scale):
         scores.append(s)
         values.append(v)
     if sum(s.shape[-1] for s in scores) == 0:
-        return Q * 0
+        return Q.masked_fill(torch.ones_like(Q, dtype=torch.bool), 0.0)  # (whatever Q holds)
     P = _masked_softmax(torch.cat(scores, -1))
     O = P.new_zeros(B, Hk, G * N, D)
     at = 0
