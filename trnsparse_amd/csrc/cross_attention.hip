@@ -22,7 +22,7 @@ int check_operand(const char* who, const char* name, const void* p, const int64_
   return TSP_OK;
 }
 
-Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want) {
+Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want, int64_t wide_least) {
   Plan p;
   p.narrow = rows <= 32;
   p.tiles = p.narrow ? 1 : (int)ceil_div(rows, 128);
@@ -34,7 +34,7 @@ Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide
   // range 8.4 / 25 / 55 / 197. In fp32 a stage of 32 keys is 3.4 us of matrix
   // instructions and a CU holds one workgroup: shorter ranges, fewer of them.
   const bool f32 = dtype == TSP_F32;
-  const int64_t want = p.narrow ? (f32 ? 256 : 512) : wide_want, least = p.narrow ? (f32 ? 128 : 512) : (f32 ? 64 : 256);
+  const int64_t want = p.narrow ? (f32 ? 256 : 512) : wide_want, least = p.narrow ? (f32 ? 128 : 512) : wide_least;
   const int64_t wgs = units * p.tiles, step = p.narrow ? 128 : 64;
   int64_t n = wgs >= (p.narrow && f32 ? want : want / 2) ? 1 : ceil_div(want, wgs);
   if (n > ceil_div(keys, least)) n = ceil_div(keys, least);
@@ -43,6 +43,14 @@ Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide
   p.chunk = ceil_div(ceil_div(keys > 0 ? keys : 1, n), step) * step;
   p.nsplit = (int)(keys > 0 ? ceil_div(keys, p.chunk) : 1);
   return p;
+}
+
+// Wide, 16 bit: one workgroup of eight wavefronts to a CU (fwd_wide<T, 2>) and
+// ranges of 512 keys at least: 16 heads of 1500 x 1500 x 64 21.0 us, two
+// workgroups of four with ranges of 256 34.7; 8 heads of 512 x 4000 x 128 29.3
+// and 32.4; 2 x 8 of 512 x 512 x 128 14.3 and 18.4.
+static Plan cross_plan(int dtype, int64_t units, int64_t rows, int64_t keys) {
+  return dtype == TSP_F32 ? fwd_plan(dtype, units, rows, keys, 512, 64) : fwd_plan(dtype, units, rows, keys, 256, 512);
 }
 
 static void set_plan(FwdArgs& a, const Plan& p) {
@@ -62,8 +70,10 @@ int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st) {
     typedef decltype(tile) T;
     if (p.narrow)
       hipLaunchKernelGGL((fwd_narrow<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else if (T::ESZ == 2 && grid <= 256)  // a CU has one workgroup at most
+      hipLaunchKernelGGL((fwd_wide<T, T::ESZ == 2 ? 2 : 1>), dim3((unsigned)grid), dim3(T::ESZ == 2 ? 512 : 256), 0, st, a);
     else
-      hipLaunchKernelGGL((fwd_wide<T>), dim3((unsigned)grid), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((fwd_wide<T, 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
     return check_launch("attention launch");
   });
 }
@@ -130,7 +140,7 @@ extern "C" int64_t tsp_cross_attn_workspace_size(int dtype, int64_t B, int64_t H
                                                  int64_t D) {
   if (xat::check_sizes("tsp_cross_attn_workspace_size", dtype, B, Hq, Hkv, Sq, L, D)) return -1;
   if (B * Hq * Sq == 0) return 0;
-  const xat::Plan p = xat::fwd_plan(dtype, B * Hkv, Hq / Hkv * Sq, L, 512);
+  const xat::Plan p = xat::cross_plan(dtype, B * Hkv, Hq / Hkv * Sq, L);
   return p.nsplit > 1 ? p.nsplit * B * Hq * Sq * (D + 1) * 4 : 0;
 }
 
@@ -154,7 +164,7 @@ extern "C" int tsp_cross_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const int64_t need = tsp_cross_attn_workspace_size(dtype, B, Hq, Hkv, Sq, L, D);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   const int64_t none[3] = {0, 0, 0};
-  const xat::Plan p = xat::fwd_plan(dtype, B * Hkv, Hq / Hkv * Sq, L, 512);
+  const xat::Plan p = xat::cross_plan(dtype, B * Hkv, Hq / Hkv * Sq, L);
   xat::FwdArgs a{};
   a.Q = xat::operand(Q, qs, dtype);
   a.K = xat::operand(K, L > 0 ? ks : none, dtype);

@@ -32,8 +32,9 @@ PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq
   // (64 sequences, 32 heads on 8 key heads, 8192 + up to 1024 keys: the prefix
   // in ranges for 128 workgroups 38.1 us, for 96 42.1, 192 40.8, 256 46.1; each
   // range writes and reads back a result of every row)
-  if (P > 0) p.shared = fwd_plan(dtype, Hkv, B * G * Sq, P, 128);
-  if (S > 0) p.own = fwd_plan(dtype, B * Hkv, G * Sq, S, 512);
+  const int64_t least = dtype == TSP_F32 ? 64 : 256;
+  if (P > 0) p.shared = fwd_plan(dtype, Hkv, B * G * Sq, P, 128, least);
+  if (S > 0) p.own = fwd_plan(dtype, B * Hkv, G * Sq, S, 512, least);
   p.nsplit = p.shared.nsplit + p.own.nsplit;
   return p;
 }

@@ -112,15 +112,19 @@ __device__ inline int keys_from(int64_t sees, int64_t k1, int64_t at) {
   return n < 0 ? 0 : n > 64 ? 64 : (int)n;
 }
 
-template <typename T, int NT>
+// KG 2: eight wavefronts, two for every 32 rows, each pair's stages in two halves
+// (the first half's results joined with the second's through LDS at the end).
+template <typename T, int NT, int KG>
 struct Wide {
-  static constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES, LDS = 2 * STAGE;
+  static constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
+  static constexpr int RING = KG * 2 * STAGE, XW = (16 * T::NU + 2) * 256, LDS = KG == 2 && 4 * XW > RING ? 4 * XW : RING;
   static __device__ inline void run(const FwdArgs& a, uint32_t block, uint8_t* lds) {
     Item it;
     if (!item_of(a, block, a.tiles, a.nsplit, it)) return;
     const int tile = it.tile, split = it.split;
     const int64_t ub = it.ub, hk = it.hk;
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int w = wave & 3, kg = wave >> 2;
     const int r = tile * 128 + w * 32 + (lane & 31);
     const bool live = r < a.R, some = tile * 128 + w * 32 < a.R;  // this row, a row of the wavefront's
     const RowId id = row_id(a, ub, hk, live ? r : 0);
@@ -129,16 +133,18 @@ struct Wide {
     T::load(q, a.Q.p + id.b * a.Q.b + id.head * a.Q.h + id.i * a.Q.s, live, a.D, h);
 
     const int64_t n = unit_length(a, ub);
-    const int64_t k0 = split * a.chunk, k1 = k0 + a.chunk < n ? k0 + a.chunk : n;
+    const int64_t c0 = split * a.chunk, k1 = c0 + a.chunk < n ? c0 + a.chunk : n;
     const int64_t sees = a.causal ? n - (a.Sq - 1 - id.i) : n;  // keys of this row
-    const int nst = k1 > k0 ? (int)ceil_div(k1 - k0, HK) : 0;
+    const int all = k1 > c0 ? (int)ceil_div(k1 - c0, HK) : 0, turns = KG == 2 ? (all + 1) / 2 : all;
+    const int nst = kg ? all - turns : turns;  // (no more than the first half's)
+    const int64_t k0 = c0 + (int64_t)kg * turns * HK;
     const char* Kp = a.K.p + ub * a.K.b + hk * a.K.h;
     const char* Vp = a.V.p + ub * a.V.b + hk * a.V.h;
     Stager<T, HK, 4> ks, vs;
     ks.init(w, lane, a.K.s, a.D);
     vs.init(w, lane, a.V.s, a.D);
     const typename T::Lane ln = T::lane_of(lane);
-    const uint32_t lds0 = dma::lds_addr(lds);
+    const uint32_t lds0 = dma::lds_addr(lds) + kg * 2 * STAGE;
     auto issue = [&](int s) {
       const uint32_t st = lds0 + (s & 1) * STAGE;
       ks.issue(Kp, k0 + (int64_t)s * HK, k1, a.K.s, a.D, st, w);
@@ -147,15 +153,39 @@ struct Wide {
     RowState<T> x;
     x.clear();
     if (nst > 0) issue(0);
-    for (int s = 0; s < nst; ++s) {
+    for (int s = 0; s < turns; ++s) {
       dma::wait_vm<0>();
       dma::barrier();
       if (s + 1 < nst) issue(s + 1);
-      if (!some) continue;
+      if (!some || (KG == 2 && s >= nst)) continue;
       const int64_t at = k0 + (int64_t)s * HK;
       const uint32_t st = lds0 + (s & 1) * STAGE;
       softmax_stage<T, NT>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,
                            keys_from(sees, k1, at), [] {});
+    }
+    if constexpr (KG == 2) {
+      float* xp = (float*)lds + w * (XW / 4) + lane;  // a register of the 64 lanes at a time
+      __syncthreads();
+      if (kg == 1) {
+#pragma unroll
+        for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) xp[64 * (16 * u + v)] = x.acc[u][v];
+        xp[64 * 16 * T::NU] = x.m;
+        xp[64 * (16 * T::NU + 1)] = x.l;
+      }
+      __syncthreads();
+      if (kg == 1) return;
+      const float m1 = xp[64 * 16 * T::NU], l1 = xp[64 * (16 * T::NU + 1)], m = fmaxf(x.m, m1);
+      // (a half without keys for the row has m = -inf and nothing to add)
+      const float f0 = x.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x.m - m);
+      const float f1 = m1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m1 - m);
+#pragma unroll
+      for (int u = 0; u < T::NU; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x.acc[u][v] = x.acc[u][v] * f0 + xp[64 * (16 * u + v)] * f1;
+      x.l = x.l * f0 + l1 * f1;
+      x.m = m;
     }
     const float l = halves_sum(x.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (!live) return;
@@ -344,14 +374,15 @@ struct Narrow {
 
 template <typename T>
 struct Kernels {
-  typedef Wide<T, T::ESZ == 2 ? 2 : 1> W;
+  static constexpr int NT = T::ESZ == 2 ? 2 : 1;
   typedef Narrow<T> N;
   static constexpr int PER_CU = N::LDS <= 80 * 1024 ? 2 : 1;
 };
-template <typename T>
-__global__ __launch_bounds__(256, 2) void fwd_wide(const FwdArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[Kernels<T>::W::LDS];
-  Kernels<T>::W::run(a, blockIdx.x, lds);
+template <typename T, int KG>
+__global__ __launch_bounds__(256 * KG, 2 / KG) void fwd_wide(const FwdArgs a) {
+  typedef Wide<T, Kernels<T>::NT, KG> W;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS];
+  W::run(a, blockIdx.x, lds);
 }
 template <typename T>
 __global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_narrow(const FwdArgs a) {
@@ -364,18 +395,21 @@ __global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_joint(const FwdAr
   Kernels<T>::N::run_joint(a, first, blockIdx.x, lds);
 }
 // Two sets of keys in one launch: the first `grid0` workgroups take the first.
+// (Workgroups of eight wavefronts for either: 64 sequences behind 8192 keys 54
+// us, of four 51.)
 template <typename T>
 __global__ __launch_bounds__(256, Kernels<T>::PER_CU) void fwd_two(const FwdArgs a, const FwdArgs b, uint32_t grid0,
                                                                    bool wide_a, bool wide_b) {
-  typedef Kernels<T> K;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[K::W::LDS > K::N::LDS ? K::W::LDS : K::N::LDS];
+  typedef Wide<T, Kernels<T>::NT, 1> W;
+  typedef typename Kernels<T>::N N;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS > N::LDS ? W::LDS : N::LDS];
   const bool first = blockIdx.x < grid0;
   const FwdArgs& x = first ? a : b;
   const uint32_t block = first ? blockIdx.x : blockIdx.x - grid0;
   if (first ? wide_a : wide_b)
-    K::W::run(x, block, lds);
+    W::run(x, block, lds);
   else
-    K::N::run(x, block, lds);
+    N::run(x, block, lds);
 }
 
 // The ranges' results of every row in one: weights 2^(lse_j - max lse). Rows
@@ -447,7 +481,8 @@ struct Plan {
   int tiles, nsplit;
   int64_t chunk;
 };
-Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want);
+Plan fwd_plan(int dtype, int64_t units, int64_t rows, int64_t keys, int64_t wide_want,
+              int64_t wide_least);
 int launch_fwd(int dtype, const Plan& p, FwdArgs a, hipStream_t st);
 int launch_fwd_joint(int dtype, FwdArgs a, const FwdArgs& first, hipStream_t st);
 int launch_fwd_two(int dtype, const Plan& pa, FwdArgs a, const Plan& pb, FwdArgs b, hipStream_t st);
