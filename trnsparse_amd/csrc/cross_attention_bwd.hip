@@ -11,11 +11,14 @@
 //
 //   row_pass     128 rows of a unit to a workgroup (rows and units as in
 //                xattn_fwd.h), a wavefront to 32 with their Q and dO in
-//                registers; K and V stages stream through LDS. Leaves each
-//                row's log2(e) lse and D for the column pass.
+//                registers; K and V stages stream through LDS.
 //   column_pass  128 keys of a unit to a workgroup, a wavefront to 32 with
 //                their K and V in registers; the Q and dO rows of all heads of
-//                the group stream through LDS with their rows' two numbers.
+//                the group stream through LDS with their rows' two numbers,
+//                log2(e) lse and D.
+//   both_passes  the two as one launch, after row_stats has left the rows'
+//                numbers: 16-bit types without FINE (else the row pass leaves
+//                them and the column pass follows).
 // S and dO V^T are formed in both passes (7 products instead of 5) so that
 // neither adds across workgroups: results do not depend on any order of
 // arrival. Where a pass has few workgroups its inner axis is split, each part
@@ -42,15 +45,18 @@ struct BwdArgs {
   float scale;
 };
 
-// FINE: P and dS as sums of two 16-bit numbers (see fine() below).
-// (fp32 at 128: Q, dO and dQ alone take 192 registers of a lane)
-template <typename T, int NT, bool FINE>
-__global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(const BwdArgs b) {
+// FINE: P and dS as sums of two 16-bit numbers (see fine() below). STATS: forms
+// and leaves the rows' numbers itself (else row_stats has left them).
+template <typename T, int NT, bool FINE, bool STATS>
+struct RowPass {
+  static constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES, LDS = 2 * STAGE;
+  static __device__ inline void run(const BwdArgs& b, uint32_t block, uint8_t* lds);
+};
+template <typename T, int NT, bool FINE, bool STATS>
+__device__ inline void RowPass<T, NT, FINE, STATS>::run(const BwdArgs& b, uint32_t block, uint8_t* lds) {
   const FwdArgs& a = b.f;
-  constexpr int HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
   Item it;
-  if (!item_of(a, blockIdx.x, a.tiles, a.nsplit, it)) return;
+  if (!item_of(a, block, a.tiles, a.nsplit, it)) return;
   const int tile = it.tile, split = it.split;
   const int64_t unit = it.unit, ub = it.ub, hk = it.hk;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
@@ -80,7 +86,10 @@ __global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(c
   T::load(q, row_of(a.Q), live, a.D, h);
   T::load(g, row_of(b.dO), live, a.D, h);
   float Dr, rq, out_scale = b.scale;
-  {
+  if constexpr (!STATS) {
+    rq = live ? b.stat[id.orow] : 0.f;
+    Dr = live ? b.stat[a.prows + id.orow] : 0.f;
+  } else {
     typename T::Rows o;
     T::load(o, row_of(b.O), live, a.D, h);
     Dr = halves_sum(T::dot(g, o));
@@ -101,9 +110,11 @@ __global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(c
     Dr *= c;
     back = unit_scale(c);
     out_scale = b.scale * back;
+    if constexpr (STATS) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    if (split == 0 && lane == 0) b.gmax[(unit * a.tiles + tile) * 4 + w] = mx;
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+      if (split == 0 && lane == 0) b.gmax[(unit * a.tiles + tile) * 4 + w] = mx;
+    }
   }
   f32x16 acc[T::NU];
 #pragma unroll
@@ -160,12 +171,16 @@ __global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(c
 }
 
 template <typename T, int NQ, bool FINE>
-__global__ __launch_bounds__(256, T::ESZ == 4 || FINE ? 1 : 2) void column_pass(const BwdArgs b) {
+struct ColumnPass {
+  static constexpr int HQ = 32 * NQ, HBYTES = HQ * T::ROWB, STAGE = 2 * HBYTES + 1024;  // Q, dO, two numbers of each row
+  static constexpr int LDS = 2 * STAGE;
+  static __device__ inline void run(const BwdArgs& b, uint32_t block, uint8_t* lds);
+};
+template <typename T, int NQ, bool FINE>
+__device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t block, uint8_t* lds) {
   const FwdArgs& a = b.f;
-  constexpr int HQ = 32 * NQ, HBYTES = HQ * T::ROWB, STAGE = 2 * HBYTES + 1024;  // Q, dO, two numbers of each row
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
   Item it;
-  if (!item_of(a, blockIdx.x, b.ktiles, b.ksplit, it)) return;
+  if (!item_of(a, block, b.ktiles, b.ksplit, it)) return;
   const int tile = it.tile, split = it.split;
   const int64_t unit = it.unit, ub = it.ub, hk = it.hk;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
@@ -258,6 +273,79 @@ __global__ __launch_bounds__(256, T::ESZ == 4 || FINE ? 1 : 2) void column_pass(
   put(dv, ov, pk ? pk + krows * a.D : nullptr, 1.f);
 }
 
+// (fp32 at 128: Q, dO and dQ alone take 192 registers of a lane)
+template <typename T, int NT, bool FINE>
+__global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(const BwdArgs b) {
+  typedef RowPass<T, NT, FINE, true> R;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS];
+  R::run(b, blockIdx.x, lds);
+}
+template <typename T, int NQ, bool FINE>
+__global__ __launch_bounds__(256, T::ESZ == 4 || FINE ? 1 : 2) void column_pass(const BwdArgs b) {
+  typedef ColumnPass<T, NQ, FINE> C;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
+  C::run(b, blockIdx.x, lds);
+}
+// Both passes in one launch, the column pass' workgroups (the longer) first:
+// with lengths of their own the key tiles are never a whole number to a CU, and
+// the row pass fills what they leave. bf16, 4 x 32 heads of 128 over 8, 1024 rows
+// x 2048 keys: lengths of 700 to 1800 take 316 us this way, 359 as two launches;
+// all of 2048, 474 and 469; 2 x 16 heads of 64, 2048 x 2048: 131 and 134.
+template <typename T, int N>
+__global__ __launch_bounds__(256, 2) void both_passes(const BwdArgs b, uint32_t columns) {
+  typedef RowPass<T, N, false, false> R;
+  typedef ColumnPass<T, N, false> C;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS > R::LDS ? C::LDS : R::LDS];
+  if (blockIdx.x < columns)
+    C::run(b, blockIdx.x, lds);
+  else
+    R::run(b, blockIdx.x - columns, lds);
+}
+
+// The rows' two numbers (and, fp16, the largest |dO| of every 32 rows of a unit)
+// ahead of both passes: 16 lanes to a row, 32 rows of a unit to a workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void row_stats(const BwdArgs b) {
+  static_assert(T::ESZ == 2, "8 elements to a lane");
+  const FwdArgs& a = b.f;
+  const uint32_t chunks = 4u * a.tiles, unit = blockIdx.x / chunks, chunk = blockIdx.x - unit * chunks;
+  const uint32_t ub = unit / (uint32_t)a.Hkv, hk = unit - ub * (uint32_t)a.Hkv;
+  const int lane = threadIdx.x & 15, d = 8 * lane;
+  float mx = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = (int)chunk * 32 + 16 * k + (threadIdx.x >> 4);
+    if (r >= a.R) continue;
+    const RowId id = row_id(a, ub, hk, r);
+    typedef typename T::elem vec8 __attribute__((ext_vector_type(8)));
+    vec8 g = vec8{}, o = vec8{};
+    if (d < a.D) {
+      g = *(const vec8*)(b.dO.p + id.b * b.dO.b + id.head * b.dO.h + id.i * b.dO.s + 2 * d);
+      o = *(const vec8*)(b.O.p + id.b * b.O.b + id.head * b.O.h + id.i * b.O.s + 2 * d);
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sum += (float)g[e] * (float)o[e];
+      mx = fmaxf(mx, fabsf((float)g[e]));
+    }
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
+    if (lane == 0) {
+      b.stat[id.orow] = b.lse[id.orow] * LOG2E;
+      b.stat[a.prows + id.orow] = sum;
+    }
+  }
+  if constexpr (T::SHORT_RANGE) {
+    __shared__ float top[4];
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    if (threadIdx.x == 0) b.gmax[blockIdx.x] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  }
+}
+
 // Sums of the parts of each result's rows in order, rounded once: 32 lanes to a
 // row; blockIdx.y is the result (dQ, dK, dV; no rows where there is one part).
 struct SumArgs {
@@ -316,6 +404,22 @@ BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int6
   return p;
 }
 
+template <typename T>
+int sums(const BwdPlan& p, const BwdArgs& b, bool columns, hipStream_t st) {
+  const FwdArgs& a = b.f;
+  const int64_t units = (int64_t)a.units_b * a.Hkv;
+  const int64_t krows = units * a.L, qsum = p.nsplit > 1 ? a.prows : 0, ksum = p.ksplit > 1 && columns ? krows : 0;
+  const int64_t most = qsum > ksum ? qsum : ksum;
+  if (most == 0) return TSP_OK;
+  SumsArgs s{};
+  s.D = a.D;
+  s.of[0] = SumArgs{b.qpart, qsum, a.prows * a.D, p.nsplit, a.Hkv * a.G, a.Sq, b.dQ};
+  s.of[1] = SumArgs{b.kpart, ksum, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dK};
+  s.of[2] = SumArgs{b.kpart + krows * a.D, ksum, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dV};
+  hipLaunchKernelGGL((sum_parts<T>), dim3((unsigned)ceil_div(most, 8), 3), dim3(256), 0, st, s);
+  return check_launch("sum_parts launch");
+}
+
 // P and dS rounded to 16 bits move a gradient as far as the rounding of its
 // result does: 1.41 times the error of that alone, of few rows or keys up to
 // 1.6. A sum of two 16-bit numbers leaves the result's own, for 4 products in
@@ -333,22 +437,23 @@ int run_t(const BwdPlan& p, const BwdArgs& b, hipStream_t st) {
   const int64_t g1 = head_grid((int64_t)p.tiles * p.nsplit, units), g2 = b.dK.p ? head_grid((int64_t)p.ktiles * p.ksplit, units) : 0;
   if (g1 > INT32_MAX || g2 > INT32_MAX) return fail(TSP_EUNSUPPORTED, "tsp_cross_attn_bwd: too large a grid");
   int rc;
+  if constexpr (!FINE && T::ESZ == 2) {
+    const int64_t g0 = units * p.tiles * 4;
+    if (g2 > 0 && g0 <= INT32_MAX && g1 + g2 <= INT32_MAX) {
+      hipLaunchKernelGGL((row_stats<T>), dim3((unsigned)g0), dim3(256), 0, st, b);
+      if ((rc = check_launch("row_stats launch"))) return rc;
+      hipLaunchKernelGGL((both_passes<T, N>), dim3((unsigned)(g1 + g2)), dim3(256), 0, st, b, (uint32_t)g2);
+      if ((rc = check_launch("both_passes launch"))) return rc;
+      return sums<T>(p, b, g2 > 0, st);
+    }
+  }
   hipLaunchKernelGGL((row_pass<T, N, FINE>), dim3((unsigned)g1), dim3(256), 0, st, b);
   if ((rc = check_launch("row_pass launch"))) return rc;
   if (g2 > 0) {
     hipLaunchKernelGGL((column_pass<T, N, FINE>), dim3((unsigned)g2), dim3(256), 0, st, b);
     if ((rc = check_launch("column_pass launch"))) return rc;
   }
-  const int64_t krows = units * a.L, qsum = p.nsplit > 1 ? a.prows : 0, ksum = p.ksplit > 1 && g2 > 0 ? krows : 0;
-  const int64_t most = qsum > ksum ? qsum : ksum;
-  if (most == 0) return TSP_OK;
-  SumsArgs s{};
-  s.D = a.D;
-  s.of[0] = SumArgs{b.qpart, qsum, a.prows * a.D, p.nsplit, a.Hkv * a.G, a.Sq, b.dQ};
-  s.of[1] = SumArgs{b.kpart, ksum, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dK};
-  s.of[2] = SumArgs{b.kpart + krows * a.D, ksum, 2 * krows * a.D, p.ksplit, a.Hkv, a.L, b.dV};
-  hipLaunchKernelGGL((sum_parts<T>), dim3((unsigned)ceil_div(most, 8), 3), dim3(256), 0, st, s);
-  return check_launch("sum_parts launch");
+  return sums<T>(p, b, g2 > 0, st);
 }
 
 // zeros in a strided result
