@@ -201,6 +201,31 @@ def test_graph_qk_norm_rope(hip_backend, dt):
     _grads_replay_match(lambda q, w: ts.qk_norm_rope(q, sets[1][1], w, w, pos, f)[0], leaves, (2, 4, 300, D), dt, 7)
 
 
+def test_capture_beside_an_eager_graph(hip_backend):
+    """A training step is not captured while an eager graph of the same leaves
+    lives: refused before it records anything; released, it is captured."""
+    g = torch.Generator(device="cuda").manual_seed(10)
+    Q, K, V = (torch.randn(1, 2, 40, D, device="cuda", generator=g).requires_grad_() for _ in range(3))
+    w, pos, f = torch.ones(D, device="cuda"), torch.arange(40, device="cuda"), ts.rope_frequencies(D, device="cuda")
+    for fn in (lambda: ts.cross_attention(Q, K, V), lambda: ts.qk_norm_rope(Q, K, w, w, pos, f)[0]):
+        held = fn()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="release it before the capture"):
+            with torch.cuda.graph(graph):
+                fn()
+        with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fn()  # (no gradients: nothing to join)
+        want = torch.autograd.grad(held, Q, torch.ones_like(held))[0]
+        del held
+        ones = torch.ones_like(want)
+        graph, (got,) = _capture(lambda: torch.autograd.grad(fn(), Q, ones)[0])
+        for _ in range(2):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
 def test_two_threads_two_streams(hip_backend):
     """Calls from two threads, each on its own stream, do not disturb each other."""
     g = torch.Generator(device="cuda").manual_seed(8)

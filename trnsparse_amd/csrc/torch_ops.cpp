@@ -16,8 +16,10 @@
 // the attention backward's column plan) and the autograd wrappers.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -808,6 +810,27 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return std::any_of(ts.begin(), ts.end(), [](const at::Tensor* t) { return t->requires_grad(); });
 }
 
+// A captured backward joins the stream on which its leaves' gradient
+// accumulators were made. One that an eager graph (or a hook) of the same leaves
+// keeps alive belongs to a stream outside the capture, and joining that ends the
+// process: refused here, before anything of the step is recorded.
+void capture_owns(const char* who, std::initializer_list<const at::Tensor*> ts) {
+  if ((*ts.begin())->key_set().has(c10::DispatchKey::Python)) return;  // traced: no stream
+  const at::Device dev = (*ts.begin())->device();
+  const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (!st || hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const c10::Stream here = c10::impl::VirtualGuardImpl(dev.type()).getStream(dev);
+  for (const at::Tensor* t : ts) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto acc = ag::impl::try_get_grad_accumulator(*t);
+    const auto made = acc ? acc->stream() : c10::nullopt;
+    TORCH_CHECK(!made || *made == here, who, ": an input that needs its gradient is held by an autograd graph or hook "
+                "made on another stream than the one being captured; release it before the capture, or call under "
+                "torch.no_grad()");
+  }
+}
+
 void first_order(const char* who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, " has no second derivatives: backward with create_graph=False");
 }
@@ -847,7 +870,10 @@ struct CrossAttention : public ag::Function<CrossAttention> {
 
 at::Tensor cross_attention_autograd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
                                     const c10::optional<at::Tensor>& key_lengths, double scale) {
-  if (wants_grad({&Q, &K, &V})) return CrossAttention::apply(Q, K, V, key_lengths, scale);
+  if (wants_grad({&Q, &K, &V})) {
+    capture_owns("cross_attention", {&Q, &K, &V});
+    return CrossAttention::apply(Q, K, V, key_lengths, scale);
+  }
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = op_of("trnsparse_hip::cross_attention", &cross_attention);
   return op.call(Q, K, V, key_lengths, scale);
@@ -884,6 +910,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& Q, co
                                                          const at::Tensor& wk, const at::Tensor& pos,
                                                          const at::Tensor& freq, double eps, bool interleaved) {
   if (wants_grad({&Q, &K, &wq, &wk})) {
+    capture_owns("qk_norm_rope", {&Q, &K, &wq, &wk});
     auto r = QKNormRope::apply(Q, K, wq, wk, pos, freq, eps, interleaved);
     return {r[0], r[1]};
   }

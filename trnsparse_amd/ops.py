@@ -629,8 +629,9 @@ def shared_prefix_attention(
     first lengths[b] rows hold its own tokens, the new ones last (None: all
     rows; values are taken into [0, keys]); rows behind them are not read.
     Query i sees the prefix and own tokens j < lengths[b] - (queries - 1 - i);
-    a query that sees nothing gives zeros. Types, heads, scale, strides and the
-    result's order as in `cross_attention`.
+    a query that sees nothing gives zeros. What stands in V of a token that only
+    some queries see has to be finite: the others weigh it with zero. Types,
+    heads, scale, strides and the result's order as in `cross_attention`.
     """
     who = "shared_prefix_attention"
     if scale is None:
