@@ -38,6 +38,11 @@ PrefixPlan prefix_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq
   p.nsplit = p.shared.nsplit + p.own.nsplit;
   return p;
 }
+// Bytes of workspace: none where one range has all keys (and writes the result),
+// an fp32 result and log-sum-exp of every row for each of more.
+int64_t part_bytes(const PrefixPlan& p, int64_t rows, int64_t D) {
+  return p.nsplit > 1 ? p.nsplit * rows * (D + 1) * 4 : 0;
+}
 }  // namespace
 }  // namespace xat
 }  // namespace tsp
@@ -49,7 +54,7 @@ extern "C" int64_t tsp_prefix_attn_workspace_size(int dtype, int64_t B, int64_t 
   if (xat::check_sizes("tsp_prefix_attn_workspace_size", dtype, B, Hq, Hkv, Sq, P > S ? P : S, D)) return -1;
   if (P < 0 || S < 0) return fail(TSP_EINVAL, "tsp_prefix_attn_workspace_size: negative length"), -1;
   if (B * Hq * Sq == 0) return 0;
-  return xat::prefix_plan(dtype, B, Hq, Hkv, Sq, P, S).nsplit * B * Hq * Sq * (D + 1) * 4;
+  return xat::part_bytes(xat::prefix_plan(dtype, B, Hq, Hkv, Sq, P, S), B * Hq * Sq, D);
 }
 
 extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void* PK, const int64_t* pks, const void* PV,
@@ -77,7 +82,7 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
   if (!(scale > 1e-30) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
   if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
   const xat::PrefixPlan p = xat::prefix_plan(dtype, B, Hq, Hkv, Sq, P, S);
-  const int64_t rows = B * Hq * Sq, need = p.nsplit * rows * (D + 1) * 4;
+  const int64_t rows = B * Hq * Sq, need = xat::part_bytes(p, rows, D);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   xat::FwdArgs a{};
   a.Q = xat::operand(Q, qs, dtype);
@@ -85,7 +90,7 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
   a.O = (char*)O;
   a.ob = o.b, a.oh = o.h, a.os = o.s;
   a.prows = rows;
-  if (!p.joint) {
+  if (p.nsplit > 1) {
     a.part = (float*)workspace;
     a.plse = a.part + p.nsplit * rows * D;
   }
@@ -117,7 +122,7 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
     rc = xat::launch_fwd(dtype, p.shared, sh, st);
   else if (S > 0)
     rc = xat::launch_fwd(dtype, p.own, own, st);
-  if (rc) return rc;
+  if (rc || p.nsplit == 1) return rc;
   const xat::CombineArgs c{a.part, a.plse, rows, p.nsplit, a.D, (int)Hq, a.Sq, a.O, a.ob, a.oh, a.os, nullptr};
   return xat::launch_combine(dtype, c, st);
 }
