@@ -608,7 +608,7 @@ int tsp_csr_transpose(const void* values, int dtype, const int64_t* col_indices,
  * and below 16 MiB (TSP_EINVAL / TSP_EUNSUPPORTED otherwise). dtype is
  * TSP_F32, TSP_BF16 or TSP_F16, the same for all operands; sums, maxima and
  * partial results are fp32. heads is a multiple of kv_heads; query head h
- * reads key head h / (heads / kv_heads). scale is positive.
+ * reads key head h / (heads / kv_heads). scale lies in (1e-30, 1e30).
  * `key_lengths` / `lengths` (batch,) of `index_type`, or NULL for all keys:
  * values are taken into [0, keys]; K and V rows behind them are not read.
  * A row without a key to see is zero.

@@ -5,7 +5,9 @@ formats (CSRMatrix, COOMatrix, BSRMatrix, from_dense, from_scipy,
 eye_sparse), ops (spmv, spmm, bsr_spmm, screened_spmm,
 block_sparse_attention_tiled and the small CSR helpers) and the backend
 switch (set_backend / get_backend / HAS_NKI), plus the fixed-step solvers
-(richardson_bsr, chebyshev_bsr, chebyshev_coeffs). The compute runs in
+(richardson_bsr, chebyshev_bsr, chebyshev_coeffs) and what a decoder layer has
+next to the block-sparse attention (cross_attention, shared_prefix_attention,
+qk_norm_rope), which the reference lacks. The compute runs in
 hand-written gfx950 HIP kernels behind the C ABI in include/trnsparse_hip.h.
 """
 

@@ -523,7 +523,7 @@ def _check_heads(who: str, Q, K, V, lengths, scale: float) -> None:
         raise RuntimeError(f"{who}: Q, K, V must have one floating dtype, got {dt}, {K.dtype}, {V.dtype}")
     if not 1 <= q[3] <= 128:
         raise RuntimeError(f"{who}: head_dim {q[3]} is not in 1 .. 128")
-    if not 0 < scale < math.inf:
+    if not 1e-30 < scale < 1e30:
         raise RuntimeError(f"{who}: scale must be positive, got {scale}")
     if lengths is not None:
         if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != q[:1]:
@@ -589,7 +589,7 @@ def cross_attention(
     int64 gives each sample's number of valid keys (values are taken into
     [0, keys]); what stands in K and V behind them is not read, and its
     gradient is zero. A sample without keys gives zeros. `scale` defaults to
-    head_dim**-0.5 and is positive; head_dim is at most 128.
+    head_dim**-0.5 and lies in (1e-30, 1e30); head_dim is at most 128.
 
     float32, bfloat16 and float16 on the HIP backend, accumulated in float32.
     Operands may be strided views (heads of a projection's output); the result
