@@ -160,7 +160,7 @@ struct Wide {
       if (!some || (KG == 2 && s >= nst)) continue;
       const int64_t at = k0 + (int64_t)s * HK;
       const uint32_t st = lds0 + (s & 1) * STAGE;
-      softmax_stage<T, NT>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,
+      softmax_stage<T, NT, false>(x, q, st, st + HBYTES, ln, h, a.scale_log2, a.causal || at + HK > k1,
                            keys_from(sees, k1, at), [] {});
     }
     if constexpr (KG == 2) {
@@ -203,6 +203,10 @@ struct Wide {
 // share a CU (16 bit; 128 wide fp32 has one): one streams while the other
 // starts or joins its wavefronts (16 sequences of up to 1500 keys, 8 heads of
 // 128: rings of two with one workgroup to a CU 21.7 us).
+// P enters its product as the sum of two 16-bit numbers: the wavefront waits for
+// memory here, not for the matrix cores (that case 24.0 us with cold caches, of one
+// number 23.6; 64 sequences behind 8192 shared keys 51.1 and 50.2), and a result
+// then is as near as its own rounding (of one number up to 1.5 times as far).
 template <typename T>
 struct Narrow {
   static constexpr int NW = 4, HBYTES = 32 * T::ROWB, XLD = T::DP + 4;
@@ -244,7 +248,7 @@ struct Narrow {
       const int64_t at = key(s);
       dma::wait_vm<St::NI>();  // K is there once only V's loads are out
       fence();
-      softmax_stage<T, 1>(x, q, kst, vst, ln, h, a.scale_log2, a.causal || at + 32 > k1, keys_from(sees, k1, at), [&] {
+      softmax_stage<T, 1, true>(x, q, kst, vst, ln, h, a.scale_log2, a.causal || at + 32 > k1, keys_from(sees, k1, at), [&] {
         drained();  // this wavefront's reads of K have returned: its place is free
         if (more) {
           ks.issue(Kp, key(s + 1), k1, a.K.s, a.D, kst, 0);
@@ -312,7 +316,7 @@ struct Narrow {
       const int64_t at = 32 * (int64_t)(own ? stage(s) - np : stage(s)), end = own ? n : P;
       dma::wait_vm<St::NI>();
       fence();
-      softmax_stage<T, 1>(x, q, kst, vst, ln, h, a.scale_log2, (own && a.causal) || at + 32 > end,
+      softmax_stage<T, 1, true>(x, q, kst, vst, ln, h, a.scale_log2, (own && a.causal) || at + 32 > end,
                           keys_from(own ? sees : P, end, at), [&] {
                             drained();
                             if (more) {

@@ -147,30 +147,32 @@ struct Tile16 {
 #pragma unroll
       for (int v = 0; v < 16; ++v) p[t][v] -= (float)kept.b[t][v >> 3][v & 7];
   }
+  // acc += X^T p, and X^T rest, of X's tile at st
   template <int NT>
-  static __device__ inline void outer(f32x16* acc, uint32_t st, const Lane& ln, const Prob<NT>& p) {
+  static __device__ inline void outer(f32x16* acc, uint32_t st, const Lane& ln, const Prob<NT>& p,
+                                      const Prob<NT>* rest = nullptr) {
     const uint32_t t0 = st + ln.t0, t1 = st + ln.t1;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
-          acc[u] = mfma16(__builtin_bit_cast(vec8, abw::lds_trp(t0, t1, u, (32 * t + 16 * a) * ROWB)), p.b[t][a],
-                          acc[u]);
+        for (int u = 0; u < NU; ++u) {
+          const vec8 x = __builtin_bit_cast(vec8, abw::lds_trp(t0, t1, u, (32 * t + 16 * a) * ROWB));
+          acc[u] = mfma16(x, p.b[t][a], acc[u]);
+          if (rest) acc[u] = mfma16(x, rest->b[t][a], acc[u]);
+        }
   }
   // acc += X^T p, with p in 16 bits or (TWICE) as the sum of two such numbers
   template <int NT, bool TWICE>
   static __device__ inline void product(f32x16* acc, uint32_t st, const Lane& ln, f32x16* p) {
-    Prob<NT> a;
+    Prob<NT> a, b;
     pack<NT>(a, p);
-    outer<NT>(acc, st, ln, a);
     if constexpr (TWICE) {
-      Prob<NT> b;
       rest<NT>(p, a);
       pack<NT>(b, p);
-      outer<NT>(acc, st, ln, b);
     }
+    outer<NT>(acc, st, ln, a, TWICE ? &b : nullptr);
   }
   // f(d, four consecutive values at d) over the lane's part of its own row
   template <typename F>
@@ -331,7 +333,7 @@ struct RowState {
   }
 };
 // `between` runs once the scores have left the K stage, before V is read.
-template <typename T, int NT, typename F>
+template <typename T, int NT, bool TWICE, typename F>
 __device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, uint32_t kst, uint32_t vst,
                                      const typename T::Lane& ln, int h, float scale_log2, bool check, int keys,
                                      F&& between) {
@@ -369,9 +371,7 @@ __device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, 
       sum += s[t][v];
     }
   r.l += sum;
-  typename T::template Prob<NT> p;
-  T::template pack<NT>(p, s);
-  T::template outer<NT>(r.acc, vst, ln, p);
+  T::template product<NT, TWICE>(r.acc, vst, ln, s);
 }
 
 }  // namespace xat
