@@ -106,7 +106,14 @@ struct Angles {
         const double turns = __builtin_rint(angle * 0.15915494309189535);
         angle = __builtin_fma(-turns, 6.283185307179586477, angle);
         angle = __builtin_fma(-turns, 2.449293598294706414e-16, angle);
-        sincospif((float)(angle * 0.31830988618379067154), &s[k], &c[k]);
+        // in half turns, and what 32 bits leave of them to first order: 2^-24 of a
+        // half turn would move a result by more than its own rounding
+        const double halves = angle * 0.31830988618379067154;
+        const float head = (float)halves, rest = (float)((halves - head) * 3.14159265358979323846);
+        float c0, s0;
+        sincospif(head, &s0, &c0);
+        c[k] = c0 - rest * s0;
+        s[k] = s0 + rest * c0;
       }
     }
   }
@@ -186,6 +193,15 @@ __device__ inline float lanes_sum(float v) {
   return v;
 }
 
+// 1 / sqrt(x): the instruction's value, and for fp32 rows a Newton step from it
+// (it is off by up to 2^-23, twice a result's rounding).
+template <typename E>
+__device__ inline float inv_sqrt(float x) {
+  const float r = __builtin_amdgcn_rsqf(x);
+  if constexpr (sizeof(E) == 2) return r;
+  return r > 0.f && r < INFINITY ? __builtin_fmaf(0.5f * r, __builtin_fmaf(-x * r, r, 1.f), r) : r;
+}
+
 // A row's chunks as they lie in memory: loaded a step before they are used.
 template <typename E, int CE, int J>
 struct Raw {
@@ -258,7 +274,7 @@ __global__ __launch_bounds__(256) void norm_rope_fwd(const Args g) {
         fetch(sd, step + 1);
       else if (sd == 0 && n[1] > 0)
         fetch(1, 0);
-      const float r = __builtin_amdgcn_rsqf(lanes_sum<G>(ss) / (float)g.D + g.eps);
+      const float r = inv_sqrt<E>(lanes_sum<G>(ss) / (float)g.D + g.eps);
       const int hd = head(step);
       char* out = (char*)rows_at(s.y, hd);
 #pragma unroll
@@ -335,7 +351,7 @@ __global__ __launch_bounds__(256) void norm_rope_bwd(const Args g) {
             sw += x[j][e] * (w[sd][j][e] * d[j][e]);
           }
         }
-        const float r = __builtin_amdgcn_rsqf(lanes_sum<G>(ss) * invD + g.eps);
+        const float r = inv_sqrt<E>(lanes_sum<G>(ss) / (float)g.D + g.eps);
         const float c = r * r * r * invD * lanes_sum<G>(sw);
         const int hd = step * GW + grp;
         char* out = (char*)s.y.p + b * s.y.b + hd * s.y.h + i * s.y.s;
@@ -371,13 +387,15 @@ __global__ __launch_bounds__(256) void norm_rope_bwd(const Args g) {
   }
 }
 
-// dw of 16 columns of (2, D): 64 threads to a column, then their sums in order.
+// dw of 16 columns of (2, D): 64 threads to a column, then their sums in order,
+// in fp64: as a chain of fp32 sums of up to 1024 parts they alone were off by 1.6
+// times a result's rounding.
 template <typename E>
 __global__ __launch_bounds__(1024) void wgrad_kernel(const float* __restrict__ part, int n, int D, int w32, void* dwq,
                                                      void* dwk) {
-  __shared__ float sum[64][17];
+  __shared__ double sum[64][17];
   const int c = threadIdx.x & 15, rg = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
-  float v = 0.f;
+  double v = 0.;
   if (col < 2 * D) {
 #pragma unroll 8
     for (int k = rg; k < n; k += 64) v += part[(int64_t)k * 2 * D + col];
@@ -385,7 +403,7 @@ __global__ __launch_bounds__(1024) void wgrad_kernel(const float* __restrict__ p
   sum[rg][c] = v;
   __syncthreads();
   if (rg >= 4) return;
-  float t = 0.f;
+  double t = 0.;
 #pragma unroll
   for (int k = 0; k < 16; ++k) t += sum[16 * rg + k][c];
   t += __shfl_xor(t, 16, 64);
@@ -395,9 +413,9 @@ __global__ __launch_bounds__(1024) void wgrad_kernel(const float* __restrict__ p
   const int d = col < D ? col : col - D;
   if (!out) return;
   if (w32)
-    ((float*)out)[d] = t;
+    ((float*)out)[d] = (float)t;
   else
-    ((E*)out)[d] = (E)t;
+    ((E*)out)[d] = (E)(float)t;
 }
 
 // Workgroups of the backward (and parts of a weight gradient): four to a CU.
