@@ -177,3 +177,52 @@ def test_fp16_gradients_of_any_size(hip_backend, size, N):
     dO = (dO * 2.0 ** -(torch.arange(N, device="cuda") % 5).view(N, 1)).to(HF)
     check_backward(Q, K, V, dO=dO)
     check_backward(Q, K, V, dO=torch.zeros_like(dO))
+
+
+# Steps of 2^29 products of the scores and more in 16 bits: both passes in one
+# launch, P and dS as one number each. With ranges of keys and of queries that are
+# added (one head; one row tile), 65 to 96 elements, 64, odd edges.
+LARGE = [(2, 8, 2, 401, 701, 128), (4, 8, 8, 300, 721, 80), (2, 16, 16, 513, 520, 64), (1, 1, 1, 2103, 2001, 128),
+         (1, 8, 1, 16, 33000, 128)]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("size", LARGE)
+def test_large_steps(hip_backend, size, dt):
+    B, H, _, N, L, D = size
+    assert B * H * N * L * D >= 2**29
+    (dQ, _, _), r = check_backward(*make(*size, dt, seed=11))
+    # the queries' gradient alone takes the row pass alone: within two results'
+    # bounds (3 u of the scale each, and the fp32 steps) of the one beside it
+    Q, K, V = make(*size, dt, seed=11)
+    g = torch.Generator(device="cuda").manual_seed(50)
+    dO = torch.randn(B, N, H, D, device="cuda", generator=g).to(dt).transpose(1, 2)
+    q = Q.detach().requires_grad_()
+    alone = torch.autograd.grad(ts.cross_attention(q, K, V), q, dO)[0]
+    u = torch.finfo(dt).eps / 2
+    assert ((alone.double() - dQ.double()).abs().cpu() <= 8 * u * r["aQ"] + 2.0**-22).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_large_steps_with_lengths(hip_backend, dt):
+    L = 1300
+    lengths = torch.tensor([0, 1, 640, 1299, 1300, 5000], device="cuda", dtype=torch.int32)
+    Q, K, V = make(6, 4, 2, 300, L, 64, dt, seed=12)
+    K, V = K.clone(), V.clone()
+    for b, n in enumerate(lengths.clamp(0, L).tolist()):
+        K[b, :, n:], V[b, :, n:] = float("inf"), float("nan")
+    (dQ, dK, dV), _ = check_backward(Q, K, V, lengths)
+    assert (dQ[0] == 0).all()
+    for b, n in enumerate(lengths.clamp(0, L).tolist()):
+        assert (dK[b, :, n:] == 0).all() and (dV[b, :, n:] == 0).all()
+
+
+@pytest.mark.parametrize("size", [2.0**-16, 2.0**10])
+def test_large_fp16_gradients_of_any_size(hip_backend, size):
+    N = 400
+    g = torch.Generator(device="cuda").manual_seed(61)
+    Q, K, V = make(2, 8, 2, N, 1400, 64, HF, seed=13)
+    dO = size * torch.randn(2, 8, N, 64, device="cuda", generator=g)
+    dO = (dO * 2.0 ** -(torch.arange(N, device="cuda") % 5).view(N, 1)).to(HF)
+    check_backward(Q, K, V, dO=dO)
+    check_backward(Q, K, V, dO=torch.zeros_like(dO))
