@@ -202,3 +202,26 @@ def test_float64_is_refused(hip_backend):
     Q, K, V = (t.double() for t in make(1, 2, 2, 3, 4, 64, F32))
     with pytest.raises(RuntimeError, match="not supported"):
         ts.cross_attention(Q, K, V)
+
+
+# More workgroups than CUs, of four wavefronts each in 16 bits too; more narrow
+# ones than fit at once; units that do not divide over the XCDs.
+FULL = [(3, 32, 32, 300, 100, 64), (2, 40, 8, 700, 333, 128), (5, 21, 21, 290, 70, 90), (70, 24, 8, 2, 150, 128)]
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("size", FULL)
+def test_full_grids(hip_backend, size, dt):
+    check_forward(*make(*size, dt, seed=20))
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_full_grid_with_lengths(hip_backend, dt):
+    L = 300
+    lengths = torch.tensor([0, 1, 63, 64, 299, 400], device="cuda")
+    Q, K, V = make(6, 16, 16, 400, L, 64, dt, seed=21)
+    K, V = K.clone(), V.clone()
+    for b, n in enumerate(lengths.clamp(0, L).tolist()):
+        K[b, :, n:], V[b, :, n:] = float("nan"), float("inf")
+    O, _ = check_forward(Q, K, V, lengths)
+    assert (O[0] == 0).all()

@@ -92,3 +92,10 @@ def test_views_and_slices_of_a_cache(hip_backend):
     long = lambda t: torch.cat([t, t.new_full((2, 50, 64), float("nan"))], 1)[:, :200]  # noqa: E731
     assert torch.equal(ts.shared_prefix_attention(Q, long(pK), long(pV), turn(K), turn(V)), want)
     assert torch.equal(ts.shared_prefix_attention(Q, turn(pK[None])[0], pV, K, V), want)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("size", [(64, 16, 8, 1, 2100, 500, 128), (24, 32, 4, 5, 3001, 300, 80), (33, 12, 3, 40, 700, 400, 64)])
+def test_full_grids(hip_backend, size, dt):
+    """A prefix in wide workgroups, in several ranges, next to many sequences."""
+    check(*make(*size, dt))
