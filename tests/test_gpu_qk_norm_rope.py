@@ -146,3 +146,12 @@ def test_weight_gradients_repeat(hip_backend):
         grads = torch.autograd.grad(ts.qk_norm_rope(*leaves, pos, f), leaves, args[4:])
         first = first or grads
         assert all(torch.equal(a, b) for a, b in zip(first, grads))
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("size", [(1, 2, 1, 9001, 64, 64), (3, 5, 2, 1801, 128, 32), (2, 1, 3, 4999, 20, 10), (1, 9, 1, 4200, 256, 200)])
+def test_long_sequences(hip_backend, size, dt):
+    """More tokens than the backward's wavefronts: each takes several in turn."""
+    *s, rot = size
+    pos = torch.arange(s[0] * s[3], device="cuda").view(s[0], s[3])
+    check(*make(*s, dt, seed=3), pos, ts.rope_frequencies(rot, device="cuda"), interleaved=s[4] == 20)
