@@ -226,3 +226,12 @@ def test_large_fp16_gradients_of_any_size(hip_backend, size):
     dO = (dO * 2.0 ** -(torch.arange(N, device="cuda") % 5).view(N, 1)).to(HF)
     check_backward(Q, K, V, dO=dO)
     check_backward(Q, K, V, dO=torch.zeros_like(dO))
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("B", [2, 64, 65])
+def test_many_lengths(hip_backend, B, dt):
+    """Entries of equal and of different lengths, as many as are taken longest
+    first and more."""
+    lengths = torch.arange(B, device="cuda") * 37 % 5 * 40
+    check_backward(*make(B, 4, 2, 45, 150, 24, dt, seed=14), lengths)

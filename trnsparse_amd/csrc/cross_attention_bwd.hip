@@ -58,7 +58,7 @@ __device__ inline void RowPass<T, NT, FINE, STATS>::run(const BwdArgs& b, uint32
   Item it;
   if (!item_of(a, block, a.tiles, a.nsplit, it)) return;
   const int tile = it.tile, split = it.split;
-  const int64_t unit = it.unit, ub = it.ub, hk = it.hk;
+  const int64_t ub = longest_first(a, it.ub), hk = it.hk, unit = ub * a.Hkv + hk;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
   const int r = tile * 128 + w * 32 + l32;
   const bool live = r < a.R, some = tile * 128 + w * 32 < a.R;
