@@ -380,18 +380,28 @@ struct BwdPlan {
   int64_t stat, gmax, qpart, kpart;  // bytes
   int64_t bytes() const { return stat + gmax + qpart + kpart; }
 };
-BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D) {
+// Ranges for 512 workgroups, where there are less than half of that. An fp32
+// workgroup has a CU to itself, so one round of them is 256 and the ranges are as
+// many as fit (2 x 8 heads of 512 x 512 x 128 108 us, for 512 workgroups 142; 12
+// heads over 4 of 1000 x 200 x 64 52 and 66) - but not with lengths, which leave
+// ranges empty: 3 x 8 heads of 257 x up to 383 x 80 94 us, for 512 87. Lengths
+// never take fewer ranges, so the workspace that does for them does for all.
+BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D, bool lengths) {
   BwdPlan p{};
-  const int64_t G = Hq / Hkv, units = B * Hkv, stage = dtype == TSP_F32 ? 32 : 64, want = 512;
+  const int64_t G = Hq / Hkv, units = B * Hkv, stage = dtype == TSP_F32 ? 32 : 64;
+  const auto ranges = [&](int64_t wgs) {
+    if (wgs == 0 || wgs >= 256) return int64_t(1);
+    return dtype == TSP_F32 && !lengths ? 256 / wgs : ceil_div(512, wgs);
+  };
   p.tiles = (int)ceil_div(G * Sq, 128);
-  int64_t n = units * p.tiles >= want / 2 ? 1 : ceil_div(want, units * p.tiles);
+  int64_t n = ranges(units * p.tiles);
   const int64_t kst = ceil_div(L > 0 ? L : 1, stage);  // stages of keys
   if (n > kst / 2) n = kst / 2 > 1 ? kst / 2 : 1;
   p.chunk = ceil_div(kst, n) * stage;
   p.nsplit = (int)ceil_div(L > 0 ? L : 1, p.chunk);
   p.ktiles = (int)ceil_div(L, 128);
-  const int64_t total = G * ceil_div(Sq, stage), wgs = units * p.ktiles;
-  n = wgs == 0 || wgs >= want / 2 ? 1 : ceil_div(want, wgs);
+  const int64_t total = G * ceil_div(Sq, stage);
+  n = ranges(units * p.ktiles);
   if (n > total / 2) n = total / 2 > 1 ? total / 2 : 1;
   p.per = (int)ceil_div(total, n);
   p.ksplit = (int)ceil_div(total, p.per > 0 ? p.per : 1);
@@ -480,8 +490,7 @@ extern "C" int64_t tsp_cross_attn_bwd_workspace_size(int dtype, int64_t B, int64
                                                      int64_t L, int64_t D) {
   if (xat::check_sizes("tsp_cross_attn_bwd_workspace_size", dtype, B, Hq, Hkv, Sq, L, D)) return -1;
   if (B * Hq * Sq == 0) return 0;
-  const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D);
-  return p.bytes();
+  return xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D, true).bytes();
 }
 
 extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* K, const int64_t* ks, const void* V,
@@ -520,7 +529,7 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
     if ((rc = xat::check_operand(who, "K", K, ks, L, D, dtype)) || (rc = xat::check_operand(who, "V", V, vs, L, D, dtype)))
       return rc;
   if (!lse) return fail(TSP_EINVAL, "%s: null lse", who);
-  const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D);
+  const xat::BwdPlan p = xat::bwd_plan(dtype, B, Hq, Hkv, Sq, L, D, key_lengths != nullptr);
   if (!workspace || workspace_bytes < p.bytes())
     return fail(TSP_EINVAL, "%s: workspace too small", who);
   if (ceil_div(B * Hq * Sq, 8) > INT32_MAX || ceil_div(B * Hkv * L, 8) > INT32_MAX)
