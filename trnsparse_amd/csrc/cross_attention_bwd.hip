@@ -15,7 +15,7 @@
 //   column_pass  128 keys of a unit to a workgroup, a wavefront to 32 with
 //                their K and V in registers; the Q and dO rows of all heads of
 //                the group stream through LDS with their rows' two numbers,
-//                log2(e) lse and D.
+//                log2(e) lse (less P_EXP) and D.
 //   both_passes  the two as one launch, after row_stats has left the rows'
 //                numbers: 16-bit types without FINE (else the row pass leaves
 //                them and the column pass follows).
@@ -32,12 +32,19 @@ int check_sizes(const char* who, int dtype, int64_t B, int64_t Hq, int64_t Hkv, 
 
 namespace {
 
+// P enters dV's product as 2^P_EXP P. In fp16 that fills the type's range: P of n
+// keys is about 1 / n, and from 2^-14 down fp16 has a fixed step of 2^-24 (131072
+// keys: dV off by 1.3e-3 of its norm as P itself, 2.9e-4 this way; its own
+// rounding 2.1e-4). P <= 1, so 2^15 P stays finite.
+template <typename T>
+constexpr int P_EXP = T::SHORT_RANGE ? 15 : 0;
+
 struct BwdArgs {
   FwdArgs f;           // Q, K, V, lengths and sizes; tiles, nsplit, chunk of the row pass
   Operand O, dO;
   Operand dQ, dK, dV;  // written
   const float* lse;
-  float *stat;         // (2, rows): log2(e) lse, D
+  float *stat;         // (2, rows): log2(e) lse - P_EXP, D
   float *gmax;         // fp16: (units, tiles, 4) largest |dO| of each wavefront's rows
   float *qpart;        // (nsplit, rows, D), null with one range
   float *kpart;        // (ksplit, 2, batch * kv_heads * keys, D), null with one range
@@ -87,7 +94,7 @@ __device__ inline void RowPass<T, NT, FINE, STATS>::run(const BwdArgs& b, uint32
   T::load(g, row_of(b.dO), live, a.D, h);
   float Dr, rq, out_scale = b.scale;
   if constexpr (!STATS) {
-    rq = live ? b.stat[id.orow] : 0.f;
+    rq = live ? b.stat[id.orow] + P_EXP<T> : 0.f;
     Dr = live ? b.stat[a.prows + id.orow] : 0.f;
   } else {
     typename T::Rows o;
@@ -95,7 +102,7 @@ __device__ inline void RowPass<T, NT, FINE, STATS>::run(const BwdArgs& b, uint32
     Dr = halves_sum(T::dot(g, o));
     rq = live ? b.lse[id.orow] * LOG2E : 0.f;
     if (live && split == 0 && h == 0) {
-      b.stat[id.orow] = rq;
+      b.stat[id.orow] = rq - P_EXP<T>;
       if (!short_rows) b.stat[a.prows + id.orow] = Dr;
     }
   }
@@ -202,7 +209,7 @@ __device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t b
     const uint32_t st = lds0 + (s & 1) * STAGE;
     qs.issue(a.Q.p + ub * a.Q.b + head * a.Q.h, i0, a.Sq, a.Q.s, a.D, st, w);
     gs.issue(b.dO.p + ub * b.dO.b + head * b.dO.h, i0, a.Sq, b.dO.s, a.D, st + HBYTES, w);
-    if (w < 2) {  // rows past the last one: both numbers zero, so P = 1 meets dO = 0 and dS = 0
+    if (w < 2) {  // rows past the last one: both numbers zero, so a finite P meets dO = 0 and dS = 0
       const float* x = b.stat + w * a.prows + (ub * a.Hkv * a.G + head) * a.Sq + i0;
       const int left = a.Sq - i0;
       dma::buffer4(dma::make_rsrc(x, 4u * (left < HQ ? left : HQ)), 4u * lane, st + 2 * HBYTES + w * 256);
@@ -212,14 +219,15 @@ __device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t b
   typename T::Rows k, v;
   T::load(k, a.K.p + ub * a.K.b + hk * a.K.h + key * a.K.s, key < n, a.D, h);
   T::load(v, a.V.p + ub * a.V.b + hk * a.V.h + key * a.V.s, key < n, a.D, h);
-  float c = 1.f;
+  constexpr float back = 1.f / (1 << P_EXP<T>);
+  float cs = 1.f;  // makes dS of what P makes
   if constexpr (T::SHORT_RANGE) {  // as in the row pass, one factor for the rows of the unit
     float mx = 0.f;
     for (int e = lane; e < a.tiles * 4; e += 64) mx = fmaxf(mx, b.gmax[unit * a.tiles * 4 + e]);
     mx = halves_max(mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    c = unit_scale(mx);
+    cs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit_scale(mx) * back)));
   }
   f32x16 dk[T::NU], dv[T::NU];
 #pragma unroll
@@ -246,7 +254,7 @@ __device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t b
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][4 * x + e], a.scale_log2, -rq[e]));
           sc[0][4 * x + e] = p;
           const float ds = p * (dp[0][4 * x + e] - Dr[e]);
-          dp[0][4 * x + e] = T::SHORT_RANGE ? ds * c : ds;
+          dp[0][4 * x + e] = T::SHORT_RANGE ? ds * cs : ds;
         }
       }
       T::template product<1, FINE>(dv, at + HBYTES, ln, sc);
@@ -269,8 +277,8 @@ __device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t b
         T::store4(o + d * T::ESZ, y);
     });
   };
-  put(dk, ok, pk, b.scale * unit_scale(c));
-  put(dv, ov, pk ? pk + krows * a.D : nullptr, 1.f);
+  put(dk, ok, pk, b.scale * (T::SHORT_RANGE ? unit_scale(cs) * back : 1.f));
+  put(dv, ov, pk ? pk + krows * a.D : nullptr, back);
 }
 
 // (fp32 at 128: Q, dO and dQ alone take 192 registers of a lane)
@@ -332,7 +340,7 @@ __global__ __launch_bounds__(256) void row_stats(const BwdArgs b) {
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
     if (lane == 0) {
-      b.stat[id.orow] = b.lse[id.orow] * LOG2E;
+      b.stat[id.orow] = b.lse[id.orow] * LOG2E - P_EXP<T>;
       b.stat[a.prows + id.orow] = sum;
     }
   }
