@@ -19,7 +19,7 @@ import torch
 
 import trnsparse_amd as ts
 from oracle import layer
-from test_gpu_cross_attention import BF, HF, make
+from test_gpu_cross_attention import BF, E, HF, make
 
 NORM = 1.25  # of u
 
@@ -41,6 +41,30 @@ def step(size, dt, seed=15):
     return Q, K, V, (2.0**8 * torch.randn(Q.shape, device="cuda", generator=g)).to(dt)
 
 
+def check_fp16_gradients(Q, K, V, dO):
+    """Elementwise, on the bounds of test_gpu_cross_attention_backward but for
+    what fp16 cannot hold: P enters as 2^15 P, dS with its bound 2 D max |dO| max
+    |V| at 2^14 or more, so a term below the normal range is off by 2^-40, or by
+    2^-39 of that bound. O below the normal range is off by 2^-25, so D by 2^-25
+    sum |dO|, which weighs rows of K with P of sum 1, and of Q with P <= 1. A
+    gradient past fp16's range is infinite: both sides are clamped to it."""
+    leaves = [t.requires_grad_() for t in (Q, K, V)]
+    grads = torch.autograd.grad(ts.cross_attention(*leaves), leaves, dO)
+    torch.cuda.synchronize()
+    N, D, L, sc, top = Q.shape[2], Q.shape[3], K.shape[2], Q.shape[3] ** -0.5, torch.finfo(HF).max
+    r = layer.attention(Q, K, V, sc, None, dO)
+    inner = 2 * (D + 4) * r["smax"] + 2 * L + 64 + 4 * float(r["lse"].abs().max()) + 2 * D
+    dS = 2.0**-39 * 2 * D * float(dO.abs().max()) * float(V.abs().max()) * sc
+    off = 2.0**-25 * float(dO.abs().sum(3).max()) * sc
+    size = lambda t: t.detach().double().cpu().abs()  # noqa: E731
+    col = lambda t: size(t).sum(2, keepdim=True)  # noqa: E731
+    lows = (dS * col(K) + off * size(K).amax(2, keepdim=True), (dS + off) * col(Q), 2.0**-40 * col(dO))
+    for got, k, terms, low in zip(grads, "QKV", (L, N, N), lows):
+        bound = (3 * 2.0**-11 + E * (inner + terms)) * r["a" + k] + 2.0**-25 + low
+        far = (got.double().cpu().clamp(-top, top) - r["d" + k].clamp(-top, top)).abs() - bound
+        assert not got.isnan().any() and far.max() <= 0, ("d" + k, float(far.max()))
+
+
 # (batch, heads, kv_heads, queries, keys, head_dim): many keys, with few queries
 # (P and dS as sums of two numbers) and with more
 MANY_KEYS = [(1, 1, 1, 32, 131072, 64), (1, 2, 1, 64, 131072, 64), (1, 1, 1, 8, 524288, 64), (1, 2, 1, 64, 33000, 128)]
@@ -50,6 +74,22 @@ MANY_KEYS = [(1, 1, 1, 32, 131072, 64), (1, 2, 1, 64, 131072, 64), (1, 1, 1, 8, 
 @pytest.mark.parametrize("dt", [BF, HF])
 @pytest.mark.parametrize("size", MANY_KEYS)
 def test_many_keys(hip_backend, size, dt):
-    """P of many keys is small: fp16 keeps its digits all the same."""
+    """P and dS of many keys are small: fp16 keeps their digits all the same."""
     e = gradient_errors(*step(size, dt))
-    assert e["dV"] <= NORM, e
+    assert max(e.values()) <= NORM, e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value,grad", [(3000.0, 1.0), (65504.0, 2.0**-6), (2.0**-24, 1.0), (0.0, 1.0)])
+@pytest.mark.parametrize("H,N,L", [(2, 3, 2), (2, 40, 50), (2, 200, 700), (16, 400, 1500)])
+def test_values_of_any_size(hip_backend, H, N, L, value, grad):
+    """fp16: dO V^T and dS of large values pass 65504 where the gradients do not.
+    Two keys of opposite values share each row's weight."""
+    g = torch.Generator(device="cuda").manual_seed(17)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    Q, K, V = 1 + 0.1 * r(1, H, N, 64), 0.1 * r(1, H, L, 64), 0.1 * value * r(1, H, L, 64)
+    K[:, :, :2] += 1.5
+    V[:, :, 0], V[:, :, 1] = value, -value
+    dO = torch.full((1, H, N, 64), grad, device="cuda")
+    dO[:, :, ::2] = -grad
+    check_fp16_gradients(*(t.clamp(-65504, 65504).to(HF) for t in (Q, K, V)), dO.to(HF))

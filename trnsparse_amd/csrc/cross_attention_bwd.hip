@@ -16,9 +16,10 @@
 //                their K and V in registers; the Q and dO rows of all heads of
 //                the group stream through LDS with their rows' two numbers,
 //                log2(e) lse (less P_EXP) and D.
-//   both_passes  the two as one launch, after row_stats has left the rows'
-//                numbers: 16-bit types without FINE (else the row pass leaves
-//                them and the column pass follows).
+//   both_passes  the two as one launch: 16-bit types without FINE.
+//   row_stats    leaves the rows' numbers ahead of both_passes, and in fp16
+//                ahead of the separate passes too, with the largest |dO| and
+//                |V| (else the row pass leaves the numbers for the column pass).
 // S and dO V^T are formed in both passes (7 products instead of 5) so that
 // neither adds across workgroups: results do not depend on any order of
 // arrival. Where a pass has few workgroups its inner axis is split, each part
@@ -39,18 +40,38 @@ namespace {
 template <typename T>
 constexpr int P_EXP = T::SHORT_RANGE ? 15 : 0;
 
+// And dS, in fp16, as c dS: the power of two that brings what dS can be to just
+// below 2^15. |dS_ij| <= P_ij (|dO_i . V_j| + |D_i|) <= 2 head_dim max |dO| max
+// |V|, whatever the scores. So no loss scale and no size of V takes dS out of
+// fp16's range, and of many keys it keeps its digits (131072 keys: dQ and dK off
+// by 7e-4 of their norms with dO near 1 alone; 3e-4 this way). The launch that
+// finds the two sizes is 3 us of a small step (8 x 8 heads of 128 x 128 x 64 17.8 ->
+// 20.7 us), 1 to 2 % of a large one.
+__device__ inline float ds_scale(float dO, float V, int D) { return unit_scale(2.f * D * dO * V) * 16384.f; }
+
 struct BwdArgs {
   FwdArgs f;           // Q, K, V, lengths and sizes; tiles, nsplit, chunk of the row pass
   Operand O, dO;
   Operand dQ, dK, dV;  // written
   const float* lse;
   float *stat;         // (2, rows): log2(e) lse - P_EXP, D
-  float *gmax;         // fp16: (units, tiles, 4) largest |dO| of each wavefront's rows
+  float *gmax, *vmax;  // fp16: (units, tiles, 4) largest |dO| of 32 rows, (units, vparts) |V| of vkeys keys
+  int vparts;
+  int64_t vkeys;
   float *qpart;        // (nsplit, rows, D), null with one range
   float *kpart;        // (ksplit, 2, batch * kv_heads * keys, D), null with one range
   int ktiles, ksplit, per;  // column pass: key tiles, ranges of `per` stages
   float scale;
 };
+
+// Largest |V| of a unit's valid keys.
+__device__ inline float largest_value(const BwdArgs& b, int64_t unit) {
+  const int lane = threadIdx.x & 63;
+  float mx = lane < b.vparts ? b.vmax[unit * b.vparts + lane] : 0.f;  // (at most 64 parts)
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  return mx;
+}
 
 // FINE: P and dS as sums of two 16-bit numbers (see fine() below). STATS: forms
 // and leaves the rows' numbers itself (else row_stats has left them).
@@ -106,22 +127,12 @@ __device__ inline void RowPass<T, NT, FINE, STATS>::run(const BwdArgs& b, uint32
       if (!short_rows) b.stat[a.prows + id.orow] = Dr;
     }
   }
-  float back = 1.f;  // of dO's scale
-  if constexpr (T::SHORT_RANGE) {
-    // dS in fp16: with each row's dO near 1 it neither leaves fp16's range where
-    // the loss is scaled up nor loses its digits where gradients are small. A
-    // power of two, so nothing is rounded by it.
-    float mx = halves_max(T::largest(g));
-    const float c = unit_scale(mx);
-    T::scale(g, c);
-    Dr *= c;
+  float back = 1.f;  // of dS's scale
+  if constexpr (T::SHORT_RANGE) {  // c P in place of P: one factor for a row
+    const float c = ds_scale(halves_max(T::largest(g)), largest_value(b, unit), a.D);
+    rq -= (float)((int)(__float_as_uint(c) >> 23) - 127);
     back = unit_scale(c);
     out_scale = b.scale * back;
-    if constexpr (STATS) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-      if (split == 0 && lane == 0) b.gmax[(unit * a.tiles + tile) * 4 + w] = mx;
-    }
   }
   f32x16 acc[T::NU];
 #pragma unroll
@@ -148,8 +159,8 @@ __device__ inline void RowPass<T, NT, FINE, STATS>::run(const BwdArgs& b, uint32
           const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v], a.scale_log2, -rq));
           if (32 * t + 8 * (v >> 2) + 4 * h + (v & 3) < keys) sum += p * dp[t][v];
         }
-      Dr = halves_sum(sum);
-      if (live && h == 0) b.stat[a.prows + id.orow] = Dr * back;
+      Dr = halves_sum(sum) * back;
+      if (live && h == 0) b.stat[a.prows + id.orow] = Dr;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -221,13 +232,13 @@ __device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t b
   T::load(v, a.V.p + ub * a.V.b + hk * a.V.h + key * a.V.s, key < n, a.D, h);
   constexpr float back = 1.f / (1 << P_EXP<T>);
   float cs = 1.f;  // makes dS of what P makes
-  if constexpr (T::SHORT_RANGE) {  // as in the row pass, one factor for the rows of the unit
+  if constexpr (T::SHORT_RANGE) {  // one factor for the unit
     float mx = 0.f;
     for (int e = lane; e < a.tiles * 4; e += 64) mx = fmaxf(mx, b.gmax[unit * a.tiles * 4 + e]);
     mx = halves_max(mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    cs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit_scale(mx) * back)));
+    cs = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ds_scale(mx, largest_value(b, unit), a.D) * back)));
   }
   f32x16 dk[T::NU], dv[T::NU];
 #pragma unroll
@@ -284,7 +295,7 @@ __device__ inline void ColumnPass<T, NQ, FINE>::run(const BwdArgs& b, uint32_t b
 // (fp32 at 128: Q, dO and dQ alone take 192 registers of a lane)
 template <typename T, int NT, bool FINE>
 __global__ __launch_bounds__(256, T::ROWB > 256 || FINE ? 1 : 2) void row_pass(const BwdArgs b) {
-  typedef RowPass<T, NT, FINE, true> R;
+  typedef RowPass<T, NT, FINE, !T::SHORT_RANGE> R;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS];
   R::run(b, blockIdx.x, lds);
 }
@@ -310,39 +321,52 @@ __global__ __launch_bounds__(256, 2) void both_passes(const BwdArgs b, uint32_t 
     R::run(b, blockIdx.x - columns, lds);
 }
 
-// The rows' two numbers (and, fp16, the largest |dO| of every 32 rows of a unit)
-// ahead of both passes: 16 lanes to a row, 32 rows of a unit to a workgroup.
+// The rows' two numbers ahead of the passes: 16 lanes to a row, 32 rows of a unit
+// to a workgroup. fp16: also their largest |dO|, and behind those workgroups
+// vparts for each unit's largest |V|.
 template <typename T>
 __global__ __launch_bounds__(256) void row_stats(const BwdArgs b) {
   static_assert(T::ESZ == 2, "8 elements to a lane");
+  typedef typename T::elem vec8 __attribute__((ext_vector_type(8)));
   const FwdArgs& a = b.f;
-  const uint32_t chunks = 4u * a.tiles, unit = blockIdx.x / chunks, chunk = blockIdx.x - unit * chunks;
-  const uint32_t ub = unit / (uint32_t)a.Hkv, hk = unit - ub * (uint32_t)a.Hkv;
+  const uint32_t chunks = 4u * a.tiles, row_wgs = (uint32_t)a.units_b * a.Hkv * chunks;
   const int lane = threadIdx.x & 15, d = 8 * lane;
   float mx = 0.f;
+  auto largest = [&](vec8 x) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int r = (int)chunk * 32 + 16 * k + (threadIdx.x >> 4);
-    if (r >= a.R) continue;
-    const RowId id = row_id(a, ub, hk, r);
-    typedef typename T::elem vec8 __attribute__((ext_vector_type(8)));
-    vec8 g = vec8{}, o = vec8{};
-    if (d < a.D) {
-      g = *(const vec8*)(b.dO.p + id.b * b.dO.b + id.head * b.dO.h + id.i * b.dO.s + 2 * d);
-      o = *(const vec8*)(b.O.p + id.b * b.O.b + id.head * b.O.h + id.i * b.O.s + 2 * d);
-    }
-    float sum = 0.f;
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf((float)x[e]));
+  };
+  if (blockIdx.x < row_wgs) {
+    const uint32_t unit = blockIdx.x / chunks, chunk = blockIdx.x - unit * chunks;
+    const uint32_t ub = unit / (uint32_t)a.Hkv, hk = unit - ub * (uint32_t)a.Hkv;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      sum += (float)g[e] * (float)o[e];
-      mx = fmaxf(mx, fabsf((float)g[e]));
-    }
+    for (int k = 0; k < 2; ++k) {
+      const int r = (int)chunk * 32 + 16 * k + (threadIdx.x >> 4);
+      if (r >= a.R) continue;
+      const RowId id = row_id(a, ub, hk, r);
+      vec8 g = vec8{}, o = vec8{};
+      if (d < a.D) {
+        g = *(const vec8*)(b.dO.p + id.b * b.dO.b + id.head * b.dO.h + id.i * b.dO.s + 2 * d);
+        o = *(const vec8*)(b.O.p + id.b * b.O.b + id.head * b.O.h + id.i * b.O.s + 2 * d);
+      }
+      float sum = 0.f;
 #pragma unroll
-    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
-    if (lane == 0) {
-      b.stat[id.orow] = b.lse[id.orow] * LOG2E - P_EXP<T>;
-      b.stat[a.prows + id.orow] = sum;
+      for (int e = 0; e < 8; ++e) sum += (float)g[e] * (float)o[e];
+      if constexpr (T::SHORT_RANGE) largest(g);
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
+      if (lane == 0) {
+        b.stat[id.orow] = b.lse[id.orow] * LOG2E - P_EXP<T>;
+        b.stat[a.prows + id.orow] = sum;
+      }
     }
+  } else if constexpr (T::SHORT_RANGE) {
+    const uint32_t i = blockIdx.x - row_wgs, unit = i / (uint32_t)b.vparts, part = i - unit * (uint32_t)b.vparts;
+    const uint32_t ub = unit / (uint32_t)a.Hkv, hk = unit - ub * (uint32_t)a.Hkv;
+    const int64_t n = unit_length(a, ub), k0 = part * b.vkeys, k1 = k0 + b.vkeys < n ? k0 + b.vkeys : n;
+    const char* V = a.V.p + ub * a.V.b + hk * a.V.h + 2 * d;
+    if (d < a.D)
+      for (int64_t k = k0 + (threadIdx.x >> 4); k < k1; k += 16) largest(*(const vec8*)(V + k * a.V.s));
   }
   if constexpr (T::SHORT_RANGE) {
     __shared__ float top[4];
@@ -350,7 +374,9 @@ __global__ __launch_bounds__(256) void row_stats(const BwdArgs b) {
     for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
     if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = mx;
     __syncthreads();
-    if (threadIdx.x == 0) b.gmax[blockIdx.x] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if (threadIdx.x == 0)
+      *(blockIdx.x < row_wgs ? b.gmax + blockIdx.x : b.vmax + (blockIdx.x - row_wgs)) =
+          fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   }
 }
 
@@ -383,10 +409,10 @@ __global__ __launch_bounds__(256) void sum_parts(const SumsArgs all) {
 }
 
 struct BwdPlan {
-  int tiles, nsplit, ktiles, ksplit, per;
-  int64_t chunk;
-  int64_t stat, gmax, qpart, kpart;  // bytes
-  int64_t bytes() const { return stat + gmax + qpart + kpart; }
+  int tiles, nsplit, ktiles, ksplit, per, vparts;
+  int64_t chunk, vkeys;
+  int64_t stat, gmax, vmax, qpart, kpart;  // bytes
+  int64_t bytes() const { return stat + gmax + vmax + qpart + kpart; }
 };
 // Ranges for 512 workgroups, where there are less than half of that. An fp32
 // workgroup has a CU to itself, so one round of them is 256 and the ranges are as
@@ -416,7 +442,12 @@ BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int6
   if (p.ksplit < 1) p.ksplit = 1;
   const int64_t rows = B * Hq * Sq, up = 255;
   p.stat = (2 * rows * 4 + up) & ~up;
+  // the largest |V| of a unit in at most 64 parts, one to a lane of what reads them
+  p.vkeys = ceil_div(L > 0 ? L : 1, 64);
+  if (p.vkeys < 64) p.vkeys = 64;
+  p.vparts = (int)ceil_div(L > 0 ? L : 1, p.vkeys);
   p.gmax = dtype == TSP_F16 ? (units * p.tiles * 16 + up) & ~up : 0;
+  p.vmax = dtype == TSP_F16 ? (units * p.vparts * 4 + up) & ~up : 0;
   p.qpart = p.nsplit > 1 ? (p.nsplit * rows * D * 4 + up) & ~up : 0;
   p.kpart = p.ksplit > 1 ? p.ksplit * 2 * units * L * D * 4 : 0;
   return p;
@@ -455,15 +486,20 @@ int run_t(const BwdPlan& p, const BwdArgs& b, hipStream_t st) {
   const int64_t g1 = head_grid((int64_t)p.tiles * p.nsplit, units), g2 = b.dK.p ? head_grid((int64_t)p.ktiles * p.ksplit, units) : 0;
   if (g1 > INT32_MAX || g2 > INT32_MAX) return fail(TSP_EUNSUPPORTED, "tsp_cross_attn_bwd: too large a grid");
   int rc;
-  if constexpr (!FINE && T::ESZ == 2) {
-    const int64_t g0 = units * p.tiles * 4;
-    if (g2 > 0 && g0 <= INT32_MAX && g1 + g2 <= INT32_MAX) {
+  if constexpr (T::ESZ == 2) {
+    const bool both = !FINE && g2 > 0 && g1 + g2 <= INT32_MAX;
+    if (both || T::SHORT_RANGE) {
+      const int64_t g0 = units * (4 * p.tiles + (T::SHORT_RANGE ? p.vparts : 0));
+      if (g0 > INT32_MAX) return fail(TSP_EUNSUPPORTED, "tsp_cross_attn_bwd: too large a grid");
       hipLaunchKernelGGL((row_stats<T>), dim3((unsigned)g0), dim3(256), 0, st, b);
       if ((rc = check_launch("row_stats launch"))) return rc;
-      hipLaunchKernelGGL((both_passes<T, N>), dim3((unsigned)(g1 + g2)), dim3(256), 0, st, b, (uint32_t)g2);
-      if ((rc = check_launch("both_passes launch"))) return rc;
-      return sums<T>(p, b, g2 > 0, st);
     }
+    if constexpr (!FINE)
+      if (both) {
+        hipLaunchKernelGGL((both_passes<T, N>), dim3((unsigned)(g1 + g2)), dim3(256), 0, st, b, (uint32_t)g2);
+        if ((rc = check_launch("both_passes launch"))) return rc;
+        return sums<T>(p, b, g2 > 0, st);
+      }
   }
   hipLaunchKernelGGL((row_pass<T, N, FINE>), dim3((unsigned)g1), dim3(256), 0, st, b);
   if ((rc = check_launch("row_pass launch"))) return rc;
@@ -557,8 +593,12 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   b.stat = (float*)workspace;
   char* at = (char*)workspace + p.stat;
   if (p.gmax) b.gmax = (float*)at;
-  if (p.qpart) b.qpart = (float*)(at + p.gmax);
-  if (p.kpart) b.kpart = (float*)(at + p.gmax + p.qpart);
+  at += p.gmax;
+  if (p.vmax) b.vmax = (float*)at;
+  at += p.vmax;
+  if (p.qpart) b.qpart = (float*)at;
+  if (p.kpart) b.kpart = (float*)(at + p.qpart);
+  b.vparts = p.vparts, b.vkeys = p.vkeys;
   b.ktiles = p.ktiles, b.ksplit = p.ksplit, b.per = p.per;
   b.scale = (float)scale;
   a.prows = B * Hq * Sq;

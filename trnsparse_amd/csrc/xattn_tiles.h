@@ -94,12 +94,6 @@ struct Tile16 {
       for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf((float)a.f[s][i]));
     return t;
   }
-  static __device__ inline void scale(Rows& a, float c) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a.f[s][i] = (E)((float)a.f[s][i] * c);
-  }
 
   // LDS addresses of one stage, formed once per stage
   struct Lane {
