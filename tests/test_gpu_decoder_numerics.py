@@ -93,3 +93,24 @@ def test_values_of_any_size(hip_backend, H, N, L, value, grad):
     dO = torch.full((1, H, N, 64), grad, device="cuda")
     dO[:, :, ::2] = -grad
     check_fp16_gradients(*(t.clamp(-65504, 65504).to(HF) for t in (Q, K, V)), dO.to(HF))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [(5,), (0, 32, 64, 96), (524287,)])
+@pytest.mark.parametrize("H,N", [(512, 1), (16, 4100), (1, 1)])
+def test_one_key_outweighs_many(hip_backend, H, N, at):
+    """fp16: the many keys of a long row weigh 2^-20.4 each beside a few of 1, and
+    half of all or a tenth together. All of one weight, its rounding is theirs: u
+    of the result, whose own rounding (u / sqrt(3) of its norm) comes on top."""
+    L, D = 524288, 64
+    K = torch.zeros(1, 1, L, D, dtype=HF, device="cuda")
+    K[0, 0, list(at), 0] = 1
+    Q = torch.zeros(1, H, N, D, dtype=HF, device="cuda")
+    Q[..., 0] = 14.109375
+    g = torch.Generator(device="cuda").manual_seed(18)
+    V = (1 + torch.rand(1, 1, L, D, device="cuda", generator=g)).to(HF)
+    O = ts.cross_attention(Q, K.expand(1, H, L, D), V.expand(1, H, L, D), scale=1.0)
+    want = layer.attention(Q[:, :1, :1], K, V, 1.0)["O"]
+    assert (O == O[:, :1, :1]).all()
+    far = (O[:, :1, :1].double().cpu() - want).norm() / want.norm()
+    assert far <= (1 + 3**-0.5) * 2.0**-11, float(far) * 2**11

@@ -314,7 +314,12 @@ struct Stager {
 // l = this lane half's part of sum 2^(s - m), s = log2(e) * scale * score. m
 // follows the running maximum only when that has moved by more than 8 (log2
 // units), so 2^(s - m) <= 2^8 and acc is rarely rescaled; acc / l does not
-// depend on m. `keys` (with check): the staged keys that this row sees.
+// depend on m. In fp16, m lies 7 below the maximum that it follows, so that
+// 2^(s - m) <= 2^15 takes up the type's range: from 2^-14 down it has a fixed step
+// of 2^-24, and the many keys of a long row that one key outweighs lose digits
+// together (one of weight 1 and 524287 of 2^-20.4 in one range: results off by
+// 23 u, u = 2^-11; by less than 1.6 u this way).
+// `keys` (with check): the staged keys that this row sees.
 template <typename T>
 struct RowState {
   f32x16 acc[T::NU];
@@ -346,7 +351,7 @@ __device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, 
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[t][v]);
-  mx = halves_max(mx) * scale_log2;
+  mx = halves_max(mx) * scale_log2 - (T::SHORT_RANGE ? 7.f : 0.f);
   const bool move = mx > r.m + 8.f;
   if (__builtin_amdgcn_ballot_w64(move) != 0) {
     const float f = move ? (r.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r.m - mx)) : 1.f;
