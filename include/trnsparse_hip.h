@@ -605,7 +605,8 @@ int tsp_csr_transpose(const void* values, int dtype, const int64_t* col_indices,
  * in elements of the batch, head and row dimensions. Pointers and strides
  * are whole 16-byte pieces, head_dim is at most 128 and a whole number of
  * them (8 elements of 16 bits, 4 of 32), row strides are at least head_dim
- * and below 16 MiB (TSP_EINVAL / TSP_EUNSUPPORTED otherwise). dtype is
+ * and below 16 MiB (TSP_EINVAL / TSP_EUNSUPPORTED otherwise); the row stride
+ * of an operand of one row is not used. dtype is
  * TSP_F32, TSP_BF16 or TSP_F16, the same for all operands; sums, maxima and
  * partial results are fp32. heads is a multiple of kv_heads; query head h
  * reads key head h / (heads / kv_heads). scale lies in (1e-30, 1e30).

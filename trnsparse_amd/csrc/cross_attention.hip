@@ -12,12 +12,12 @@ namespace xat {
 
 int check_operand(const char* who, const char* name, const void* p, const int64_t* s, int64_t rows, int64_t D,
                   int dtype) {
-  const int e = esize(dtype);
   if (!p || !s) return fail(TSP_EINVAL, "%s: null %s", who, name);
-  if (((uintptr_t)p | (uint64_t)(s[0] * e) | (uint64_t)(s[1] * e) | (uint64_t)(s[2] * e)) & 15)
+  const int64_t e = esize(dtype), rs = row_stride(s, rows, D);
+  if (((uintptr_t)p | (uint64_t)(s[0] * e) | (uint64_t)(s[1] * e) | (uint64_t)(rs * e)) & 15)
     return fail(TSP_EINVAL, "%s: %s and its strides must be whole 16-byte pieces", who, name);
-  if (rows > 1 && (s[2] < D || s[2] * e >= MAX_ROW_BYTES))
-    return fail(TSP_EINVAL, "%s: row stride %lld of %s is not in [%lld, %lld)", who, (long long)s[2], name, (long long)D,
+  if (rs < D || rs * e >= MAX_ROW_BYTES)
+    return fail(TSP_EINVAL, "%s: row stride %lld of %s is not in [%lld, %lld)", who, (long long)rs, name, (long long)D,
                 (long long)(MAX_ROW_BYTES / e));
   return TSP_OK;
 }
@@ -166,10 +166,10 @@ extern "C" int tsp_cross_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const int64_t none[3] = {0, 0, 0};
   const xat::Plan p = xat::cross_plan(dtype, B * Hkv, Hq / Hkv * Sq, L);
   xat::FwdArgs a{};
-  a.Q = xat::operand(Q, qs, dtype);
-  a.K = xat::operand(K, L > 0 ? ks : none, dtype);
-  a.V = xat::operand(V, L > 0 ? vs : none, dtype);
-  const xat::Operand o = xat::operand(O, os, dtype);
+  a.Q = xat::operand(Q, qs, Sq, D, dtype);
+  a.K = xat::operand(K, L > 0 ? ks : none, L, D, dtype);
+  a.V = xat::operand(V, L > 0 ? vs : none, L, D, dtype);
+  const xat::Operand o = xat::operand(O, os, Sq, D, dtype);
   a.O = (char*)O;
   a.ob = o.b, a.oh = o.h, a.os = o.s;
   a.lse = lse;

@@ -557,7 +557,7 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   if (!rows) {  // no query: the keys' gradients are zero
     if (!cols) return TSP_OK;
     const int64_t n = B * Hkv * L;
-    for (const xat::Operand& o : {xat::operand(dK, dks, dtype), xat::operand(dV, dvs, dtype)}) {
+    for (const xat::Operand& o : {xat::operand(dK, dks, L, D, dtype), xat::operand(dV, dvs, L, D, dtype)}) {
       const xat::ZeroArgs z{o, n, L, (int)Hkv, (int)(D * xat::esize(dtype))};
       if (ceil_div(n, 8) > INT32_MAX) return fail(TSP_EUNSUPPORTED, "%s: too many rows", who);
       hipLaunchKernelGGL(xat::zero_rows, dim3((unsigned)ceil_div(n, 8)), dim3(256), 0, st, z);
@@ -581,14 +581,14 @@ extern "C" int tsp_cross_attn_bwd(const void* Q, const int64_t* qs, const void* 
   const int64_t none[3] = {0, 0, 0};
   xat::BwdArgs b{};
   xat::FwdArgs& a = b.f;
-  a.Q = xat::operand(Q, qs, dtype);
-  a.K = xat::operand(K, keys ? ks : none, dtype);
-  a.V = xat::operand(V, keys ? vs : none, dtype);
-  b.O = xat::operand(O, os, dtype);
-  b.dO = xat::operand(dO, gs, dtype);
-  b.dQ = xat::operand(dQ, dqs, dtype);
-  b.dK = xat::operand(dK, cols ? dks : none, dtype);
-  b.dV = xat::operand(dV, cols ? dvs : none, dtype);
+  a.Q = xat::operand(Q, qs, Sq, D, dtype);
+  a.K = xat::operand(K, keys ? ks : none, L, D, dtype);
+  a.V = xat::operand(V, keys ? vs : none, L, D, dtype);
+  b.O = xat::operand(O, os, Sq, D, dtype);
+  b.dO = xat::operand(dO, gs, Sq, D, dtype);
+  b.dQ = xat::operand(dQ, dqs, Sq, D, dtype);
+  b.dK = xat::operand(dK, cols ? dks : none, L, D, dtype);
+  b.dV = xat::operand(dV, cols ? dvs : none, L, D, dtype);
   b.lse = lse;
   b.stat = (float*)workspace;
   char* at = (char*)workspace + p.stat;

@@ -85,8 +85,8 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
   const int64_t rows = B * Hq * Sq, need = xat::part_bytes(p, rows, D);
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   xat::FwdArgs a{};
-  a.Q = xat::operand(Q, qs, dtype);
-  const xat::Operand o = xat::operand(O, os, dtype);
+  a.Q = xat::operand(Q, qs, Sq, D, dtype);
+  const xat::Operand o = xat::operand(O, os, Sq, D, dtype);
   a.O = (char*)O;
   a.ob = o.b, a.oh = o.h, a.os = o.s;
   a.prows = rows;
@@ -98,15 +98,15 @@ extern "C" int tsp_prefix_attn_fwd(const void* Q, const int64_t* qs, const void*
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   xat::FwdArgs sh = a, own = a;
   if (P > 0) {
-    sh.K = xat::operand(PK, pks, dtype);
-    sh.V = xat::operand(PV, pvs, dtype);
+    sh.K = xat::operand(PK, pks, P, D, dtype);
+    sh.V = xat::operand(PV, pvs, P, D, dtype);
     sh.units_b = 1;
     sh.R = (int)(B * Hq / Hkv * Sq);
     sh.L = P;
   }
   if (S > 0) {
-    own.K = xat::operand(K, ks, dtype);
-    own.V = xat::operand(V, vs, dtype);
+    own.K = xat::operand(K, ks, S, D, dtype);
+    own.V = xat::operand(V, vs, S, D, dtype);
     own.lengths = lengths;
     own.len64 = index_type == TSP_I64;
     own.units_b = (int)B;

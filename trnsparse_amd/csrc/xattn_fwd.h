@@ -525,9 +525,12 @@ int with_tile(int dtype, int64_t D, F&& f) {
 int check_operand(const char* who, const char* name, const void* p, const int64_t* strides, int64_t rows, int64_t D,
                   int dtype);
 inline int esize(int dtype) { return dtype == TSP_F32 ? 4 : 2; }
-inline Operand operand(const void* p, const int64_t* strides, int dtype) {
+// One row's stride is not the caller's: a stage of it goes on behind the row, where
+// offsets have to pass the end of the stage's buffer to read as zero.
+inline int64_t row_stride(const int64_t* strides, int64_t rows, int64_t D) { return rows > 1 ? strides[2] : D; }
+inline Operand operand(const void* p, const int64_t* strides, int64_t rows, int64_t D, int dtype) {
   const int e = esize(dtype);
-  return Operand{(const char*)p, strides[0] * e, strides[1] * e, strides[2] * e};
+  return Operand{(const char*)p, strides[0] * e, strides[1] * e, row_stride(strides, rows, D) * e};
 }
 
 }  // namespace xat
