@@ -1,0 +1,59 @@
+"""Derivatives of the decoder layer's operators that they do not have are refused,
+not answered with zeros; those that they have also trace whole."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import trnsparse_amd as ts
+
+pytestmark = pytest.mark.gpu
+
+D = 64
+
+
+def _operators():
+    """(call, inputs that could carry a derivative)"""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    pos, f = torch.arange(5, device="cuda"), ts.rope_frequencies(D, device="cuda")
+    heads = (r(2, 4, 5, D), r(2, 2, 5, D))
+    return [
+        (ts.cross_attention, (*heads, r(2, 2, 5, D))),
+        (lambda *t: ts.qk_norm_rope(*t[:4], pos, t[4])[0], (*heads, r(D), r(D), f)),
+        (ts.shared_prefix_attention, (heads[0], r(2, 7, D), r(2, 7, D), heads[1], r(2, 2, 5, D))),
+    ]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_is_refused(hip_backend, which):
+    """No operator has forward-mode derivatives: an input with a tangent is
+    refused, whichever it is, not answered with a tangent of zero."""
+    fn, inputs = _operators()[which]
+    want = fn(*inputs)
+    with fwAD.dual_level():
+        assert torch.equal(fn(*inputs), want)
+        for i in range(len(inputs)):
+            args = list(inputs)
+            args[i] = fwAD.make_dual(inputs[i], torch.ones_like(inputs[i]))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    fn(*args)
+    ones = tuple(torch.ones_like(t) for t in inputs)
+    for call in (lambda: torch.func.jvp(fn, inputs, ones), lambda: torch.func.vjp(fn, *inputs),
+                 lambda: torch.func.grad(lambda q: fn(q, *inputs[1:]).sum())(inputs[0])):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.mark.parametrize("which", range(2))
+def test_forward_mode_of_a_gradient_is_refused(hip_backend, which):
+    fn, inputs = _operators()[which]
+    q = inputs[0].clone().requires_grad_()
+    out = fn(q, *inputs[1:])
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, q, dual)

@@ -810,6 +810,14 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return std::any_of(ts.begin(), ts.end(), [](const at::Tensor* t) { return t->requires_grad(); });
 }
 
+// Forward-mode derivatives are not formed. An input with a tangent need not
+// require a gradient, and below autograd its tangent would be lost: refused.
+void no_tangents(const char* who, std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), who, " has no forward-mode derivatives: an input has a "
+                "tangent");
+}
+
 // A captured backward joins the stream on which its leaves' gradient
 // accumulators were made. One that an eager graph (or a hook) of the same leaves
 // keeps alive belongs to a stream outside the capture, and joining that ends the
@@ -831,8 +839,9 @@ void capture_owns(const char* who, std::initializer_list<const at::Tensor*> ts) 
   }
 }
 
-void first_order(const char* who) {
+void first_order(const char* who, const ag::variable_list& grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, " has no second derivatives: backward with create_graph=False");
+  for (const at::Tensor& g : grads) no_tangents(who, {&g});
 }
 
 at::Tensor cross_attention(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
@@ -856,7 +865,7 @@ struct CrossAttention : public ag::Function<CrossAttention> {
     return O;
   }
   static ag::variable_list backward(ag::AutogradContext* ctx, const ag::variable_list& grads) {
-    first_order("cross_attention");
+    first_order("cross_attention", grads);
     const auto s = ctx->get_saved_variables();
     const bool need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     static const auto op = op_of("trnsparse_hip::cross_attn_bwd", &cross_attn_bwd);
@@ -870,6 +879,7 @@ struct CrossAttention : public ag::Function<CrossAttention> {
 
 at::Tensor cross_attention_autograd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V,
                                     const c10::optional<at::Tensor>& key_lengths, double scale) {
+  no_tangents("cross_attention", {&Q, &K, &V});
   if (wants_grad({&Q, &K, &V})) {
     capture_owns("cross_attention", {&Q, &K, &V});
     return CrossAttention::apply(Q, K, V, key_lengths, scale);
@@ -877,6 +887,14 @@ at::Tensor cross_attention_autograd(const at::Tensor& Q, const at::Tensor& K, co
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = op_of("trnsparse_hip::cross_attention", &cross_attention);
   return op.call(Q, K, V, key_lengths, scale);
+}
+
+at::Tensor prefix_attn_autograd(const at::Tensor& Q, const at::Tensor& PK, const at::Tensor& PV, const at::Tensor& K,
+                                const at::Tensor& V, const c10::optional<at::Tensor>& lengths, double scale) {
+  no_tangents("shared_prefix_attention", {&Q, &PK, &PV, &K, &V});
+  at::AutoDispatchBelowADInplaceOrView below;
+  static const auto op = op_of("trnsparse_hip::prefix_attn_fwd", &prefix_attn_fwd);
+  return op.call(Q, PK, PV, K, V, lengths, scale);
 }
 
 struct QKNormRope : public ag::Function<QKNormRope> {
@@ -892,7 +910,7 @@ struct QKNormRope : public ag::Function<QKNormRope> {
     return {q, k};
   }
   static ag::variable_list backward(ag::AutogradContext* ctx, const ag::variable_list& grads) {
-    first_order("qk_norm_rope");
+    first_order("qk_norm_rope", grads);
     const auto s = ctx->get_saved_variables();
     const bool need_w = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
     auto grad = [&](int i) {  // a result that was not used
@@ -909,6 +927,7 @@ struct QKNormRope : public ag::Function<QKNormRope> {
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& wq,
                                                          const at::Tensor& wk, const at::Tensor& pos,
                                                          const at::Tensor& freq, double eps, bool interleaved) {
+  no_tangents("qk_norm_rope", {&Q, &K, &wq, &wk, &freq});
   if (wants_grad({&Q, &K, &wq, &wk})) {
     capture_owns("qk_norm_rope", {&Q, &K, &wq, &wk});
     auto r = QKNormRope::apply(Q, K, wq, wk, pos, freq, eps, interleaved);
@@ -984,6 +1003,7 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(trnsparse_hip, AutogradCUDA, m) {
   m.impl("cross_attention", &cross_attention_autograd);
+  m.impl("prefix_attn_fwd", &prefix_attn_autograd);
   m.impl("qk_norm_rope", &qk_norm_rope_autograd);
 }
 
