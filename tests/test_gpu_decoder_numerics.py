@@ -19,7 +19,8 @@ import torch
 
 import trnsparse_amd as ts
 from oracle import layer
-from test_gpu_cross_attention import BF, E, HF, make
+import test_gpu_qk_norm_rope as norm_rope
+from test_gpu_cross_attention import BF, E, F32, HF, make
 
 NORM = 1.25  # of u
 
@@ -54,7 +55,7 @@ def check_fp16_gradients(Q, K, V, dO):
     N, D, L, sc, top = Q.shape[2], Q.shape[3], K.shape[2], Q.shape[3] ** -0.5, torch.finfo(HF).max
     r = layer.attention(Q, K, V, sc, None, dO)
     inner = 2 * (D + 4) * r["smax"] + 2 * L + 64 + 4 * float(r["lse"].abs().max()) + 2 * D
-    dS = 2.0**-39 * 2 * D * float(dO.abs().max()) * float(V.abs().max()) * sc
+    dS = 2.0**-39 * 2 * D * float(dO.abs().max()) * float(V.detach().abs().max()) * sc
     off = 2.0**-25 * float(dO.abs().sum(3).max()) * sc
     size = lambda t: t.detach().double().cpu().abs()  # noqa: E731
     col = lambda t: size(t).sum(2, keepdim=True)  # noqa: E731
@@ -114,3 +115,23 @@ def test_one_key_outweighs_many(hip_backend, H, N, at):
     assert (O == O[:, :1, :1]).all()
     far = (O[:, :1, :1].double().cpu() - want).norm() / want.norm()
     assert far <= (1 + 3**-0.5) * 2.0**-11, float(far) * 2**11
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-6), (1e-13, 0.0), (1e-16, 1e-30)])
+def test_norms_of_any_size(hip_backend, size, eps, dt):
+    """Rows whose inverse norm's third power leaves 32 bits, on the bounds of
+    test_gpu_qk_norm_rope."""
+    Q, K, *rest = norm_rope.make(2, 4, 2, 30, 128, dt)
+    Q, K = ((size * t.float()).to(dt) for t in (Q, K))
+    f, pos = ts.rope_frequencies(128, device="cuda"), torch.arange(30, device="cuda")
+    norm_rope.check(Q, K, *rest, pos, f, eps)
+
+
+@pytest.mark.gpu
+def test_zero_rows_and_a_small_eps(hip_backend):
+    """A row of zeros has the gradient w dn / sqrt(eps)."""
+    Q, K, *rest = norm_rope.make(2, 4, 2, 30, 128, F32)
+    f, pos = ts.rope_frequencies(128, device="cuda"), torch.arange(30, device="cuda")
+    norm_rope.check(torch.zeros_like(Q), K, *rest, pos, f, 1e-28)

@@ -6,7 +6,7 @@
 // for the pair (a, b) of every frequency f_j, j < rot / 2: (j, j + rot / 2), or
 // (2 j, 2 j + 1) interleaved; elements from rot on are not rotated. Backward:
 // dn is dy rotated back, dw = sum_rows dn x r and
-//   dx_d = r (w_d dn_d) - x_d r^3 / D sum_e x_e w_e dn_e.
+//   dx_d = r (w_d dn_d - x_d r (r / D sum_e x_e w_e dn_e)).
 // No counterpart in the reference, whose attention takes Q and K as they are
 // (trnsparse/ops.py:549-625).
 //
@@ -352,7 +352,8 @@ __global__ __launch_bounds__(256) void norm_rope_bwd(const Args g) {
           }
         }
         const float r = inv_sqrt<E>(lanes_sum<G>(ss) / (float)g.D + g.eps);
-        const float c = r * r * r * invD * lanes_sum<G>(sw);
+        // (r before the sums: r^3 alone leaves 32 bits for rows of 1e-13 or 1e13)
+        const float c = r * lanes_sum<G>(sw) * invD;
         const int hd = step * GW + grp;
         char* out = (char*)s.y.p + b * s.y.b + hd * s.y.h + i * s.y.s;
 #pragma unroll
@@ -360,8 +361,9 @@ __global__ __launch_bounds__(256) void norm_rope_bwd(const Args g) {
 #pragma unroll
           for (int e = 0; e < 2 * CE; ++e) {
             // (a lane without a row holds zeros, and r may be infinite there)
-            dw[sd][j][e] += hd < s.H ? d[j][e] * (x[j][e] * r) : 0.f;
-            x[j][e] = r * (w[sd][j][e] * d[j][e]) - x[j][e] * c;
+            const float u = x[j][e] * r;
+            dw[sd][j][e] += hd < s.H ? d[j][e] * u : 0.f;
+            x[j][e] = r * (w[sd][j][e] * d[j][e] - u * c);
           }
           if (hd < s.H) store2<E, CE>(out, x[j], p[j]);
         }
