@@ -57,3 +57,15 @@ def test_forward_mode_of_a_gradient_is_refused(hip_backend, which):
         dual = fwAD.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(out, q, dual)
+
+
+def test_frequencies_have_no_gradient(hip_backend):
+    """inv_freq that asks for a gradient is refused, in either float type and
+    whatever else asks for one; under no_grad it is taken."""
+    fn, inputs = _operators()[1]
+    for f in (inputs[4], inputs[4].float()):
+        for q in (inputs[0], inputs[0].clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="inv_freq"):
+                fn(q, *inputs[1:4], f.clone().requires_grad_())
+        with torch.no_grad():
+            fn(*inputs[:4], f.clone().requires_grad_())

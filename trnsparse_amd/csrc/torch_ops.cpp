@@ -928,6 +928,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& Q, co
                                                          const at::Tensor& wk, const at::Tensor& pos,
                                                          const at::Tensor& freq, double eps, bool interleaved) {
   no_tangents("qk_norm_rope", {&Q, &K, &wq, &wk, &freq});
+  TORCH_CHECK(!wants_grad({&freq}), "qk_norm_rope has no gradient of inv_freq: pass inv_freq.detach()");
   if (wants_grad({&Q, &K, &wq, &wk})) {
     capture_owns("qk_norm_rope", {&Q, &K, &wq, &wk});
     auto r = QKNormRope::apply(Q, K, wq, wk, pos, freq, eps, interleaved);

@@ -972,6 +972,6 @@ def hip_qk_norm_rope(Q, K, q_weight, k_weight, positions, inv_freq, eps: float, 
     if freq.dtype != torch.float64 or not freq.is_contiguous():
         if not freq.is_floating_point():
             raise RuntimeError(f"qk_norm_rope: inv_freq must be floating values, got {freq.dtype}")
-        freq = freq.detach().double().contiguous()
+        freq = freq.double().contiguous()
     out = _lib.ops().qk_norm_rope(q, k, wq.contiguous(), wk.contiguous(), pos, freq, eps, interleaved)
     return out if q is Q else tuple(t.to(Q.device) for t in out)

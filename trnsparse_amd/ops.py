@@ -708,7 +708,9 @@ def qk_norm_rope(
     are int32 or int64.
 
     float32, bfloat16 and float16 on the HIP backend, head_dim even and at most
-    256. Differentiable in Q, K and the weights.
+    256; squares are summed in float32, whose range they have to stay in.
+    Differentiable in Q, K and the weights; the HIP backend refuses an inv_freq
+    that requires a gradient.
     """
     if _use_hip():
         from .hip.dispatch import hip_qk_norm_rope
