@@ -8,6 +8,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 import trnsparse_amd as ts
+from test_gpu_graphs import _capture
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,35 @@ def test_frequencies_have_no_gradient(hip_backend):
                 fn(q, *inputs[1:4], f.clone().requires_grad_())
         with torch.no_grad():
             fn(*inputs[:4], f.clone().requires_grad_())
+
+
+def test_capture_from_leaves_that_an_eager_graph_holds(hip_backend):
+    """The operators' inputs come from a fused projection within the capture:
+    an eager graph of its leaves is found there too, and refused before anything
+    is recorded; one of other leaves does not matter, and released, the step is
+    captured."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x, W, other = r(1, 40, 32), r(32, 6 * D).requires_grad_(), r(D).requires_grad_()
+    pos, f = torch.arange(40, device="cuda"), ts.rope_frequencies(D, device="cuda")
+
+    def heads():
+        q, k, v = ((x @ W).view(1, 40, 6, D)[:, :, 2 * i : 2 * i + 2].transpose(1, 2) for i in range(3))
+        return q, k, v
+
+    for fn in (lambda: ts.cross_attention(*heads()), lambda: ts.qk_norm_rope(*heads()[:2], other, other, pos, f)[0]):
+        held = fn()
+        with pytest.raises(RuntimeError, match="release it before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fn()
+        ones = torch.ones_like(held)
+        want = torch.autograd.grad(held, W, ones)[0]
+        del held
+        apart = (r(D).requires_grad_() * 2).sum()
+        graph, (got,) = _capture(lambda: torch.autograd.grad(fn(), W, ones)[0])
+        for _ in range(2):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        del apart

@@ -19,12 +19,15 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <string>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "trnsparse_hip.h"
 
@@ -821,7 +824,9 @@ void no_tangents(const char* who, std::initializer_list<const at::Tensor*> ts) {
 // A captured backward joins the stream on which its leaves' gradient
 // accumulators were made. One that an eager graph (or a hook) of the same leaves
 // keeps alive belongs to a stream outside the capture, and joining that ends the
-// process: refused here, before anything of the step is recorded.
+// process: refused here, before anything of the step is recorded. The leaves are
+// the inputs themselves, or those that the capture has come from to an input (its
+// graph is followed as far as it was made on the captured stream).
 void capture_owns(const char* who, std::initializer_list<const at::Tensor*> ts) {
   if ((*ts.begin())->key_set().has(c10::DispatchKey::Python)) return;  // traced: no stream
   const at::Device dev = (*ts.begin())->device();
@@ -829,13 +834,25 @@ void capture_owns(const char* who, std::initializer_list<const at::Tensor*> ts) 
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (!st || hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
   const c10::Stream here = c10::impl::VirtualGuardImpl(dev.type()).getStream(dev);
+  std::vector<ag::Node*> todo;
+  std::unordered_set<ag::Node*> seen;
+  auto add = [&](ag::Node* n) {
+    if (n && seen.insert(n).second) todo.push_back(n);
+  };
   for (const at::Tensor* t : ts) {
-    if (!t->requires_grad() || !t->is_leaf()) continue;
-    const auto acc = ag::impl::try_get_grad_accumulator(*t);
-    const auto made = acc ? acc->stream() : c10::nullopt;
-    TORCH_CHECK(!made || *made == here, who, ": an input that needs its gradient is held by an autograd graph or hook "
-                "made on another stream than the one being captured; release it before the capture, or call under "
-                "torch.no_grad()");
+    if (!t->requires_grad()) continue;
+    add(t->is_leaf() ? ag::impl::try_get_grad_accumulator(*t).get() : t->grad_fn().get());
+  }
+  while (!todo.empty()) {
+    ag::Node* n = todo.back();
+    todo.pop_back();
+    const auto made = n->stream();
+    const bool ours = !made || *made == here;
+    TORCH_CHECK(ours || !dynamic_cast<ag::AccumulateGrad*>(n), who, ": an input that needs its gradient, or what it "
+                "comes from, is held by an autograd graph or hook made on another stream than the one being captured; "
+                "release it before the capture, or call under torch.no_grad()");
+    if (ours)
+      for (const ag::Edge& e : n->next_edges()) add(e.function.get());
   }
 }
 
