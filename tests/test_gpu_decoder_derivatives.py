@@ -9,6 +9,7 @@ import torch.autograd.forward_ad as fwAD
 
 import trnsparse_amd as ts
 from test_gpu_graphs import _capture
+from trnsparse_amd.hip import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +103,22 @@ def test_capture_from_leaves_that_an_eager_graph_holds(hip_backend):
             torch.cuda.synchronize()
             assert torch.equal(got, want)
         del apart
+
+
+def test_fullgraph_with_gradients(hip_backend):
+    """The operators trace whole with their gradients, in one graph."""
+    ops = _lib.ops()
+    g = torch.Generator(device="cuda").manual_seed(13)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    w, pos, f = r(D), torch.arange(20, device="cuda"), ts.rope_frequencies(D, device="cuda")
+
+    def whole(q, k, v, wq):
+        q2, k2 = ops.qk_norm_rope(q, k, wq, w, pos, f, 1e-6, False)
+        return ops.cross_attention(q2 * 2.0, k2, v, None, 0.125) + 1.0
+
+    leaves = [t.requires_grad_() for t in (r(1, 4, 20, D), r(1, 2, 20, D), r(1, 2, 20, D), r(D))]
+    out = whole(*leaves)
+    want = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    traced = torch.compile(whole, fullgraph=True, backend="aot_eager")(*leaves)
+    got = torch.autograd.grad(traced, leaves, torch.ones_like(out))
+    assert torch.equal(traced, out) and all(torch.equal(a, b) for a, b in zip(got, want))

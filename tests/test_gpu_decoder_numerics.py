@@ -21,6 +21,7 @@ import trnsparse_amd as ts
 from oracle import layer
 import test_gpu_qk_norm_rope as norm_rope
 from test_gpu_cross_attention import BF, E, F32, HF, make
+from test_gpu_cross_attention_backward import LARGE
 
 NORM = 1.25  # of u
 
@@ -40,6 +41,18 @@ def step(size, dt, seed=15):
     Q, K, V = make(*size, dt, seed=seed)
     g = torch.Generator(device="cuda").manual_seed(seed + 1)
     return Q, K, V, (2.0**8 * torch.randn(Q.shape, device="cuda", generator=g)).to(dt)
+
+
+def test_the_norm_notices_a_missing_range():
+    """A range of 128 of 33000 keys left out of one head's dQ, in the oracle."""
+    g = torch.Generator().manual_seed(19)
+    Q, dO, K, V = (torch.randn(n, 128, generator=g, dtype=torch.float64) for n in (16, 16, 33000, 33000))
+    p = (Q @ K.t() * 128**-0.5).softmax(1)
+    dp = dO @ V.t()
+    ds = p * (dp - (p * dp).sum(1, keepdim=True))
+    dQ = ds @ K
+    ds[:, 640:768] = 0
+    assert (ds @ K - dQ).norm() > 10 * NORM * 2.0**-8 * dQ.norm()  # bf16's bound
 
 
 def check_fp16_gradients(Q, K, V, dO):
@@ -78,6 +91,22 @@ def test_many_keys(hip_backend, size, dt):
     """P and dS of many keys are small: fp16 keeps their digits all the same."""
     e = gradient_errors(*step(size, dt))
     assert max(e.values()) <= NORM, e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("size", LARGE + [(2, 4, 2, 70, 90, 64), (1, 4, 2, 200, 300, 96)])
+def test_steps(hip_backend, size, dt):
+    """Both passes in one launch and apart, keys and queries in ranges; the
+    queries' gradient alone, from the row pass alone."""
+    Q, K, V, dO = step(size, dt)
+    e = gradient_errors(Q, K, V, dO)
+    assert max(e.values()) <= NORM, e
+    q = Q.detach().requires_grad_()
+    alone = torch.autograd.grad(ts.cross_attention(q, K, V), q, dO)[0].double()
+    leaves = [t.detach().requires_grad_() for t in (Q, K, V)]
+    dQ = torch.autograd.grad(ts.cross_attention(*leaves), leaves, dO)[0].double()
+    assert (alone - dQ).norm() <= 2 * NORM * torch.finfo(dt).eps / 2 * dQ.norm()
 
 
 @pytest.mark.gpu
