@@ -164,3 +164,23 @@ def test_zero_rows_and_a_small_eps(hip_backend):
     Q, K, *rest = norm_rope.make(2, 4, 2, 30, 128, F32)
     f, pos = ts.rope_frequencies(128, device="cuda"), torch.arange(30, device="cuda")
     norm_rope.check(torch.zeros_like(Q), K, *rest, pos, f, 1e-28)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(11, 64, 16, 1, 128, 128), (2, 64, 8, 554, 128, 128), (1, 128, 16, 1, 96, 96),
+                                  (2, 32, 8, 4096, 128, 128)])
+def test_weight_gradients_in_fp32(hip_backend, size):
+    """The 2-norm of a weight gradient's error. A term dn x r takes about eight
+    roundings to 24 bits (cosine and sine, two products and their sum, r, x r, the
+    workgroup's part, the result), 2^-24 / sqrt(3) each at most: 1.63 times 2^-24.
+    Sums of the terms in 24 bits would add to it with their number."""
+    *shape, rot = size
+    Q, K, wq, wk, gQ, gK = norm_rope.make(*shape, F32, seed=21)
+    g = torch.Generator(device="cuda").manual_seed(22)
+    pos = torch.randint(0, 4_000_000, (shape[0], shape[3]), device="cuda", generator=g)
+    f = ts.rope_frequencies(rot, device="cuda")
+    leaves = [t.detach().requires_grad_() for t in (Q, K, wq, wk)]
+    grads = torch.autograd.grad(ts.qk_norm_rope(*leaves, pos, f), leaves[2:], (gQ, gK))
+    for got, x, w, dy in zip(grads, (Q, K), (wq, wk), (gQ, gK)):
+        want = layer.norm_rope(x, w, pos, f, 1e-6, False, dy)["dw"]
+        assert (got.double().cpu() - want).norm() <= 1.75 * 2.0**-24 * want.norm()
