@@ -824,16 +824,24 @@ void no_tangents(const char* who, std::initializer_list<const at::Tensor*> ts) {
 // A captured backward joins the stream on which its leaves' gradient
 // accumulators were made. One that an eager graph (or a hook) of the same leaves
 // keeps alive belongs to a stream outside the capture, and joining that ends the
-// process: refused here, before anything of the step is recorded. The leaves are
-// the inputs themselves, or those that the capture has come from to an input (its
-// graph is followed as far as it was made on the captured stream).
+// process: refused here, before anything of the step is recorded. Inputs that are
+// leaves: any other stream. Inputs that the capture has made of leaves: the default
+// stream, which no capture can take in (a side stream's accumulators, as a data
+// parallel wrapper keeps them, wait for the captured work and so come into the
+// capture); their graph is followed as far as it was made on the captured stream.
 void capture_owns(const char* who, std::initializer_list<const at::Tensor*> ts) {
   if ((*ts.begin())->key_set().has(c10::DispatchKey::Python)) return;  // traced: no stream
   const at::Device dev = (*ts.begin())->device();
   const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (!st || hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
-  const c10::Stream here = c10::impl::VirtualGuardImpl(dev.type()).getStream(dev);
+  const c10::impl::VirtualGuardImpl impl(dev.type());
+  const c10::Stream here = impl.getStream(dev), outside = impl.getDefaultStream(dev);
+  auto refuse_if = [&](bool held) {
+    TORCH_CHECK(!held, who, ": an input that needs its gradient, or what it comes from, is held by an autograd graph or "
+                "hook made on another stream than the one being captured; release it before the capture, or call "
+                "under torch.no_grad()");
+  };
   std::vector<ag::Node*> todo;
   std::unordered_set<ag::Node*> seen;
   auto add = [&](ag::Node* n) {
@@ -841,17 +849,20 @@ void capture_owns(const char* who, std::initializer_list<const at::Tensor*> ts) 
   };
   for (const at::Tensor* t : ts) {
     if (!t->requires_grad()) continue;
-    add(t->is_leaf() ? ag::impl::try_get_grad_accumulator(*t).get() : t->grad_fn().get());
+    if (!t->is_leaf()) {
+      add(t->grad_fn().get());
+      continue;
+    }
+    const auto acc = ag::impl::try_get_grad_accumulator(*t);
+    const auto made = acc ? acc->stream() : c10::nullopt;
+    refuse_if(made && *made != here);
   }
   while (!todo.empty()) {
     ag::Node* n = todo.back();
     todo.pop_back();
     const auto made = n->stream();
-    const bool ours = !made || *made == here;
-    TORCH_CHECK(ours || !dynamic_cast<ag::AccumulateGrad*>(n), who, ": an input that needs its gradient, or what it "
-                "comes from, is held by an autograd graph or hook made on another stream than the one being captured; "
-                "release it before the capture, or call under torch.no_grad()");
-    if (ours)
+    refuse_if(made && *made == outside && dynamic_cast<ag::AccumulateGrad*>(n));
+    if (!made || *made == here)
       for (const ag::Edge& e : n->next_edges()) add(e.function.get());
   }
 }
