@@ -417,9 +417,14 @@ struct BwdPlan {
 // Ranges for 512 workgroups, where there are less than half of that. An fp32
 // workgroup has a CU to itself, so one round of them is 256 and the ranges are as
 // many as fit (2 x 8 heads of 512 x 512 x 128 108 us, for 512 workgroups 142; 12
-// heads over 4 of 1000 x 200 x 64 52 and 66) - but not with lengths, which leave
-// ranges empty: 3 x 8 heads of 257 x up to 383 x 80 94 us, for 512 87. Lengths
-// never take fewer ranges, so the workspace that does for them does for all.
+// heads over 4 of 1000 x 200 x 64 52 and 66) - but not of a padded batch. Its
+// lengths, which the host does not know, leave ranges empty, and one round then
+// takes as long as its longest: with entries a quarter to all full, 3 x 6 heads of
+// 700 x 900 x 96 take 190 to 210 us, in one round 279; 3 x 8 of 257 x 383 x 80 with
+// an empty one 65 to 71 and 75. What a batch whose entries are all full pays for that: 2 x 8 heads of 512
+// x 512 x 128 141 us for 109, 2 x 4 over 2 of 300 x 2000 x 128 160 for 126, 3 x 6 of
+// 700 x 900 x 96 the same. Padded batches never take fewer ranges, so the workspace
+// that does for them does for all.
 BwdPlan bwd_plan(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D, bool lengths) {
   BwdPlan p{};
   const int64_t G = Hq / Hkv, units = B * Hkv, stage = dtype == TSP_F32 ? 32 : 64;

@@ -20,8 +20,8 @@
 // angles of one pair for all of them (every lane its own chunk's: 77 and 128
 // us; without the next rows' loads ahead 95 and 147). Angles are products in 64
 // bits, reduced to half turns there: a position of 10^6 would leave an fp32
-// product no correct digit after the point. Sums, norms and weight gradients
-// are fp32; a result is rounded once.
+// product no correct digit after the point. Sums and norms are fp32; a result is
+// rounded once.
 //
 // Weight gradients: every workgroup sums its tokens' rows in registers and
 // writes one part; wgrad_kernel adds the parts in a fixed order, so results do
@@ -106,7 +106,8 @@ struct Angles {
       c[k] = 1.f;
       s[k] = 0.f;
       if (k < rounds && lane + 64 * k < g.rot / 2) {
-        // less whole turns, 2 pi in two parts: right to 2^-50 at any angle
+        // less whole turns, 2 pi in two parts: adds at most 2^-50 up to 2^53 turns.
+        // (The product itself is off by 2^-53 of the angle.)
         double angle = t * g.freq[lane + 64 * k];
         const double turns = __builtin_rint(angle * 0.15915494309189535);
         angle = __builtin_fma(-turns, 6.283185307179586477, angle);

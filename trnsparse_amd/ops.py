@@ -593,7 +593,8 @@ def cross_attention(
 
     float32, bfloat16 and float16 on the HIP backend, accumulated in float32.
     Operands may be strided views (heads of a projection's output); the result
-    has Q's order of heads and rows. Differentiable in Q, K and V.
+    has Q's order of heads and rows (contiguous where head_dim is not whole
+    16-byte pieces). Differentiable in Q, K and V.
     """
     if scale is None:
         scale = _default_scale(Q)
