@@ -678,6 +678,89 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
                         int64_t workspace_bytes, void* stream);
 
 /* ====================================================================
+ * A key and value cache in pages (serving): its attention, the write of new
+ * tokens into it, and the eviction that keeps a budget of its rows.
+ *
+ * K_pages and V_pages are (pages, kv_heads, page_size, head_dim) views with
+ * unit stride over head_dim; `*_pages_strides` points to three int64 in host
+ * memory: the strides in elements of the page, head and row dimensions.
+ * Pointers and strides are whole 16-byte pieces and not negative, row strides
+ * at least head_dim and below 16 MiB; page_size is a multiple of 16; head_dim
+ * and dtype as above. Row j of sequence b is row j % page_size of page
+ * block_table[b * table_stride + j / page_size], a column below `columns`;
+ * entries are of table_type (TSP_I32 or TSP_I64). slots = columns * page_size,
+ * the rows a sequence may have, is at most 2^30, and slots * page_size below
+ * 2^40. An entry outside [0, pages) is a page of zeros that cannot be written.
+ * A page that is written belongs to one sequence: what two writes to one row
+ * leave is not defined.
+ * lengths and new_lengths (batch,) are of index_type and are taken into
+ * [0, slots] and [0, queries or tokens]; new_lengths NULL: all. weights
+ * (batch, kv_heads, slots) fp32, unit stride over slots; weight_strides: two
+ * int64 in host memory, the strides of batch and head.
+ * No counterpart in the reference, whose attention takes one sequence's K and
+ * V whole (trnsparse/ops.py:549-625).
+ *
+ * tsp_paged_attn_fwd: lengths[b] rows are in the cache, the last m =
+ *   new_lengths[b] of them the new tokens', whose queries are Q[b, :, :m] of Q
+ *   (batch, heads, queries, head_dim):
+ *     O[b,h,i] = sum_j softmax_j(scale Q[b,h,i].K_j) V_j, j < lengths[b] - (m - 1 - i)
+ *   with key head h / (heads / kv_heads); rows i >= m, and rows that see no key,
+ *   are zero. With weights not NULL, weights[b,hk,j] += the softmax weight of
+ *   key j, summed over the key head's query heads and the queries. Strides,
+ *   alignment and scale of Q and O as in tsp_cross_attn_fwd. workspace:
+ *   tsp_paged_attn_workspace_size bytes, `keys` being slots, `ragged` whether
+ *   new_lengths is given and `weights` whether weights is.
+ *
+ * tsp_paged_append: K[b, :, i] and V[b, :, i] of (batch, kv_heads, tokens,
+ *   head_dim), i < new_lengths[b], become row lengths[b] + i; rows past slots
+ *   are left out. weights, where not NULL, is set to zero there. lengths_out
+ *   (batch,), not lengths itself, receives min(lengths[b] + new_lengths[b], slots).
+ *
+ * tsp_paged_evict: a sequence of more than `budget` rows keeps, for each key
+ *   head, its last `recent` rows (0 <= recent <= budget) and of the others the
+ *   budget - recent of the largest weights: of equal ones the first, NaN above
+ *   all numbers. The kept rows of K, V and weights move to rows [0, budget) in
+ *   their order; what stands behind is left as it was. lengths_out, not lengths
+ *   itself, receives min(lengths[b], budget). K_pages and V_pages must not
+ *   overlap.
+ * ==================================================================== */
+int64_t tsp_paged_attn_workspace_size(int dtype, int64_t batch, int64_t heads,
+                                      int64_t kv_heads, int64_t queries,
+                                      int64_t keys, int64_t head_dim, int ragged,
+                                      int weights);
+int tsp_paged_attn_fwd(const void* Q, const int64_t* q_strides,
+                       const void* K_pages, const int64_t* k_pages_strides,
+                       const void* V_pages, const int64_t* v_pages_strides,
+                       int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                       int64_t queries, int64_t pages, int64_t page_size,
+                       int64_t head_dim, const void* block_table, int table_type,
+                       int64_t table_stride, int64_t columns, const void* lengths,
+                       const void* new_lengths, int index_type, double scale,
+                       void* O, const int64_t* o_strides, float* weights,
+                       const int64_t* weight_strides, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int tsp_paged_append(const void* K, const int64_t* k_strides, const void* V,
+                     const int64_t* v_strides, void* K_pages,
+                     const int64_t* k_pages_strides, void* V_pages,
+                     const int64_t* v_pages_strides, int dtype, int64_t batch,
+                     int64_t kv_heads, int64_t tokens, int64_t pages,
+                     int64_t page_size, int64_t head_dim, const void* block_table,
+                     int table_type, int64_t table_stride, int64_t columns,
+                     const void* lengths, const void* new_lengths, int index_type,
+                     void* lengths_out, float* weights,
+                     const int64_t* weight_strides, void* stream);
+int64_t tsp_paged_evict_workspace_size(int64_t batch, int64_t kv_heads,
+                                       int64_t budget);
+int tsp_paged_evict(void* K_pages, const int64_t* k_pages_strides, void* V_pages,
+                    const int64_t* v_pages_strides, int dtype, int64_t batch,
+                    int64_t kv_heads, int64_t pages, int64_t page_size,
+                    int64_t head_dim, const void* block_table, int table_type,
+                    int64_t table_stride, int64_t columns, const void* lengths,
+                    int index_type, float* weights, const int64_t* weight_strides,
+                    int64_t budget, int64_t recent, void* lengths_out,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ====================================================================
  * RMS norm of query and key heads and their rotation by position.
  *
  * For every head vector x of Q (batch, q_heads, tokens, head_dim) and K

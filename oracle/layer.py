@@ -16,7 +16,8 @@ import torch
 def attention(Q, K, V, scale, seen=None, dO=None):
     """Q (B, H, N, D); K, V (B, Hk, L, D); seen (B, N, L) bool or None.
 
-    Returns a dict in float64: O; lse; A = P |V| (the error scale of O); smax =
+    Returns a dict in float64: O; lse; A = P |V| (the error scale of O); W (B, Hk,
+    L), the weight P of every key summed over its heads and queries; smax =
     largest sum_d scale |q_d k_d| of a seen pair; with dO also dQ, dK, dV and
     their scales aQ = (P W) |K| scale, aK = (P W)^T |Q| scale, aV = P^T |dO|, W
     = |dO| |V|^T + rowsum |dO| A.
@@ -27,6 +28,7 @@ def attention(Q, K, V, scale, seen=None, dO=None):
     G = H // Hk
     f = dict(dtype=torch.float64)
     r = {"O": torch.zeros(B, H, N, D, **f), "A": torch.zeros(B, H, N, D, **f), "lse": torch.zeros(B, H, N, **f), "smax": 0.0}
+    r["W"] = torch.zeros(B, Hk, L, **f)
     if dO is not None:
         dO = dO.detach().double().cpu()
         for k, t in (("dQ", Q), ("aQ", Q), ("dK", K), ("aK", K), ("dV", K), ("aV", K)):
@@ -47,6 +49,7 @@ def attention(Q, K, V, scale, seen=None, dO=None):
             r["lse"][b, h] = (m + tot.log()).squeeze(1)
             p = p / torch.where(tot == 0, torch.ones_like(tot), tot)
             r["O"][b, h], r["A"][b, h] = p @ v, p @ v.abs()
+            r["W"][b, h // G] += p.sum(0)
             mag = torch.where(ok, q.abs() @ k.abs().t() * scale, torch.zeros((), **f))
             if mag.numel():
                 r["smax"] = max(r["smax"], float(mag.max()))
@@ -69,6 +72,83 @@ def lengths_seen(lengths, N, L, causal=False):
     if causal:
         n = n - (N - 1 - torch.arange(N)).view(1, N, 1)
     return (torch.arange(L) < n).expand(-1, N, -1)
+
+
+def paged_rows(pages, table):
+    """Every sequence's rows in order, (B, Hk, columns * page_size, D), row by row
+    from pages (P, Hk, page_size, D) and table (B, columns); zeros where a table
+    entry names no page."""
+    pages, table = pages.detach().cpu(), table.cpu()
+    count, Hk, size, D = pages.shape
+    B, cols = table.shape
+    out = torch.zeros(B, Hk, cols * size, D, dtype=pages.dtype)
+    for b in range(B):
+        for c in range(cols):
+            if 0 <= int(table[b, c]) < count:
+                out[b, :, c * size : (c + 1) * size] = pages[int(table[b, c])]
+    return out
+
+
+def chunk_seen(lengths, new_lengths, N, L):
+    """seen (B, N, L) of the last m of n cached rows' queries, query i with the
+    rows up to its own: j <= n - m + i. Queries i >= m see nothing."""
+    B = lengths.numel()
+    seen = torch.zeros(B, N, L, dtype=torch.bool)
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), L)
+        m = N if new_lengths is None else min(max(int(new_lengths[b]), 0), N)
+        for i in range(m):
+            seen[b, i, : max(n - m + i + 1, 0)] = True
+    return seen
+
+
+def paged_append(K, V, K_pages, V_pages, table, lengths, new_lengths=None, weights=None):
+    """New copies of (K_pages, V_pages, weights) with the new rows written one at
+    a time, and the new lengths."""
+    K, V, table = K.detach().cpu(), V.detach().cpu(), table.cpu()
+    kp, vp = K_pages.detach().cpu().clone(), V_pages.detach().cpu().clone()
+    w = None if weights is None else weights.cpu().clone()
+    count, _, size, _ = kp.shape
+    L, after = table.shape[1] * size, []
+    for b in range(table.shape[0]):
+        n = min(max(int(lengths[b]), 0), L)
+        m = K.shape[2] if new_lengths is None else min(max(int(new_lengths[b]), 0), K.shape[2])
+        after.append(min(n + m, L))
+        for i in range(after[-1] - n):
+            j = n + i
+            if w is not None:
+                w[b, :, j] = 0
+            p = int(table[b, j // size])
+            if 0 <= p < count:
+                kp[p, :, j % size], vp[p, :, j % size] = K[b, :, i], V[b, :, i]
+    return kp, vp, w, torch.tensor(after, dtype=lengths.dtype)
+
+
+def paged_evict(K_pages, V_pages, weights, table, lengths, budget, recent):
+    """New copies of (K_pages, V_pages, weights) after the eviction, and the new
+    lengths: rows ranked by (NaN, weight, first place) with Python's sort."""
+    kp, vp, w, table = K_pages.detach().cpu().clone(), V_pages.detach().cpu().clone(), weights.cpu().clone(), table.cpu()
+    count, Hk, size, D = kp.shape
+    L, after = table.shape[1] * size, []
+    for b in range(table.shape[0]):
+        n = min(max(int(lengths[b]), 0), L)
+        after.append(min(n, budget))
+        if n <= budget:
+            continue
+        ids = [int(p) for p in table[b]]
+        for h in range(Hk):
+            old = w[b, h].tolist()
+            order = sorted(range(n - recent), key=lambda j: (0, 0.0, j) if math.isnan(old[j]) else (1, -old[j], j))  # noqa: B023
+            kept = sorted(order[: budget - recent]) + list(range(n - recent, n))
+            for pages in (kp, vp):
+                rows = [pages[ids[j // size], h, j % size].clone() if 0 <= ids[j // size] < count
+                        else torch.zeros(D, dtype=pages.dtype) for j in kept]
+                for d, row in enumerate(rows):
+                    if 0 <= ids[d // size] < count:
+                        pages[ids[d // size], h, d % size] = row
+            for d, j in enumerate(kept):
+                w[b, h, d] = old[j]
+    return kp, vp, w, torch.tensor(after, dtype=lengths.dtype)
 
 
 def norm_rope(x, w, positions, inv_freq, eps, interleaved, dy=None):

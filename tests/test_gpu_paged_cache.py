@@ -1,0 +1,147 @@
+"""GPU parity of paged_cache_append and paged_cache_evict: every value is a copy
+of one that was there, so results are equal to the oracle's bit for bit."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import trnsparse_amd as ts
+from oracle import layer
+from test_gpu_paged_attention import BF, F32, HF, make
+
+pytestmark = pytest.mark.gpu
+
+
+def same(got, want):
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a.cpu(), b.cpu(), rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("size", [(1, 1, 1, 1, 16, 64), (5, 3, 7, 6, 48, 40), (3, 8, 40, 9, 16, 128), (2, 2, 300, 3, 128, 8)])
+@pytest.mark.parametrize("itype", [torch.int32, torch.int64])
+def test_append(hip_backend, size, dt, itype):
+    B, Hk, N, cols, ps, D = size
+    K, kp, vp, table = make(B, Hk, Hk, N, cols, ps, D, dt)
+    V = torch.randn_like(K)
+    L = cols * ps
+    table[B - 1, cols - 1] = -1  # a page that is not there
+    for lengths in ([0, 1, ps - 1, L, L - 1], [L // 2, -9, L + 9, ps, 0]):
+        lengths = torch.tensor(lengths[:B], dtype=itype, device="cuda")
+        for new in (None, torch.tensor([N, 0, 1, -1, 9999][:B], dtype=itype, device="cuda")):
+            w = torch.rand(B, Hk, L, device="cuda")
+            want = layer.paged_append(K, V, kp, vp, table, lengths, new, w)
+            after = ts.paged_cache_append(K, V, kp, vp, table, lengths, new, w)
+            assert after.dtype == itype
+            same((kp, vp, w, after), want)
+            ts.paged_cache_append(V, K, kp, vp, table, lengths, new)  # without weights, other values
+            same((w,), (want[2],))
+
+
+def test_append_views(hip_backend):
+    """New rows that are not whole pieces apart; pages in (page, row, head) order;
+    mixed index types."""
+    K, kp, vp, table = make(3, 2, 2, 5, 4, 16, 64, BF)
+    odd = torch.zeros(3, 2, 5, 67, dtype=BF, device="cuda")[..., 1:65]
+    odd.copy_(K)
+    lengths, new = torch.tensor([0, 14, 60], device="cuda"), torch.tensor([5, 2, 5], dtype=torch.int32, device="cuda")
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (kp, vp)]
+    want = layer.paged_append(K, K, kp, vp, table, lengths, new)
+    after = ts.paged_cache_append(odd, odd, *turned, table, lengths, new)
+    same((*turned, after), (want[0], want[1], want[3]))
+    with pytest.raises(RuntimeError):  # written rows on top of each other
+        ts.paged_cache_append(K, K, kp[:1].expand(9, -1, -1, -1), vp[:1].expand(9, -1, -1, -1), table, lengths)
+    with pytest.raises(RuntimeError):
+        ts.paged_cache_append(K, K, kp[..., 1:], vp[..., 1:], table, lengths)
+
+
+# (batch, kv_heads, columns, page_size, head_dim, budget, recent)
+EVICT = [
+    (1, 1, 1, 16, 64, 1, 0), (4, 2, 8, 16, 64, 40, 9), (3, 3, 5, 48, 80, 100, 100), (2, 8, 12, 64, 128, 333, 41),
+    (5, 2, 40, 16, 40, 77, 0), (2, 1, 9, 256, 16, 2000, 300), (2, 2, 600, 16, 8, 4000, 17), (3, 2, 4, 16, 128, 63, 3),
+]
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("size", EVICT)
+@pytest.mark.parametrize("kind", ["random", "ties", "equal"])
+def test_evict(hip_backend, size, dt, kind):
+    B, Hk, cols, ps, D, budget, recent = size
+    _, kp, vp, table = make(B, Hk, Hk, 1, cols, ps, D, dt)
+    L = cols * ps
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn(B, Hk, L, device="cuda", generator=g)
+    w = {"random": w.exp(), "ties": (3 * w).round(), "equal": torch.zeros_like(w)}[kind]
+    lengths = torch.tensor([L, L - 1, budget, budget + 1, 0][:B], device="cuda").int()
+    want = layer.paged_evict(kp, vp, w, table, lengths, budget, recent)
+    after = ts.paged_cache_evict(kp, vp, w, table, lengths, budget, recent)
+    assert after.dtype == torch.int32
+    same((kp, vp, w, after), want)
+
+
+def test_evict_special_weights(hip_backend):
+    """Infinities, NaN of either sign, zeros of either sign, subnormal and negative weights."""
+    _, kp, vp, table = make(2, 3, 3, 1, 4, 64, 32, F32)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(2, 3, 256, device="cuda", generator=g)
+    for i, x in enumerate((float("inf"), float("-inf"), float("nan"), 0.0, -0.0, 1e-45, -1e-45, 1e-40, 3e38)):
+        w[:, :, i::17] = x
+    w[1, 0, 5::31] = -torch.tensor(float("nan"))
+    w[1, 1], w[1, 2] = float("nan"), float("-inf")
+    lengths = torch.tensor([256, 200], device="cuda")
+    for budget, recent in ((9, 0), (30, 4), (120, 60)):
+        k, v, x = kp.clone(), vp.clone(), w.clone()
+        want = layer.paged_evict(k, v, x, table, lengths, budget, recent)
+        same((k, v, x, ts.paged_cache_evict(k, v, x, table, lengths, budget, recent)), want)
+
+
+def test_evict_to_nothing_and_bad_pages(hip_backend):
+    _, kp, vp, table = make(3, 2, 2, 1, 8, 16, 64, BF)
+    table[0, 1], table[1, 6], table[2] = -1, 10**6, 10**6
+    w = torch.rand(3, 2, 128, device="cuda")
+    lengths = torch.tensor([128, 120, 99], device="cuda")
+    for budget, recent in ((50, 20), (0, 0)):
+        want = layer.paged_evict(kp, vp, w, table, lengths, budget, recent)
+        after = ts.paged_cache_evict(kp, vp, w, table, lengths, budget, recent)
+        same((kp, vp, w, after), want)
+    k0 = kp[:0]
+    want = layer.paged_evict(k0, k0, w, table, lengths, 7, 2)
+    same((w,), (layer.paged_evict(k0, k0, w, table, lengths, 128, 2)[2],))
+    after = ts.paged_cache_evict(k0, vp[:0], w, table, lengths, 7, 2)
+    same((w, after), (want[2], want[3]))
+    assert ts.paged_cache_evict(kp, vp, w[..., :0], table[:, :0], lengths, 7).tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("dt,size", [(BF, (2, 4, 300, 128, 128, 9000, 700)), (F32, (1, 2, 2200, 16, 64, 30000, 0)),
+                                     (HF, (20, 8, 40, 32, 96, 501, 60))])
+def test_evict_long(hip_backend, dt, size):
+    """Many parts of a row list, against the "pytorch" backend."""
+    B, Hk, cols, ps, D, budget, recent = size
+    _, kp, vp, table = make(B, Hk, Hk, 1, cols, ps, D, dt)
+    L = cols * ps
+    w = torch.randn(B, Hk, L, device="cuda").exp()
+    w[:, :, ::3] = 0.0
+    lengths = torch.randint(budget - 50, L + 1, (B,), device="cuda")
+    lengths[0] = L
+    k, v, x = kp.clone(), vp.clone(), w.clone()
+    ts.set_backend("pytorch")
+    want = ts.paged_cache_evict(k, v, x, table, lengths, budget, recent)
+    ts.set_backend("hip")
+    after = ts.paged_cache_evict(kp, vp, w, table, lengths, budget, recent)
+    same((kp, vp, w, after), (k, v, x, want))
+
+
+def test_evict_again_and_again(hip_backend):
+    """One row over the budget at a time, as a decoding loop does."""
+    _, kp, vp, table = make(2, 2, 2, 1, 4, 16, 64, BF)
+    w = torch.rand(2, 2, 64, device="cuda")
+    lengths = torch.tensor([41, 41], device="cuda")
+    for i in range(12):
+        want = layer.paged_evict(kp, vp, w, table, lengths, 40, 8)
+        n = ts.paged_cache_evict(kp, vp, w, table, lengths, 40, 8)
+        same((kp, vp, w, n), want)
+        K = torch.full((2, 2, 1, 64), float(i), dtype=BF, device="cuda")
+        lengths = ts.paged_cache_append(K, K, kp, vp, table, n, weights=w)
+        w[:, :, 40] = torch.rand(2, 2, device="cuda")

@@ -7,8 +7,9 @@ block_sparse_attention_tiled and the small CSR helpers) and the backend
 switch (set_backend / get_backend / HAS_NKI), plus the fixed-step solvers
 (richardson_bsr, chebyshev_bsr, chebyshev_coeffs) and what a decoder layer has
 next to the block-sparse attention (cross_attention, shared_prefix_attention,
-qk_norm_rope), which the reference lacks. The compute runs in
-hand-written gfx950 HIP kernels behind the C ABI in include/trnsparse_hip.h.
+qk_norm_rope, and a key and value cache in pages: paged_attention,
+paged_cache_append, paged_cache_evict), which the reference lacks. The compute
+runs in hand-written gfx950 HIP kernels behind the C ABI in include/trnsparse_hip.h.
 """
 
 __version__ = "0.1.0"
@@ -21,6 +22,9 @@ from .ops import (
     bsr_spmm,
     cross_attention,
     nnz_per_row,
+    paged_attention,
+    paged_cache_append,
+    paged_cache_evict,
     qk_norm_rope,
     rope_frequencies,
     screened_mask,
@@ -50,6 +54,9 @@ __all__ = [
     "block_sparse_attention_tiled",
     "cross_attention",
     "shared_prefix_attention",
+    "paged_attention",
+    "paged_cache_append",
+    "paged_cache_evict",
     "qk_norm_rope",
     "rope_frequencies",
     "sparse_add",

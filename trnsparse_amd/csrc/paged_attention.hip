@@ -1,0 +1,751 @@
+// Attention of a chunk of new tokens over a key and value cache in pages
+// (serving): sequence b has n = lengths[b] rows in its pages, the last m =
+// new_lengths[b] of them the new tokens'. Query i of head h, key head hk = h / G:
+//   O[b, h, i] = sum_j p_ij V[b, hk, j],  p_i = softmax_j(scale Q[b, h, i] . K[b, hk, j])
+// over j < n - (m - 1 - i), and on request
+//   W[b, hk, j] += sum over the heads of hk and the queries i of p_ij.
+// No counterpart in the reference, whose attention is one sequence's over its
+// whole K and V (trnsparse/ops.py:549-625).
+//
+// A unit is one (sequence, key head) pair; its rows are r = i G + g (token,
+// head of the group), so that the keys which a run of rows sees end close
+// together. Tiles, softmax and products: xattn_tiles.h.
+//   wide    128 rows to a workgroup, a wavefront to 32; stages of keys that the
+//           four wavefronts share in an LDS ring of two
+//   narrow  up to 32 rows to a workgroup: every wavefront has all of them and
+//           takes every fourth stage of 32 keys through LDS of its own
+// The host does not see the lengths. It gives every unit `items` workgroups;
+// each finds the unit's tiles of rows from its number of new tokens, and where
+// workgroups are left, they take ranges of the keys (share_of). Ranges write
+// their own normalised result and log-sum-exp in fp32, which combine_kernel
+// joins in the ranges' order.
+//
+// The accumulated weights need the final log-sum-exp of every row. Few rows:
+// the narrow kernel keeps its scores (4 bytes a pair, where reading K again is 2
+// head_dim bytes a key) and weigh_kernel adds up their exponentials. Many: the
+// scores are formed again, a wavefront having 32 keys as its own rows and the
+// queries staged, so that a key's sum stays in its lane (weights_wide). Either
+// way one workgroup owns a key and adds in a fixed order: no atomics.
+#include "lds_dma.h"
+#include "paged_cache.h"
+#include "xattn_fwd.h"
+
+namespace tsp {
+namespace xat {
+int check_sizes(const char* who, int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t L, int64_t D);
+}
+namespace paged {
+namespace {
+
+using xat::LOG2E;
+using xat::Operand;
+using xat::OUT_OF_RANGE;
+
+struct Args {
+  Operand Q;
+  char* O;
+  int64_t ob, oh, os;  // strides of O in bytes
+  Pages K, V;
+  Table t;
+  Lengths len;
+  int B, Hkv, G, Sq, R, D;   // R: rows of a unit, G Sq
+  int items;                 // workgroups of a unit
+  int slots;                 // results of ranges that a unit has room for (0: keys stay whole)
+  int least, step;           // a range's least keys, and what it is a multiple of
+  int slot_rows;             // rows of one such result
+  float *part, *plse;        // [unit][slot][row]: results, log-sum-exps (base 2)
+  float* lse;                // [unit][R]: log-sum-exps (base 2) where the weights need them, else null
+  float* scores;             // [unit][stage of 32 keys][R][32], log2 units; else null
+  int stages;                // of a unit
+  float scale_log2;
+  float* W;
+  int64_t wb, wh;
+};
+
+struct Share {
+  int n, m, rows, tiles, splits, chunk;
+};
+// What a unit's workgroups do. Uniform: scalar loads and arithmetic.
+__device__ inline Share share_of(const Args& a, int64_t b, int tile_rows) {
+  Share s;
+  s.n = (int)cached_rows(a.len, b);
+  s.m = (int)new_rows(a.len, b);
+  s.rows = s.m * a.G;
+  s.tiles = (s.rows + tile_rows - 1) / tile_rows;
+  int k = s.tiles ? a.slots / s.tiles : 0;
+  const int most = (s.n + a.least - 1) / a.least;
+  k = k < most ? k : most;
+  k = k < 1 ? 1 : k;
+  const int per = (s.n + k - 1) / k;
+  s.chunk = (per + a.step - 1) / a.step * a.step;
+  s.chunk = s.chunk < a.step ? a.step : s.chunk;
+  s.splits = s.n > 0 ? (s.n + s.chunk - 1) / s.chunk : 1;
+  return s;
+}
+// Keys that a row's token sees.
+__device__ inline int sees_of(const Share& s, int i) { return s.n - (s.m - 1 - i); }
+
+__device__ inline bool unit_of(const Args& a, uint32_t block, int per_unit, uint32_t& unit, uint32_t& b, uint32_t& hk,
+                               int& item) {
+  int64_t u, i;
+  if (!head_item(block, per_unit, (int64_t)a.B * a.Hkv, u, i)) return false;
+  unit = (uint32_t)u;
+  b = unit / (uint32_t)a.Hkv;
+  hk = unit - b * (uint32_t)a.Hkv;
+  item = (int)i;
+  return true;
+}
+
+__device__ inline const char* q_row(const Args& a, int64_t b, int64_t hk, int i, int g) {
+  return a.Q.p + b * a.Q.b + (hk * a.G + g) * a.Q.h + i * a.Q.s;
+}
+__device__ inline char* o_row(const Args& a, int64_t b, int64_t hk, int i, int g) {
+  return a.O + b * a.ob + (hk * a.G + g) * a.oh + i * a.os;
+}
+
+// Rows behind a sequence's new tokens are zero; the unit's workgroups share them.
+__device__ inline void clear_rest(const Args& a, const Share& s, int64_t b, int64_t hk, int item, int esz) {
+  const int c = 16 * (threadIdx.x & 31);
+  for (int r = s.rows + item * 8 + (threadIdx.x >> 5); r < a.R; r += 8 * a.items) {
+    const int i = r / a.G, g = r - i * a.G;
+    if (c < a.D * esz) *(u32x4*)(o_row(a, b, hk, i, g) + c) = u32x4{};
+  }
+}
+
+// A wavefront's rows of a stage: `ROWS` consecutive cached rows of one page.
+template <typename T, int ROWS>
+struct Loader {
+  static constexpr int RPI = 64 / T::CPR, NI = ROWS / RPI;
+  static_assert(NI >= 1 && ROWS == NI * RPI && PIECE % ROWS == 0, "whole instructions, one page");
+  uint32_t off[NI];
+  // `first`: the rows' place in the stage
+  __device__ inline void init(int first, int lane, int64_t row_bytes, int D) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = RPI * i + lane / T::CPR, c = (lane % T::CPR) ^ T::swz(first + r);
+      off[i] = c * T::CE < D ? (uint32_t)(r * row_bytes) + 16u * c : OUT_OF_RANGE;
+    }
+  }
+  // The rows at `base` of which `rows` exist (none: all zero) into LDS dst.
+  __device__ inline void issue(const char* base, int rows, int64_t row_bytes, int D, uint32_t dst) const {
+    const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * row_bytes) + (uint32_t)(D * T::ESZ) : 0;
+    const dma::i32x4 rs = dma::make_rsrc(base, bytes);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma::buffer16(rs, off[i], dst + i * 1024);
+  }
+};
+
+// Where the rows from key `key` on lie: looked up before a wait that takes in the scalar load.
+struct Spot {
+  uint32_t page;
+  int row;
+};
+__device__ inline Spot spot_of(const Table& t, int64_t trow, int key, int end) {
+  Spot s{NO_PAGE, 0};
+  if (key < end) {
+    const uint32_t col = column_of(t, (uint32_t)key / PIECE);
+    s.page = page_at(t, trow, col);
+    s.row = key - (int)col * t.page_size;
+  }
+  return s;
+}
+// Rows [key, end) of the piece or part of one that starts at the spot.
+template <typename L>
+__device__ inline void fetch(const L& ld, const Pages& p, const char* head, const Spot& s, int key, int end, int most,
+                             int D, uint32_t dst) {
+  const int left = end - key, rows = s.page == NO_PAGE ? 0 : left < most ? left : most;
+  const int64_t page = s.page == NO_PAGE ? 0 : s.page;
+  ld.issue(head + page * p.page + s.row * p.s, rows, p.s, D, dst);
+}
+
+template <typename T>
+struct Final {
+  char* o;
+  float* p;
+  __device__ inline void put(int d, f32x4 v) const {
+    if (p)
+      *(f32x4*)(p + d) = v;
+    else
+      T::store4(o + d * T::ESZ, v);
+  }
+};
+
+// ------------------------------------------------------------------- wide
+template <typename T>
+struct Wide {
+  static constexpr int NT = T::ESZ == 2 ? 2 : 1, HK = 32 * NT, HBYTES = HK * T::ROWB, STAGE = 2 * HBYTES;
+  static constexpr int LDS = 2 * STAGE, MINE = HK / 4;
+  typedef Loader<T, MINE> Ld;
+
+  static __device__ inline void run(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int item,
+                                    uint8_t* lds) {
+    const int split = item / (s.tiles ? s.tiles : 1);
+    if (s.tiles == 0 || split >= s.splits) return;
+    const int slot = item, tile = s.tiles - 1 - (item - split * s.tiles);  // the tiles that see most first
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int r0 = tile * 128 + w * 32, r = r0 + (lane & 31);
+    const bool live = r < s.rows, some = r0 < s.rows;
+    const int i = live ? r / a.G : 0, g = live ? r - i * a.G : 0;
+    typename T::Rows q;
+    T::load(q, q_row(a, b, hk, i, g), live, a.D, h);
+
+    const int c0 = split * s.chunk;
+    const int tile_last = tile * 128 + 127 < s.rows ? tile * 128 + 127 : s.rows - 1;
+    const int last = sees_of(s, tile_last / a.G);                   // keys that any row of the tile sees
+    const int k1 = c0 + s.chunk < last ? c0 + s.chunk : last;
+    const int sees = live ? sees_of(s, i) : 0;
+    const int least = some ? sees_of(s, r0 / a.G) : 0;              // and that all rows of the wavefront see
+    const int nst = k1 > c0 ? (k1 - c0 + HK - 1) / HK : 0;
+    const char* Kh = a.K.p + hk * a.K.h;
+    const char* Vh = a.V.p + hk * a.V.h;
+    const int64_t trow = b * a.t.ld;
+    Ld kl, vl;
+    kl.init(MINE * w, lane, a.K.s, a.D);
+    vl.init(MINE * w, lane, a.V.s, a.D);
+    const typename T::Lane ln = T::lane_of(lane);
+    const uint32_t lds0 = dma::lds_addr(lds), mine = w * (MINE * T::ROWB);
+    auto key = [&](int st) { return c0 + st * HK + MINE * w; };
+    auto issue = [&](int st, const Spot& sp) {
+      const uint32_t at = lds0 + (st & 1) * STAGE + mine;
+      fetch(kl, a.K, Kh, sp, key(st), k1, MINE, a.D, at);
+      fetch(vl, a.V, Vh, sp, key(st), k1, MINE, a.D, at + HBYTES);
+    };
+    xat::RowState<T> x;
+    x.clear();
+    if (nst > 0) issue(0, spot_of(a.t, trow, key(0), k1));
+    for (int st = 0; st < nst; ++st) {
+      Spot sp = spot_of(a.t, trow, key(st + 1), k1);
+      asm volatile("" : "+s"(sp.page));
+      dma::wait_vm<0>();
+      dma::barrier();
+      if (st + 1 < nst) issue(st + 1, sp);
+      const int at = c0 + st * HK;
+      if (!some) continue;
+      const uint32_t stage = lds0 + (st & 1) * STAGE;
+      const int lim = least < k1 ? least : k1;
+      xat::softmax_stage<T, NT, false>(x, q, stage, stage + HBYTES, ln, h, a.scale_log2, at + HK > lim,
+                                       xat::keys_from(sees, k1, at), [] {});
+    }
+    const float l = xat::halves_sum(x.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (!live) return;
+    const bool whole = s.splits == 1;
+    const int64_t at = ((int64_t)unit * a.slots + slot) * a.slot_rows + (r - tile * 128);
+    const Final<T> out{o_row(a, b, hk, i, g), whole ? nullptr : a.part + at * a.D};
+    T::quads(x.acc, h, [&](int d, f32x4 v) {
+      if (d < a.D) out.put(d, v * inv);
+    });
+    if (h == 0) {
+      const float e = x.m + __builtin_amdgcn_logf(l);
+      if (!whole)
+        a.plse[at] = e;
+      else if (a.lse)
+        a.lse[(int64_t)unit * a.R + r] = e;
+    }
+  }
+};
+
+// ----------------------------------------------------------------- narrow
+template <typename T>
+struct Narrow {
+  static constexpr int NW = 4, HBYTES = 32 * T::ROWB, XLD = T::DP + 4;
+  static constexpr int RING = NW * 2 * HBYTES, XB = NW * 32 * (XLD + 2) * 4, LDS = RING > XB ? RING : XB;
+  typedef Loader<T, PIECE> Ld;
+  static constexpr int NI = 2 * Ld::NI;  // instructions of a stage's K
+
+  static __device__ inline void fence() { asm volatile("" ::: "memory"); }
+  static __device__ inline void drained() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+  template <bool SCORES>
+  static __device__ inline void run(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int item,
+                                    uint8_t* lds) {
+    const int split = item;
+    if (s.rows == 0 || split >= s.splits) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int l32 = lane & 31;
+    const bool live = l32 < s.rows;
+    const int i = live ? l32 / a.G : 0, g = live ? l32 - i * a.G : 0;
+    const int k0 = split * s.chunk, k1 = k0 + s.chunk < s.n ? k0 + s.chunk : s.n;
+    const int sees = live ? sees_of(s, i) : 0, lim = sees_of(s, 0);  // keys of this row, and keys that all rows see
+    const int nst = k1 > k0 ? (k1 - k0 + 31) / 32 : 0, mine = nst > w ? (nst - w + NW - 1) / NW : 0;
+    const char* Kh = a.K.p + hk * a.K.h;
+    const char* Vh = a.V.p + hk * a.V.h;
+    const int64_t trow = b * a.t.ld;
+    // rows 16 and on of a stage are swizzled as the first 16 are
+    static_assert(T::swz(16) == T::swz(0) && T::swz(19) == T::swz(3), "one set of offsets");
+    Ld kl, vl;
+    kl.init(0, lane, a.K.s, a.D);
+    vl.init(0, lane, a.V.s, a.D);
+    const uint32_t kst = dma::lds_addr(lds) + w * 2 * HBYTES, vst = kst + HBYTES;
+    auto key = [&](int st) { return k0 + 32 * (st * NW + w); };
+    struct Two {
+      Spot p[2];
+    };
+    auto look = [&](int st) {
+      Two t;
+      t.p[0] = spot_of(a.t, trow, key(st), k1);
+      t.p[1] = spot_of(a.t, trow, key(st) + PIECE, k1);
+      return t;
+    };
+    auto issue = [&](const Ld& ld, const Pages& p, const char* head, int st, const Two& t, uint32_t dst) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        fetch(ld, p, head, t.p[j], key(st) + PIECE * j, k1, PIECE, a.D, dst + j * PIECE * T::ROWB);
+    };
+    Two now = look(0);
+    if (mine > 0) {
+      issue(kl, a.K, Kh, 0, now, kst);
+      issue(vl, a.V, Vh, 0, now, vst);
+    }
+    typename T::Rows q;
+    T::load(q, q_row(a, b, hk, i, g), live, a.D, h);
+    const typename T::Lane ln = T::lane_of(lane);
+    xat::RowState<T> x;
+    x.clear();
+    float* sc = nullptr;
+    if constexpr (SCORES) sc = a.scores + ((int64_t)unit * a.stages * a.R + l32) * 32 + 4 * h;
+    for (int st = 0; st < mine; ++st) {
+      const bool more = st + 1 < mine;
+      const int at = key(st);
+      Two next = look(st + 1);
+      asm volatile("" : "+s"(next.p[0].page), "+s"(next.p[1].page));
+      dma::wait_vm<NI>();  // K is there once only V's loads are out
+      fence();
+      f32x16 c[1];
+      T::template scores<1>(c, kst, ln, q);
+      drained();  // this wavefront's reads of K have returned: its place is free
+      if (more) issue(kl, a.K, Kh, st + 1, next, kst);
+      const bool check = at + 32 > (lim < k1 ? lim : k1);
+      xat::weigh_stage<T, 1, true>(
+          x, c, vst, ln, h, a.scale_log2, check, xat::keys_from(sees, k1, at),
+          [&] {
+            if constexpr (SCORES) {
+              // four stores of every wavefront, its first row being there
+              float* p = sc + (int64_t)(at / 32) * a.R * 32;
+              if (live) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                  *(f32x4*)(p + 8 * v) = f32x4{c[0][4 * v], c[0][4 * v + 1], c[0][4 * v + 2], c[0][4 * v + 3]} * a.scale_log2;
+              }
+            }
+          },
+          [&] {
+            if (more)
+              dma::wait_vm<NI + (SCORES ? 4 : 0)>();
+            else
+              dma::wait_vm<0>();
+            fence();
+          });
+      drained();
+      if (more) issue(vl, a.V, Vh, st + 1, next, vst);
+    }
+    join(a, s, unit, b, hk, split, x, lds, w, h, l32, live);
+  }
+
+  // m, l, acc of each row over the wavefronts, through LDS
+  static __device__ inline void join(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int split,
+                                     const xat::RowState<T>& x, uint8_t* lds, int w, int h, int l32, bool live) {
+    const float l = xat::halves_sum(x.l);
+    float* xo = (float*)lds;
+    float* xm = xo + NW * 32 * XLD;
+    float* xl = xm + NW * 32;
+    __syncthreads();
+    if (live) {
+      T::quads(x.acc, h, [&](int d, f32x4 v) { *(f32x4*)(xo + (w * 32 + l32) * XLD + d) = v; });
+      if (h == 0) {
+        xm[w * 32 + l32] = x.m;
+        xl[w * 32 + l32] = l;
+      }
+    }
+    __syncthreads();
+    constexpr int QPR = T::DP / 4;  // quads of a row
+    for (int e = threadIdx.x; e < s.rows * QPR; e += 64 * NW) {
+      const int row = e / QPR, d = 4 * (e % QPR), i = row / a.G, g = row - i * a.G;
+      float m = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NW; ++j) m = fmaxf(m, xm[j * 32 + row]);
+      float total = 0.f;
+      f32x4 sum = f32x4{};
+#pragma unroll
+      for (int j = 0; j < NW; ++j) {
+        const float lj = xl[j * 32 + row], mj = xm[j * 32 + row];
+        // (a wavefront without keys for the row has m = -inf, l = 0; a NaN score leaves NaN in l)
+        const float f = mj == -INFINITY ? (lj == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mj - m);
+        total += f * lj;
+        sum += *(const f32x4*)(xo + (j * 32 + row) * XLD + d) * f;
+      }
+      const float inv = total > 0.f || total != total ? 1.f / total : 0.f, lse = m + __builtin_amdgcn_logf(total);
+      const bool whole = s.splits == 1;
+      const int64_t at = ((int64_t)unit * a.slots + split) * a.slot_rows + row;
+      const Final<T> out{o_row(a, b, hk, i, g), whole ? nullptr : a.part + at * a.D};
+      if (d < a.D) out.put(d, sum * inv);
+      if (d == 0) {
+        if (!whole)
+          a.plse[at] = lse;
+        else if (a.lse)
+          a.lse[(int64_t)unit * a.R + row] = lse;
+      }
+    }
+  }
+};
+
+template <typename T>
+constexpr int narrow_per_cu = Narrow<T>::LDS <= 80 * 1024 ? 2 : 1;
+
+// Units of up to 32 rows each.
+template <typename T, bool SCORES>
+__global__ __launch_bounds__(256, narrow_per_cu<T>) void narrow_kernel(const Args a) {
+  typedef Narrow<T> N;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[N::LDS];
+  uint32_t unit, b, hk;
+  int item;
+  if (!unit_of(a, blockIdx.x, a.items, unit, b, hk, item)) return;
+  const Share s = share_of(a, b, 32);
+  clear_rest(a, s, b, hk, item, T::ESZ);
+  N::template run<SCORES>(a, s, unit, b, hk, item, lds);
+}
+// Units of any number of rows, each narrow or wide by its own.
+template <typename T>
+__global__ __launch_bounds__(256, narrow_per_cu<T>) void chunk_kernel(const Args a) {
+  typedef Wide<T> W;
+  typedef Narrow<T> N;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS > N::LDS ? W::LDS : N::LDS];
+  uint32_t unit, b, hk;
+  int item;
+  if (!unit_of(a, blockIdx.x, a.items, unit, b, hk, item)) return;
+  const Share s = share_of(a, b, 128);
+  clear_rest(a, s, b, hk, item, T::ESZ);
+  if (s.rows <= 32)
+    N::template run<false>(a, s, unit, b, hk, item, lds);
+  else
+    W::run(a, s, unit, b, hk, item, lds);
+}
+
+// ---------------------------------------------------------------- joining
+// One row: the ranges' results with weights 2^(lse_j - max lse); 32 lanes to a
+// row, four values each. Returns the row's log-sum-exp.
+template <typename T>
+__device__ inline float combine_row(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int tile_rows,
+                                    int r) {
+  const int lane = threadIdx.x & 31, d = 4 * lane;
+  const int tile = r / tile_rows;
+  const int64_t stride = (int64_t)s.tiles * a.slot_rows;  // of a row between ranges
+  const int64_t at = ((int64_t)unit * a.slots + (s.tiles - 1 - tile)) * a.slot_rows + (r - tile * tile_rows);
+  float m = -INFINITY, total = 0.f;
+  f32x4 sum = f32x4{};
+  for (int j0 = 0; j0 < s.splits; j0 += 32) {
+    const float lse = j0 + lane < s.splits ? a.plse[at + (j0 + lane) * stride] : -INFINITY;
+    float mx = lse;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    const float mn = fmaxf(m, mx);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    total *= f;
+    sum *= f;
+    // (a range without keys for the row weighs nothing; a NaN goes on)
+    const float wgt = lse == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse - mn);
+    const int n = s.splits - j0 < 32 ? s.splits - j0 : 32;
+    const float* p = a.part + (at + j0 * stride) * a.D + (d < a.D ? d : 0);
+    for (int j = 0; j < n; j += 8) {
+      f32x4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = j + u < n ? *(const f32x4*)(p + (j + u) * stride * a.D) : f32x4{};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float wj = __shfl(wgt, (threadIdx.x & 32) + j + u, 64);  // (zero behind the last range)
+        total += wj;
+        sum += wj == 0.f ? f32x4{} : v[u] * wj;
+      }
+    }
+  }
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  const int i = r / a.G, g = r - i * a.G;
+  if (d < a.D) T::store4(o_row(a, b, hk, i, g) + d * T::ESZ, sum * inv);
+  return m + __builtin_amdgcn_logf(total);
+}
+
+// `per` workgroups to a unit, 8 rows to each.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const Args a, int per, int tile_rows) {
+  const uint32_t unit = blockIdx.x / (uint32_t)per, part = blockIdx.x - unit * (uint32_t)per;
+  const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
+  const Share s = share_of(a, b, tile_rows);
+  const int r = (int)part * 8 + (int)(threadIdx.x >> 5);
+  if (s.splits == 1 || r >= s.rows) return;
+  const float lse = combine_row<T>(a, s, unit, b, hk, tile_rows, r);
+  if (a.lse && (threadIdx.x & 31) == 0) a.lse[(int64_t)unit * a.R + r] = lse;
+}
+
+// After the narrow kernel: workgroups [0, cw) of a unit join its rows (where the
+// keys were taken in ranges), the other `kw` add up the keys' weights, 256 keys
+// at a time, from the scores and the rows' log-sum-exps.
+template <typename T>
+__global__ __launch_bounds__(256) void weigh_kernel(const Args a, int cw, int kw) {
+  __shared__ float lse[32];
+  const uint32_t per = (uint32_t)(cw + kw), unit = blockIdx.x / per;
+  const int part = (int)(blockIdx.x - unit * per);
+  const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
+  const Share s = share_of(a, b, 32);
+  if (part < cw) {
+    const int r = part * 8 + (int)(threadIdx.x >> 5);
+    if (s.splits > 1 && r < s.rows) combine_row<T>(a, s, unit, b, hk, 32, r);
+    return;
+  }
+  if (s.splits > 1) {
+    // 8 threads to a row; ranges in order
+    const int r = threadIdx.x >> 3, l8 = threadIdx.x & 7;
+    float m = -INFINITY, total = 0.f;
+    if (r < s.rows) {
+      const int64_t at = (int64_t)unit * a.slots * a.slot_rows + r;
+      for (int j = l8; j < s.splits; j += 8) m = fmaxf(m, a.plse[at + (int64_t)j * a.slot_rows]);
+      for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+      for (int j = l8; j < s.splits; j += 8) {
+        const float e = a.plse[at + (int64_t)j * a.slot_rows];
+        total += e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e - m);
+      }
+      for (int o = 4; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+      if (l8 == 0) lse[r] = m + __builtin_amdgcn_logf(total);
+    }
+  } else if ((int)threadIdx.x < s.rows) {
+    lse[threadIdx.x] = a.lse[(int64_t)unit * a.R + threadIdx.x];
+  }
+  __syncthreads();
+  float* w = a.W + b * a.wb + hk * a.wh;
+  for (int k = (part - cw) * 256 + (int)threadIdx.x; k < s.n; k += 256 * kw) {
+    const float* p = a.scores + ((int64_t)unit * a.stages + k / 32) * a.R * 32 + k % 32;
+    float sum = 0.f;
+    for (int r = 0; r < s.rows; ++r) {
+      const float c = p[r * 32];
+      // (a key that the row does not see has a score of -inf)
+      sum += c == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(c - lse[r]);
+    }
+    w[k] += sum;
+  }
+}
+
+// ------------------------------------------------- weights of many rows
+// 128 keys to a workgroup, a wavefront to 32; the unit's rows staged 64 (fp32:
+// 32) at a time with their log-sum-exps.
+template <typename T>
+struct Weigh {
+  static constexpr int NT = T::ESZ == 2 ? 2 : 1, HR = 32 * NT, STAGE = HR * T::ROWB, LDS = 2 * STAGE;
+  static constexpr int RPI = 64 / T::CPR, MINE = HR / 4, NI = MINE / RPI;
+};
+template <typename T>
+__global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
+  typedef Weigh<T> G;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[G::LDS];
+  __shared__ __attribute__((aligned(16))) float neg[2][G::HR];  // minus the rows' log-sum-exps
+  uint32_t unit, b, hk;
+  int item;
+  if (!unit_of(a, blockIdx.x, per, unit, b, hk, item)) return;
+  const Share s = share_of(a, b, 128);
+  const int j0 = item * 128;
+  if (j0 >= s.n || s.rows == 0) return;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int j = j0 + w * 32 + (lane & 31);
+  const bool live = j < s.n;
+  typename T::Rows k;
+  {
+    const uint32_t col = live ? column_of(a.t, (uint32_t)j / PIECE) : 0;
+    const uint32_t page = live ? page_of_lane(a.t, b * a.t.ld, col) : NO_PAGE;
+    const char* p = a.K.p + (page == NO_PAGE ? 0 : page) * a.K.page + hk * a.K.h + (j - (int)col * a.t.page_size) * a.K.s;
+    T::load(k, p, live && page != NO_PAGE, a.D, h);
+  }
+  const int before = s.n - s.m;  // token i sees keys up to before + i
+  const int first = j0 > before ? (j0 - before) * a.G / G::HR * G::HR : 0;  // the first row that sees a key
+  const int seen_by = (j > before ? j - before : 0) * a.G;                  // ... that sees this lane's
+  const int all_from = (j0 + w * 32 + 31 > before ? j0 + w * 32 + 31 - before : 0) * a.G;
+  const char* Qh = a.Q.p + b * a.Q.b + hk * a.G * a.Q.h;
+  const typename T::Lane ln = T::lane_of(lane);
+  const uint32_t lds0 = dma::lds_addr(lds), mine = w * (G::MINE * T::ROWB);
+  // A stage's rows through a buffer that begins with the first row's token.
+  auto issue = [&](int r0, int buf) {
+    const int i0 = r0 / a.G;
+    const dma::i32x4 rs = dma::make_rsrc(Qh + i0 * a.Q.s, OUT_OF_RANGE);
+#pragma unroll
+    for (int u = 0; u < G::NI; ++u) {
+      const int x = G::MINE * w + G::RPI * u + lane / T::CPR, r = r0 + x, c = (lane % T::CPR) ^ T::swz(x);
+      const int i = r / a.G, g = r - i * a.G;
+      const uint32_t off = (uint32_t)((i - i0) * a.Q.s + g * a.Q.h) + 16u * c;
+      dma::buffer16(rs, r < s.rows && c * T::CE < a.D ? off : OUT_OF_RANGE, lds0 + buf * G::STAGE + mine + u * 1024);
+    }
+  };
+  // The log-sum-exps go through a register, loaded a stage ahead of the stage's
+  // rows: waited for with the loads before them. Rows behind the last, and rows
+  // that see nothing, weigh nothing.
+  auto lse_of = [&](int r0) {
+    const int r = r0 + (int)threadIdx.x;
+    return (int)threadIdx.x < G::HR && r < s.rows ? a.lse[(int64_t)unit * a.R + r] : -INFINITY;
+  };
+  auto put_neg = [&](int buf, float e) {
+    if ((int)threadIdx.x < G::HR) neg[buf][threadIdx.x] = e == -INFINITY ? e : -e;
+  };
+  float sum = 0.f;
+  put_neg(0, lse_of(first));
+  float ahead = lse_of(first + G::HR);
+  issue(first, 0);
+  for (int r0 = first, st = 0; r0 < s.rows; r0 += G::HR, st ^= 1) {
+    asm volatile("" : "+v"(ahead));
+    dma::wait_vm<0>();
+    dma::barrier();
+    put_neg(st ^ 1, ahead);
+    ahead = lse_of(r0 + 2 * G::HR);
+    if (r0 + G::HR < s.rows) issue(r0 + G::HR, st ^ 1);
+    f32x16 c[G::NT];
+    T::template scores<G::NT>(c, lds0 + st * G::STAGE, ln, k);
+    const bool check = r0 < all_from;
+#pragma unroll
+    for (int t = 0; t < G::NT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 e = *(const f32x4*)&neg[st][32 * t + 8 * q + 4 * h];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[t][4 * q + v], a.scale_log2, e[v]));
+          if (e[v] == -INFINITY || (check && r0 + 32 * t + 8 * q + 4 * h + v < seen_by)) p = 0.f;
+          sum += p;
+        }
+      }
+  }
+  sum = xat::halves_sum(sum);
+  if (live && h == 0) a.W[b * a.wb + hk * a.wh + j] += sum;
+}
+
+// ------------------------------------------------------------------- host
+
+struct Plan {
+  bool narrow;
+  int items, slots, least, step, slot_rows;
+  int64_t part, lse, scores;  // floats
+};
+Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t keys, int64_t D, bool ragged, bool weights) {
+  Plan p{};
+  const int64_t G = Hq / Hkv, R = G * Sq, units = B * Hkv;
+  const bool f32 = dtype == TSP_F32;
+  p.narrow = R <= 32;
+  const int64_t tiles = p.narrow ? 1 : ceil_div(R, 128);
+  p.least = p.narrow ? (f32 ? 128 : 512) : 256;
+  p.step = 128;
+  p.slot_rows = (int)(p.narrow ? R : 128);
+  const int64_t want = p.narrow && f32 ? 256 : 512, wgs = units * tiles;
+  int64_t n = wgs >= (p.narrow && f32 ? want : want / 2) ? 1 : ceil_div(want, wgs);
+  const int64_t most = ceil_div(keys > 0 ? keys : 1, p.least);
+  n = n < most ? n : most;
+  n = n < 32 ? n : 32;
+  p.items = (int)(tiles * n);
+  p.slots = n > 1 ? p.items : 0;
+  if (ragged && !p.narrow && n == 1) {
+    // sequences of few new tokens leave workgroups over, which take ranges
+    const int64_t room = ceil_div(1024, units);
+    p.slots = (int)(p.items < room ? p.items : room);
+    if (p.slots < 2) p.slots = 0;
+  }
+  auto pad = [](int64_t v) { return ceil_div(v, 64) * 64; };
+  p.part = pad(p.slots * units * p.slot_rows * (D + 1));
+  p.lse = weights ? pad(units * R) : 0;
+  p.scores = weights && p.narrow ? units * ceil_div(keys, 32) * R * 32 : 0;
+  return p;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace tsp
+
+using namespace tsp;
+
+extern "C" int64_t tsp_paged_attn_workspace_size(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t keys,
+                                                 int64_t D, int ragged, int weights) {
+  if (xat::check_sizes("tsp_paged_attn_workspace_size", dtype, B, Hq, Hkv, Sq, keys, D)) return -1;
+  if (B * Hq * Sq == 0) return 0;
+  const paged::Plan p = paged::plan_of(dtype, B, Hq, Hkv, Sq, keys, D, ragged != 0, weights != 0);
+  return 4 * (p.part + p.lse + p.scores);
+}
+
+extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* K_pages, const int64_t* kps,
+                                  const void* V_pages, const int64_t* vps, int dtype, int64_t B, int64_t Hq, int64_t Hkv,
+                                  int64_t Sq, int64_t pages, int64_t page_size, int64_t D, const void* table,
+                                  int table_type, int64_t table_stride, int64_t cols, const void* lengths,
+                                  const void* new_lengths, int index_type, double scale, void* O, const int64_t* os,
+                                  float* weights, const int64_t* ws, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+  const char* who = "tsp_paged_attn_fwd";
+  const hipStream_t st = (hipStream_t)stream;
+  int rc = paged::check_cache(who, dtype, B, Hkv, pages, page_size, D, table, table_type, table_stride, cols);
+  if (rc) return rc;
+  const int64_t keys = cols * page_size;
+  if ((rc = xat::check_sizes(who, dtype, B, Hq, Hkv, Sq, keys, D))) return rc;
+  if ((rc = paged::check_lengths(who, B, lengths, index_type))) return rc;
+  if (!(scale > 1e-30) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
+  if (B * Hq * Sq == 0) return TSP_OK;
+  if ((rc = xat::check_operand(who, "Q", Q, qs, Sq, D, dtype))) return rc;
+  if ((rc = xat::check_operand(who, "O", O, os, Sq, D, dtype))) return rc;
+  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, D))) return rc;
+  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, D))) return rc;
+  if ((rc = paged::check_weights(who, weights, ws))) return rc;
+  const bool weigh = weights && keys > 0;
+  const paged::Plan p = paged::plan_of(dtype, B, Hq, Hkv, Sq, keys, D, new_lengths != nullptr, weigh);
+  const int64_t need = 4 * (p.part + p.lse + p.scores);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
+  paged::Args a{};
+  a.Q = xat::operand(Q, qs, Sq, D, dtype);
+  const xat::Operand o = xat::operand(O, os, Sq, D, dtype);
+  a.O = (char*)O;
+  a.ob = o.b, a.oh = o.h, a.os = o.s;
+  a.K = paged::pages_of(K_pages, kps, dtype);
+  a.V = paged::pages_of(V_pages, vps, dtype);
+  a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
+  a.len = paged::Lengths{lengths, new_lengths, index_type == TSP_I64, keys, Sq};
+  a.B = (int)B, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
+  a.items = p.items, a.slots = p.slots, a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
+  const int64_t units = B * Hkv;
+  a.part = (float*)workspace;
+  a.plse = a.part + p.slots * units * p.slot_rows * D;
+  if (weigh) {
+    a.lse = (float*)workspace + p.part;
+    a.scores = p.narrow ? a.lse + p.lse : nullptr;
+    a.stages = (int)ceil_div(keys, 32);
+    a.W = weights, a.wb = ws[0], a.wh = ws[1];
+    // a stage of queries is read at 32-bit offsets from its first token
+    if (!p.narrow && (double)(a.G - 1) * a.Q.h + 66.0 * a.Q.s + 512 >= 2147483632.0)
+      return fail(TSP_EUNSUPPORTED, "%s: weights of query heads that lie 2 GiB apart", who);
+  }
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  const int64_t grid = head_grid(p.items, units);
+  const int64_t wper = ceil_div(keys, 128), wgrid = weigh && !p.narrow ? head_grid(wper, units) : 0;
+  const int tile_rows = p.narrow ? 32 : 128;
+  const int64_t joined = p.narrow ? a.R : (int64_t)(p.slots / 2) * 128 < a.R ? (int64_t)(p.slots / 2) * 128 : a.R;
+  const int64_t cper = p.slots > 1 ? ceil_div(joined, 8) : 0;
+  // 1024 keys and more to a workgroup, as many as fill the CUs
+  int64_t kper = ceil_div(2048, units);
+  if (kper > ceil_div(keys, 1024)) kper = ceil_div(keys, 1024);
+  if (kper < 1) kper = 1;
+  if (grid > INT32_MAX || wgrid > INT32_MAX || units * (cper + kper) > INT32_MAX)
+    return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
+  return xat::with_tile(dtype, D, [&](auto tile) {
+    typedef decltype(tile) T;
+    const dim3 g((unsigned)grid), t(256);
+    if (p.narrow && weigh)
+      hipLaunchKernelGGL((paged::narrow_kernel<T, true>), g, t, 0, st, a);
+    else if (p.narrow)
+      hipLaunchKernelGGL((paged::narrow_kernel<T, false>), g, t, 0, st, a);
+    else
+      hipLaunchKernelGGL((paged::chunk_kernel<T>), g, t, 0, st, a);
+    int rc = check_launch("paged attention launch");
+    if (rc) return rc;
+    if (p.narrow && weigh) {
+      hipLaunchKernelGGL((paged::weigh_kernel<T>), dim3((unsigned)(units * (cper + kper))), t, 0, st, a, (int)cper,
+                         (int)kper);
+      return check_launch("weights launch");
+    }
+    if (cper > 0) {
+      hipLaunchKernelGGL((paged::combine_kernel<T>), dim3((unsigned)(units * cper)), t, 0, st, a, (int)cper, tile_rows);
+      if ((rc = check_launch("combine launch"))) return rc;
+    }
+    if (weigh) {
+      hipLaunchKernelGGL((paged::weights_wide<T>), dim3((unsigned)wgrid), t, 0, st, a, (int)wper);
+      return check_launch("weights launch");
+    }
+    return TSP_OK;
+  });
+}

@@ -700,6 +700,163 @@ at::Tensor prefix_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at
   return Q.size(3) == piece_dim(Q) ? attn_like(Q, Q.size(3)) : at::empty(Q.sizes(), Q.options());
 }
 
+// ------------------------------------ a key and value cache in pages
+
+// The pages, the table and the lengths of a call, checked.
+struct PagedArgs {
+  int code, tcode, icode;
+  int64_t B, Hk, pages, page_size, D, cols, slots, tstride;
+  const void *lens, *fresh = nullptr;
+  int64_t ks[3], vs[3];
+
+  static void page_strides(const at::Tensor& t, int64_t* s) {
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) <= 1 ? (i == 2 ? t.size(3) : 0) : t.stride(i);
+  }
+  void need_pages(const at::Tensor& t, const at::Tensor& like, const char* who, const char* name, bool written) const {
+    TORCH_CHECK(t.device() == like.device(), who, ": ", name, " is on ", t.device(), ", expected ", like.device());
+    need_dtype(t, like.scalar_type(), who, name);
+    TORCH_CHECK(t.dim() == 4, who, ": ", name, " must be (pages, kv_heads, page_size, head_dim)");
+    const int64_t ce = 16 / t.element_size();
+    TORCH_CHECK(t.size(2) > 0 && t.size(2) % 16 == 0, who, ": page_size ", t.size(2), " must be a multiple of 16");
+    TORCH_CHECK(t.size(3) >= 1 && t.size(3) <= 128 && t.size(3) % ce == 0, who, ": head_dim ", t.size(3),
+                " must be at most 128 and a multiple of ", ce);
+    bool ok = (t.stride(3) == 1 || t.size(3) == 1) && (t.numel() == 0 || (uintptr_t)t.data_ptr() % 16 == 0);
+    for (int i = 0; i < 3; ++i)
+      ok = ok && (t.size(i) <= 1 || (t.stride(i) % ce == 0 && t.stride(i) >= (i == 2 ? t.size(3) : written ? 1 : 0)));
+    TORCH_CHECK(ok, who, ": ", name, " needs unit stride over head_dim and other strides of whole 16-byte pieces, got ",
+                t.strides(), written ? " (and is written: its rows lie apart)" : "");
+  }
+  PagedArgs(const at::Tensor& K, const at::Tensor& V, const at::Tensor& table, const at::Tensor& lengths,
+            const c10::optional<at::Tensor>& new_lengths, const at::Tensor& like, bool written, const char* who) {
+    code = attn_dtype(like.scalar_type(), who);
+    need_pages(K, like, who, "K_pages", written);
+    need_pages(V, like, who, "V_pages", written);
+    TORCH_CHECK(K.sizes() == V.sizes(), who, ": K_pages ", K.sizes(), " and V_pages ", V.sizes(), " do not belong together");
+    TORCH_CHECK(!written || K.numel() == 0 || K.data_ptr() != V.data_ptr(), who, ": K_pages and V_pages are the same");
+    pages = K.size(0), Hk = K.size(1), page_size = K.size(2), D = K.size(3);
+    TORCH_CHECK(Hk > 0, who, ": no key heads");
+    page_strides(K, ks);
+    page_strides(V, vs);
+    TORCH_CHECK(table.device() == like.device(), who, ": block_table is on ", table.device());
+    TORCH_CHECK(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), who,
+                ": block_table must be (batch, columns) with unit stride over columns");
+    tcode = index_code(table.scalar_type());
+    B = table.size(0), cols = table.size(1), slots = cols * page_size;
+    tstride = B > 1 ? table.stride(0) : cols;
+    lens = lengths_ptr(lengths, B, like, who, icode);
+    if (new_lengths.has_value()) {
+      int c;
+      fresh = lengths_ptr(new_lengths, B, like, who, c);
+      TORCH_CHECK(c == icode, who, ": lengths and new_lengths must have one dtype");
+    }
+  }
+};
+
+// accumulated weights (batch, kv_heads, slots)
+const int64_t* need_weights(const at::Tensor& w, const PagedArgs& p, const at::Tensor& like, const char* who, int64_t* s) {
+  TORCH_CHECK(w.device() == like.device(), who, ": weights are on ", w.device());
+  need_dtype(w, at::kFloat, who, "weights");
+  TORCH_CHECK(w.dim() == 3 && w.size(0) == p.B && w.size(1) == p.Hk && w.size(2) == p.slots, who, ": weights ", w.sizes(),
+              " must be (batch, kv_heads, slots) = (", p.B, ", ", p.Hk, ", ", p.slots, ")");
+  for (int i = 0; i < 2; ++i) {
+    s[i] = w.size(i) <= 1 ? 0 : w.stride(i);
+    TORCH_CHECK(w.size(i) <= 1 || w.stride(i) >= 1, who, ": weights are written: their rows lie apart");
+  }
+  TORCH_CHECK(w.size(2) <= 1 || w.stride(2) == 1, who, ": weights need unit stride over slots");
+  return s;
+}
+
+// what an operator wrote in place
+void written(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts) t->unsafeGetTensorImpl()->bump_version();
+}
+
+at::Tensor paged_attn_fwd(const at::Tensor& Q_, const at::Tensor& K, const at::Tensor& V, const at::Tensor& table,
+                          const at::Tensor& lengths, const c10::optional<at::Tensor>& new_lengths, double scale,
+                          const c10::optional<at::Tensor>& weights) {
+  const char* who = "paged_attn_fwd";
+  const c10::DeviceGuard guard(Q_.device());
+  need_4d(Q_, Q_, who, "Q");
+  const PagedArgs p(K, V, table, lengths, new_lengths, Q_, false, who);
+  TORCH_CHECK(Q_.size(0) == p.B && Q_.size(3) == p.D && Q_.size(1) % p.Hk == 0, who, ": Q ", Q_.sizes(), ", K_pages ",
+              K.sizes(), " and block_table ", table.sizes(), " do not belong together");
+  int64_t ws2[2];
+  if (weights.has_value()) need_weights(*weights, p, Q_, who, ws2);
+  const auto Q = attn_operand(Q_);
+  const int64_t Hq = Q.size(1), Sq = Q.size(2);
+  auto O = attn_like(Q_, p.D);
+  const int64_t wsb = tsp_paged_attn_workspace_size(p.code, p.B, Hq, p.Hk, Sq, p.slots, p.D, new_lengths.has_value(),
+                                                    weights.has_value());
+  const Workspace ws(wsb, Q, who);
+  check(tsp_paged_attn_fwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), p.ks, V.data_ptr(), p.vs, p.code, p.B, Hq, p.Hk, Sq,
+                           p.pages, p.page_size, p.D, table.data_ptr(), p.tcode, p.tstride, p.cols, p.lens, p.fresh,
+                           p.icode, scale, O.data_ptr(), Strides(O).s,
+                           weights.has_value() ? weights->data_ptr<float>() : nullptr, ws2, ws.ptr(), wsb, stream_of(Q)),
+        "tsp_paged_attn_fwd");
+  if (weights.has_value()) written({&*weights});
+  return O;
+}
+
+at::Tensor paged_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                               const at::Tensor&, const c10::optional<at::Tensor>&, double,
+                               const c10::optional<at::Tensor>&) {
+  return attn_like(Q, Q.size(3));
+}
+
+at::Tensor paged_append(const at::Tensor& K_, const at::Tensor& V_, const at::Tensor& Kp, const at::Tensor& Vp,
+                        const at::Tensor& table, const at::Tensor& lengths, const c10::optional<at::Tensor>& new_lengths,
+                        const c10::optional<at::Tensor>& weights) {
+  const char* who = "paged_append";
+  const c10::DeviceGuard guard(Kp.device());
+  const PagedArgs p(Kp, Vp, table, lengths, new_lengths, Kp, true, who);
+  need_4d(K_, Kp, who, "K");
+  need_4d(V_, Kp, who, "V");
+  TORCH_CHECK(K_.sizes() == V_.sizes() && K_.size(0) == p.B && K_.size(1) == p.Hk, who, ": K ", K_.sizes(), ", V ",
+              V_.sizes(), ", K_pages ", Kp.sizes(), " and block_table ", table.sizes(), " do not belong together");
+  int64_t ws2[2];
+  if (weights.has_value()) need_weights(*weights, p, Kp, who, ws2);
+  const auto K = attn_operand(K_), V = attn_operand(V_);
+  auto out = at::empty_like(lengths);
+  check(tsp_paged_append(K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs,
+                         p.code, p.B, p.Hk, K.size(2), p.pages, p.page_size, p.D, table.data_ptr(), p.tcode, p.tstride,
+                         p.cols, p.lens, p.fresh, p.icode, out.data_ptr(),
+                         weights.has_value() ? weights->data_ptr<float>() : nullptr, ws2, stream_of(Kp)),
+        "tsp_paged_append");
+  written({&Kp, &Vp});
+  if (weights.has_value()) written({&*weights});
+  return out;
+}
+
+at::Tensor paged_append_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, const at::Tensor& lengths, const c10::optional<at::Tensor>&,
+                             const c10::optional<at::Tensor>&) {
+  return at::empty_like(lengths);
+}
+
+at::Tensor paged_evict(const at::Tensor& Kp, const at::Tensor& Vp, const at::Tensor& weights, const at::Tensor& table,
+                       const at::Tensor& lengths, int64_t budget, int64_t recent) {
+  const char* who = "paged_evict";
+  const c10::DeviceGuard guard(Kp.device());
+  const PagedArgs p(Kp, Vp, table, lengths, c10::nullopt, Kp, true, who);
+  int64_t ws2[2];
+  need_weights(weights, p, Kp, who, ws2);
+  TORCH_CHECK(0 <= recent && recent <= budget, who, ": recent ", recent, " is not in 0 .. budget ", budget);
+  auto out = at::empty_like(lengths);
+  const int64_t wsb = tsp_paged_evict_workspace_size(p.B, p.Hk, std::min(budget, p.slots));
+  const Workspace ws(wsb, Kp, who);
+  check(tsp_paged_evict(Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs, p.code, p.B, p.Hk, p.pages, p.page_size, p.D,
+                        table.data_ptr(), p.tcode, p.tstride, p.cols, p.lens, p.icode, weights.data_ptr<float>(), ws2,
+                        budget, recent, out.data_ptr(), ws.ptr(), wsb, stream_of(Kp)),
+        "tsp_paged_evict");
+  written({&Kp, &Vp, &weights});
+  return out;
+}
+
+at::Tensor paged_evict_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const at::Tensor& lengths, int64_t, int64_t) {
+  return at::empty_like(lengths);
+}
+
 // --------------------------------- norm and rotation of query and key heads
 
 // t with unit stride over head_dim (a contiguous copy where it has another)
@@ -810,7 +967,7 @@ auto op_of(const char* name, F*) {
 
 bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
-  return std::any_of(ts.begin(), ts.end(), [](const at::Tensor* t) { return t->requires_grad(); });
+  return std::any_of(ts.begin(), ts.end(), [](const at::Tensor* t) { return t->defined() && t->requires_grad(); });
 }
 
 // Forward-mode derivatives are not formed. An input with a tangent need not
@@ -925,6 +1082,43 @@ at::Tensor prefix_attn_autograd(const at::Tensor& Q, const at::Tensor& PK, const
   return op.call(Q, PK, PV, K, V, lengths, scale);
 }
 
+// The operators of the paged cache have no gradients: an input that needs one is
+// refused, and what they write in place counts as written.
+void no_gradients(const char* who, std::initializer_list<const at::Tensor*> ts) {
+  no_tangents(who, ts);
+  TORCH_CHECK(!wants_grad(ts), who, " has no gradients: call it under torch.no_grad()");
+}
+const at::Tensor& or_none(const c10::optional<at::Tensor>& t) {
+  static const at::Tensor none;
+  return t.has_value() ? *t : none;
+}
+
+at::Tensor paged_attn_autograd(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V, const at::Tensor& table,
+                               const at::Tensor& lengths, const c10::optional<at::Tensor>& new_lengths, double scale,
+                               const c10::optional<at::Tensor>& weights) {
+  no_gradients("paged_attention", {&Q, &K, &V, &or_none(weights)});
+  at::AutoDispatchBelowADInplaceOrView below;
+  static const auto op = op_of("trnsparse_hip::paged_attn_fwd", &paged_attn_fwd);
+  return op.call(Q, K, V, table, lengths, new_lengths, scale, weights);
+}
+
+at::Tensor paged_append_autograd(const at::Tensor& K, const at::Tensor& V, const at::Tensor& Kp, const at::Tensor& Vp,
+                                 const at::Tensor& table, const at::Tensor& lengths,
+                                 const c10::optional<at::Tensor>& new_lengths, const c10::optional<at::Tensor>& weights) {
+  no_gradients("paged_cache_append", {&K, &V, &Kp, &Vp, &or_none(weights)});
+  at::AutoDispatchBelowADInplaceOrView below;
+  static const auto op = op_of("trnsparse_hip::paged_append", &paged_append);
+  return op.call(K, V, Kp, Vp, table, lengths, new_lengths, weights);
+}
+
+at::Tensor paged_evict_autograd(const at::Tensor& Kp, const at::Tensor& Vp, const at::Tensor& weights,
+                                const at::Tensor& table, const at::Tensor& lengths, int64_t budget, int64_t recent) {
+  no_gradients("paged_cache_evict", {&Kp, &Vp, &weights});
+  at::AutoDispatchBelowADInplaceOrView below;
+  static const auto op = op_of("trnsparse_hip::paged_evict", &paged_evict);
+  return op.call(Kp, Vp, weights, table, lengths, budget, recent);
+}
+
 struct QKNormRope : public ag::Function<QKNormRope> {
   static ag::variable_list forward(ag::AutogradContext* ctx, const at::Tensor& Q, const at::Tensor& K,
                                    const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& pos,
@@ -998,6 +1192,12 @@ TORCH_LIBRARY(trnsparse_hip, m) {
         "float scale, bool need_kv) -> (Tensor, Tensor, Tensor)");
   m.def("prefix_attn_fwd(Tensor Q, Tensor prefix_K, Tensor prefix_V, Tensor K, Tensor V, Tensor? lengths, "
         "float scale) -> Tensor");
+  m.def("paged_attn_fwd(Tensor Q, Tensor K_pages, Tensor V_pages, Tensor block_table, Tensor lengths, "
+        "Tensor? new_lengths, float scale, Tensor(a!)? weights) -> Tensor");
+  m.def("paged_append(Tensor K, Tensor V, Tensor(a!) K_pages, Tensor(b!) V_pages, Tensor block_table, Tensor lengths, "
+        "Tensor? new_lengths, Tensor(c!)? weights) -> Tensor");
+  m.def("paged_evict(Tensor(a!) K_pages, Tensor(b!) V_pages, Tensor(c!) weights, Tensor block_table, Tensor lengths, "
+        "int budget, int recent) -> Tensor");
   m.def("qk_norm_rope_fwd(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
         "float eps, bool interleaved) -> (Tensor, Tensor)");
   m.def("qk_norm_rope_bwd(Tensor Q, Tensor K, Tensor q_weight, Tensor k_weight, Tensor positions, Tensor inv_freq, "
@@ -1024,6 +1224,9 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
   m.impl("cross_attn_fwd", &cross_attn_fwd);
   m.impl("cross_attn_bwd", &cross_attn_bwd);
   m.impl("prefix_attn_fwd", &prefix_attn_fwd);
+  m.impl("paged_attn_fwd", &paged_attn_fwd);
+  m.impl("paged_append", &paged_append);
+  m.impl("paged_evict", &paged_evict);
   m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
   m.impl("cross_attention", &cross_attention);
@@ -1033,6 +1236,9 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, CUDA, m) {
 TORCH_LIBRARY_IMPL(trnsparse_hip, AutogradCUDA, m) {
   m.impl("cross_attention", &cross_attention_autograd);
   m.impl("prefix_attn_fwd", &prefix_attn_autograd);
+  m.impl("paged_attn_fwd", &paged_attn_autograd);
+  m.impl("paged_append", &paged_append_autograd);
+  m.impl("paged_evict", &paged_evict_autograd);
   m.impl("qk_norm_rope", &qk_norm_rope_autograd);
 }
 
@@ -1051,6 +1257,9 @@ TORCH_LIBRARY_IMPL(trnsparse_hip, Meta, m) {
   m.impl("cross_attn_fwd", &cross_attn_fwd_meta);
   m.impl("cross_attn_bwd", &cross_attn_bwd_meta);
   m.impl("prefix_attn_fwd", &prefix_attn_fwd_meta);
+  m.impl("paged_attn_fwd", &paged_attn_fwd_meta);
+  m.impl("paged_append", &paged_append_meta);
+  m.impl("paged_evict", &paged_evict_meta);
   m.impl("qk_norm_rope_fwd", &qk_norm_rope_fwd_meta);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_meta);
   m.impl("cross_attention", &cross_attention_meta);

@@ -331,14 +331,11 @@ struct RowState {
     l = 0.f;
   }
 };
-// `between` runs once the scores have left the K stage, before V is read.
-template <typename T, int NT, bool TWICE, typename F>
-__device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, uint32_t kst, uint32_t vst,
-                                     const typename T::Lane& ln, int h, float scale_log2, bool check, int keys,
-                                     F&& between) {
-  f32x16 s[NT];
-  T::template scores<NT>(s, kst, ln, q);
-  between();
+// weigh_stage: from the stage's scores on. `masked` runs once s holds the scores
+// that the row sees (the others -inf), `ready` before V is read.
+template <typename T, int NT, bool TWICE, typename M, typename F>
+__device__ inline void weigh_stage(RowState<T>& r, f32x16* s, uint32_t vst, const typename T::Lane& ln, int h,
+                                   float scale_log2, bool check, int keys, M&& masked, F&& ready) {
   if (check) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -346,6 +343,7 @@ __device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, 
       for (int v = 0; v < 16; ++v)
         if (32 * t + 8 * (v >> 2) + 4 * h + (v & 3) >= keys) s[t][v] = -INFINITY;
   }
+  masked();
   float mx = s[0][0];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -370,7 +368,18 @@ __device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, 
       sum += s[t][v];
     }
   r.l += sum;
+  ready();
   T::template product<NT, TWICE>(r.acc, vst, ln, s);
+}
+// `between` runs once the scores have left the K stage, before V is read.
+template <typename T, int NT, bool TWICE, typename F>
+__device__ inline void softmax_stage(RowState<T>& r, const typename T::Rows& q, uint32_t kst, uint32_t vst,
+                                     const typename T::Lane& ln, int h, float scale_log2, bool check, int keys,
+                                     F&& between) {
+  f32x16 s[NT];
+  T::template scores<NT>(s, kst, ln, q);
+  between();
+  weigh_stage<T, NT, TWICE>(r, s, vst, ln, h, scale_log2, check, keys, [] {}, [] {});
 }
 
 }  // namespace xat

@@ -660,6 +660,227 @@ def shared_prefix_attention(
     return _attn_parts_pytorch(Q, [shared, (K, V, seen)], scale)
 
 
+# A key and value cache in pages: what the three operators share.
+
+
+def _no_gradients(who: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{who} has no gradients: call it under torch.no_grad()")
+
+
+def _check_cache(who: str, K_pages, V_pages, block_table, lengths, new_lengths, weights) -> None:
+    """Shapes and types of a paged cache. The HIP operators refuse the same
+    calls themselves (csrc/torch_ops.cpp)."""
+    k, dt = K_pages.shape, K_pages.dtype
+    if len(k) != 4 or V_pages.shape != k or V_pages.dtype != dt or not dt.is_floating_point:
+        raise RuntimeError(f"{who}: K_pages {tuple(k)} of {dt} and V_pages {tuple(V_pages.shape)} of {V_pages.dtype} must "
+                           "be (pages, kv_heads, page_size, head_dim) of one floating dtype")
+    if k[1] == 0 or k[2] == 0 or k[2] % 16:
+        raise RuntimeError(f"{who}: page_size {k[2]} must be a multiple of 16, kv_heads {k[1]} at least 1")
+    if not 1 <= k[3] <= 128 or k[3] * K_pages.element_size() % 16:
+        raise RuntimeError(f"{who}: head_dim {k[3]} must be at most 128 and whole 16-byte pieces")
+    whole = (torch.int32, torch.int64)
+    if block_table.dim() != 2 or block_table.dtype not in whole:
+        raise RuntimeError(f"{who}: block_table must be (batch, columns) of int32 or int64")
+    B, cols = block_table.shape
+    for name, t in (("lengths", lengths), ("new_lengths", new_lengths)):
+        if t is not None and (t.shape != (B,) or t.dtype not in whole):
+            raise RuntimeError(f"{who}: {name} must be ({B},) of int32 or int64, got {tuple(t.shape)} of {t.dtype}")
+    if weights is not None and (weights.shape != (B, k[1], cols * k[2]) or weights.dtype != torch.float32):
+        raise RuntimeError(f"{who}: weights must be ({B}, {k[1]}, {cols * k[2]}) of float32, got {tuple(weights.shape)} of "
+                           f"{weights.dtype}")
+
+
+def _page_rows(K_pages, block_table, slots):
+    """Of the given slots (batch, kv_heads, n) or (n,): pages and rows to index
+    (pages, kv_heads, page_size, head_dim) with, and whether a page is there."""
+    pages, Hk, size, _ = K_pages.shape
+    B = block_table.shape[0]
+    slots = slots.expand(B, Hk, slots.shape[-1])
+    table = block_table.to(K_pages.device).long()
+    page = table.gather(1, (slots // size).reshape(B, -1)).view(slots.shape)
+    there = (page >= 0) & (page < pages)
+    heads = torch.arange(Hk, device=K_pages.device).view(1, Hk, 1).expand(slots.shape)
+    return (torch.where(there, page, torch.zeros_like(page)), heads, slots % size), there
+
+
+def _read_rows(pages, at, there):
+    if pages.shape[0] == 0:
+        return pages.new_zeros(*there.shape, pages.shape[3])
+    return torch.where(there.unsqueeze(-1), pages[at], torch.zeros((), dtype=pages.dtype, device=pages.device))
+
+
+def paged_attention(
+    Q: torch.Tensor,
+    K_pages: torch.Tensor,
+    V_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    new_lengths: torch.Tensor | None = None,
+    scale: float | None = None,
+    weights: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of a chunk of new tokens of every sequence over its cache in
+    pages, the new tokens' own rows included (serving: no gradients).
+
+    K_pages, V_pages (pages, kv_heads, page_size, head_dim); page_size is a
+    multiple of 16, head_dim at most 128 and whole 16-byte pieces. block_table
+    (batch, columns) int32 or int64: row j of sequence b is row j % page_size of
+    page block_table[b, j // page_size]; an entry outside [0, pages) is a page
+    of zeros. lengths (batch,) int32 or int64: the rows that each sequence has
+    (taken into [0, slots], slots = columns * page_size). Its last
+    new_lengths[b] rows are the new tokens' (None: as many as Q has; taken into
+    [0, queries]), whose queries are Q[b, :, :new_lengths[b]] of Q (batch,
+    heads, queries, head_dim). Query i sees the rows j < lengths[b] -
+    (new_lengths[b] - 1 - i), heads are grouped as in `cross_attention`. Results
+    of queries behind new_lengths[b], or that see no row, are zero. What stands
+    in V of a row that only some of the new tokens see has to be finite: the
+    others weigh it with zero.
+
+    With `weights` (batch, kv_heads, slots) float32, the softmax weight of every
+    row, summed over the key head's query heads and the new tokens, is added to
+    it: what `paged_cache_evict` goes by.
+
+    Types, scale, strides of Q and the result's order as in `cross_attention`;
+    pages and weights may be views with unit stride over the last dimension and
+    (pages) other strides of whole 16-byte pieces. head_dim**-0.5 is the default
+    scale.
+    """
+    who = "paged_attention"
+    if scale is None:
+        scale = _default_scale(Q)
+    _no_gradients(who, Q, K_pages, V_pages, weights)
+    if _use_hip():
+        from .hip.dispatch import hip_paged_attention
+
+        return hip_paged_attention(Q, K_pages, V_pages, block_table, lengths, new_lengths, scale, weights)
+    _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+    B, cols = block_table.shape
+    _, Hk, size, D = K_pages.shape
+    if Q.dim() != 4 or Q.shape[0] != B or Q.shape[3] != D or Q.shape[1] % Hk or Q.dtype != K_pages.dtype:
+        raise RuntimeError(f"{who}: Q {tuple(Q.shape)} of {Q.dtype} does not belong to K_pages {tuple(K_pages.shape)} of "
+                           f"{K_pages.dtype} and block_table {tuple(block_table.shape)}")
+    if not 1e-30 < scale < 1e30:
+        raise RuntimeError(f"{who}: scale must be positive, got {scale}")
+    H, N, L, dev = Q.shape[1], Q.shape[2], cols * size, Q.device
+    if Q.numel() == 0 or L == 0:
+        return torch.zeros_like(Q)
+    j, i = torch.arange(L, device=dev), torch.arange(N, device=dev)
+    n = lengths.to(dev).long().clamp(0, L).view(B, 1)
+    m = torch.full_like(n, N) if new_lengths is None else new_lengths.to(dev).long().clamp(0, N).view(B, 1)
+    sees = torch.where(i < m, n - (m - 1 - i), torch.zeros_like(n))  # (batch, queries)
+    seen = j < sees.view(B, 1, N, 1)
+    at, there = _page_rows(K_pages, block_table, j)
+    K, V = (_wide(_read_rows(p, at, there & (j < n).view(B, 1, L))) for p in (K_pages, V_pages))
+    G = H // Hk
+    q = torch.where((i < m).view(B, 1, N, 1), _wide(Q), torch.zeros((), dtype=_wide(Q).dtype, device=dev))
+    S = (q.reshape(B, Hk, G * N, D) @ K.transpose(2, 3)) * scale
+    P = _masked_softmax(S.view(B, H, N, L).masked_fill(~seen, float("-inf")).view(B, Hk, G * N, L))
+    if weights is not None:
+        weights += P.sum(2).to(weights.dtype)
+    return (P @ V).reshape(B, H, N, D).to(Q.dtype)
+
+
+def paged_cache_append(
+    K: torch.Tensor,
+    V: torch.Tensor,
+    K_pages: torch.Tensor,
+    V_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    new_lengths: torch.Tensor | None = None,
+    weights: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Writes new tokens' keys and values behind the rows that a cache in pages
+    has (`paged_attention`), in place, and returns the new lengths.
+
+    K, V (batch, kv_heads, tokens, head_dim) in the pages' dtype, strided views
+    allowed: row i < new_lengths[b] (None: all) becomes row lengths[b] + i of
+    sequence b. Rows past the table's columns, or in a page that is not there,
+    are left out. `weights` (batch, kv_heads, slots), where given, is set to
+    zero at the new rows. A page that is written belongs to one sequence.
+    """
+    who = "paged_cache_append"
+    _no_gradients(who, K, V, K_pages, V_pages, weights)
+    if _use_hip():
+        from .hip.dispatch import hip_paged_cache_append
+
+        return hip_paged_cache_append(K, V, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+    _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+    B, cols = block_table.shape
+    _, Hk, size, D = K_pages.shape
+    if K.dim() != 4 or K.shape != V.shape or (K.shape[0], K.shape[1], K.shape[3]) != (B, Hk, D):
+        raise RuntimeError(f"{who}: K {tuple(K.shape)} and V {tuple(V.shape)} must be ({B}, {Hk}, tokens, {D})")
+    if K.dtype != K_pages.dtype or V.dtype != K_pages.dtype:
+        raise RuntimeError(f"{who}: K and V must have the pages' dtype {K_pages.dtype}")
+    if K_pages.numel() and K_pages.data_ptr() == V_pages.data_ptr():
+        raise RuntimeError(f"{who}: K_pages and V_pages are the same")
+    N, L, dev = K.shape[2], cols * size, K_pages.device
+    n = lengths.to(dev).long().clamp(0, L)
+    m = torch.full_like(n, N) if new_lengths is None else new_lengths.to(dev).long().clamp(0, N)
+    for b in range(B):
+        new = min(int(m[b]), L - int(n[b]))
+        if new <= 0:
+            continue
+        slots = int(n[b]) + torch.arange(new, device=dev)
+        (page, head, row), there = _page_rows(K_pages, block_table[b : b + 1], slots)
+        for pages, rows in ((K_pages, K), (V_pages, V)):
+            pages[page[there], head[there], row[there]] = rows[b : b + 1, :, :new].to(dev)[there]
+        if weights is not None:
+            weights[b, :, int(n[b]) : int(n[b]) + new] = 0
+    return (n + m).clamp_max(L).to(lengths.dtype).to(lengths.device)
+
+
+def paged_cache_evict(
+    K_pages: torch.Tensor,
+    V_pages: torch.Tensor,
+    weights: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    budget: int,
+    recent: int = 0,
+) -> torch.Tensor:
+    """Cuts every sequence of a cache in pages (`paged_attention`) that has more
+    than `budget` rows down to it, in place, and returns the new lengths.
+
+    Each key head of such a sequence keeps its last `recent` rows (at most
+    `budget`) and, of the others, the budget - recent with the largest
+    accumulated `weights` (batch, kv_heads, slots) float32; of equal weights the
+    first rows, a NaN counts as above all numbers. The kept rows of K_pages,
+    V_pages and weights move to rows [0, budget) in their order; what stands
+    behind them is left as it was. Heads keep rows of their own. A sequence of
+    at most `budget` rows stays as it is. A page that a cut sequence has belongs
+    to it alone.
+    """
+    who = "paged_cache_evict"
+    _no_gradients(who, K_pages, V_pages, weights)
+    if _use_hip():
+        from .hip.dispatch import hip_paged_cache_evict
+
+        return hip_paged_cache_evict(K_pages, V_pages, weights, block_table, lengths, budget, recent)
+    _check_cache(who, K_pages, V_pages, block_table, lengths, None, weights)
+    if not 0 <= recent <= budget:
+        raise RuntimeError(f"{who}: recent {recent} is not in 0 .. budget {budget}")
+    if K_pages.numel() and K_pages.data_ptr() == V_pages.data_ptr():
+        raise RuntimeError(f"{who}: K_pages and V_pages are the same")
+    B, cols = block_table.shape
+    L, dev = cols * K_pages.shape[2], K_pages.device
+    n = lengths.to(dev).long().clamp(0, L)
+    for b in range(B):
+        rows = int(n[b])
+        if rows <= budget:
+            continue
+        heavy = weights[b, :, : rows - recent].sort(dim=-1, descending=True, stable=True).indices[:, : budget - recent]
+        last = torch.arange(rows - recent, rows, device=dev).expand(heavy.shape[0], recent)
+        kept = torch.cat([heavy.sort(-1).values, last], 1)
+        source, there = _page_rows(K_pages, block_table[b : b + 1], kept.unsqueeze(0))
+        (page, head, row), room = _page_rows(K_pages, block_table[b : b + 1], torch.arange(budget, device=dev))
+        for pages in (K_pages, V_pages):
+            pages[page[room], head[room], row[room]] = _read_rows(pages, source, there)[room]
+        weights[b, :, :budget] = weights[b].gather(1, kept)
+    return n.clamp_max(budget).to(lengths.dtype).to(lengths.device)
+
+
 def rope_frequencies(rot_dim: int, theta: float = 10000.0, device=None) -> torch.Tensor:
     """The angles per position of `qk_norm_rope`: theta**(-2 j / rot_dim) for
     j < rot_dim / 2, in float64."""
