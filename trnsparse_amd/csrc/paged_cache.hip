@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, int64_t
 // place at or before its own, and the list rises: a workgroup that takes the list
 // in order, and writes a part only once all of its rows are read, never writes
 // over a row that is still to be read. Workgroups share no byte: each has one
-// head's K or V and a slice of 128 bytes of its rows.
+// head's K or V and a slice of its rows.
 struct EvictArgs {
   Pages Kp, Vp;
   Table t;
@@ -123,11 +123,12 @@ struct EvictArgs {
   int64_t B;
   int Hkv, D, esz;
   int budget, recent;
-  int32_t* list;   // [batch][head][budget]: kept rows
+  u32x2* list;     // [batch][head][budget]: kept rows, page and row of it
   int32_t* first;  // [batch][head]: the first kept row that moves
+  char* spare;     // 16 bytes
 };
 
-constexpr int ST = 1024, SPT = 8, BINS = 2048;  // threads of select_kernel, rows of one in a part of the pass
+constexpr int ST = 1024, SPT = 8, PART = ST * SPT, BINS = 2048;  // threads of select_kernel, rows of one in a part
 
 __device__ inline uint32_t order_key(float w) {
   if (w != w) return 0xffffffffu;
@@ -147,10 +148,27 @@ __device__ inline int wave_scan(int v, int lane, int& total) {
   return x - v;
 }
 
+// A thread's rows of a part, consecutive ones; rows from `end` on are not read.
+struct Part {
+  float v[SPT];
+  __device__ inline void load(const float* w, int j, int end, bool aligned) {
+    if (aligned && j + SPT <= end) {
+#pragma unroll
+      for (int i = 0; i < SPT; i += 4) {
+        const f32x4 x = *(const f32x4*)(w + j + i);
+        v[i] = x[0], v[i + 1] = x[1], v[i + 2] = x[2], v[i + 3] = x[3];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) v[i] = j + i < end ? w[j + i] : 0.f;
+    }
+  }
+};
+
 __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
   __shared__ uint32_t hist[BINS];
   __shared__ int sums[2][2][ST / 64];
-  __shared__ uint32_t lo_hi[2], pick[2];
+  __shared__ uint32_t lo_hi[2][ST / 64], pick[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t unit = blockIdx.x, b = unit / a.Hkv, h = unit - b * a.Hkv;
   const int64_t n64 = cached_rows(a.len, b);
@@ -167,50 +185,71 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
     return;
   }
   float* w = a.W + b * a.wb + h * a.wh;
-  const int E = n - a.recent;             // rows that may go
-  const int keep = a.budget - a.recent;   // of those, the ones that stay (fewer than E)
+  const bool aligned = ((uintptr_t)w & 15) == 0;
+  const int E = n - a.recent;            // rows that may go
+  const int keep = a.budget - a.recent;  // of those, the ones that stay (fewer than E)
+  // The rows of up to one part stay in registers; of more, each pass reads them
+  // again, the next part's while one is worked on.
+  const bool once = n <= PART;
+  Part held;
+  held.load(w, tid * SPT, n, aligned);
+  auto each = [&](int end, auto&& f) {
+    Part now = held;
+    for (int j0 = 0; j0 < end; j0 += PART) {
+      Part next;
+      if (!once) next.load(w, j0 + PART + tid * SPT, n, aligned);
+      f(j0 + tid * SPT, now);
+      if (!once) now = next;
+    }
+  };
   // the key of the last that stays, and how many with that key do
   uint32_t last = 0xffffffffu;
   int equal = 0;
   if (keep > 0) {
     uint32_t lo = 0xffffffffu, hi = 0;
-    for (int j = tid; j < E; j += ST) {
-      const uint32_t k = order_key(w[j]);
-      lo = k < lo ? k : lo;
-      hi = k > hi ? k : hi;
-    }
+    each(E, [&](int j, const Part& p) {
+#pragma unroll
+      for (int i = 0; i < SPT; ++i) {
+        const uint32_t k = order_key(p.v[i]);
+        lo = j + i < E && k < lo ? k : lo;
+        hi = j + i < E && k > hi ? k : hi;
+      }
+    });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       const uint32_t l = __shfl_xor(lo, o, 64), g = __shfl_xor(hi, o, 64);
       lo = l < lo ? l : lo;
       hi = g > hi ? g : hi;
     }
-    if (tid == 0) lo_hi[0] = 0xffffffffu, lo_hi[1] = 0;
+    if (lane == 0) lo_hi[0][wave] = lo, lo_hi[1][wave] = hi;
+    for (int i = tid; i < BINS; i += ST) hist[i] = 0;
     __syncthreads();
-    if (lane == 0) {
-      atomicMin(&lo_hi[0], lo);
-      atomicMax(&lo_hi[1], hi);
+#pragma unroll
+    for (int i = 0; i < ST / 64; ++i) {
+      lo = lo_hi[0][i] < lo ? lo_hi[0][i] : lo;
+      hi = lo_hi[1][i] > hi ? lo_hi[1][i] : hi;
     }
-    __syncthreads();
-    lo = lo_hi[0], hi = lo_hi[1];
     int want = keep;  // the place of the wanted key among those of [lo, hi], from the largest
     while (lo < hi) {
       const uint32_t span = hi - lo;
       const int shift = 32 - __builtin_clz(span) > 11 ? 32 - __builtin_clz(span) - 11 : 0;  // BINS digits
-      for (int i = tid; i < BINS; i += ST) hist[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < E; j += ST) {
-        const uint32_t k = order_key(w[j]);
-        if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
-      }
+      each(E, [&](int j, const Part& p) {
+#pragma unroll
+        for (int i = 0; i < SPT; ++i) {
+          const uint32_t k = order_key(p.v[i]);
+          if (j + i < E && k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+        }
+      });
       __syncthreads();
       // two digits to a thread, from the largest; the one where the count passes `want`
       const int d = BINS - 1 - 2 * tid;
       const int c0 = (int)hist[d], c1 = (int)hist[d - 1];
+      hist[d] = hist[d - 1] = 0;  // (for the next turn)
       int total, before = wave_scan(c0 + c1, lane, total);
       if (lane == 0) sums[0][0][wave] = total;
       __syncthreads();
-      for (int i = 0; i < wave; ++i) before += sums[0][0][i];
+#pragma unroll
+      for (int i = 0; i < ST / 64; ++i) before += i < wave ? sums[0][0][i] : 0;
       if (before < want && want <= before + c0 + c1) {
         const bool second = want > before + c0;
         pick[0] = (uint32_t)(second ? d - 1 : d);
@@ -221,126 +260,147 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
       const uint32_t low = lo + (pick[0] << shift), width = shift ? (1u << shift) - 1 : 0;
       hi = hi - low < width ? hi : low + width;
       lo = low;
-      __syncthreads();
     }
     last = lo;
     equal = want;
   }
+  __syncthreads();
   // the kept rows in order; those that equal the last one's key as far as they go
-  int32_t* list = a.list + unit * a.budget;
-  int base = 0, equal_base = 0, first = a.budget;
-  for (int j0 = 0, turn = 0; j0 < n; j0 += ST * SPT, turn ^= 1) {
-    const int j = j0 + tid * SPT;
-    float v[SPT];
+  u32x2* list = a.list + unit * a.budget;
+  int base = 0, equal_base = 0, first = a.budget, turn = 0;
+  each(n, [&](int j, Part p) {
+    // (a thread's rows lie in one page)
+    const uint32_t col = column_of(a.t, (uint32_t)j / PIECE), row = (uint32_t)j - col * (uint32_t)a.t.page_size;
+    const uint32_t page = j < n ? page_of_lane(a.t, b * a.t.ld, col) : NO_PAGE;
     uint32_t above = 0, same = 0;
 #pragma unroll
     for (int i = 0; i < SPT; ++i) {
-      v[i] = j + i < n ? w[j + i] : 0.f;
-      const uint32_t k = order_key(v[i]);
+      const uint32_t k = order_key(p.v[i]);
       if (j + i < n && (j + i >= E || (keep > 0 && k > last))) above |= 1u << i;
       if (j + i < E && keep > 0 && k == last) same |= 1u << i;
     }
-    int total_e, total_a;
-    int eb = wave_scan(__builtin_popcount(same), lane, total_e);
-    int ab = wave_scan(__builtin_popcount(above), lane, total_a);
-    if (lane == 0) sums[turn][0][wave] = total_e, sums[turn][1][wave] = total_a;
+    // both counts in one scan: at most PART of each
+    int total, before = wave_scan(__builtin_popcount(same) << 16 | __builtin_popcount(above), lane, total);
+    if (lane == 0) sums[turn][0][wave] = total;
     // every row of this part is read before one is written
 #pragma unroll
-    for (int i = 0; i < SPT; ++i) asm volatile("" : "+v"(v[i]));
+    for (int i = 0; i < SPT; ++i) asm volatile("" : "+v"(p.v[i]));
     __syncthreads();
-    int se = 0, sa = 0;
+    int all = 0;
 #pragma unroll
     for (int i = 0; i < ST / 64; ++i) {
-      const int e = sums[turn][0][i], c = sums[turn][1][i];
-      eb += i < wave ? e : 0;
-      ab += i < wave ? c : 0;
-      se += e;
-      sa += c;
+      const int c = sums[turn][0][i];
+      before += i < wave ? c : 0;
+      all += c;
     }
-    int e = equal_base + eb;                                  // equal ones before this thread's
-    int d = base + ab + (e < equal ? e : equal) - (equal_base < equal ? equal_base : equal);
+    turn ^= 1;
+    int e = equal_base + (before >> 16);  // equal ones before this thread's
+    const int e0 = equal_base < equal ? equal_base : equal;
+    int d = base + (before & 0xffff) + (e < equal ? e : equal) - e0;
 #pragma unroll
     for (int i = 0; i < SPT; ++i) {
       bool stays = above >> i & 1;
       if (same >> i & 1) stays = e++ < equal;
       if (!stays) continue;
-      list[d] = j + i;
+      list[d] = u32x2{page, row + i};
       if (d != j + i) {
-        w[d] = v[i];
+        w[d] = p.v[i];
         first = d < first ? d : first;
       }
       ++d;
     }
-    const int e0 = equal_base < equal ? equal_base : equal;
-    equal_base += se;
-    base += sa + (equal_base < equal ? equal_base : equal) - e0;
-  }
+    equal_base += all >> 16;
+    base += (all & 0xffff) + (equal_base < equal ? equal_base : equal) - e0;
+  });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const int f = __shfl_xor(first, o, 64);
     first = f < first ? f : first;
   }
-  __syncthreads();
-  if (lane == 0) sums[0][0][wave] = first;
+  if (lane == 0) sums[turn][1][wave] = first;
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < ST / 64; ++i) first = sums[0][0][i] < first ? sums[0][0][i] : first;
+    for (int i = 1; i < ST / 64; ++i) first = sums[turn][1][i] < first ? sums[turn][1][i] : first;
     a.first[unit] = first;
   }
 }
 
-// A row's place in the pages, in bytes from their start; -1 without a page.
-__device__ inline int64_t place_of_row(const Pages& p, const Table& t, int64_t row, int64_t h, uint32_t j) {
-  const uint32_t col = column_of(t, j / PIECE), r = j - col * (uint32_t)t.page_size;
-  const uint32_t page = page_of_lane(t, row, col);
-  return page == NO_PAGE ? -1 : page * p.page + h * p.h + r * p.s;
-}
-
-constexpr int MT = 512, MU = 4;  // threads of move_kernel, rows of one in a part of the list
+// LPR lanes (16 bytes each) to a row's slice, MU rows of a thread in a part of the
+// list. The list's entries come two parts ahead, the rows one. A thread without
+// a row takes the last one's (and stores the same once more), one without a page
+// the spare place, so that no branch keeps a wait from being counted.
+constexpr int MT = 512, MU = 8;
+struct Move {
+  u32x2 from[MU];   // page and row
+  uint32_t to[MU];  // page
+};
+template <int LPR>
 __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t slices) {
-  const uint32_t slice = blockIdx.x % slices, x = blockIdx.x / slices;
-  const int64_t unit = x >> 1, b = unit / a.Hkv, h = unit - b * a.Hkv;
+  // the slices of a row in consecutive slots of one XCD
+  const uint32_t xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, slice = at8 % slices, x = at8 / slices * 8 + xcd;
+  const int64_t unit = x >> 1;
+  if (unit >= a.B * a.Hkv) return;
+  const int64_t b = unit / a.Hkv, h = unit - b * a.Hkv;
   const int first = a.first[unit];
   if (first >= a.budget) return;
   const Pages& p = x & 1 ? a.Vp : a.Kp;
-  const int32_t* list = a.list + unit * a.budget;
+  const u32x2* list = a.list + unit * a.budget;
   const int64_t trow = b * a.t.ld;
-  const uint32_t c = 128 * slice + 16 * (threadIdx.x & 7);
-  const bool on = c < (uint32_t)(a.D * a.esz);
-  constexpr int RP = MT / 8;  // rows at once
-  const int at = threadIdx.x >> 3;
-  auto load = [&](u32x4* v, int d0) {
+  constexpr int RP = MT / LPR, PR = RP * MU;  // rows at once, and of a part
+  const uint32_t row_bytes = (uint32_t)(a.D * a.esz);
+  uint32_t c = 16 * (LPR * slice + threadIdx.x % LPR);
+  c = c < row_bytes ? c : row_bytes - 16;
+  char* base = p.p + h * p.h + c;
+  const int at = threadIdx.x / LPR, end = a.budget - 1;
+  auto place = [&](int d0, int u) {
+    const int d = d0 + RP * u + at;
+    return (uint32_t)(d < end ? d : end);
+  };
+  auto look = [&](Move& m, int d0) {
 #pragma unroll
     for (int u = 0; u < MU; ++u) {
-      const int d = d0 + RP * u + at;
-      v[u] = u32x4{};
-      if (d < a.budget && on) {
-        const int64_t s = place_of_row(p, a.t, trow, h, (uint32_t)list[d]);
-        if (s >= 0) v[u] = *(const u32x4*)(p.p + s + c);
-      }
+      const uint32_t d = place(d0, u);
+      m.from[u] = list[d];
+      m.to[u] = page_of_lane(a.t, trow, column_of(a.t, d / PIECE));
     }
   };
+  auto load = [&](u32x4* v, const Move& m) {
+#pragma unroll
+    for (int u = 0; u < MU; ++u) {
+      const bool there = m.from[u].x != NO_PAGE;
+      const char* q = there ? base + m.from[u].x * p.page + m.from[u].y * p.s : a.spare;
+      v[u] = *(const u32x4*)q;
+      if (!there) v[u] = u32x4{};
+    }
+  };
+  Move m0, m1, m2;
   u32x4 now[MU], next[MU];
-  load(now, first);
-  for (int d0 = first; d0 < a.budget; d0 += RP * MU) {
-    load(next, d0 + RP * MU);
+  look(m0, first);
+  look(m1, first + PR);
+  load(now, m0);
+  for (int d0 = first; d0 <= end; d0 += PR) {
+    look(m2, d0 + 2 * PR);
+    load(next, m1);
     // the rows of this part have arrived in every wavefront before one is written
 #pragma unroll
     for (int u = 0; u < MU; ++u) asm volatile("" : "+v"(now[u]));
     asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int u = 0; u < MU; ++u) {
-      const int d = d0 + RP * u + at;
-      if (d < a.budget && on) {
-        const int64_t s = place_of_row(p, a.t, trow, h, (uint32_t)d);
-        if (s >= 0) *(u32x4*)(p.p + s + c) = now[u];
-      }
+      const uint32_t d = place(d0, u), r = d - column_of(a.t, d / PIECE) * (uint32_t)a.t.page_size;
+      char* q = m0.to[u] != NO_PAGE ? base + m0.to[u] * p.page + r * p.s : a.spare;
+      *(u32x4*)q = now[u];
       now[u] = next[u];
     }
+    m0 = m1;
+    m1 = m2;
   }
 }
 
-int64_t list_bytes(int64_t B, int64_t Hkv, int64_t budget) { return 4 * B * Hkv * (budget + 1); }
+// Workspace: 16 bytes that writes to no page go to, the units' first rows that
+// move, then the lists.
+int64_t list_at(int64_t B, int64_t Hkv) { return 16 + ceil_div(4 * B * Hkv, 16) * 16; }
+int64_t list_bytes(int64_t B, int64_t Hkv, int64_t budget) { return list_at(B, Hkv) + 8 * B * Hkv * budget; }
 
 }  // namespace
 }  // namespace paged
@@ -420,7 +480,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, D))) return rc;
   if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, D))) return rc;
   if (pages > 0 && K_pages == V_pages) return fail(TSP_EINVAL, "%s: K_pages and V_pages are the same", who);
-  if (!workspace || workspace_bytes < paged::list_bytes(B, Hkv, budget)) return fail(TSP_EINVAL, "%s: workspace too small", who);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < paged::list_bytes(B, Hkv, budget)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   paged::EvictArgs a{};
   a.Kp = paged::pages_of(K_pages, kps, dtype);
   a.Vp = paged::pages_of(V_pages, vps, dtype);
@@ -430,13 +490,20 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   a.W = weights, a.wb = ws[0], a.wh = ws[1];
   a.B = B, a.Hkv = (int)Hkv, a.D = (int)D, a.esz = paged::esize(dtype);
   a.budget = (int)budget, a.recent = (int)recent;
-  a.first = (int32_t*)workspace;
-  a.list = a.first + B * Hkv;
-  const int64_t slices = ceil_div(D * a.esz, 128), grid = B * Hkv * 2 * slices;
+  a.spare = (char*)workspace;
+  a.first = (int32_t*)(a.spare + 16);
+  a.list = (u32x2*)(a.spare + paged::list_at(B, Hkv));
+  // slices of 128 bytes, a line of the cache; of 64 where they leave CUs without one
+  const int64_t units = B * Hkv * 2, row = D * a.esz;
+  const bool thin = units * ceil_div(row, 128) < 256;
+  const int64_t slices = ceil_div(row, thin ? 64 : 128), grid = ceil_div(units, 8) * 8 * slices;
   if (grid > INT32_MAX) return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
   hipLaunchKernelGGL(paged::select_kernel, dim3((unsigned)(B * Hkv)), dim3(paged::ST), 0, st, a);
   if ((rc = check_launch("select launch"))) return rc;
   if (pages == 0 || budget == 0) return TSP_OK;
-  hipLaunchKernelGGL(paged::move_kernel, dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices);
+  if (thin)
+    hipLaunchKernelGGL(paged::move_kernel<4>, dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices);
+  else
+    hipLaunchKernelGGL(paged::move_kernel<8>, dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices);
   return check_launch("move launch");
 }
