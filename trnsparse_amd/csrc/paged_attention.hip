@@ -96,6 +96,28 @@ __device__ inline bool unit_of(const Args& a, uint32_t block, int per_unit, uint
   return true;
 }
 
+// The sequence whose work is the k-th largest (of up to 64; a lane has one's), so
+// that a long one does not start last and run alone.
+__device__ inline uint32_t longest_first(const Args& a, uint32_t k) {
+  if (a.B < 2 || a.B > 64) return k;
+  const int lane = threadIdx.x & 63;
+  const bool on = lane < a.B;
+  float work = -1.f;
+  if (on) {
+    const auto at = [&](const void* p) {
+      return a.len.wide ? ((const int64_t*)p)[lane] : (int64_t)((const int32_t*)p)[lane];
+    };
+    const float n = (float)clamped(at(a.len.p), a.len.slots);
+    work = n * (a.len.fresh ? (float)clamped(at(a.len.fresh), a.len.most) : 1.f);
+  }
+  uint32_t rank = 0;
+  for (int j = 0; j < a.B; ++j) {
+    const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), j));
+    rank += other > work || (other == work && j < lane);
+  }
+  return __builtin_amdgcn_readfirstlane(__builtin_ctzll(__builtin_amdgcn_ballot_w64(on && rank == k)));
+}
+
 __device__ inline const char* q_row(const Args& a, int64_t b, int64_t hk, int i, int g) {
   return a.Q.p + b * a.Q.b + (hk * a.G + g) * a.Q.h + i * a.Q.s;
 }
@@ -403,18 +425,23 @@ __global__ __launch_bounds__(256, narrow_per_cu<T>) void narrow_kernel(const Arg
   clear_rest(a, s, b, hk, item, T::ESZ);
   N::template run<SCORES>(a, s, unit, b, hk, item, lds);
 }
-// Units of any number of rows, each narrow or wide by its own.
+// Units of any number of rows, each narrow or wide by its own (wide where the
+// narrow kernel's LDS would leave one workgroup to a CU: fp32 rows of 128).
 template <typename T>
-__global__ __launch_bounds__(256, narrow_per_cu<T>) void chunk_kernel(const Args a) {
+constexpr bool chunk_has_narrow = narrow_per_cu<T> == 2;
+template <typename T>
+__global__ __launch_bounds__(256, 2) void chunk_kernel(const Args a) {
   typedef Wide<T> W;
   typedef Narrow<T> N;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[W::LDS > N::LDS ? W::LDS : N::LDS];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[chunk_has_narrow<T> && N::LDS > W::LDS ? N::LDS : W::LDS];
   uint32_t unit, b, hk;
   int item;
   if (!unit_of(a, blockIdx.x, a.items, unit, b, hk, item)) return;
+  b = longest_first(a, b);
+  unit = b * (uint32_t)a.Hkv + hk;
   const Share s = share_of(a, b, 128);
   clear_rest(a, s, b, hk, item, T::ESZ);
-  if (s.rows <= 32)
+  if (chunk_has_narrow<T> && s.rows <= 32)
     N::template run<false>(a, s, unit, b, hk, item, lds);
   else
     W::run(a, s, unit, b, hk, item, lds);
@@ -464,16 +491,17 @@ __device__ inline float combine_row(const Args& a, const Share& s, uint32_t unit
   return m + __builtin_amdgcn_logf(total);
 }
 
-// `per` workgroups to a unit, 8 rows to each.
+// `per` workgroups to a unit, 8 rows of each at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(const Args a, int per, int tile_rows) {
   const uint32_t unit = blockIdx.x / (uint32_t)per, part = blockIdx.x - unit * (uint32_t)per;
   const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
   const Share s = share_of(a, b, tile_rows);
-  const int r = (int)part * 8 + (int)(threadIdx.x >> 5);
-  if (s.splits == 1 || r >= s.rows) return;
-  const float lse = combine_row<T>(a, s, unit, b, hk, tile_rows, r);
-  if (a.lse && (threadIdx.x & 31) == 0) a.lse[(int64_t)unit * a.R + r] = lse;
+  if (s.splits == 1) return;
+  for (int r = (int)part * 8 + (int)(threadIdx.x >> 5); r < s.rows; r += 8 * per) {
+    const float lse = combine_row<T>(a, s, unit, b, hk, tile_rows, r);
+    if (a.lse && (threadIdx.x & 31) == 0) a.lse[(int64_t)unit * a.R + r] = lse;
+  }
 }
 
 // After the narrow kernel: workgroups [0, cw) of a unit join its rows (where the
@@ -581,7 +609,7 @@ __global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
   auto put_neg = [&](int buf, float e) {
     if ((int)threadIdx.x < G::HR) neg[buf][threadIdx.x] = e == -INFINITY ? e : -e;
   };
-  float sum = 0.f;
+  f32x4 sum = f32x4{};
   put_neg(0, lse_of(first));
   float ahead = lse_of(first + G::HR);
   issue(first, 0);
@@ -594,22 +622,33 @@ __global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
     if (r0 + G::HR < s.rows) issue(r0 + G::HR, st ^ 1);
     f32x16 c[G::NT];
     T::template scores<G::NT>(c, lds0 + st * G::STAGE, ln, k);
-    const bool check = r0 < all_from;
+    // rows that do not see the key, and rows behind the last (zeros, which an
+    // infinite key would turn into NaN)
+    const bool check = r0 < all_from || r0 + G::HR > s.rows;
+    auto add = [&](auto masked) {
 #pragma unroll
-    for (int t = 0; t < G::NT; ++t)
+      for (int t = 0; t < G::NT; ++t)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 e = *(const f32x4*)&neg[st][32 * t + 8 * q + 4 * h];
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 e = *(const f32x4*)&neg[st][32 * t + 8 * q + 4 * h];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[t][4 * q + v], a.scale_log2, e[v]));
-          if (e[v] == -INFINITY || (check && r0 + 32 * t + 8 * q + 4 * h + v < seen_by)) p = 0.f;
-          sum += p;
+          for (int v = 0; v < 4; ++v) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[t][4 * q + v], a.scale_log2, e[v]));
+            if constexpr (decltype(masked)::value) {
+              const int r = r0 + 32 * t + 8 * q + 4 * h + v;
+              if (r < seen_by || r >= s.rows) p = 0.f;
+            }
+            sum[v] += p;
+          }
         }
-      }
+    };
+    if (check)
+      add(std::true_type{});
+    else
+      add(std::false_type{});
   }
-  sum = xat::halves_sum(sum);
-  if (live && h == 0) a.W[b * a.wb + hk * a.wh + j] += sum;
+  const float total = xat::halves_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (live && h == 0) a.W[b * a.wb + hk * a.wh + j] += total;
 }
 
 // ------------------------------------------------------------------- host
@@ -624,15 +663,19 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   const int64_t G = Hq / Hkv, R = G * Sq, units = B * Hkv;
   const bool f32 = dtype == TSP_F32;
   p.narrow = R <= 32;
-  const int64_t tiles = p.narrow ? 1 : ceil_div(R, 128);
-  p.least = p.narrow ? (f32 ? 128 : 512) : 256;
-  p.step = 128;
+  const int64_t tiles = p.narrow ? 1 : ceil_div(R, 128), wgs = units * tiles;
+  // Ranges of keys: as many as bring the rounds of workgroups that fit the CUs
+  // at once, each of its keys and of as much as `least` keys more (starting,
+  // joining), to the shortest time.
+  p.least = p.narrow ? (f32 ? 128 : 512) : (f32 ? 64 : 256);
+  p.step = p.narrow ? 128 : 64;
   p.slot_rows = (int)(p.narrow ? R : 128);
-  const int64_t want = p.narrow && f32 ? 256 : 512, wgs = units * tiles;
-  int64_t n = wgs >= (p.narrow && f32 ? want : want / 2) ? 1 : ceil_div(want, wgs);
-  const int64_t most = ceil_div(keys > 0 ? keys : 1, p.least);
-  n = n < most ? n : most;
-  n = n < 32 ? n : 32;
+  const int64_t room = p.narrow && f32 && D > 64 ? 256 : 512, most = ceil_div(keys > 0 ? keys : 1, p.least);
+  int64_t n = 1, best = INT64_MAX;
+  for (int64_t k = 1; k <= 32 && k <= most; ++k) {
+    const int64_t cost = ceil_div(wgs * k, room) * (ceil_div(keys, k) + p.least);
+    if (cost < best) best = cost, n = k;
+  }
   p.items = (int)(tiles * n);
   p.slots = n > 1 ? p.items : 0;
   if (ragged && !p.narrow && n == 1) {
@@ -715,7 +758,8 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const int64_t wper = ceil_div(keys, 128), wgrid = weigh && !p.narrow ? head_grid(wper, units) : 0;
   const int tile_rows = p.narrow ? 32 : 128;
   const int64_t joined = p.narrow ? a.R : (int64_t)(p.slots / 2) * 128 < a.R ? (int64_t)(p.slots / 2) * 128 : a.R;
-  const int64_t cper = p.slots > 1 ? ceil_div(joined, 8) : 0;
+  int64_t cper = p.slots > 1 ? ceil_div(joined, 8) : 0;
+  if (!p.narrow && new_lengths && cper > ceil_div(2048, units)) cper = ceil_div(2048, units);  // (most have few rows)
   // 1024 keys and more to a workgroup, as many as fill the CUs
   int64_t kper = ceil_div(2048, units);
   if (kper > ceil_div(keys, 1024)) kper = ceil_div(keys, 1024);
