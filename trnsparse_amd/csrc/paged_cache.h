@@ -20,7 +20,7 @@ struct Table {
   const void* p;
   int64_t ld;      // entries between rows
   int64_t pages;   // below 2^31
-  int wide;        // entries are int64 (else int32)
+  int wide;        // 1: entries are int64 (0: int32)
   int cols;
   int page_size;
   uint64_t recip;  // ceil(2^32 / (page_size / PIECE))
@@ -63,10 +63,19 @@ __device__ inline uint32_t page_at(const Table& t, int64_t row, uint32_t col) {
   const int64_t id = index_at(t.p, t.wide, row + col);
   return id >= 0 && id < t.pages ? (uint32_t)id : NO_PAGE;
 }
-// The same where the lanes of a wavefront ask for different columns.
+// The same where the lanes of a wavefront ask for different columns: an entry's
+// halves as they are (int32 entries: the entry twice), and what page they name.
+// Both without a branch, which would wait for other loads in flight.
+__device__ inline u32x2 entry_of_lane(const Table& t, int64_t row, uint32_t col) {
+  const uint32_t* p = (const uint32_t*)t.p + ((row + col) << t.wide);
+  return u32x2{p[0], p[t.wide]};
+}
+__device__ inline uint32_t page_of_entry(const Table& t, u32x2 e) {
+  const uint32_t bad = (uint32_t)(e.x >= (uint32_t)t.pages) | ((uint32_t)t.wide & (uint32_t)(e.y != 0));
+  return e.x | (0u - bad);
+}
 __device__ inline uint32_t page_of_lane(const Table& t, int64_t row, uint32_t col) {
-  const int64_t id = t.wide ? ((const int64_t*)t.p)[row + col] : (int64_t)((const int32_t*)t.p)[row + col];
-  return id >= 0 && id < t.pages ? (uint32_t)id : NO_PAGE;
+  return page_of_entry(t, entry_of_lane(t, row, col));
 }
 
 // ------------------------------------------------------------------- host

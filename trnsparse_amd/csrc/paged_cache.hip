@@ -105,9 +105,9 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, int64_t
 // -------------------------------------------------------------- eviction
 // select_kernel, one workgroup to a (sequence, head) pair: the key (an unsigned
 // number in the order of the weights, NaN above all) of the k-th largest of the
-// rows that may go, by three histograms of the keys' digits between the smallest
-// and the largest; then one pass in the rows' order that lists the kept ones and
-// moves their weights, each to a place at or before its own.
+// rows that may go, by histograms of the keys' digits of 11, 11 and 10 bits, fewer
+// where all rows with the digits so far stay; then one pass in the rows' order that
+// lists the kept ones and moves their weights, each to a place at or before its own.
 // move_kernel moves the listed rows of K and V to their places. A row goes to a
 // place at or before its own, and the list rises: a workgroup that takes the list
 // in order, and writes a part only once all of its rows are read, never writes
@@ -168,7 +168,7 @@ struct Part {
 __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
   __shared__ uint32_t hist[BINS];
   __shared__ int sums[2][2][ST / 64];
-  __shared__ uint32_t lo_hi[2][ST / 64], pick[2];
+  __shared__ uint32_t pick[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t unit = blockIdx.x, b = unit / a.Hkv, h = unit - b * a.Hkv;
   const int64_t n64 = cached_rows(a.len, b);
@@ -189,50 +189,30 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
   const int E = n - a.recent;            // rows that may go
   const int keep = a.budget - a.recent;  // of those, the ones that stay (fewer than E)
   // The rows of up to one part stay in registers; of more, each pass reads them
-  // again, the next part's while one is worked on.
+  // again, two parts ahead of the one that is worked on.
   const bool once = n <= PART;
   Part held;
   held.load(w, tid * SPT, n, aligned);
   auto each = [&](int end, auto&& f) {
-    Part now = held;
-    for (int j0 = 0; j0 < end; j0 += PART) {
-      Part next;
-      if (!once) next.load(w, j0 + PART + tid * SPT, n, aligned);
-      f(j0 + tid * SPT, now);
-      if (!once) now = next;
+    Part even = held, odd;
+    if (!once) odd.load(w, PART + tid * SPT, n, aligned);
+    for (int j0 = 0; j0 < end; j0 += 2 * PART) {
+      f(j0 + tid * SPT, even);
+      if (once) break;
+      even.load(w, j0 + 2 * PART + tid * SPT, n, aligned);
+      if (j0 + PART < end) f(j0 + PART + tid * SPT, odd);
+      odd.load(w, j0 + 3 * PART + tid * SPT, n, aligned);
     }
   };
-  // the key of the last that stays, and how many with that key do
+  // `last`: the keys above it stay, and of those equal to it the first `equal` ones
   uint32_t last = 0xffffffffu;
   int equal = 0;
   if (keep > 0) {
-    uint32_t lo = 0xffffffffu, hi = 0;
-    each(E, [&](int j, const Part& p) {
-#pragma unroll
-      for (int i = 0; i < SPT; ++i) {
-        const uint32_t k = order_key(p.v[i]);
-        lo = j + i < E && k < lo ? k : lo;
-        hi = j + i < E && k > hi ? k : hi;
-      }
-    });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint32_t l = __shfl_xor(lo, o, 64), g = __shfl_xor(hi, o, 64);
-      lo = l < lo ? l : lo;
-      hi = g > hi ? g : hi;
-    }
-    if (lane == 0) lo_hi[0][wave] = lo, lo_hi[1][wave] = hi;
     for (int i = tid; i < BINS; i += ST) hist[i] = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ST / 64; ++i) {
-      lo = lo_hi[0][i] < lo ? lo_hi[0][i] : lo;
-      hi = lo_hi[1][i] > hi ? lo_hi[1][i] : hi;
-    }
+    uint32_t lo = 0, hi = 0xffffffffu;
     int want = keep;  // the place of the wanted key among those of [lo, hi], from the largest
-    while (lo < hi) {
-      const uint32_t span = hi - lo;
-      const int shift = 32 - __builtin_clz(span) > 11 ? 32 - __builtin_clz(span) - 11 : 0;  // BINS digits
+    for (int shift = 21;; shift = shift > 10 ? shift - 11 : 0) {
       each(E, [&](int j, const Part& p) {
 #pragma unroll
         for (int i = 0; i < SPT; ++i) {
@@ -254,15 +234,22 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
         const bool second = want > before + c0;
         pick[0] = (uint32_t)(second ? d - 1 : d);
         pick[1] = (uint32_t)(want - before - (second ? c0 : 0));
+        pick[2] = (uint32_t)(second ? c1 : c0);
       }
       __syncthreads();
       want = (int)pick[1];
-      const uint32_t low = lo + (pick[0] << shift), width = shift ? (1u << shift) - 1 : 0;
-      hi = hi - low < width ? hi : low + width;
-      lo = low;
+      lo += pick[0] << shift;
+      hi = lo + (shift ? (1u << shift) - 1 : 0);
+      if (want == (int)pick[2]) {  // all with this digit stay
+        last = lo - 1;             // (no key is zero: it would be a NaN's)
+        break;
+      }
+      if (shift == 0) {
+        last = lo;
+        equal = want;
+        break;
+      }
     }
-    last = lo;
-    equal = want;
   }
   __syncthreads();
   // the kept rows in order; those that equal the last one's key as far as they go
@@ -326,13 +313,15 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
 }
 
 // LPR lanes (16 bytes each) to a row's slice, MU rows of a thread in a part of the
-// list. The list's entries come two parts ahead, the rows one. A thread without
-// a row takes the last one's (and stores the same once more), one without a page
-// the spare place, so that no branch keeps a wait from being counted.
+// list. The list's entries come two parts ahead, the rows one, in three sets of
+// registers by turns. A thread without a row takes the last one's (and stores the
+// same once more), one without a page the spare place, so that no branch keeps a
+// wait from being counted.
 constexpr int MT = 512, MU = 8;
 struct Move {
-  u32x2 from[MU];   // page and row
-  uint32_t to[MU];  // page
+  u32x2 from[MU];  // page and row
+  u32x2 to[MU];    // the table's entry
+  u32x4 v[MU];
 };
 template <int LPR>
 __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t slices) {
@@ -356,44 +345,51 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
     const int d = d0 + RP * u + at;
     return (uint32_t)(d < end ? d : end);
   };
+  // a row's place, or the spare one
+  auto spot = [&](uint32_t page, uint32_t row) {
+    const uint64_t none = 0 - (uint64_t)(page == NO_PAGE);
+    const uint64_t there = (uint64_t)(base + (int64_t)(page & ~(uint32_t)none) * p.page + row * p.s);
+    return (u32x4*)((there & ~none) | ((uint64_t)a.spare & none));
+  };
   auto look = [&](Move& m, int d0) {
 #pragma unroll
     for (int u = 0; u < MU; ++u) {
       const uint32_t d = place(d0, u);
       m.from[u] = list[d];
-      m.to[u] = page_of_lane(a.t, trow, column_of(a.t, d / PIECE));
+      m.to[u] = entry_of_lane(a.t, trow, column_of(a.t, d / PIECE));
     }
   };
-  auto load = [&](u32x4* v, const Move& m) {
+  auto load = [&](Move& m) {
 #pragma unroll
     for (int u = 0; u < MU; ++u) {
-      const bool there = m.from[u].x != NO_PAGE;
-      const char* q = there ? base + m.from[u].x * p.page + m.from[u].y * p.s : a.spare;
-      v[u] = *(const u32x4*)q;
-      if (!there) v[u] = u32x4{};
+      m.v[u] = *spot(m.from[u].x, m.from[u].y);
     }
   };
-  Move m0, m1, m2;
-  u32x4 now[MU], next[MU];
-  look(m0, first);
-  look(m1, first + PR);
-  load(now, m0);
-  for (int d0 = first; d0 <= end; d0 += PR) {
-    look(m2, d0 + 2 * PR);
-    load(next, m1);
+  auto step = [&](Move& now, Move& next, Move& later, int d0) {
+    look(later, d0 + 2 * PR);
+    load(next);
     // the rows of this part have arrived in every wavefront before one is written
 #pragma unroll
-    for (int u = 0; u < MU; ++u) asm volatile("" : "+v"(now[u]));
+    for (int u = 0; u < MU; ++u) asm volatile("" : "+v"(now.v[u]));
     asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int u = 0; u < MU; ++u) {
       const uint32_t d = place(d0, u), r = d - column_of(a.t, d / PIECE) * (uint32_t)a.t.page_size;
-      char* q = m0.to[u] != NO_PAGE ? base + m0.to[u] * p.page + r * p.s : a.spare;
-      *(u32x4*)q = now[u];
-      now[u] = next[u];
+      const uint32_t keep = 0u - (uint32_t)(now.from[u].x != NO_PAGE);
+      *spot(page_of_entry(a.t, now.to[u]), r) = now.v[u] & keep;
     }
-    m0 = m1;
-    m1 = m2;
+  };
+  Move m0, m1, m2;
+  look(m0, first);
+  look(m1, first + PR);
+  load(m0);
+  for (int d0 = first;; d0 += 3 * PR) {
+    step(m0, m1, m2, d0);
+    if (d0 + PR > end) break;
+    step(m1, m2, m0, d0 + PR);
+    if (d0 + 2 * PR > end) break;
+    step(m2, m0, m1, d0 + 2 * PR);
+    if (d0 + 3 * PR > end) break;
   }
 }
 
