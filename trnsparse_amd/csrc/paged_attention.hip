@@ -20,11 +20,11 @@
 // their own normalised result and log-sum-exp in fp32, which combine_kernel
 // joins in the ranges' order.
 //
-// The accumulated weights need the final log-sum-exp of every row. Few rows:
+// The accumulated weights need the final log-sum-exp of every row. Up to 16 rows:
 // the narrow kernel keeps its scores (4 bytes a pair, where reading K again is 2
-// head_dim bytes a key) and weigh_kernel adds up their exponentials. Many: the
+// head_dim bytes a key), whose exponentials are added up afterwards. More: the
 // scores are formed again, a wavefront having 32 keys as its own rows and the
-// queries staged, so that a key's sum stays in its lane (weights_wide). Either
+// queries staged, so that a key's sum stays in its lane (weights_kernel). Either
 // way one workgroup owns a key and adds in a fixed order: no atomics.
 #include "lds_dma.h"
 #include "paged_cache.h"
@@ -55,7 +55,8 @@ struct Args {
   int slot_rows;             // rows of one such result
   float *part, *plse;        // [unit][slot][row]: results, log-sum-exps (base 2)
   float* lse;                // [unit][R]: log-sum-exps (base 2) where the weights need them, else null
-  float* scores;             // [unit][stage of 32 keys][R][32], log2 units; else null
+  float* scores;             // [unit][stage of 32 keys][sr][32], log2 units, of units of up to sr rows
+  int sr;
   int stages;                // of a unit
   float scale_log2;
   float* W;
@@ -324,7 +325,7 @@ struct Narrow {
     xat::RowState<T> x;
     x.clear();
     float* sc = nullptr;
-    if constexpr (SCORES) sc = a.scores + ((int64_t)unit * a.stages * a.R + l32) * 32 + 4 * h;
+    if constexpr (SCORES) sc = a.scores + ((int64_t)unit * a.stages * a.sr + l32) * 32 + 4 * h;
     for (int st = 0; st < mine; ++st) {
       const bool more = st + 1 < mine;
       const int at = key(st);
@@ -342,7 +343,7 @@ struct Narrow {
           [&] {
             if constexpr (SCORES) {
               // four stores of every wavefront, its first row being there
-              float* p = sc + (int64_t)(at / 32) * a.R * 32;
+              float* p = sc + (int64_t)(at / 32) * a.sr * 32;
               if (live) {
 #pragma unroll
                 for (int v = 0; v < 4; ++v)
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(256, narrow_per_cu<T>) void narrow_kernel(const Arg
 // narrow kernel's LDS would leave one workgroup to a CU: fp32 rows of 128).
 template <typename T>
 constexpr bool chunk_has_narrow = narrow_per_cu<T> == 2;
-template <typename T>
+template <typename T, bool SCORES>
 __global__ __launch_bounds__(256, 2) void chunk_kernel(const Args a) {
   typedef Wide<T> W;
   typedef Narrow<T> N;
@@ -441,7 +442,9 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const Args a) {
   unit = b * (uint32_t)a.Hkv + hk;
   const Share s = share_of(a, b, 128);
   clear_rest(a, s, b, hk, item, T::ESZ);
-  if (chunk_has_narrow<T> && s.rows <= 32)
+  if (SCORES && s.rows <= a.sr)
+    N::template run<true>(a, s, unit, b, hk, item, lds);
+  else if (chunk_has_narrow<T> && s.rows <= 32)
     N::template run<false>(a, s, unit, b, hk, item, lds);
   else
     W::run(a, s, unit, b, hk, item, lds);
@@ -504,6 +507,18 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a, int per, int
   }
 }
 
+// The weight of key k of a unit whose scores are kept (a key that a row does not
+// see has a score of -inf).
+__device__ inline float weight_of(const Args& a, const Share& s, uint32_t unit, const float* lse, int k) {
+  const float* p = a.scores + ((int64_t)unit * a.stages + k / 32) * a.sr * 32 + k % 32;
+  float sum = 0.f;
+  for (int r = 0; r < s.rows; ++r) {
+    const float c = p[r * 32];
+    sum += c == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(c - lse[r]);
+  }
+  return sum;
+}
+
 // After the narrow kernel: workgroups [0, cw) of a unit join its rows (where the
 // keys were taken in ranges), the other `kw` add up the keys' weights, 256 keys
 // at a time, from the scores and the rows' log-sum-exps.
@@ -539,39 +554,44 @@ __global__ __launch_bounds__(256) void weigh_kernel(const Args a, int cw, int kw
   }
   __syncthreads();
   float* w = a.W + b * a.wb + hk * a.wh;
-  for (int k = (part - cw) * 256 + (int)threadIdx.x; k < s.n; k += 256 * kw) {
-    const float* p = a.scores + ((int64_t)unit * a.stages + k / 32) * a.R * 32 + k % 32;
-    float sum = 0.f;
-    for (int r = 0; r < s.rows; ++r) {
-      const float c = p[r * 32];
-      // (a key that the row does not see has a score of -inf)
-      sum += c == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(c - lse[r]);
-    }
-    w[k] += sum;
-  }
+  for (int k = (part - cw) * 256 + (int)threadIdx.x; k < s.n; k += 256 * kw) w[k] += weight_of(a, s, unit, lse, k);
 }
 
 // ------------------------------------------------- weights of many rows
-// 128 keys to a workgroup, a wavefront to 32; the unit's rows staged 64 (fp32:
-// 32) at a time with their log-sum-exps.
-template <typename T>
+// 32 keys to a wavefront as its own rows; the unit's rows staged 64 or 32 at a
+// time with their log-sum-exps.
+//   RW 1  128 keys to a workgroup, whose four wavefronts share the stages
+//   RW 4  32 keys to a workgroup, every wavefront with every fourth stage of 32
+//         rows through LDS of its own, their sums added at the end: four times as
+//         many workgroups, each a quarter as long, for launches that have few
+template <typename T, int RW>
 struct Weigh {
-  static constexpr int NT = T::ESZ == 2 ? 2 : 1, HR = 32 * NT, STAGE = HR * T::ROWB, LDS = 2 * STAGE;
-  static constexpr int RPI = 64 / T::CPR, MINE = HR / 4, NI = MINE / RPI;
+  static constexpr int NT = RW == 1 && T::ESZ == 2 ? 2 : 1, HR = 32 * NT, STAGE = HR * T::ROWB;
+  static constexpr int KEYS = 128 / RW, RINGS = RW, LDS = RINGS * 2 * STAGE;
+  static constexpr int RPI = 64 / T::CPR, MINE = RW == 1 ? HR / 4 : HR, NI = MINE / RPI;
 };
-template <typename T>
-__global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
-  typedef Weigh<T> G;
+template <typename T, int RW>
+__global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void weights_kernel(const Args a, int per) {
+  typedef Weigh<T, RW> G;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[G::LDS];
-  __shared__ __attribute__((aligned(16))) float neg[2][G::HR];  // minus the rows' log-sum-exps
+  __shared__ __attribute__((aligned(256))) float lse[G::RINGS][2][64];  // of a stage's rows
   uint32_t unit, b, hk;
   int item;
   if (!unit_of(a, blockIdx.x, per, unit, b, hk, item)) return;
+  b = longest_first(a, b);
+  unit = b * (uint32_t)a.Hkv + hk;
   const Share s = share_of(a, b, 128);
-  const int j0 = item * 128;
+  const int j0 = item * G::KEYS;
   if (j0 >= s.n || s.rows == 0) return;
+  float* W = a.W + b * a.wb + hk * a.wh;
+  if (s.rows <= a.sr) {
+    const int k = j0 + (int)threadIdx.x;
+    if ((int)threadIdx.x < G::KEYS && k < s.n) W[k] += weight_of(a, s, unit, a.lse + (int64_t)unit * a.R, k);
+    return;
+  }
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int j = j0 + w * 32 + (lane & 31);
+  const int k0 = RW == 1 ? j0 + w * 32 : j0, j = k0 + (lane & 31);  // this wavefront's keys, this lane's
+  const int ring = RW == 1 ? 0 : w, w4 = RW == 1 ? w : 0;
   const bool live = j < s.n;
   typename T::Rows k;
   {
@@ -581,47 +601,55 @@ __global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
     T::load(k, p, live && page != NO_PAGE, a.D, h);
   }
   const int before = s.n - s.m;  // token i sees keys up to before + i
-  const int first = j0 > before ? (j0 - before) * a.G / G::HR * G::HR : 0;  // the first row that sees a key
-  const int seen_by = (j > before ? j - before : 0) * a.G;                  // ... that sees this lane's
-  const int all_from = (j0 + w * 32 + 31 > before ? j0 + w * 32 + 31 - before : 0) * a.G;
+  const int first = j0 > before ? (j0 - before) * a.G / G::HR : 0;  // the first stage with a row that sees a key
+  const int stages = (s.rows + G::HR - 1) / G::HR;
+  const int seen_by = (j > before ? j - before : 0) * a.G;          // the first row that sees this lane's key
+  const int all_from = (k0 + 31 > before ? k0 + 31 - before : 0) * a.G;
   const char* Qh = a.Q.p + b * a.Q.b + hk * a.G * a.Q.h;
+  const float* L = a.lse + (int64_t)unit * a.R;
   const typename T::Lane ln = T::lane_of(lane);
-  const uint32_t lds0 = dma::lds_addr(lds), mine = w * (G::MINE * T::ROWB);
-  // A stage's rows through a buffer that begins with the first row's token.
-  auto issue = [&](int r0, int buf) {
-    const int i0 = r0 / a.G;
+  const uint32_t lds0 = dma::lds_addr(lds) + ring * 2 * G::STAGE, mine = w4 * (G::MINE * T::ROWB);
+  const uint32_t lse0 = dma::lds_addr(lse) + ring * 512;
+  // A stage's rows through a buffer that begins with the first row's token, rows
+  // behind the last as zeros; then their log-sum-exps.
+  auto issue = [&](int st, int buf) {
+    const int r0 = st * G::HR, i0 = r0 / a.G;
     const dma::i32x4 rs = dma::make_rsrc(Qh + i0 * a.Q.s, OUT_OF_RANGE);
 #pragma unroll
     for (int u = 0; u < G::NI; ++u) {
-      const int x = G::MINE * w + G::RPI * u + lane / T::CPR, r = r0 + x, c = (lane % T::CPR) ^ T::swz(x);
+      const int x = G::MINE * w4 + G::RPI * u + lane / T::CPR, r = r0 + x, c = (lane % T::CPR) ^ T::swz(x);
       const int i = r / a.G, g = r - i * a.G;
       const uint32_t off = (uint32_t)((i - i0) * a.Q.s + g * a.Q.h) + 16u * c;
       dma::buffer16(rs, r < s.rows && c * T::CE < a.D ? off : OUT_OF_RANGE, lds0 + buf * G::STAGE + mine + u * 1024);
     }
-  };
-  // The log-sum-exps go through a register, loaded a stage ahead of the stage's
-  // rows: waited for with the loads before them. Rows behind the last, and rows
-  // that see nothing, weigh nothing.
-  auto lse_of = [&](int r0) {
-    const int r = r0 + (int)threadIdx.x;
-    return (int)threadIdx.x < G::HR && r < s.rows ? a.lse[(int64_t)unit * a.R + r] : -INFINITY;
-  };
-  auto put_neg = [&](int buf, float e) {
-    if ((int)threadIdx.x < G::HR) neg[buf][threadIdx.x] = e == -INFINITY ? e : -e;
+    if (RW > 1 || w == 0) {
+      const int left = s.rows - r0;
+      const dma::i32x4 ls = dma::make_rsrc(L + r0, 4u * (uint32_t)(left < G::HR ? left : G::HR));
+      dma::buffer4(ls, 4u * (uint32_t)lane, lse0 + buf * 256);
+    }
   };
   f32x4 sum = f32x4{};
-  put_neg(0, lse_of(first));
-  float ahead = lse_of(first + G::HR);
-  issue(first, 0);
-  for (int r0 = first, st = 0; r0 < s.rows; r0 += G::HR, st ^= 1) {
-    asm volatile("" : "+v"(ahead));
-    dma::wait_vm<0>();
-    dma::barrier();
-    put_neg(st ^ 1, ahead);
-    ahead = lse_of(r0 + 2 * G::HR);
-    if (r0 + G::HR < s.rows) issue(r0 + G::HR, st ^ 1);
+  constexpr int STEP = RW;
+  int st = RW == 1 ? first : first + (w + RW - first % RW) % RW;
+  if (st < stages) issue(st, 0);
+  for (int buf = 0; st < stages; st += STEP, buf ^= 1) {
+    if constexpr (RW == 1) {
+      dma::wait_vm<0>();
+      dma::barrier();
+      if (st + STEP < stages) issue(st + STEP, buf ^ 1);
+    } else {
+      if (st + STEP < stages) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage before has been read
+        issue(st + STEP, buf ^ 1);
+        dma::wait_vm<G::NI + 1>();
+      } else {
+        dma::wait_vm<0>();
+      }
+      asm volatile("" ::: "memory");
+    }
     f32x16 c[G::NT];
-    T::template scores<G::NT>(c, lds0 + st * G::STAGE, ln, k);
+    T::template scores<G::NT>(c, lds0 + buf * G::STAGE, ln, k);
+    const int r0 = st * G::HR;
     // rows that do not see the key, and rows behind the last (zeros, which an
     // infinite key would turn into NaN)
     const bool check = r0 < all_from || r0 + G::HR > s.rows;
@@ -630,10 +658,10 @@ __global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
       for (int t = 0; t < G::NT; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4 e = *(const f32x4*)&neg[st][32 * t + 8 * q + 4 * h];
+          const f32x4 e = *(const f32x4*)&lse[ring][buf][32 * t + 8 * q + 4 * h];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[t][4 * q + v], a.scale_log2, e[v]));
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[t][4 * q + v], a.scale_log2, -e[v]));
             if constexpr (decltype(masked)::value) {
               const int r = r0 + 32 * t + 8 * q + 4 * h + v;
               if (r < seen_by || r >= s.rows) p = 0.f;
@@ -647,8 +675,17 @@ __global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
     else
       add(std::false_type{});
   }
-  const float total = xat::halves_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-  if (live && h == 0) a.W[b * a.wb + hk * a.wh + j] += total;
+  float total = xat::halves_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if constexpr (RW > 1) {
+    float* x = &lse[0][0][0];
+    __syncthreads();
+    if (h == 0) x[w * 32 + (lane & 31)] = total;
+    __syncthreads();
+    if (w) return;
+    const int l32 = lane & 31;
+    total = (x[l32] + x[32 + l32]) + (x[64 + l32] + x[96 + l32]);
+  }
+  if (live && h == 0) W[j] += total;
 }
 
 // ------------------------------------------------------------------- host
@@ -656,6 +693,7 @@ __global__ __launch_bounds__(256, 2) void weights_wide(const Args a, int per) {
 struct Plan {
   bool narrow;
   int items, slots, least, step, slot_rows;
+  int sr;
   int64_t part, lse, scores;  // floats
 };
 Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t keys, int64_t D, bool ragged, bool weights) {
@@ -687,7 +725,10 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   auto pad = [](int64_t v) { return ceil_div(v, 64) * 64; };
   p.part = pad(p.slots * units * p.slot_rows * (D + 1));
   p.lse = weights ? pad(units * R) : 0;
-  p.scores = weights && p.narrow ? units * ceil_div(keys, 32) * R * 32 : 0;
+  // scores of up to 16 rows are kept (with a chunk's workgroups, those of the
+  // sequences that have so few)
+  p.sr = (int)(!weights || (p.narrow ? R > 16 : !ragged || (f32 && D > 64)) ? 0 : R < 16 ? R : 16);
+  p.scores = units * ceil_div(keys, 32) * p.sr * 32;
   return p;
 }
 
@@ -746,16 +787,21 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   a.plse = a.part + p.slots * units * p.slot_rows * D;
   if (weigh) {
     a.lse = (float*)workspace + p.part;
-    a.scores = p.narrow ? a.lse + p.lse : nullptr;
+    a.scores = a.lse + p.lse;
+    a.sr = p.sr;
     a.stages = (int)ceil_div(keys, 32);
     a.W = weights, a.wb = ws[0], a.wh = ws[1];
     // a stage of queries is read at 32-bit offsets from its first token
-    if (!p.narrow && (double)(a.G - 1) * a.Q.h + 66.0 * a.Q.s + 512 >= 2147483632.0)
+    if ((double)(a.G - 1) * a.Q.h + 66.0 * a.Q.s + 512 >= 2147483632.0)
       return fail(TSP_EUNSUPPORTED, "%s: weights of query heads that lie 2 GiB apart", who);
   }
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   const int64_t grid = head_grid(p.items, units);
-  const int64_t wper = ceil_div(keys, 128), wgrid = weigh && !p.narrow ? head_grid(wper, units) : 0;
+  // (9 units of 1008 keys and up to 399 rows in fp32: 28 us with 128 keys to a workgroup)
+  const bool few = units * ceil_div(keys, 128) < 512;
+  const int64_t wper = ceil_div(keys, few ? 32 : 128);
+  const bool again = weigh && !(p.narrow && p.sr > 0);  // some scores are formed again
+  const int64_t wgrid = again ? head_grid(wper, units) : 0;
   const int tile_rows = p.narrow ? 32 : 128;
   const int64_t joined = p.narrow ? a.R : (int64_t)(p.slots / 2) * 128 < a.R ? (int64_t)(p.slots / 2) * 128 : a.R;
   int64_t cper = p.slots > 1 ? ceil_div(joined, 8) : 0;
@@ -769,15 +815,17 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   return xat::with_tile(dtype, D, [&](auto tile) {
     typedef decltype(tile) T;
     const dim3 g((unsigned)grid), t(256);
-    if (p.narrow && weigh)
+    if (p.narrow && p.sr > 0)
       hipLaunchKernelGGL((paged::narrow_kernel<T, true>), g, t, 0, st, a);
     else if (p.narrow)
       hipLaunchKernelGGL((paged::narrow_kernel<T, false>), g, t, 0, st, a);
+    else if (p.sr > 0)
+      hipLaunchKernelGGL((paged::chunk_kernel<T, paged::chunk_has_narrow<T>>), g, t, 0, st, a);
     else
-      hipLaunchKernelGGL((paged::chunk_kernel<T>), g, t, 0, st, a);
+      hipLaunchKernelGGL((paged::chunk_kernel<T, false>), g, t, 0, st, a);
     int rc = check_launch("paged attention launch");
     if (rc) return rc;
-    if (p.narrow && weigh) {
+    if (p.narrow && p.sr > 0) {
       hipLaunchKernelGGL((paged::weigh_kernel<T>), dim3((unsigned)(units * (cper + kper))), t, 0, st, a, (int)cper,
                          (int)kper);
       return check_launch("weights launch");
@@ -786,8 +834,11 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
       hipLaunchKernelGGL((paged::combine_kernel<T>), dim3((unsigned)(units * cper)), t, 0, st, a, (int)cper, tile_rows);
       if ((rc = check_launch("combine launch"))) return rc;
     }
-    if (weigh) {
-      hipLaunchKernelGGL((paged::weights_wide<T>), dim3((unsigned)wgrid), t, 0, st, a, (int)wper);
+    if (again) {
+      if (few)
+        hipLaunchKernelGGL((paged::weights_kernel<T, 4>), dim3((unsigned)wgrid), t, 0, st, a, (int)wper);
+      else
+        hipLaunchKernelGGL((paged::weights_kernel<T, 1>), dim3((unsigned)wgrid), t, 0, st, a, (int)wper);
       return check_launch("weights launch");
     }
     return TSP_OK;
