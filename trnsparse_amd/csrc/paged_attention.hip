@@ -611,16 +611,33 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
   const uint32_t lds0 = dma::lds_addr(lds) + ring * 2 * G::STAGE, mine = w4 * (G::MINE * T::ROWB);
   const uint32_t lse0 = dma::lds_addr(lse) + ring * 512;
   // A stage's rows through a buffer that begins with the first row's token, rows
-  // behind the last as zeros; then their log-sum-exps.
+  // behind the last as zeros; then their log-sum-exps. Where stages are whole
+  // tokens, the rows' offsets are the same in all of them.
+  const uint32_t qs = (uint32_t)a.Q.s, qh = (uint32_t)a.Q.h;
+  const uint32_t group_recip = 0xffffffffu / (uint32_t)a.G + 1;
+  uint32_t offs[G::NI];
+  auto offset = [&](int u, int skip) {
+    const int x = G::MINE * w4 + G::RPI * u + lane / T::CPR, c = (lane % T::CPR) ^ T::swz(x);
+    // v / G of v below 64 + G: one or none from G = 64 on; below, by the reciprocal
+    // ceil(2^32 / G), which is exact for v G < 2^32 (and passes 32 bits for G = 1)
+    const uint32_t v = (uint32_t)(skip + x), G1 = (uint32_t)a.G;
+    const uint32_t i = G1 >= 64 ? (uint32_t)(v >= G1) : G1 == 1 ? v : __umulhi(v, group_recip), g = v - i * G1;
+    return c * T::CE < a.D ? i * qs + g * qh + 16u * c : OUT_OF_RANGE;
+  };
+  const bool even = G::HR % a.G == 0;
+#pragma unroll
+  for (int u = 0; u < G::NI; ++u) offs[u] = offset(u, 0);
   auto issue = [&](int st, int buf) {
     const int r0 = st * G::HR, i0 = r0 / a.G;
     const dma::i32x4 rs = dma::make_rsrc(Qh + i0 * a.Q.s, OUT_OF_RANGE);
+    if (!even) {
+#pragma unroll
+      for (int u = 0; u < G::NI; ++u) offs[u] = offset(u, r0 - i0 * a.G);
+    }
 #pragma unroll
     for (int u = 0; u < G::NI; ++u) {
-      const int x = G::MINE * w4 + G::RPI * u + lane / T::CPR, r = r0 + x, c = (lane % T::CPR) ^ T::swz(x);
-      const int i = r / a.G, g = r - i * a.G;
-      const uint32_t off = (uint32_t)((i - i0) * a.Q.s + g * a.Q.h) + 16u * c;
-      dma::buffer16(rs, r < s.rows && c * T::CE < a.D ? off : OUT_OF_RANGE, lds0 + buf * G::STAGE + mine + u * 1024);
+      const int x = G::MINE * w4 + G::RPI * u + lane / T::CPR;
+      dma::buffer16(rs, r0 + x < s.rows ? offs[u] : OUT_OF_RANGE, lds0 + buf * G::STAGE + mine + u * 1024);
     }
     if (RW > 1 || w == 0) {
       const int left = s.rows - r0;

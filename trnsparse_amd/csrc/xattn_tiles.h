@@ -337,6 +337,7 @@ template <typename T, int NT, bool TWICE, typename M, typename F>
 __device__ inline void weigh_stage(RowState<T>& r, f32x16* s, uint32_t vst, const typename T::Lane& ln, int h,
                                    float scale_log2, bool check, int keys, M&& masked, F&& ready) {
   if (check) {
+    asm volatile("");  // a branch, not selections that every stage would go through
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
