@@ -14,11 +14,12 @@
 //           four wavefronts share in an LDS ring of two
 //   narrow  up to 32 rows to a workgroup: every wavefront has all of them and
 //           takes every fourth stage of 32 keys through LDS of its own
-// The host does not see the lengths. It gives every unit `items` workgroups;
-// each finds the unit's tiles of rows from its number of new tokens, and where
-// workgroups are left, they take ranges of the keys (share_of). Ranges write
-// their own normalised result and log-sum-exp in fp32, which combine_kernel
-// joins in the ranges' order.
+// The host does not see the lengths. It launches `items` workgroups for every
+// unit; they find from the lengths how many tiles of rows each unit has and, where
+// these are few, ranges of the keys (share_of), and the work is dealt to the
+// first workgroups of the launch, the longest first (work_of); the others end.
+// Ranges write their own normalised result and log-sum-exp in fp32, which
+// combine_kernel joins in the ranges' order.
 //
 // The accumulated weights need the final log-sum-exp of every row. Up to 16 rows:
 // the narrow kernel keeps its scores (4 bytes a pair, where reading K again is 2
@@ -49,7 +50,8 @@ struct Args {
   Table t;
   Lengths len;
   int B, Hkv, G, Sq, R, D;   // R: rows of a unit, G Sq
-  int items;                 // workgroups of a unit
+  int items;                 // workgroups of a unit at most
+  int deal;                  // work goes to the launch's first workgroups, longest first (up to 64 sequences)
   int slots;                 // results of ranges that a unit has room for (0: keys stay whole)
   int least, step;           // a range's least keys, and what it is a multiple of
   int slot_rows;             // rows of one such result
@@ -63,25 +65,30 @@ struct Args {
   int64_t wb, wh;
 };
 
+constexpr int TILE = 128;  // rows of a wide workgroup (a narrow one has all of its unit's)
 struct Share {
   int n, m, rows, tiles, splits, chunk;
 };
-// What a unit's workgroups do. Uniform: scalar loads and arithmetic.
-__device__ inline Share share_of(const Args& a, int64_t b, int tile_rows) {
+// What the workgroups of a unit of n cached and m new rows do.
+__device__ inline Share share_of(const Args& a, int n, int m) {
   Share s;
-  s.n = (int)cached_rows(a.len, b);
-  s.m = (int)new_rows(a.len, b);
-  s.rows = s.m * a.G;
-  s.tiles = (s.rows + tile_rows - 1) / tile_rows;
-  int k = s.tiles ? a.slots / s.tiles : 0;
-  const int most = (s.n + a.least - 1) / a.least;
+  s.n = n;
+  s.m = m;
+  s.rows = m * a.G;
+  s.tiles = (s.rows + TILE - 1) / TILE;
+  s.splits = 1;
+  s.chunk = n > 0 ? n : 1;
+  int k = s.tiles && a.slots ? a.slots / s.tiles : 0;
+  const int most = (n + a.least - 1) / a.least;
   k = k < most ? k : most;
-  k = k < 1 ? 1 : k;
-  const int per = (s.n + k - 1) / k;
-  s.chunk = (per + a.step - 1) / a.step * a.step;
-  s.chunk = s.chunk < a.step ? a.step : s.chunk;
-  s.splits = s.n > 0 ? (s.n + s.chunk - 1) / s.chunk : 1;
+  if (k > 1) {
+    s.chunk = ((n + k - 1) / k + a.step - 1) / a.step * a.step;
+    s.splits = (n + s.chunk - 1) / s.chunk;
+  }
   return s;
+}
+__device__ inline Share share_of(const Args& a, int64_t b) {
+  return share_of(a, (int)cached_rows(a.len, b), (int)new_rows(a.len, b));
 }
 // Keys that a row's token sees.
 __device__ inline int sees_of(const Share& s, int i) { return s.n - (s.m - 1 - i); }
@@ -97,26 +104,73 @@ __device__ inline bool unit_of(const Args& a, uint32_t block, int per_unit, uint
   return true;
 }
 
-// The sequence whose work is the k-th largest (of up to 64; a lane has one's), so
-// that a long one does not start last and run alone.
-__device__ inline uint32_t longest_first(const Args& a, uint32_t k) {
-  if (a.B < 2 || a.B > 64) return k;
+// The lengths of the lane's sequence, of up to 64 (none: zero).
+struct Lane64 {
+  int n, m;
+};
+__device__ inline Lane64 lane_lengths(const Args& a) {
   const int lane = threadIdx.x & 63;
-  const bool on = lane < a.B;
-  float work = -1.f;
-  if (on) {
+  Lane64 l{0, 0};
+  if (lane < a.B) {
     const auto at = [&](const void* p) {
       return a.len.wide ? ((const int64_t*)p)[lane] : (int64_t)((const int32_t*)p)[lane];
     };
-    const float n = (float)clamped(at(a.len.p), a.len.slots);
-    work = n * (a.len.fresh ? (float)clamped(at(a.len.fresh), a.len.most) : 1.f);
+    l.n = (int)clamped(at(a.len.p), a.len.slots);
+    l.m = (int)(a.len.fresh ? clamped(at(a.len.fresh), a.len.most) : a.len.most);
   }
+  return l;
+}
+// What a workgroup does: item `item` of the `wgs` that its unit has.
+struct Work {
+  uint32_t unit, b, hk;
+  int item, wgs;
+  Share s;
+};
+__device__ inline bool work_of(const Args& a, uint32_t block, Work& w) {
+  if (!a.deal) {
+    if (!unit_of(a, block, a.items, w.unit, w.b, w.hk, w.item)) return false;
+    w.wgs = a.items;
+    w.s = share_of(a, (int64_t)w.b);
+    return true;
+  }
+  // A lane has one sequence: its workgroups for one key head, and how long the
+  // first of them takes. The longest go first.
+  const int lane = threadIdx.x & 63;
+  const Lane64 l = lane_lengths(a);
+  const Share v = share_of(a, l.n, l.m);
+  const int rest = (a.R - v.rows + 255) / 256;  // (rows to clear)
+  int wgs = v.tiles * v.splits;
+  wgs = lane < a.B ? (wgs > rest ? wgs : rest) : 0;
+  const int keys = v.chunk < l.n ? v.chunk : l.n, time = v.rows > 32 ? 4 * keys : keys;
+  int total = 0, start = 0;
+  for (int j = 0; j < a.B; ++j) {
+    const int wj = __builtin_amdgcn_readlane(wgs, j), tj = __builtin_amdgcn_readlane(time, j);
+    total += wj;
+    start += tj > time || (tj == time && j < lane) ? wj : 0;
+  }
+  int64_t hk, at;
+  if (!head_item(block, total, a.Hkv, hk, at)) return false;
+  const int p = (int)at;
+  w.b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__builtin_amdgcn_ballot_w64(start <= p && p < start + wgs)));
+  w.hk = (uint32_t)hk;
+  w.unit = w.b * (uint32_t)a.Hkv + w.hk;
+  w.item = p - __builtin_amdgcn_readlane(start, w.b);
+  w.wgs = __builtin_amdgcn_readlane(wgs, w.b);
+  w.s = share_of(a, __builtin_amdgcn_readlane(l.n, w.b), __builtin_amdgcn_readlane(l.m, w.b));
+  return true;
+}
+// The sequence whose cache is the k-th longest (of up to 64, weighed with its new rows).
+__device__ inline uint32_t longest_first(const Args& a, uint32_t k) {
+  if (a.B < 2 || a.B > 64) return k;
+  const int lane = threadIdx.x & 63;
+  const Lane64 l = lane_lengths(a);
+  const float work = lane < a.B ? (float)l.n * (float)l.m : -1.f;
   uint32_t rank = 0;
   for (int j = 0; j < a.B; ++j) {
     const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), j));
     rank += other > work || (other == work && j < lane);
   }
-  return __builtin_amdgcn_readfirstlane(__builtin_ctzll(__builtin_amdgcn_ballot_w64(on && rank == k)));
+  return __builtin_amdgcn_readfirstlane(__builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < a.B && rank == k)));
 }
 
 __device__ inline const char* q_row(const Args& a, int64_t b, int64_t hk, int i, int g) {
@@ -127,12 +181,21 @@ __device__ inline char* o_row(const Args& a, int64_t b, int64_t hk, int i, int g
 }
 
 // Rows behind a sequence's new tokens are zero; the unit's workgroups share them.
-__device__ inline void clear_rest(const Args& a, const Share& s, int64_t b, int64_t hk, int item, int esz) {
+__device__ inline void clear_rest(const Args& a, const Work& w, int esz) {
   const int c = 16 * (threadIdx.x & 31);
-  for (int r = s.rows + item * 8 + (threadIdx.x >> 5); r < a.R; r += 8 * a.items) {
+  for (int r = w.s.rows + w.item * 8 + (int)(threadIdx.x >> 5); r < a.R; r += 8 * w.wgs) {
     const int i = r / a.G, g = r - i * a.G;
-    if (c < a.D * esz) *(u32x4*)(o_row(a, b, hk, i, g) + c) = u32x4{};
+    if (c < a.D * esz) *(u32x4*)(o_row(a, w.b, w.hk, i, g) + c) = u32x4{};
   }
+}
+
+// A buffer whose place and size are the same for the whole wavefront, in scalar registers.
+__device__ inline dma::i32x4 buffer_at(const char* base, uint32_t bytes) {
+  dma::i32x4 r = dma::make_rsrc(base, bytes);
+  r.x = __builtin_amdgcn_readfirstlane(r.x);
+  r.y = __builtin_amdgcn_readfirstlane(r.y);
+  r.z = __builtin_amdgcn_readfirstlane(r.z);
+  return r;
 }
 
 // A wavefront's rows of a stage: `ROWS` consecutive cached rows of one page.
@@ -152,7 +215,7 @@ struct Loader {
   // The rows at `base` of which `rows` exist (none: all zero) into LDS dst.
   __device__ inline void issue(const char* base, int rows, int64_t row_bytes, int D, uint32_t dst) const {
     const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * row_bytes) + (uint32_t)(D * T::ESZ) : 0;
-    const dma::i32x4 rs = dma::make_rsrc(base, bytes);
+    const dma::i32x4 rs = buffer_at(base, bytes);
 #pragma unroll
     for (int i = 0; i < NI; ++i) dma::buffer16(rs, off[i], dst + i * 1024);
   }
@@ -171,6 +234,11 @@ __device__ inline Spot spot_of(const Table& t, int64_t trow, int key, int end) {
     s.row = key - (int)col * t.page_size;
   }
   return s;
+}
+// Keeps the look-up before the wait that follows.
+__device__ inline void settle(Spot& s) {
+  s.page = __builtin_amdgcn_readfirstlane(s.page);
+  asm volatile("" : "+s"(s.page));
 }
 // Rows [key, end) of the piece or part of one that starts at the spot.
 template <typename L>
@@ -200,20 +268,22 @@ struct Wide {
   static constexpr int LDS = 2 * STAGE, MINE = HK / 4;
   typedef Loader<T, MINE> Ld;
 
-  static __device__ inline void run(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int item,
-                                    uint8_t* lds) {
-    const int split = item / (s.tiles ? s.tiles : 1);
-    if (s.tiles == 0 || split >= s.splits) return;
-    const int slot = item, tile = s.tiles - 1 - (item - split * s.tiles);  // the tiles that see most first
+  static __device__ inline void run(const Args& a, const Work& wk, uint8_t* lds) {
+    const Share& s = wk.s;
+    const int64_t b = wk.b, hk = wk.hk;
+    if (s.tiles == 0) return;
+    const int split = wk.item / s.tiles;
+    if (split >= s.splits) return;
+    const int tile = s.tiles - 1 - (wk.item - split * s.tiles);  // the tiles that see most first
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-    const int r0 = tile * 128 + w * 32, r = r0 + (lane & 31);
+    const int r0 = tile * TILE + w * 32, r = r0 + (lane & 31);
     const bool live = r < s.rows, some = r0 < s.rows;
     const int i = live ? r / a.G : 0, g = live ? r - i * a.G : 0;
     typename T::Rows q;
     T::load(q, q_row(a, b, hk, i, g), live, a.D, h);
 
     const int c0 = split * s.chunk;
-    const int tile_last = tile * 128 + 127 < s.rows ? tile * 128 + 127 : s.rows - 1;
+    const int tile_last = tile * TILE + TILE - 1 < s.rows ? tile * TILE + TILE - 1 : s.rows - 1;
     const int last = sees_of(s, tile_last / a.G);                   // keys that any row of the tile sees
     const int k1 = c0 + s.chunk < last ? c0 + s.chunk : last;
     const int sees = live ? sees_of(s, i) : 0;
@@ -238,12 +308,12 @@ struct Wide {
     if (nst > 0) issue(0, spot_of(a.t, trow, key(0), k1));
     for (int st = 0; st < nst; ++st) {
       Spot sp = spot_of(a.t, trow, key(st + 1), k1);
-      asm volatile("" : "+s"(sp.page));
+      settle(sp);
       dma::wait_vm<0>();
       dma::barrier();
       if (st + 1 < nst) issue(st + 1, sp);
-      const int at = c0 + st * HK;
       if (!some) continue;
+      const int at = c0 + st * HK;
       const uint32_t stage = lds0 + (st & 1) * STAGE;
       const int lim = least < k1 ? least : k1;
       xat::softmax_stage<T, NT, false>(x, q, stage, stage + HBYTES, ln, h, a.scale_log2, at + HK > lim,
@@ -252,7 +322,7 @@ struct Wide {
     const float l = xat::halves_sum(x.l), inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (!live) return;
     const bool whole = s.splits == 1;
-    const int64_t at = ((int64_t)unit * a.slots + slot) * a.slot_rows + (r - tile * 128);
+    const int64_t at = ((int64_t)wk.unit * a.slots + wk.item) * a.slot_rows + (r - tile * TILE);
     const Final<T> out{o_row(a, b, hk, i, g), whole ? nullptr : a.part + at * a.D};
     T::quads(x.acc, h, [&](int d, f32x4 v) {
       if (d < a.D) out.put(d, v * inv);
@@ -262,7 +332,7 @@ struct Wide {
       if (!whole)
         a.plse[at] = e;
       else if (a.lse)
-        a.lse[(int64_t)unit * a.R + r] = e;
+        a.lse[(int64_t)wk.unit * a.R + r] = e;
     }
   }
 };
@@ -279,9 +349,10 @@ struct Narrow {
   static __device__ inline void drained() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
   template <bool SCORES>
-  static __device__ inline void run(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int item,
-                                    uint8_t* lds) {
-    const int split = item;
+  static __device__ inline void run(const Args& a, const Work& wk, uint8_t* lds) {
+    const Share& s = wk.s;
+    const uint32_t unit = wk.unit, b = wk.b, hk = wk.hk;
+    const int split = wk.item;
     if (s.rows == 0 || split >= s.splits) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int l32 = lane & 31;
@@ -330,7 +401,8 @@ struct Narrow {
       const bool more = st + 1 < mine;
       const int at = key(st);
       Two next = look(st + 1);
-      asm volatile("" : "+s"(next.p[0].page), "+s"(next.p[1].page));
+      settle(next.p[0]);
+      settle(next.p[1]);
       dma::wait_vm<NI>();  // K is there once only V's loads are out
       fence();
       f32x16 c[1];
@@ -419,12 +491,10 @@ template <typename T, bool SCORES>
 __global__ __launch_bounds__(256, narrow_per_cu<T>) void narrow_kernel(const Args a) {
   typedef Narrow<T> N;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[N::LDS];
-  uint32_t unit, b, hk;
-  int item;
-  if (!unit_of(a, blockIdx.x, a.items, unit, b, hk, item)) return;
-  const Share s = share_of(a, b, 32);
-  clear_rest(a, s, b, hk, item, T::ESZ);
-  N::template run<SCORES>(a, s, unit, b, hk, item, lds);
+  Work w;
+  if (!work_of(a, blockIdx.x, w)) return;
+  clear_rest(a, w, T::ESZ);
+  N::template run<SCORES>(a, w, lds);
 }
 // Units of any number of rows, each narrow or wide by its own (wide where the
 // narrow kernel's LDS would leave one workgroup to a CU: fp32 rows of 128).
@@ -435,31 +505,26 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const Args a) {
   typedef Wide<T> W;
   typedef Narrow<T> N;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[chunk_has_narrow<T> && N::LDS > W::LDS ? N::LDS : W::LDS];
-  uint32_t unit, b, hk;
-  int item;
-  if (!unit_of(a, blockIdx.x, a.items, unit, b, hk, item)) return;
-  b = longest_first(a, b);
-  unit = b * (uint32_t)a.Hkv + hk;
-  const Share s = share_of(a, b, 128);
-  clear_rest(a, s, b, hk, item, T::ESZ);
-  if (SCORES && s.rows <= a.sr)
-    N::template run<true>(a, s, unit, b, hk, item, lds);
-  else if (chunk_has_narrow<T> && s.rows <= 32)
-    N::template run<false>(a, s, unit, b, hk, item, lds);
+  Work w;
+  if (!work_of(a, blockIdx.x, w)) return;
+  clear_rest(a, w, T::ESZ);
+  if (SCORES && w.s.rows <= a.sr)
+    N::template run<true>(a, w, lds);
+  else if (chunk_has_narrow<T> && w.s.rows <= 32)
+    N::template run<false>(a, w, lds);
   else
-    W::run(a, s, unit, b, hk, item, lds);
+    W::run(a, w, lds);
 }
 
 // ---------------------------------------------------------------- joining
 // One row: the ranges' results with weights 2^(lse_j - max lse); 32 lanes to a
 // row, four values each. Returns the row's log-sum-exp.
 template <typename T>
-__device__ inline float combine_row(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int tile_rows,
-                                    int r) {
+__device__ inline float combine_row(const Args& a, const Share& s, uint32_t unit, uint32_t b, uint32_t hk, int r) {
   const int lane = threadIdx.x & 31, d = 4 * lane;
-  const int tile = r / tile_rows;
+  const int tile = r / TILE;
   const int64_t stride = (int64_t)s.tiles * a.slot_rows;  // of a row between ranges
-  const int64_t at = ((int64_t)unit * a.slots + (s.tiles - 1 - tile)) * a.slot_rows + (r - tile * tile_rows);
+  const int64_t at = ((int64_t)unit * a.slots + (s.tiles - 1 - tile)) * a.slot_rows + (r - tile * TILE);
   float m = -INFINITY, total = 0.f;
   f32x4 sum = f32x4{};
   for (int j0 = 0; j0 < s.splits; j0 += 32) {
@@ -496,13 +561,13 @@ __device__ inline float combine_row(const Args& a, const Share& s, uint32_t unit
 
 // `per` workgroups to a unit, 8 rows of each at a time.
 template <typename T>
-__global__ __launch_bounds__(256) void combine_kernel(const Args a, int per, int tile_rows) {
+__global__ __launch_bounds__(256) void combine_kernel(const Args a, int per) {
   const uint32_t unit = blockIdx.x / (uint32_t)per, part = blockIdx.x - unit * (uint32_t)per;
   const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
-  const Share s = share_of(a, b, tile_rows);
+  const Share s = share_of(a, (int64_t)b);
   if (s.splits == 1) return;
   for (int r = (int)part * 8 + (int)(threadIdx.x >> 5); r < s.rows; r += 8 * per) {
-    const float lse = combine_row<T>(a, s, unit, b, hk, tile_rows, r);
+    const float lse = combine_row<T>(a, s, unit, b, hk, r);
     if (a.lse && (threadIdx.x & 31) == 0) a.lse[(int64_t)unit * a.R + r] = lse;
   }
 }
@@ -528,10 +593,10 @@ __global__ __launch_bounds__(256) void weigh_kernel(const Args a, int cw, int kw
   const uint32_t per = (uint32_t)(cw + kw), unit = blockIdx.x / per;
   const int part = (int)(blockIdx.x - unit * per);
   const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
-  const Share s = share_of(a, b, 32);
+  const Share s = share_of(a, (int64_t)b);
   if (part < cw) {
     const int r = part * 8 + (int)(threadIdx.x >> 5);
-    if (s.splits > 1 && r < s.rows) combine_row<T>(a, s, unit, b, hk, 32, r);
+    if (s.splits > 1 && r < s.rows) combine_row<T>(a, s, unit, b, hk, r);
     return;
   }
   if (s.splits > 1) {
@@ -580,7 +645,7 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
   if (!unit_of(a, blockIdx.x, per, unit, b, hk, item)) return;
   b = longest_first(a, b);
   unit = b * (uint32_t)a.Hkv + hk;
-  const Share s = share_of(a, b, 128);
+  const Share s = share_of(a, (int64_t)b);  // (its lengths)
   const int j0 = item * G::KEYS;
   if (j0 >= s.n || s.rows == 0) return;
   float* W = a.W + b * a.wb + hk * a.wh;
@@ -629,7 +694,7 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
   for (int u = 0; u < G::NI; ++u) offs[u] = offset(u, 0);
   auto issue = [&](int st, int buf) {
     const int r0 = st * G::HR, i0 = r0 / a.G;
-    const dma::i32x4 rs = dma::make_rsrc(Qh + i0 * a.Q.s, OUT_OF_RANGE);
+    const dma::i32x4 rs = buffer_at(Qh + i0 * a.Q.s, OUT_OF_RANGE);
     if (!even) {
 #pragma unroll
       for (int u = 0; u < G::NI; ++u) offs[u] = offset(u, r0 - i0 * a.G);
@@ -641,7 +706,7 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
     }
     if (RW > 1 || w == 0) {
       const int left = s.rows - r0;
-      const dma::i32x4 ls = dma::make_rsrc(L + r0, 4u * (uint32_t)(left < G::HR ? left : G::HR));
+      const dma::i32x4 ls = buffer_at((const char*)(L + r0), 4u * (uint32_t)(left < G::HR ? left : G::HR));
       dma::buffer4(ls, 4u * (uint32_t)lane, lse0 + buf * 256);
     }
   };
@@ -718,13 +783,13 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   const int64_t G = Hq / Hkv, R = G * Sq, units = B * Hkv;
   const bool f32 = dtype == TSP_F32;
   p.narrow = R <= 32;
-  const int64_t tiles = p.narrow ? 1 : ceil_div(R, 128), wgs = units * tiles;
+  const int64_t tiles = p.narrow ? 1 : ceil_div(R, TILE), wgs = units * tiles;
   // Ranges of keys: as many as bring the rounds of workgroups that fit the CUs
   // at once, each of its keys and of as much as `least` keys more (starting,
   // joining), to the shortest time.
   p.least = p.narrow ? (f32 ? 128 : 512) : (f32 ? 64 : 256);
   p.step = p.narrow ? 128 : 64;
-  p.slot_rows = (int)(p.narrow ? R : 128);
+  p.slot_rows = (int)(p.narrow ? R : TILE);
   const int64_t room = p.narrow && f32 && D > 64 ? 256 : 512, most = ceil_div(keys > 0 ? keys : 1, p.least);
   int64_t n = 1, best = INT64_MAX;
   for (int64_t k = 1; k <= 32 && k <= most; ++k) {
@@ -735,8 +800,8 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   p.slots = n > 1 ? p.items : 0;
   if (ragged && !p.narrow && n == 1) {
     // sequences of few new tokens leave workgroups over, which take ranges
-    const int64_t room = ceil_div(1024, units);
-    p.slots = (int)(p.items < room ? p.items : room);
+    const int64_t more = ceil_div(1024, units);
+    p.slots = (int)(p.items < more ? p.items : more);
     if (p.slots < 2) p.slots = 0;
   }
   auto pad = [](int64_t v) { return ceil_div(v, 64) * 64; };
@@ -814,13 +879,15 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   }
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   const int64_t grid = head_grid(p.items, units);
+  // (where all workgroups start at once, dealing costs 1 us and gives nothing: 24
+  // sequences of five tokens 34.7 and 36.7 us; 64 of one token 287 and 279)
+  a.deal = B <= 64 && (new_lengths || units * p.items > 512);
   // (9 units of 1008 keys and up to 399 rows in fp32: 28 us with 128 keys to a workgroup)
   const bool few = units * ceil_div(keys, 128) < 512;
   const int64_t wper = ceil_div(keys, few ? 32 : 128);
   const bool again = weigh && !(p.narrow && p.sr > 0);  // some scores are formed again
   const int64_t wgrid = again ? head_grid(wper, units) : 0;
-  const int tile_rows = p.narrow ? 32 : 128;
-  const int64_t joined = p.narrow ? a.R : (int64_t)(p.slots / 2) * 128 < a.R ? (int64_t)(p.slots / 2) * 128 : a.R;
+  const int64_t joined = p.narrow || (int64_t)(p.slots / 2) * paged::TILE > a.R ? a.R : (int64_t)(p.slots / 2) * paged::TILE;
   int64_t cper = p.slots > 1 ? ceil_div(joined, 8) : 0;
   if (!p.narrow && new_lengths && cper > ceil_div(2048, units)) cper = ceil_div(2048, units);  // (most have few rows)
   // 1024 keys and more to a workgroup, as many as fill the CUs
@@ -848,7 +915,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
       return check_launch("weights launch");
     }
     if (cper > 0) {
-      hipLaunchKernelGGL((paged::combine_kernel<T>), dim3((unsigned)(units * cper)), t, 0, st, a, (int)cper, tile_rows);
+      hipLaunchKernelGGL((paged::combine_kernel<T>), dim3((unsigned)(units * cper)), t, 0, st, a, (int)cper);
       if ((rc = check_launch("combine launch"))) return rc;
     }
     if (again) {
