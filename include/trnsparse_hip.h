@@ -722,7 +722,7 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  *   all numbers. The kept rows of K, V and weights move to rows [0, budget) in
  *   their order; what stands behind is left as it was. lengths_out, not lengths
  *   itself, receives min(lengths[b], budget). K_pages and V_pages must not
- *   overlap.
+ *   overlap. workspace: tsp_paged_evict_workspace_size bytes, 16-byte aligned.
  * ==================================================================== */
 int64_t tsp_paged_attn_workspace_size(int dtype, int64_t batch, int64_t heads,
                                       int64_t kv_heads, int64_t queries,
@@ -749,8 +749,9 @@ int tsp_paged_append(const void* K, const int64_t* k_strides, const void* V,
                      const void* lengths, const void* new_lengths, int index_type,
                      void* lengths_out, float* weights,
                      const int64_t* weight_strides, void* stream);
-int64_t tsp_paged_evict_workspace_size(int64_t batch, int64_t kv_heads,
-                                       int64_t budget);
+int64_t tsp_paged_evict_workspace_size(int dtype, int64_t batch,
+                                       int64_t kv_heads, int64_t slots,
+                                       int64_t head_dim, int64_t budget);
 int tsp_paged_evict(void* K_pages, const int64_t* k_pages_strides, void* V_pages,
                     const int64_t* v_pages_strides, int dtype, int64_t batch,
                     int64_t kv_heads, int64_t pages, int64_t page_size,

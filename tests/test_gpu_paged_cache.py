@@ -114,16 +114,27 @@ def test_evict_to_nothing_and_bad_pages(hip_backend):
     assert ts.paged_cache_evict(kp, vp, w[..., :0], table[:, :0], lengths, 7).tolist() == [0, 0, 0]
 
 
-@pytest.mark.parametrize("dt,size", [(BF, (2, 4, 300, 128, 128, 9000, 700)), (F32, (1, 2, 2200, 16, 64, 30000, 0)),
-                                     (HF, (20, 8, 40, 32, 96, 501, 60))])
-def test_evict_long(hip_backend, dt, size):
-    """Many parts of a row list, against the "pytorch" backend."""
+@pytest.mark.parametrize("dt,size", [
+    (BF, (2, 4, 300, 128, 128, 9000, 700)), (F32, (1, 2, 2200, 16, 64, 30000, 0)), (HF, (20, 8, 40, 32, 96, 501, 60)),
+    (BF, (3, 1, 130, 256, 8, 300, 300)), (F32, (4, 2, 1100, 16, 40, 17000, 5)), (BF, (1, 1, 1300, 64, 128, 80000, 100)),
+    (HF, (40, 8, 12, 64, 64, 300, 17)), (BF, (130, 1, 300, 64, 16, 9000, 100)),
+])
+@pytest.mark.parametrize("kind", ["random", "ties", "special"])
+def test_evict_long(hip_backend, dt, size, kind):
+    """Many parts of a row list and of the weights, against the "pytorch" backend."""
     B, Hk, cols, ps, D, budget, recent = size
     _, kp, vp, table = make(B, Hk, Hk, 1, cols, ps, D, dt)
     L = cols * ps
-    w = torch.randn(B, Hk, L, device="cuda").exp()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randn(B, Hk, L, device="cuda", generator=g).exp()
     w[:, :, ::3] = 0.0
-    lengths = torch.randint(budget - 50, L + 1, (B,), device="cuda")
+    if kind == "ties":
+        w = (w * 2).round()
+    if kind == "special":
+        table[0, 2], table[-1, cols // 2] = -1, len(kp)
+        w[0, 0], w[-1, -1, ::2] = float("nan"), float("-inf")
+        w[:, :, 1::7], w[:, :, 5::11] = float("inf"), -1.0
+    lengths = torch.randint(budget - 50, L + 1, (B,), device="cuda", generator=g)
     lengths[0] = L
     k, v, x = kp.clone(), vp.clone(), w.clone()
     ts.set_backend("pytorch")

@@ -235,7 +235,9 @@ def test_c_abi_refusals():
     assert evict(w=None) == -1 and evict(recent=9) == -1 and evict(recent=-1) == -1 and evict(out=d) == -1
     assert evict(vp=d) == -1 and evict(ws=None) == -1 and evict(wsb=16) == -1
     assert lib.tsp_paged_attn_workspace_size(7, 1, 2, 2, 1, 64, 64, 0, 0) == -1
-    assert lib.tsp_paged_evict_workspace_size(1, 0, 5) == -1 and lib.tsp_paged_evict_workspace_size(2, 3, 5) >= 4 * 30
+    size = lambda *v: lib.tsp_paged_evict_workspace_size(_lib.TSP_BF16, *v)  # noqa: E731
+    assert size(1, 0, 64, 64, 5) == -1 and size(2, 3, 64, 64, -1) == -1 and size(2, 3, 64, 64, 5) >= 8 * 30
+    assert size(1, 2, 1 << 17, 64, 1 << 15) >= 2 * 2 * 2 * 64 * (1 << 15)  # rows copied aside
 
 
 SCHEMAS = {

@@ -842,7 +842,7 @@ at::Tensor paged_evict(const at::Tensor& Kp, const at::Tensor& Vp, const at::Ten
   need_weights(weights, p, Kp, who, ws2);
   TORCH_CHECK(0 <= recent && recent <= budget, who, ": recent ", recent, " is not in 0 .. budget ", budget);
   auto out = at::empty_like(lengths);
-  const int64_t wsb = tsp_paged_evict_workspace_size(p.B, p.Hk, std::min(budget, p.slots));
+  const int64_t wsb = tsp_paged_evict_workspace_size(p.code, p.B, p.Hk, p.slots, p.D, budget);
   const Workspace ws(wsb, Kp, who);
   check(tsp_paged_evict(Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs, p.code, p.B, p.Hk, p.pages, p.page_size, p.D,
                         table.data_ptr(), p.tcode, p.tstride, p.cols, p.lens, p.icode, weights.data_ptr<float>(), ws2,

@@ -112,7 +112,7 @@ SIGNATURES: dict[str, tuple] = {
                                   _I64, _P, _P, _INT, _DBL, _P, _P, _P, _P, _P, _I64, _P]),
     "tsp_paged_append": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _INT, _I64,
                                 _I64, _P, _P, _INT, _P, _P, _P, _P]),
-    "tsp_paged_evict_workspace_size": (_I64, [_I64, _I64, _I64]),
+    "tsp_paged_evict_workspace_size": (_I64, [_INT, _I64, _I64, _I64, _I64, _I64]),
     "tsp_paged_evict": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _INT, _I64, _I64, _P, _INT, _P, _P,
                                _I64, _I64, _P, _P, _I64, _P]),
     "tsp_qk_norm_rope_fwd": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _INT, _P, _INT, _I64,
