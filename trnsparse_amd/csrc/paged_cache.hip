@@ -56,9 +56,9 @@ int check_weights(const char* who, const void* w, const int64_t* s) {
 
 namespace {
 
-// ---------------------------------------------------------------- append
-// One thread to a 16-byte piece of a new row: K's, V's, then the zeros of the
-// weights and the lengths. Bound by the rows' bytes, or by the launch.
+// A workgroup to `tokens` new tokens of one sequence, all heads, a thread to a piece
+// of 16 bytes of K's row and V's, AU of them at a time. Bound by the rows' bytes, or by
+// the launch (TODO). Workgroups behind a sequence's new tokens end at once.
 struct AppendArgs {
   const char *K, *V;
   int64_t kb, kh, ks, vb, vh, vs;  // strides in bytes
@@ -68,38 +68,53 @@ struct AppendArgs {
   void* out;  // lengths after
   float* W;
   int64_t wb, wh;
-  int64_t B;
-  uint32_t Hkv, N, chunks;  // chunks: 16-byte pieces of a row
+  uint32_t Hkv, chunks, pieces;  // pieces of a row, and of a token's rows
+  uint32_t tokens, per;          // of a workgroup, workgroups of a sequence
 };
-__global__ __launch_bounds__(256) void append_kernel(const AppendArgs a, int64_t total) {
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (x < a.B) {
-    const int64_t n = cached_rows(a.len, x) + new_rows(a.len, x), v = n < a.len.slots ? n : a.len.slots;
+constexpr int AU = 4;
+__global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
+  const uint32_t b = blockIdx.x / a.per, part = blockIdx.x - b * a.per;
+  const int64_t n = cached_rows(a.len, b), m = new_rows(a.len, b);
+  if (part == 0 && threadIdx.x == 0) {
+    const int64_t v = n + m < a.len.slots ? n + m : a.len.slots;
     if (a.len.wide)
-      ((int64_t*)a.out)[x] = v;
+      ((int64_t*)a.out)[b] = v;
     else
-      ((int32_t*)a.out)[x] = (int32_t)v;
+      ((int32_t*)a.out)[b] = (int32_t)v;
   }
-  if (x >= total) return;
-  // (batch, token, head, piece), the order of a projection's output
-  const int64_t row = x / a.chunks, tok = row / a.Hkv;
-  const uint32_t c = (uint32_t)(x - row * a.chunks), h = (uint32_t)(row - tok * a.Hkv);
-  const int64_t b = tok / a.N, i = tok - b * a.N;
-  const int64_t m = a.len.fresh ? clamped(a.len.wide ? ((const int64_t*)a.len.fresh)[b]
-                                                     : (int64_t)((const int32_t*)a.len.fresh)[b], a.len.most)
-                                : a.len.most;
-  if (i >= m) return;
-  const int64_t n = clamped(a.len.wide ? ((const int64_t*)a.len.p)[b] : (int64_t)((const int32_t*)a.len.p)[b], a.len.slots);
-  const int64_t j = n + i;
-  if (j >= a.len.slots) return;
-  if (a.W && c == 0) a.W[b * a.wb + h * a.wh + j] = 0.f;
-  const uint32_t col = (uint32_t)j / (uint32_t)a.t.page_size, r = (uint32_t)j - col * (uint32_t)a.t.page_size;
-  const uint32_t page = page_of_lane(a.t, b * a.t.ld, col);
-  if (page == NO_PAGE) return;
-  const u32x4 k = *(const u32x4*)(a.K + b * a.kb + h * a.kh + i * a.ks + 16 * c);
-  const u32x4 v = *(const u32x4*)(a.V + b * a.vb + h * a.vh + i * a.vs + 16 * c);
-  *(u32x4*)(a.Kp.p + page * a.Kp.page + h * a.Kp.h + r * a.Kp.s + 16 * c) = k;
-  *(u32x4*)(a.Vp.p + page * a.Vp.page + h * a.Vp.h + r * a.Vp.s + 16 * c) = v;
+  const int64_t i0 = (int64_t)part * a.tokens, room = a.len.slots - n, last = m < room ? m : room;
+  const int64_t left = last - i0;
+  if (left <= 0) return;
+  // (both below 2^32: a workgroup has 2^11 pieces, or one token)
+  const uint32_t total = (uint32_t)(left < a.tokens ? left : a.tokens) * a.pieces;
+  const char* K = a.K + b * a.kb;
+  const char* V = a.V + b * a.vb;
+  for (uint32_t p0 = threadIdx.x; p0 < total; p0 += 256 * AU) {
+    u32x4 k[AU], v[AU];
+    uint32_t head[AU], c[AU], row[AU];
+    u32x2 entry[AU];
+#pragma unroll
+    for (int u = 0; u < AU; ++u) {
+      const uint32_t p = p0 + 256 * u < total ? p0 + 256 * u : total - 1;  // (the last piece, once more)
+      const uint32_t tok = p / a.pieces, rest = p - tok * a.pieces;
+      head[u] = rest / a.chunks;
+      c[u] = 16 * (rest - head[u] * a.chunks);
+      const int64_t i = i0 + tok;
+      row[u] = (uint32_t)(n + i);
+      entry[u] = entry_of_lane(a.t, b * a.t.ld, column_of(a.t, row[u] / PIECE));
+      k[u] = *(const u32x4*)(K + head[u] * a.kh + i * a.ks + c[u]);
+      v[u] = *(const u32x4*)(V + head[u] * a.vh + i * a.vs + c[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AU; ++u) {
+      if (a.W && c[u] == 0) a.W[b * a.wb + head[u] * a.wh + row[u]] = 0.f;
+      const uint32_t page = page_of_entry(a.t, entry[u]);
+      if (page == NO_PAGE) continue;
+      const uint32_t r = row[u] - column_of(a.t, row[u] / PIECE) * (uint32_t)a.t.page_size;
+      *(u32x4*)(a.Kp.p + page * a.Kp.page + head[u] * a.Kp.h + r * a.Kp.s + c[u]) = k[u];
+      *(u32x4*)(a.Vp.p + page * a.Vp.page + head[u] * a.Vp.h + r * a.Vp.s + c[u]) = v[u];
+    }
+  }
 }
 
 }  // namespace
@@ -144,10 +159,11 @@ extern "C" int tsp_paged_append(const void* K, const int64_t* ks, const void* V,
   a.out = lengths_out;
   a.W = weights;
   if (weights) a.wb = ws[0], a.wh = ws[1];
-  a.B = B, a.Hkv = (uint32_t)Hkv, a.N = (uint32_t)(N > 0 ? N : 1), a.chunks = (uint32_t)(D * e / 16);
-  const int64_t total = cols > 0 ? B * N * Hkv * a.chunks : 0;
-  const int64_t grid = ceil_div(total > B ? total : B, 256);
-  if (grid > INT32_MAX) return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
-  hipLaunchKernelGGL(paged::append_kernel, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a, total);
+  a.Hkv = (uint32_t)Hkv, a.chunks = (uint32_t)(D * e / 16), a.pieces = a.Hkv * a.chunks;
+  if (Hkv > (int64_t(1) << 26)) return fail(TSP_EUNSUPPORTED, "%s: too many heads", who);
+  a.tokens = a.pieces < 2048 ? 2048 / a.pieces : 1;
+  a.per = (uint32_t)(N > 0 ? ceil_div(N, a.tokens) : 1);
+  if (B * a.per > INT32_MAX) return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
+  hipLaunchKernelGGL(paged::append_kernel, dim3((unsigned)(B * a.per)), dim3(256), 0, (hipStream_t)stream, a);
   return check_launch("append launch");
 }

@@ -937,9 +937,13 @@ def hip_block_sparse_attention_backward(Q, K, V, O, dO, mask_bsr, scale: float, 
 def _together(first, *rest):
     """The operands on one GPU: as they are when they share first's, else
     copied to the first GPU among them (None stays)."""
-    dev = first.device
-    if dev.type == "cuda" and all(t is None or t.device == dev for t in rest):
-        return (first, *rest)
+    at = first.get_device()  # (-1: the host)
+    if at >= 0:
+        for t in rest:
+            if t is not None and t.get_device() != at:
+                break
+        else:
+            return (first, *rest)
     dev = _target_device(first, *rest)
     return tuple(None if t is None else t.to(dev) for t in (first, *rest))
 
@@ -967,8 +971,7 @@ def hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale: flo
 
 def _one_dtype(lengths, new_lengths):
     """Contiguous lengths, and new ones of the same dtype (None stays)."""
-    if not lengths.is_contiguous():
-        lengths = lengths.contiguous()
+    lengths = lengths.contiguous()
     if new_lengths is not None and (new_lengths.dtype != lengths.dtype or not new_lengths.is_contiguous()):
         if new_lengths.dtype not in (torch.int32, torch.int64):
             raise RuntimeError(f"new_lengths must be int32 or int64, got {new_lengths.dtype}")
