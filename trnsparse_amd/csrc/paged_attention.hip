@@ -65,6 +65,7 @@ struct Args {
   int64_t wb, wh;
 };
 
+constexpr int MOST_RANGES = 64;  // of a unit's keys where the host chooses them
 constexpr int TILE = 128;  // rows of a wide workgroup (a narrow one has all of its unit's)
 struct Share {
   int n, m, rows, tiles, splits, chunk;
@@ -577,9 +578,12 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a, int per) {
 __device__ inline float weight_of(const Args& a, const Share& s, uint32_t unit, const float* lse, int k) {
   const float* p = a.scores + ((int64_t)unit * a.stages + k / 32) * a.sr * 32 + k % 32;
   float sum = 0.f;
-  for (int r = 0; r < s.rows; ++r) {
-    const float c = p[r * 32];
-    sum += c == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(c - lse[r]);
+  for (int r = 0; r < s.rows; r += 4) {
+    float c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[u] = r + u < s.rows ? p[(r + u) * 32] : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum += c[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(c[u] - lse[r + u]);
   }
   return sum;
 }
@@ -589,7 +593,7 @@ __device__ inline float weight_of(const Args& a, const Share& s, uint32_t unit, 
 // at a time, from the scores and the rows' log-sum-exps.
 template <typename T>
 __global__ __launch_bounds__(256) void weigh_kernel(const Args a, int cw, int kw) {
-  __shared__ float lse[32];
+  __shared__ float lse[36];  // (read four at a time)
   const uint32_t per = (uint32_t)(cw + kw), unit = blockIdx.x / per;
   const int part = (int)(blockIdx.x - unit * per);
   const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
@@ -600,17 +604,19 @@ __global__ __launch_bounds__(256) void weigh_kernel(const Args a, int cw, int kw
     return;
   }
   if (s.splits > 1) {
-    // 8 threads to a row; ranges in order
+    // 8 threads to a row, each with up to 8 of its ranges
     const int r = threadIdx.x >> 3, l8 = threadIdx.x & 7;
-    float m = -INFINITY, total = 0.f;
+    float e[MOST_RANGES / 8], m = -INFINITY, total = 0.f;
     if (r < s.rows) {
       const int64_t at = (int64_t)unit * a.slots * a.slot_rows + r;
-      for (int j = l8; j < s.splits; j += 8) m = fmaxf(m, a.plse[at + (int64_t)j * a.slot_rows]);
+#pragma unroll
+      for (int j = 0; j < MOST_RANGES / 8; ++j)
+        e[j] = l8 + 8 * j < s.splits ? a.plse[at + (int64_t)(l8 + 8 * j) * a.slot_rows] : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < MOST_RANGES / 8; ++j) m = fmaxf(m, e[j]);
       for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-      for (int j = l8; j < s.splits; j += 8) {
-        const float e = a.plse[at + (int64_t)j * a.slot_rows];
-        total += e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e - m);
-      }
+#pragma unroll
+      for (int j = 0; j < MOST_RANGES / 8; ++j) total += e[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[j] - m);
       for (int o = 4; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
       if (l8 == 0) lse[r] = m + __builtin_amdgcn_logf(total);
     }
@@ -792,7 +798,7 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   p.slot_rows = (int)(p.narrow ? R : TILE);
   const int64_t room = p.narrow && f32 && D > 64 ? 256 : 512, most = ceil_div(keys > 0 ? keys : 1, p.least);
   int64_t n = 1, best = INT64_MAX;
-  for (int64_t k = 1; k <= 32 && k <= most; ++k) {
+  for (int64_t k = 1; k <= MOST_RANGES && k <= most; ++k) {
     const int64_t cost = ceil_div(wgs * k, room) * (ceil_div(keys, k) + p.least);
     if (cost < best) best = cost, n = k;
   }
