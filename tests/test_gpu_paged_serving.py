@@ -1,0 +1,239 @@
+"""The operators of a paged cache together, as a server uses them: prompts in by
+chunks, tokens one at a time, sequences that come and go, eviction; captured and
+replayed, from several streams and threads, traced."""
+
+from __future__ import annotations
+
+import threading
+
+import pytest
+import torch
+
+import trnsparse_amd as ts
+from oracle import layer
+from test_gpu_graphs import _capture
+from test_gpu_paged_attention import BF, F32, HF, check, make
+from trnsparse_amd.hip import _lib
+
+pytestmark = pytest.mark.gpu
+
+H, Hk, D, SIZE = 8, 2, 64, 16
+
+
+def rand(g, *shape, dt=F32):
+    return torch.randn(*shape, device="cuda", generator=g).to(dt)
+
+
+def test_chunks_and_tokens_equal_the_whole(hip_backend):
+    """A prompt taken in by chunks, then tokens one at a time, all rotated by their
+    positions, equals attention over the whole sequence in float64."""
+    B, cols = 3, 12
+    g = torch.Generator(device="cuda").manual_seed(1)
+    total = torch.tensor([150, 77, 31], device="cuda")
+    T = int(total.max())
+    q, k, v = rand(g, B, H, T, D), rand(g, B, Hk, T, D), rand(g, B, Hk, T, D)
+    w, freq = 1 + 0.1 * rand(g, D), ts.rope_frequencies(D, device="cuda")
+    q, k = ts.qk_norm_rope(q, k, w, w, torch.arange(T, device="cuda"), freq)
+    _, kp, vp, table = make(B, H, Hk, 1, cols, SIZE, D, F32)
+    out, lengths = torch.zeros_like(q), torch.zeros(B, dtype=torch.int32, device="cuda")
+    at = 0
+    for n in (64, 33, 20, 1, 1, 17, 1, 13):
+        new = (total - at).clamp(0, n).int()
+        lengths = ts.paged_cache_append(k[:, :, at : at + n], v[:, :, at : at + n], kp, vp, table, lengths, new)
+        out[:, :, at : at + n] = ts.paged_attention(q[:, :, at : at + n], kp, vp, table, lengths, new)
+        at += n
+    assert at == T and torch.equal(lengths, total.int())
+    want = layer.attention(q, k, v, D**-0.5, layer.chunk_seen(total, total, T, T))["O"]
+    assert (out.double().cpu() - want).norm() <= 1e-5 * want.norm()  # (of 150 keys: test_gpu_paged_attention's bound is 4e-5)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_decoding_with_eviction(hip_backend, dt):
+    """Sequences decode with a budget of rows; at each step results and weights are the
+    oracle's over what the cache then holds."""
+    B, cols, budget, recent = 3, 5, 48, 16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    _, kp, vp, table = make(B, H, Hk, 1, cols, SIZE, D, dt)
+    lengths, w = torch.tensor([3, 40, 0], device="cuda"), torch.zeros(B, Hk, cols * SIZE, device="cuda")
+    for step in range(30):
+        n = 5 if step % 7 == 0 else 1
+        k, v = rand(g, B, Hk, n, D, dt=dt), rand(g, B, Hk, n, D, dt=dt)
+        lengths = ts.paged_cache_append(k, v, kp, vp, table, lengths, weights=w)
+        for b, m in enumerate(lengths.tolist()):
+            assert (w[b, :, m - n : m] == 0).all()
+            rows = layer.paged_rows(kp, table)[b, :, m - n : m]
+            assert torch.equal(rows, k[b].cpu())
+        Q = rand(g, B, n, H, D, dt=dt).transpose(1, 2)
+        check(Q, kp, vp, table, lengths)
+        ts.paged_attention(Q, kp, vp, table, lengths, weights=w)
+        want = layer.paged_evict(kp, vp, w, table, lengths, budget, recent)
+        lengths = ts.paged_cache_evict(kp, vp, w, table, lengths, budget, recent)
+        torch.cuda.synchronize()
+        for got, x in zip((kp, vp, w, lengths), want):
+            assert torch.equal(got.cpu(), x)
+        assert int(lengths.max()) <= budget
+    assert (lengths == torch.tensor([48, 48, 48], device="cuda")).sum() >= 1
+
+
+def _step(s, budget):
+    """One decoding step on static buffers: append, attend, evict, lengths in place."""
+    n = ts.paged_cache_append(s["k"], s["v"], s["kp"], s["vp"], s["table"], s["lengths"], s["new"], s["w"])
+    O = ts.paged_attention(s["q"], s["kp"], s["vp"], s["table"], n, s["new"], weights=s["w"])
+    s["lengths"].copy_(ts.paged_cache_evict(s["kp"], s["vp"], s["w"], s["table"], n, budget, budget // 4))
+    return O
+
+
+def _state(seed, dt, N, cols=40, B=4):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    _, kp, vp, table = make(B, H, Hk, 1, cols, SIZE, D, dt, seed=seed)
+    return {"q": rand(g, B, H, N, D, dt=dt), "k": rand(g, B, Hk, N, D, dt=dt), "v": rand(g, B, Hk, N, D, dt=dt), "kp": kp,
+            "vp": vp, "table": table, "lengths": torch.tensor([0, 9, 300, 510], device="cuda")[:B].clone(),
+            "new": torch.tensor([N, 1, N, max(N - 1, 1)], device="cuda")[:B].clone(),
+            "w": torch.zeros(B, Hk, cols * SIZE, device="cuda")}
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("N", [1, 6, 60])
+def test_graph_of_a_step(hip_backend, dt, N):
+    """A captured step replayed as the sequences grow and are cut: lengths, tables and
+    caches are read at every replay; eager work and synchronizations in between."""
+    budget = 400
+    s, e = _state(3, dt, N), _state(3, dt, N)
+    graph, (out,) = _capture(lambda: _step(s, budget))
+    for name, t in _state(3, dt, N).items():
+        s[name].copy_(t)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for turn in range(5):
+        for name in ("q", "k", "v"):
+            x = rand(g, *s[name].shape, dt=dt)
+            s[name].copy_(x), e[name].copy_(x)
+        if turn == 2:  # a sequence ends, another takes its pages
+            for t in (s, e):
+                t["lengths"][3] = 2
+                t["table"][3] = t["table"][3].flip(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _step(e, budget)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for name in ("kp", "vp", "w", "lengths"):
+            assert torch.equal(s[name], e[name]), name
+
+
+def test_graph_of_a_long_eviction(hip_backend):
+    """The eviction by parts and segments, captured and replayed on other weights."""
+    B, cols, budget = 2, 1300, 9000
+    _, kp, vp, table = make(B, Hk, Hk, 1, cols, SIZE, 16, BF, seed=5)
+    w, lengths = torch.zeros(B, Hk, cols * SIZE, device="cuda"), torch.tensor([cols * SIZE, 15000], device="cuda")
+    graph, (after,) = _capture(lambda: ts.paged_cache_evict(kp, vp, w, table, lengths, budget, 70))
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for _ in range(4):
+        x = rand(g, *w.shape).exp()
+        w.copy_(x)
+        k, v, y = kp.clone(), vp.clone(), x.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        n = ts.paged_cache_evict(k, v, y, table, lengths, budget, 70)
+        torch.cuda.synchronize()
+        assert torch.equal(kp, k) and torch.equal(vp, v) and torch.equal(w, y) and torch.equal(after, n)
+
+
+def test_two_graphs_and_streams(hip_backend):
+    """Two captured steps replayed at the same time: each has workspaces of its own."""
+    states = [_state(7 + i, BF, 3) for i in range(2)]
+    eager = [_state(7 + i, BF, 3) for i in range(2)]
+    graphs = [_capture(lambda s=s: _step(s, 200)) for s in states]
+    for i, s in enumerate(states):
+        for name, t in _state(7 + i, BF, 3).items():
+            s[name].copy_(t)
+    streams = [torch.cuda.Stream() for _ in states]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for (graph, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        want = [_step(e, 200) for e in eager]
+        torch.cuda.synchronize()
+        for (_, (out,)), w, s, e in zip(graphs, want, states, eager):
+            assert torch.equal(out, w) and torch.equal(s["w"], e["w"]) and torch.equal(s["kp"], e["kp"])
+
+
+def test_two_threads_two_streams(hip_backend):
+    states, eager = [_state(11 + i, BF, 1) for i in range(2)], [_state(11 + i, BF, 1) for i in range(2)]
+    want = [[_step(e, 300) for _ in range(15)] for e in eager]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [_step(states[i], 300) for _ in range(15)]
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(outs, want[i])):
+                bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    assert all(torch.equal(s[n], e[n]) for s, e in zip(states, eager) for n in ("kp", "vp", "w", "lengths"))
+
+
+def test_operands_on_the_host(hip_backend):
+    """Tables and lengths from the host, and a whole cache there: written ones come back."""
+    dev = _state(13, F32, 2, cols=6)
+    dev["lengths"] %= 90
+    host = {n: t.cpu() for n, t in dev.items()}
+    want = _step(dev, 60)
+    got = _step(host, 60)
+    torch.cuda.synchronize()
+    assert got.device.type == "cpu" and torch.equal(got, want.cpu())
+    for n in ("kp", "vp", "w", "lengths"):
+        assert torch.equal(host[n], dev[n].cpu()), n
+    O = ts.paged_attention(dev["q"], dev["kp"], dev["vp"], host["table"], host["lengths"], host["new"].int())
+    assert torch.equal(O, ts.paged_attention(dev["q"], dev["kp"], dev["vp"], dev["table"], dev["lengths"], dev["new"]))
+
+
+def test_no_gradients_and_versions(hip_backend):
+    """What is written counts as written; gradients and tangents are refused."""
+    import torch.autograd.forward_ad as fw
+
+    s = _state(14, F32, 2)
+    before = [s[n]._version for n in ("kp", "vp", "w")]
+    _step(s, 100)
+    assert all(s[n]._version > b for n, b in zip(("kp", "vp", "w"), before))
+    ops = _lib.ops()
+    q = s["q"].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.paged_attn_fwd(q, s["kp"], s["vp"], s["table"], s["lengths"], None, 0.1, None)
+    with torch.no_grad():
+        ops.paged_attn_fwd(q, s["kp"], s["vp"], s["table"], s["lengths"], None, 0.1, None)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+        ts.paged_attention(fw.make_dual(s["q"], s["q"]), s["kp"], s["vp"], s["table"], s["lengths"])
+    with pytest.raises(RuntimeError, match="not supported"):  # (a type that the pytorch backend takes)
+        ts.paged_attention(s["q"].double(), s["kp"].double(), s["vp"].double(), s["table"], s["lengths"])
+
+
+def test_traced_and_compiled(hip_backend):
+    """torch.compile reaches the operators whole, writes in place included, and the public
+    functions by graph breaks; results equal eager calls."""
+    ops = _lib.ops()
+
+    def whole(s):
+        n = ops.paged_append(s["k"], s["v"], s["kp"], s["vp"], s["table"], s["lengths"], None, s["w"])
+        O = ops.paged_attn_fwd(s["q"] * 2.0, s["kp"], s["vp"], s["table"], n, None, 0.125, s["w"]) + 1.0
+        return O, ops.paged_evict(s["kp"], s["vp"], s["w"], s["table"], n, 50, 10) + 1
+
+    def public(s):
+        n = ts.paged_cache_append(s["k"], s["v"], s["kp"], s["vp"], s["table"], s["lengths"], None, s["w"])
+        O = ts.paged_attention(s["q"] * 2.0, s["kp"], s["vp"], s["table"], n, None, 0.125, s["w"]) + 1.0
+        return O, ts.paged_cache_evict(s["kp"], s["vp"], s["w"], s["table"], n, 50, 10) + 1
+
+    for f, full in ((whole, True), (public, False)):
+        a, b = _state(15, F32, 2), _state(15, F32, 2)
+        want = f(a)
+        got = torch.compile(f, fullgraph=full, backend="aot_eager")(b)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert all(torch.equal(a[n], b[n]) for n in ("kp", "vp", "w"))
