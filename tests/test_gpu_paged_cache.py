@@ -156,3 +156,11 @@ def test_evict_again_and_again(hip_backend):
         K = torch.full((2, 2, 1, 64), float(i), dtype=BF, device="cuda")
         lengths = ts.paged_cache_append(K, K, kp, vp, table, n, weights=w)
         w[:, :, 40] = torch.rand(2, 2, device="cuda")
+
+
+@pytest.mark.parametrize("kind", ["random", "ties", "special"])
+@pytest.mark.parametrize("size", [(20, 4, 3200, 16, 8, 300, 20), (1, 2, 220, 256, 64, 20000, 3000), (3, 1, 800, 64, 40, 51000, 0),
+                                  (1, 1, 1000, 128, 16, 8192, 8192)])
+def test_evict_by_parts(hip_backend, size, kind):
+    """Weights searched part by part, rows moved in one list or in segments."""
+    test_evict_long(hip_backend, BF, size, kind)

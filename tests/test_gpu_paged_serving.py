@@ -138,6 +138,23 @@ def test_graph_of_a_long_eviction(hip_backend):
         assert torch.equal(kp, k) and torch.equal(vp, v) and torch.equal(w, y) and torch.equal(after, n)
 
 
+def test_graph_of_an_eviction_by_parts(hip_backend):
+    B, cols, budget = 1, 3300, 9000
+    _, kp, vp, table = make(B, Hk, Hk, 1, cols, SIZE, 16, BF, seed=5)
+    w, lengths = torch.zeros(B, Hk, cols * SIZE, device="cuda"), torch.tensor([cols * SIZE - 7], device="cuda")
+    graph, (after,) = _capture(lambda: ts.paged_cache_evict(kp, vp, w, table, lengths, budget, 70))
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for _ in range(4):
+        x = rand(g, *w.shape).exp().round()
+        w.copy_(x)
+        k, v, y = kp.clone(), vp.clone(), x.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        n = ts.paged_cache_evict(k, v, y, table, lengths, budget, 70)
+        torch.cuda.synchronize()
+        assert torch.equal(kp, k) and torch.equal(vp, v) and torch.equal(w, y) and torch.equal(after, n)
+
+
 def test_two_graphs_and_streams(hip_backend):
     """Two captured steps replayed at the same time: each has workspaces of its own."""
     states = [_state(7 + i, BF, 3) for i in range(2)]

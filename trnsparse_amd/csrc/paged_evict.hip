@@ -45,7 +45,7 @@ struct EvictArgs {
   struct Find* state;  // [3][unit]: the search after the first, the second and the third digit
   uint32_t* hist;  // [3][unit][part][BINS]
   int32_t* count;  // [unit][part][2]: rows above the last key, rows equal to it
-  float* kept;     // [unit][budget]: weights
+  float* kept;     // [unit][budget]: weights; null where they are in place
   char* saved;     // [unit][K, V][budget]: rows
 };
 constexpr uint32_t SAVED = 0x80000000u;  // with the row's number: the row is taken from `saved`
@@ -58,14 +58,16 @@ __device__ inline uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// sum over the lanes before this one, and the total of the wavefront
-__device__ inline int wave_scan(int v, int lane, int& total) {
+// Sum over the lanes before this one, and the total of the wavefront: within rows of
+// 16 lanes by shifts, then the rows' totals to those behind them.
+__device__ inline int wave_scan(int v, int& total) {
   int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row to the next row, rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
   total = __builtin_amdgcn_readlane(x, 63);
   return x - v;
 }
@@ -103,8 +105,9 @@ struct Find {
   }
 };
 struct Scratch {
-  int sums[2][2][ST / 64];
+  int sums[2][ST / 64];
   uint32_t pick[3];
+  int first;
 };
 __device__ inline void add_digits(uint32_t* hist, const Find& f, const Part& p, int j, int end) {
 #pragma unroll
@@ -117,11 +120,11 @@ __device__ inline void add_digits(uint32_t* hist, const Find& f, const Part& p, 
 // below: the one in which the count from the largest passes `want`.
 __device__ inline void next_digit(Find& f, int c0, int c1, Scratch& x) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, d = BINS - 1 - 2 * tid;
-  int total, before = wave_scan(c0 + c1, lane, total);
-  if (lane == 0) x.sums[0][0][wave] = total;
+  int total, before = wave_scan(c0 + c1, total);
+  if (lane == 0) x.sums[0][wave] = total;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ST / 64; ++i) before += i < wave ? x.sums[0][0][i] : 0;
+  for (int i = 0; i < ST / 64; ++i) before += i < wave ? x.sums[0][i] : 0;
   if (before < f.want && f.want <= before + c0 + c1) {
     const bool second = f.want > before + c0;
     x.pick[0] = (uint32_t)(second ? d - 1 : d);
@@ -180,20 +183,23 @@ __device__ inline void sort_out(const Unit& u, const Find& f, const Part& p, int
     if (j + i < u.E && f.equal > 0 && k == f.last) same |= 1u << i;
   }
 }
+// Page and row of row j (a thread's rows of a part lie in one page).
+__device__ inline u32x2 spot_of_row(const EvictArgs& a, const Unit& u, int j) {
+  const uint32_t col = column_of(a.t, (uint32_t)j / PIECE), row = (uint32_t)j - col * (uint32_t)a.t.page_size;
+  return u32x2{j < u.n ? page_of_lane(a.t, u.b * a.t.ld, col) : NO_PAGE, row};
+}
 // Lists the part's kept rows behind the `base` kept ones before it, of the rows that
 // equal the last key as far as they go (`equal_base` came before); counts on. Their
-// weights go to `to`, which may be the weights themselves.
-__device__ inline void list_part(const EvictArgs& a, const Unit& u, const Find& f, Part& p, int j, float* to, int& base,
-                                 int& equal_base, int& first, int turn, Scratch& x) {
+// weights go to `to`, which may be the weights themselves. `spot`: of row j. Returns
+// the first of the thread's rows that goes, n for none: the rows behind it move.
+__device__ inline int list_part(const EvictArgs& a, const Unit& u, const Find& f, Part& p, int j, u32x2 spot, float* to,
+                                int& base, int& equal_base, int turn, Scratch& x) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // (a thread's rows lie in one page)
-  const uint32_t col = column_of(a.t, (uint32_t)j / PIECE), row = (uint32_t)j - col * (uint32_t)a.t.page_size;
-  const uint32_t page = j < u.n ? page_of_lane(a.t, u.b * a.t.ld, col) : NO_PAGE;
   uint32_t above, same;
   sort_out(u, f, p, j, above, same);
   // both counts in one scan: at most PART of each
-  int total, before = wave_scan(__builtin_popcount(same) << 16 | __builtin_popcount(above), lane, total);
-  if (lane == 0) x.sums[turn][0][wave] = total;
+  int total, before = wave_scan(__builtin_popcount(same) << 16 | __builtin_popcount(above), total);
+  if (lane == 0) x.sums[turn][wave] = total;
   // every row of this part is read before one is written
 #pragma unroll
   for (int i = 0; i < SPT; ++i) asm volatile("" : "+v"(p.v[i]));
@@ -201,29 +207,30 @@ __device__ inline void list_part(const EvictArgs& a, const Unit& u, const Find& 
   int all = 0;
 #pragma unroll
   for (int i = 0; i < ST / 64; ++i) {
-    const int c = x.sums[turn][0][i];
+    const int c = x.sums[turn][i];
     before += i < wave ? c : 0;
     all += c;
   }
   int e = equal_base + (before >> 16);  // equal ones before this thread's
   const int e0 = equal_base < f.equal ? equal_base : f.equal;
-  int d = base + (before & 0xffff) + (e < f.equal ? e : f.equal) - e0;
+  int d = base + (before & 0xffff) + (e < f.equal ? e : f.equal) - e0, goes = u.n;
   u32x2* list = a.list + u.unit * a.budget;
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     bool stays = above >> i & 1;
     if (same >> i & 1) stays = e++ < f.equal;
+    const int q = j + i;
+    if (!stays && q < goes) goes = q;
     // (weights that another stream writes meanwhile could make more rows stay than there are places)
     if (!stays || d >= a.budget) continue;
-    const int q = j + i;
-    const uint32_t aside = q < a.budget && (q >> a.segment) != (d >> a.segment) && page != NO_PAGE ? SAVED : 0;
-    list[d] = u32x2{page, (row + i) | aside};
-    if (d != q) first = d < first ? d : first;
+    const uint32_t aside = q < a.budget && (q >> a.segment) != (d >> a.segment) && spot.x != NO_PAGE ? SAVED : 0;
+    list[d] = u32x2{spot.x, (spot.y + i) | aside};
     if (d != q || to != u.w) to[d] = p.v[i];
     ++d;
   }
   equal_base += all >> 16;
   base += (all & 0xffff) + (equal_base < f.equal ? equal_base : f.equal) - e0;
+  return goes;
 }
 
 __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
@@ -242,6 +249,7 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
   const bool once = n <= PART;
   Part held;
   held.load(u.w, tid * SPT, n, u.aligned);
+  const u32x2 held_spot = spot_of_row(a, u, tid * SPT);
   auto each = [&](int end, auto&& f) {
     Part even = held, odd;
     if (!once) odd.load(u.w, PART + tid * SPT, n, u.aligned);
@@ -256,6 +264,7 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
   Find f;
   f.start(u.keep);
   for (int i = tid; i < BINS; i += ST) hist[i] = 0;
+  if (tid == 0) x.first = n;
   __syncthreads();
   while (!f.done) {
     each(u.E, [&](int j, const Part& p) { add_digits(hist, f, p, j, u.E); });
@@ -265,22 +274,24 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
     next_digit(f, c0, c1, x);
   }
   __syncthreads();
-  int base = 0, equal_base = 0, first = a.budget, turn = 0;
+  int base = 0, equal_base = 0, first = n, turn = 0;
   each(n, [&](int j, Part p) {
-    list_part(a, u, f, p, j, u.w, base, equal_base, first, turn, x);
+    const int goes = list_part(a, u, f, p, j, j < PART ? held_spot : spot_of_row(a, u, j), u.w, base, equal_base, turn, x);
+    first = goes < first ? goes : first;
     turn ^= 1;
   });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const int g = __shfl_xor(first, o, 64);
-    first = g < first ? g : first;
+  // (the lowest lane with one has the wavefront's first)
+  const uint64_t some = __builtin_amdgcn_ballot_w64(first < n);
+  if (some) {
+    const int low = __builtin_amdgcn_readlane(first, __builtin_ctzll(some));
+    if (once) {
+      if (lane == 0) atomicMin(&x.first, low);
+    } else if (first < n) {  // (of several parts, any lane may)
+      atomicMin(&x.first, first);
+    }
   }
-  if (lane == 0) x.sums[turn][1][wave] = first;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < ST / 64; ++i) first = x.sums[turn][1][i] < first ? x.sums[turn][1][i] : first;
-    a.first[u.unit] = first;
-  }
+  if (tid == 0) a.first[u.unit] = x.first < a.budget ? x.first : a.budget;
 }
 
 // ------------------------------------------------- few units of many rows
@@ -331,12 +342,12 @@ __global__ __launch_bounds__(ST) void digit_kernel(const EvictArgs a, int turn) 
   uint32_t above, same;
   sort_out(u, f, p, j, above, same);
   int total;
-  wave_scan(__builtin_popcount(same) << 16 | __builtin_popcount(above), lane, total);
-  if (lane == 0) x.sums[1][0][wave] = total;
+  wave_scan(__builtin_popcount(same) << 16 | __builtin_popcount(above), total);
+  if (lane == 0) x.sums[1][wave] = total;
   __syncthreads();
   if (tid == 0) {
     int all = 0;
-    for (int i = 0; i < ST / 64; ++i) all += x.sums[1][0][i];
+    for (int i = 0; i < ST / 64; ++i) all += x.sums[1][i];
     int32_t* to = a.count + 2 * (u.unit * a.parts + part);
     to[0] = all & 0xffff;
     to[1] = all >> 16;
@@ -363,8 +374,8 @@ __global__ __launch_bounds__(ST) void list_kernel(const EvictArgs a) {
     above += __shfl_xor(above, o, 64);
     equal_base += __shfl_xor(equal_base, o, 64);
   }
-  int base = above + (equal_base < f.equal ? equal_base : f.equal), first = 0;
-  list_part(a, u, f, p, j, a.kept + u.unit * a.budget, base, equal_base, first, 0, x);
+  int base = above + (equal_base < f.equal ? equal_base : f.equal);
+  list_part(a, u, f, p, j, spot_of_row(a, u, j), a.kept + u.unit * a.budget, base, equal_base, 0, x);
 }
 
 // Copies aside the rows that come from another segment's places, and puts the kept
@@ -383,7 +394,7 @@ __global__ __launch_bounds__(256) void save_kernel(const EvictArgs a, uint32_t p
   for (int i = 0; i < SU; ++i) {
     const int d = d0 + i * step;
     e[i] = d < a.budget ? a.list[unit * a.budget + d] : u32x2{NO_PAGE, 0};
-    if (!(x & 1) && c == 0 && d < a.budget) a.W[b * a.wb + h * a.wh + d] = a.kept[unit * a.budget + d];
+    if (a.kept && !(x & 1) && c == 0 && d < a.budget) a.W[b * a.wb + h * a.wh + d] = a.kept[unit * a.budget + d];
   }
   const Pages& p = x & 1 ? a.Vp : a.Kp;
 #pragma unroll
@@ -407,7 +418,7 @@ struct Move {
   u32x2 to[MU];    // the table's entry
   u32x4 v[MU];
 };
-template <int LPR>
+template <int LPR, bool SEGMENTS>
 __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t slices, uint32_t segments) {
   // the slices of a row in consecutive slots of one XCD
   const uint32_t xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, slice = at8 % slices, y = at8 / slices * 8 + xcd;
@@ -450,7 +461,10 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
   auto load = [&](Move& m, int d0) {
 #pragma unroll
     for (int u = 0; u < MU; ++u) {
-      // (in an unsaved list no row's number has the mark)
+      if constexpr (!SEGMENTS) {
+        m.v[u] = *spot(m.from[u].x, m.from[u].y);
+        continue;
+      }
       const uint64_t aside = 0 - (uint64_t)(m.from[u].y >> 31);
       const uint64_t there = (uint64_t)spot(m.from[u].x, m.from[u].y & ~SAVED);
       const uint64_t kept = (uint64_t)(a.saved + (x * a.budget + place(d0, u)) * row_bytes + c);
@@ -485,16 +499,21 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
   }
 }
 
-// Whether a unit's weights are searched by a workgroup to each part, and its rows
-// moved by segments: units of more than two parts that leave CUs without one. (8
-// units of 131072 rows cut to 32768, head_dim 128 in 16 bits: one workgroup to each
-// selects in 110 us and 64 move in 150; by parts 45, 24 to copy rows aside, 57.)
-bool by_parts(int64_t units, int64_t slots) { return units < 128 && slots > 2 * PART; }
-int segment_of(int64_t units, int64_t budget, int64_t slices) {
-  // for 512 workgroups, none of less than 1024 places
-  int64_t want = ceil_div(512, units * 2 * slices);
+// Whether a unit's weights are searched by a workgroup to each part of them: five
+// launches, which takes less time than one workgroup's turns from 7 parts on, while
+// the units leave CUs without one (8 units of 131072 rows: 45 us for 110; 64 of 32768:
+// the eviction 298 us, with one workgroup to each unit 268).
+bool by_parts(int64_t units, int64_t slots) { return units < 128 && slots > 6 * PART; }
+// log2 of the places of a segment, 31 where all are one. Segments for 512 workgroups,
+// none of less than 1024 places, where the chains of parts are too few to take the
+// memory's rate (64 with slices of 64 bytes) and long: copying rows aside is traffic
+// of its own. (8 units, head_dim 128 in 16 bits: 32768 places of 131072 rows 150 us,
+// in segments 57 and 24 to copy; 8192 of 16384: 47.6 us and 45.6 the whole eviction.
+// 32 units, 8192 of 16384: 69 us, 104 in segments.)
+int segment_of(int64_t units, int64_t budget, int64_t row) {
+  if (units * 2 * ceil_div(row, 64) > 64 || budget <= 8192) return 31;
   int s = 10;
-  while (s < 31 && (int64_t(1) << s) * want < budget) ++s;
+  while (s < 31 && (int64_t(1) << s) * ceil_div(512, units * 2 * ceil_div(row, 128)) < budget) ++s;
   return s;
 }
 struct Space {  // of the workspace, in bytes from its start
@@ -505,15 +524,13 @@ Space space_of(int64_t units, int64_t slots, int64_t budget, int64_t row) {
   Space s{};
   s.first = 16;
   s.list = s.first + up(4 * units);
-  s.state = s.hist = s.count = s.kept = s.saved = s.end = s.list + up(8 * units * budget);
-  if (by_parts(units, slots)) {
-    const int64_t parts = ceil_div(slots, PART);
-    s.hist = s.state + up(3 * units * (int64_t)sizeof(Find));
-    s.count = s.hist + 3 * units * parts * BINS * 4;
-    s.kept = s.count + up(8 * units * parts);
-    s.saved = s.kept + up(4 * units * budget);
-    s.end = s.saved + units * 2 * budget * row;
-  }
+  s.state = s.list + up(8 * units * budget);
+  const int64_t parts = by_parts(units, slots) ? ceil_div(slots, PART) : 0;
+  s.hist = s.state + (parts ? up(3 * units * (int64_t)sizeof(Find)) : 0);
+  s.count = s.hist + 3 * units * parts * BINS * 4;
+  s.kept = s.count + up(8 * units * parts);
+  s.saved = s.kept + (parts ? up(4 * units * budget) : 0);
+  s.end = s.saved + (segment_of(units, budget, row) < 31 ? units * 2 * budget * row : 0);
   return s;
 }
 
@@ -568,16 +585,14 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   a.spare = (char*)workspace;
   a.first = (int32_t*)(a.spare + sp.first);
   a.list = (u32x2*)(a.spare + sp.list);
-  a.segment = 31;
-  uint32_t segments = 1;
+  a.segment = paged::segment_of(units, budget, row);
+  const uint32_t segments = a.segment < 31 ? (uint32_t)ceil_div(budget, int64_t(1) << a.segment) : 1;
   // slices of 128 bytes, a line of the cache; of 64 where they leave CUs without one
-  const bool parts = paged::by_parts(units, slots), thin = !parts && units * 2 * ceil_div(row, 128) < 256;
+  const bool parts = paged::by_parts(units, slots), thin = segments == 1 && units * 2 * ceil_div(row, 128) < 256;
   const int64_t slices = ceil_div(row, thin ? 64 : 128), lanes = row > 256 ? 5 : row > 128 ? 4 : 3,
                 per = ceil_div(budget, (256 >> lanes) * paged::SU);
   if (parts) {
     a.parts = (int)ceil_div(slots, paged::PART);
-    a.segment = paged::segment_of(units, budget, slices);
-    segments = (uint32_t)ceil_div(budget, int64_t(1) << a.segment);
     a.state = (paged::Find*)(a.spare + sp.state);
     a.hist = (uint32_t*)(a.spare + sp.hist);
     a.count = (int32_t*)(a.spare + sp.count);
@@ -585,22 +600,24 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   }
   a.saved = a.spare + sp.saved;
   const int64_t grid = ceil_div(units * 2 * segments, 8) * 8 * slices;
-  if (grid > INT32_MAX || units * a.parts > INT32_MAX || (parts && units * 2 * per > INT32_MAX))
+  if (grid > INT32_MAX || units * a.parts > INT32_MAX || units * 2 * per > INT32_MAX)
     return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
   if (parts) {
     for (int turn = 0; turn < 4; ++turn)
       hipLaunchKernelGGL(paged::digit_kernel, dim3((unsigned)(units * a.parts)), dim3(paged::ST), 0, st, a, turn);
     hipLaunchKernelGGL(paged::list_kernel, dim3((unsigned)(units * a.parts)), dim3(paged::ST), 0, st, a);
-    if (budget > 0)
-      hipLaunchKernelGGL(paged::save_kernel, dim3((unsigned)(units * 2 * per)), dim3(256), 0, st, a, (uint32_t)per, (int)lanes);
   } else {
     hipLaunchKernelGGL(paged::select_kernel, dim3((unsigned)units), dim3(paged::ST), 0, st, a);
   }
+  if (budget > 0 && (parts || segments > 1))
+    hipLaunchKernelGGL(paged::save_kernel, dim3((unsigned)(units * 2 * per)), dim3(256), 0, st, a, (uint32_t)per, (int)lanes);
   if ((rc = check_launch("select launch"))) return rc;
   if (pages == 0 || budget == 0) return TSP_OK;
-  if (thin)
-    hipLaunchKernelGGL(paged::move_kernel<4>, dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
+  if (segments > 1)
+    hipLaunchKernelGGL((paged::move_kernel<8, true>), dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
+  else if (thin)
+    hipLaunchKernelGGL((paged::move_kernel<4, false>), dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
   else
-    hipLaunchKernelGGL(paged::move_kernel<8>, dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
+    hipLaunchKernelGGL((paged::move_kernel<8, false>), dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
   return check_launch("move launch");
 }

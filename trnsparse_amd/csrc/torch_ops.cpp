@@ -706,8 +706,9 @@ at::Tensor prefix_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at
 struct PagedArgs {
   int code, tcode, icode;
   int64_t B, Hk, pages, page_size, D, cols, slots, tstride;
-  const void *lens, *fresh = nullptr;
+  const void *table, *lens, *fresh = nullptr;
   int64_t ks[3], vs[3];
+  at::Tensor held[3];  // the table and the lengths as the kernels take them, where these are copies
 
   static void page_strides(const at::Tensor& t, int64_t* s) {
     for (int i = 0; i < 3; ++i) s[i] = t.size(i) <= 1 ? (i == 2 ? t.size(3) : 0) : t.stride(i);
@@ -726,7 +727,7 @@ struct PagedArgs {
     TORCH_CHECK(ok, who, ": ", name, " needs unit stride over head_dim and other strides of whole 16-byte pieces, got ",
                 t.strides(), written ? " (and is written: its rows lie apart)" : "");
   }
-  PagedArgs(const at::Tensor& K, const at::Tensor& V, const at::Tensor& table, const at::Tensor& lengths,
+  PagedArgs(const at::Tensor& K, const at::Tensor& V, const at::Tensor& table_, const at::Tensor& lengths,
             const c10::optional<at::Tensor>& new_lengths, const at::Tensor& like, bool written, const char* who) {
     code = attn_dtype(like.scalar_type(), who);
     need_pages(K, like, who, "K_pages", written);
@@ -737,18 +738,27 @@ struct PagedArgs {
     TORCH_CHECK(Hk > 0, who, ": no key heads");
     page_strides(K, ks);
     page_strides(V, vs);
-    TORCH_CHECK(table.device() == like.device(), who, ": block_table is on ", table.device());
-    TORCH_CHECK(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), who,
-                ": block_table must be (batch, columns) with unit stride over columns");
-    tcode = index_code(table.scalar_type());
-    B = table.size(0), cols = table.size(1), slots = cols * page_size;
-    tstride = B > 1 ? table.stride(0) : cols;
-    lens = lengths_ptr(lengths, B, like, who, icode);
+    TORCH_CHECK(table_.device() == like.device(), who, ": block_table is on ", table_.device());
+    TORCH_CHECK(table_.dim() == 2, who, ": block_table must be (batch, columns)");
+    tcode = index_code(table_.scalar_type());
+    B = table_.size(0), cols = table_.size(1), slots = cols * page_size;
+    const at::Tensor* t = &table_;
+    if (cols > 1 && table_.stride(1) != 1) t = &(held[0] = table_.contiguous());
+    table = t->data_ptr();
+    tstride = B > 1 ? t->stride(0) : cols;
+    lens = lengths_of(lengths, "lengths", like, who, held[1]);
+    icode = index_code(lengths.scalar_type());
     if (new_lengths.has_value()) {
-      int c;
-      fresh = lengths_ptr(new_lengths, B, like, who, c);
-      TORCH_CHECK(c == icode, who, ": lengths and new_lengths must have one dtype");
+      index_code(new_lengths->scalar_type());
+      const bool one = new_lengths->scalar_type() == lengths.scalar_type();
+      fresh = lengths_of(one ? *new_lengths : new_lengths->to(lengths.scalar_type()), "new_lengths", like, who, held[2]);
     }
+  }
+  const void* lengths_of(const at::Tensor& l, const char* name, const at::Tensor& like, const char* who, at::Tensor& kept) const {
+    TORCH_CHECK(l.device() == like.device(), who, ": ", name, " is on ", l.device(), ", expected ", like.device());
+    TORCH_CHECK(l.dim() == 1 && l.numel() == B, who, ": ", name, " must be (batch,)");
+    kept = l.contiguous();
+    return kept.data_ptr();
   }
 };
 
@@ -789,7 +799,7 @@ at::Tensor paged_attn_fwd(const at::Tensor& Q_, const at::Tensor& K, const at::T
                                                     weights.has_value());
   const Workspace ws(wsb, Q, who);
   check(tsp_paged_attn_fwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), p.ks, V.data_ptr(), p.vs, p.code, p.B, Hq, p.Hk, Sq,
-                           p.pages, p.page_size, p.D, table.data_ptr(), p.tcode, p.tstride, p.cols, p.lens, p.fresh,
+                           p.pages, p.page_size, p.D, p.table, p.tcode, p.tstride, p.cols, p.lens, p.fresh,
                            p.icode, scale, O.data_ptr(), Strides(O).s,
                            weights.has_value() ? weights->data_ptr<float>() : nullptr, ws2, ws.ptr(), wsb, stream_of(Q)),
         "tsp_paged_attn_fwd");
@@ -816,9 +826,9 @@ at::Tensor paged_append(const at::Tensor& K_, const at::Tensor& V_, const at::Te
   int64_t ws2[2];
   if (weights.has_value()) need_weights(*weights, p, Kp, who, ws2);
   const auto K = attn_operand(K_), V = attn_operand(V_);
-  auto out = at::empty_like(lengths);
+  auto out = at::empty({p.B}, lengths.options());
   check(tsp_paged_append(K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs,
-                         p.code, p.B, p.Hk, K.size(2), p.pages, p.page_size, p.D, table.data_ptr(), p.tcode, p.tstride,
+                         p.code, p.B, p.Hk, K.size(2), p.pages, p.page_size, p.D, p.table, p.tcode, p.tstride,
                          p.cols, p.lens, p.fresh, p.icode, out.data_ptr(),
                          weights.has_value() ? weights->data_ptr<float>() : nullptr, ws2, stream_of(Kp)),
         "tsp_paged_append");
@@ -830,7 +840,7 @@ at::Tensor paged_append(const at::Tensor& K_, const at::Tensor& V_, const at::Te
 at::Tensor paged_append_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                              const at::Tensor&, const at::Tensor& lengths, const c10::optional<at::Tensor>&,
                              const c10::optional<at::Tensor>&) {
-  return at::empty_like(lengths);
+  return at::empty(lengths.sizes(), lengths.options());
 }
 
 at::Tensor paged_evict(const at::Tensor& Kp, const at::Tensor& Vp, const at::Tensor& weights, const at::Tensor& table,
@@ -841,11 +851,11 @@ at::Tensor paged_evict(const at::Tensor& Kp, const at::Tensor& Vp, const at::Ten
   int64_t ws2[2];
   need_weights(weights, p, Kp, who, ws2);
   TORCH_CHECK(0 <= recent && recent <= budget, who, ": recent ", recent, " is not in 0 .. budget ", budget);
-  auto out = at::empty_like(lengths);
+  auto out = at::empty({p.B}, lengths.options());
   const int64_t wsb = tsp_paged_evict_workspace_size(p.code, p.B, p.Hk, p.slots, p.D, budget);
   const Workspace ws(wsb, Kp, who);
   check(tsp_paged_evict(Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs, p.code, p.B, p.Hk, p.pages, p.page_size, p.D,
-                        table.data_ptr(), p.tcode, p.tstride, p.cols, p.lens, p.icode, weights.data_ptr<float>(), ws2,
+                        p.table, p.tcode, p.tstride, p.cols, p.lens, p.icode, weights.data_ptr<float>(), ws2,
                         budget, recent, out.data_ptr(), ws.ptr(), wsb, stream_of(Kp)),
         "tsp_paged_evict");
   written({&Kp, &Vp, &weights});
@@ -854,7 +864,7 @@ at::Tensor paged_evict(const at::Tensor& Kp, const at::Tensor& Vp, const at::Ten
 
 at::Tensor paged_evict_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                             const at::Tensor& lengths, int64_t, int64_t) {
-  return at::empty_like(lengths);
+  return at::empty(lengths.sizes(), lengths.options());
 }
 
 // --------------------------------- norm and rotation of query and key heads

@@ -969,34 +969,20 @@ def hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale: flo
     return out if q is Q else out.to(Q.device)
 
 
-def _one_dtype(lengths, new_lengths):
-    """Contiguous lengths, and new ones of the same dtype (None stays)."""
-    lengths = lengths.contiguous()
-    if new_lengths is not None and (new_lengths.dtype != lengths.dtype or not new_lengths.is_contiguous()):
-        if new_lengths.dtype not in (torch.int32, torch.int64):
-            raise RuntimeError(f"new_lengths must be int32 or int64, got {new_lengths.dtype}")
-        new_lengths = new_lengths.to(lengths.dtype).contiguous()
-    return lengths, new_lengths
-
-
 def _back(written, given):
     """Copies what was written on the GPU back to operands elsewhere."""
     for w, g in zip(written, given):
-        if w is not g and w is not None:
+        if w is not g:
             g.copy_(w)
-
-
-def _unit_columns(table):
-    return table if table.dim() != 2 or table.shape[1] <= 1 or table.stride(1) == 1 else table.contiguous()
 
 
 @_library_call
 def hip_paged_attention(Q, K_pages, V_pages, block_table, lengths, new_lengths, scale: float, weights):
     """paged_attention on the HIP kernels."""
     q, kp, vp, t, lens, new, w = _together(Q, K_pages, V_pages, block_table, lengths, new_lengths, weights)
-    lens, new = _one_dtype(lens, new)
-    out = _lib.ops().paged_attn_fwd(q, kp, vp, _unit_columns(t), lens, new, scale, w)
-    _back((w,), (weights,))
+    out = _lib.ops().paged_attn_fwd(q, kp, vp, t, lens, new, scale, w)
+    if w is not weights:
+        _back((w,), (weights,))
     return out if q is Q else out.to(Q.device)
 
 
@@ -1004,21 +990,22 @@ def hip_paged_attention(Q, K_pages, V_pages, block_table, lengths, new_lengths, 
 def hip_paged_cache_append(K, V, K_pages, V_pages, block_table, lengths, new_lengths, weights):
     """paged_cache_append on the HIP kernels."""
     kp, vp, k, v, t, lens, new, w = _together(K_pages, V_pages, K, V, block_table, lengths, new_lengths, weights)
-    lens, new = _one_dtype(lens, new)
-    out = _lib.ops().paged_append(k, v, kp, vp, _unit_columns(t), lens, new, w)
-    _back((kp, vp, w), (K_pages, V_pages, weights))
-    return out if kp is K_pages else out.to(lengths.device)
+    out = _lib.ops().paged_append(k, v, kp, vp, t, lens, new, w)
+    if lens is not lengths or kp is not K_pages or vp is not V_pages or w is not weights:
+        _back((kp, vp, w), (K_pages, V_pages, weights))
+        out = out.to(lengths.device)
+    return out
 
 
 @_library_call
 def hip_paged_cache_evict(K_pages, V_pages, weights, block_table, lengths, budget: int, recent: int):
     """paged_cache_evict on the HIP kernels."""
     kp, vp, w, t, lens = _together(K_pages, V_pages, weights, block_table, lengths)
-    if not lens.is_contiguous():
-        lens = lens.contiguous()
-    out = _lib.ops().paged_evict(kp, vp, w, _unit_columns(t), lens, budget, recent)
-    _back((kp, vp, w), (K_pages, V_pages, weights))
-    return out if kp is K_pages else out.to(lengths.device)
+    out = _lib.ops().paged_evict(kp, vp, w, t, lens, budget, recent)
+    if lens is not lengths or kp is not K_pages or vp is not V_pages or w is not weights:
+        _back((kp, vp, w), (K_pages, V_pages, weights))
+        out = out.to(lengths.device)
+    return out
 
 
 @_library_call
