@@ -245,3 +245,26 @@ def test_repeated_calls_are_equal(hip_backend):
         w = torch.zeros(3, 2, 1920, device="cuda")
         outs.append((ts.paged_attention(Q, kp, vp, table, lengths, new, weights=w), w))
     assert all(torch.equal(o, outs[0][0]) and torch.equal(w, outs[0][1]) for o, w in outs)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("R", [(8, 4), (8, 5), (4, 16), (3, 21), (13, 5)])  # 32, 40, 64, 63, 65 rows of a key head
+def test_rows_around_a_tile(hip_backend, dt, R):
+    """Units of one and two tiles of 32 rows, alone and next to others in one launch."""
+    G, N = R
+    Q, kp, vp, table = make(6, 2 * G, 2, N, 50, 16, 128, dt, seed=11)
+    lengths = torch.tensor([800, 64, 5, 333, N, 799], device="cuda")
+    check(Q, kp, vp, table, lengths)
+    check(Q, kp, vp, table, lengths, torch.tensor([N, N, 3, 1, N - 1, 0], device="cuda"))
+    Q, kp, vp, table = make(6, 2 * G, 2, N + 70, 50, 16, 128, dt, seed=12)
+    check(Q, kp, vp, table, lengths.clamp_min(90), torch.tensor([N, N + 70, N, 1, N - 1, 0], device="cuda"))
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_a_chunk_of_one_tile_next_to_few_rows(hip_backend, dt):
+    """One tile of 128 rows at most, of which some sequences have two narrow ones."""
+    Q, kp, vp, table = make(3, 4, 1, 20, 3, 16, 64, dt, seed=13)
+    check(Q, kp, vp, table, torch.tensor([48, 20, 30], device="cuda"), torch.tensor([12, 20, 9], device="cuda"))
+    Q, kp, vp, table = make(70, 4, 1, 20, 3, 16, 64, dt, seed=14)  # more than 64 sequences
+    new = torch.arange(70, device="cuda") % 21
+    check(Q, kp, vp, table, (new + torch.arange(70, device="cuda") % 29).clamp_max(48), new)

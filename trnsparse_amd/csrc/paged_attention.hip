@@ -13,7 +13,8 @@
 //   wide    128 rows to a workgroup, a wavefront to 32; stages of keys that the
 //           four wavefronts share in an LDS ring of two
 //   narrow  up to 32 rows to a workgroup: every wavefront has all of them and
-//           takes every fourth stage of 32 keys through LDS of its own
+//           takes every fourth stage of 32 keys through LDS of its own. (40 rows as
+//           two such workgroups, that read the keys twice: 40.9 us, wide 34.3.)
 // The host does not see the lengths. It launches `items` workgroups for every
 // unit; they find from the lengths how many tiles of rows each unit has and, where
 // these are few, ranges of the keys (share_of), and the work is dealt to the
@@ -887,7 +888,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const int64_t grid = head_grid(p.items, units);
   // (where all workgroups start at once, dealing costs 1 us and gives nothing: 24
   // sequences of five tokens 34.7 and 36.7 us; 64 of one token 287 and 279)
-  a.deal = B <= 64 && (new_lengths || units * p.items > 512);
+  a.deal = B <= 64 && (new_lengths || units * p.items >= 512);
   // (9 units of 1008 keys and up to 399 rows in fp32: 28 us with 128 keys to a workgroup)
   const bool few = units * ceil_div(keys, 128) < 512;
   const int64_t wper = ceil_div(keys, few ? 32 : 128);
