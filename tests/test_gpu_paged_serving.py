@@ -254,3 +254,16 @@ def test_traced_and_compiled(hip_backend):
         got = torch.compile(f, fullgraph=full, backend="aot_eager")(b)
         assert all(torch.equal(x, y) for x, y in zip(got, want))
         assert all(torch.equal(a[n], b[n]) for n in ("kp", "vp", "w"))
+
+
+def test_inference_mode(hip_backend):
+    """Caches made in and out of inference mode; one made in it is not written outside."""
+    a, b = _state(16, F32, 2), _state(16, F32, 2)
+    want = _step(a, 100)
+    with torch.inference_mode():
+        c = _state(16, F32, 2)
+        assert torch.equal(_step(b, 100), want) and torch.equal(_step(c, 100), want)
+    kept = c["kp"].clone()
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        ts.paged_cache_append(c["k"] + 1, c["v"], c["kp"], c["vp"], c["table"], c["lengths"])
+    assert torch.equal(c["kp"], kept)

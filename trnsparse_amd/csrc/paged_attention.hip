@@ -795,7 +795,7 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   // at once, each of its keys and of as much as `least` keys more (starting,
   // joining), to the shortest time.
   p.least = p.narrow ? (f32 ? 128 : 512) : (f32 ? 64 : 256);
-  p.step = p.narrow ? 128 : 64;
+  p.step = p.narrow ? 128 : 64;  // whole stages of all wavefronts
   p.slot_rows = (int)(p.narrow ? R : TILE);
   const int64_t room = p.narrow && f32 && D > 64 ? 256 : 512, most = ceil_div(keys > 0 ? keys : 1, p.least);
   int64_t n = 1, best = INT64_MAX;

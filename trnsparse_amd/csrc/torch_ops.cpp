@@ -776,7 +776,8 @@ const int64_t* need_weights(const at::Tensor& w, const PagedArgs& p, const at::T
   return s;
 }
 
-// what an operator wrote in place
+// What an operator writes in place counts as written (before it is: a tensor that may
+// not be written is refused).
 void written(std::initializer_list<const at::Tensor*> ts) {
   for (const at::Tensor* t : ts) t->unsafeGetTensorImpl()->bump_version();
 }
@@ -798,12 +799,12 @@ at::Tensor paged_attn_fwd(const at::Tensor& Q_, const at::Tensor& K, const at::T
   const int64_t wsb = tsp_paged_attn_workspace_size(p.code, p.B, Hq, p.Hk, Sq, p.slots, p.D, new_lengths.has_value(),
                                                     weights.has_value());
   const Workspace ws(wsb, Q, who);
+  if (weights.has_value()) written({&*weights});
   check(tsp_paged_attn_fwd(Q.data_ptr(), Strides(Q).s, K.data_ptr(), p.ks, V.data_ptr(), p.vs, p.code, p.B, Hq, p.Hk, Sq,
                            p.pages, p.page_size, p.D, p.table, p.tcode, p.tstride, p.cols, p.lens, p.fresh,
                            p.icode, scale, O.data_ptr(), Strides(O).s,
                            weights.has_value() ? weights->data_ptr<float>() : nullptr, ws2, ws.ptr(), wsb, stream_of(Q)),
         "tsp_paged_attn_fwd");
-  if (weights.has_value()) written({&*weights});
   return O;
 }
 
@@ -827,13 +828,13 @@ at::Tensor paged_append(const at::Tensor& K_, const at::Tensor& V_, const at::Te
   if (weights.has_value()) need_weights(*weights, p, Kp, who, ws2);
   const auto K = attn_operand(K_), V = attn_operand(V_);
   auto out = at::empty({p.B}, lengths.options());
+  written({&Kp, &Vp});
+  if (weights.has_value()) written({&*weights});
   check(tsp_paged_append(K.data_ptr(), Strides(K).s, V.data_ptr(), Strides(V).s, Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs,
                          p.code, p.B, p.Hk, K.size(2), p.pages, p.page_size, p.D, p.table, p.tcode, p.tstride,
                          p.cols, p.lens, p.fresh, p.icode, out.data_ptr(),
                          weights.has_value() ? weights->data_ptr<float>() : nullptr, ws2, stream_of(Kp)),
         "tsp_paged_append");
-  written({&Kp, &Vp});
-  if (weights.has_value()) written({&*weights});
   return out;
 }
 
@@ -854,11 +855,11 @@ at::Tensor paged_evict(const at::Tensor& Kp, const at::Tensor& Vp, const at::Ten
   auto out = at::empty({p.B}, lengths.options());
   const int64_t wsb = tsp_paged_evict_workspace_size(p.code, p.B, p.Hk, p.slots, p.D, budget);
   const Workspace ws(wsb, Kp, who);
+  written({&Kp, &Vp, &weights});
   check(tsp_paged_evict(Kp.data_ptr(), p.ks, Vp.data_ptr(), p.vs, p.code, p.B, p.Hk, p.pages, p.page_size, p.D,
                         p.table, p.tcode, p.tstride, p.cols, p.lens, p.icode, weights.data_ptr<float>(), ws2,
                         budget, recent, out.data_ptr(), ws.ptr(), wsb, stream_of(Kp)),
         "tsp_paged_evict");
-  written({&Kp, &Vp, &weights});
   return out;
 }
 
