@@ -691,8 +691,9 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  * entries are of table_type (TSP_I32 or TSP_I64). slots = columns * page_size,
  * the rows a sequence may have, is at most 2^30, and slots * page_size below
  * 2^40. An entry outside [0, pages) is a page of zeros that cannot be written.
- * A page that is written belongs to one sequence: what two writes to one row
- * leave is not defined.
+ * A page that is written (by an eviction: that holds rows of a cut sequence)
+ * stands once in the table, and K_pages and V_pages do not overlap there: what
+ * two writes to one row leave is not defined.
  * lengths and new_lengths (batch,) are of index_type and are taken into
  * [0, slots] and [0, queries or tokens]; new_lengths NULL: all. weights
  * (batch, kv_heads, slots) fp32, unit stride over slots; weight_strides: two
@@ -721,8 +722,8 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  *   budget - recent of the largest weights: of equal ones the first, NaN above
  *   all numbers. The kept rows of K, V and weights move to rows [0, budget) in
  *   their order; what stands behind is left as it was. lengths_out, not lengths
- *   itself, receives min(lengths[b], budget). K_pages and V_pages must not
- *   overlap. workspace: tsp_paged_evict_workspace_size bytes, 16-byte aligned.
+ *   itself, receives min(lengths[b], budget). workspace:
+ *   tsp_paged_evict_workspace_size bytes, 16-byte aligned.
  * ==================================================================== */
 int64_t tsp_paged_attn_workspace_size(int dtype, int64_t batch, int64_t heads,
                                       int64_t kv_heads, int64_t queries,

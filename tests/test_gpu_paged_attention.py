@@ -268,3 +268,32 @@ def test_a_chunk_of_one_tile_next_to_few_rows(hip_backend, dt):
     Q, kp, vp, table = make(70, 4, 1, 20, 3, 16, 64, dt, seed=14)  # more than 64 sequences
     new = torch.arange(70, device="cuda") % 21
     check(Q, kp, vp, table, (new + torch.arange(70, device="cuda") % 29).clamp_max(48), new)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("heads,N,cols", [((4, 2), 3, 4), ((8, 2), 6, 4), ((8, 2), 6, 400), ((2, 2), 50, 10), ((16, 16), 140, 40)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_rows_of_scores_that_are_all_minus_infinity(hip_backend, dt, heads, N, cols, mixed):
+    """Their result is zero, and they weigh nothing; the rows beside them as ever."""
+    Q, kp, vp, table = make(3, *heads, N, cols, 16, 64, dt, seed=4)
+    L = 16 * cols
+    kp = kp.abs() + 0.125
+    lengths = torch.tensor([L, L - 5, N], device="cuda")
+    new = torch.tensor([N, max(N - 20, 1), 1], device="cuda") if mixed else None
+    clean = Q.clone()
+    clean[:, 1, 1::2] = 0
+    Q[:, 1, 1::2] = float("-inf")
+    gone = torch.zeros(3, heads[0], N, 1, dtype=torch.bool, device="cuda")
+    gone[:, 1, 1::2] = True
+    w = torch.zeros(3, heads[1], L, device="cuda")
+    O = ts.paged_attention(Q, kp, vp, table, lengths, new, None, w)
+    assert not (O * gone).any() and not w.isnan().any()
+    # the rows of equal scores that stand in their places weigh 1 / (keys seen) each
+    whole = ts.paged_attention(clean, kp, vp, table, lengths, new, None, torch.zeros_like(w))
+    assert torch.equal(O.masked_fill(gone, 0), whole.masked_fill(gone, 0))
+    seen = layer.chunk_seen(lengths.cpu(), None if new is None else new.cpu(), N, L)
+    each = (seen[:, 1::2].double() / seen[:, 1::2].sum(-1, keepdim=True).clamp(min=1)).sum(1)
+    r = layer.attention(clean, layer.paged_rows(kp, table), layer.paged_rows(vp, table), 64**-0.5, seen)
+    r["W"][:, 1 // (heads[0] // heads[1])] -= each  # head 1's key head
+    far = (w.double().cpu() - r["W"]).abs() - wtol(64, L, heads[0] // heads[1] * N, r["smax"]) * r["W"]
+    assert far.max() <= 1e-15, float(far.max())

@@ -57,7 +57,7 @@ struct Args {
   int least, step;           // a range's least keys, and what it is a multiple of
   int slot_rows;             // rows of one such result
   float *part, *plse;        // [unit][slot][row]: results, log-sum-exps (base 2)
-  float* lse;                // [unit][R]: log-sum-exps (base 2) where the weights need them, else null
+  float* lse;                // [unit][R]: where the weights need them (else null), what scale_of makes of log-sum-exps
   float* scores;             // [unit][stage of 32 keys][sr][32], log2 units, of units of up to sr rows
   int sr;
   int stages;                // of a unit
@@ -92,6 +92,9 @@ __device__ inline Share share_of(const Args& a, int n, int m) {
 __device__ inline Share share_of(const Args& a, int64_t b) {
   return share_of(a, (int)cached_rows(a.len, b), (int)new_rows(a.len, b));
 }
+// A log-sum-exp (base 2) as the weights take it: of a row whose scores are all -inf,
+// whose result is zero, such that every weight 2^(score - it) is zero too.
+__device__ inline float scale_of(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 // Keys that a row's token sees.
 __device__ inline int sees_of(const Share& s, int i) { return s.n - (s.m - 1 - i); }
 
@@ -334,7 +337,7 @@ struct Wide {
       if (!whole)
         a.plse[at] = e;
       else if (a.lse)
-        a.lse[(int64_t)wk.unit * a.R + r] = e;
+        a.lse[(int64_t)wk.unit * a.R + r] = scale_of(e);
     }
   }
 };
@@ -479,7 +482,7 @@ struct Narrow {
         if (!whole)
           a.plse[at] = lse;
         else if (a.lse)
-          a.lse[(int64_t)unit * a.R + row] = lse;
+          a.lse[(int64_t)unit * a.R + row] = scale_of(lse);
       }
     }
   }
@@ -570,7 +573,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const Args a, int per) {
   if (s.splits == 1) return;
   for (int r = (int)part * 8 + (int)(threadIdx.x >> 5); r < s.rows; r += 8 * per) {
     const float lse = combine_row<T>(a, s, unit, b, hk, r);
-    if (a.lse && (threadIdx.x & 31) == 0) a.lse[(int64_t)unit * a.R + r] = lse;
+    if (a.lse && (threadIdx.x & 31) == 0) a.lse[(int64_t)unit * a.R + r] = scale_of(lse);
   }
 }
 

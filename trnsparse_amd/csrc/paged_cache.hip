@@ -57,8 +57,10 @@ int check_weights(const char* who, const void* w, const int64_t* s) {
 namespace {
 
 // A workgroup to `tokens` new tokens of one sequence, all heads, a thread to a piece
-// of 16 bytes of K's row and V's, AU of them at a time. Bound by the rows' bytes, or by
-// the launch (TODO). Workgroups behind a sequence's new tokens end at once.
+// of 16 bytes of K's row and V's, AU of them at a time. Workgroups behind a sequence's
+// new tokens end at once. Bound by the launch (64 sequences, a token of 8 heads of 128 in
+// 16 bits each: 3.6 us) or by the rows' bytes, read and written (four prompts of 1024 to
+// 2047 tokens next to 12 single ones, 50 MB: 12.5 us, 4.0 TB/s).
 struct AppendArgs {
   const char *K, *V;
   int64_t kb, kh, ks, vb, vh, vs;  // strides in bytes

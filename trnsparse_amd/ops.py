@@ -798,7 +798,8 @@ def paged_cache_append(
     allowed: row i < new_lengths[b] (None: all) becomes row lengths[b] + i of
     sequence b. Rows past the table's columns, or in a page that is not there,
     are left out. `weights` (batch, kv_heads, slots), where given, is set to
-    zero at the new rows. A page that is written belongs to one sequence.
+    zero at the new rows. A page that is written stands once in block_table, and
+    K_pages and V_pages lie apart.
     """
     who = "paged_cache_append"
     _no_gradients(who, K, V, K_pages, V_pages, weights)
@@ -849,8 +850,8 @@ def paged_cache_evict(
     first rows, a NaN counts as above all numbers. The kept rows of K_pages,
     V_pages and weights move to rows [0, budget) in their order; what stands
     behind them is left as it was. Heads keep rows of their own. A sequence of
-    at most `budget` rows stays as it is. A page that a cut sequence has belongs
-    to it alone.
+    at most `budget` rows stays as it is. A page of a cut sequence's rows stands
+    once in block_table, and K_pages and V_pages lie apart.
     """
     who = "paged_cache_evict"
     _no_gradients(who, K_pages, V_pages, weights)
