@@ -157,7 +157,7 @@ struct Unit {
 __device__ inline Unit unit_at(const EvictArgs& a, int64_t unit) {
   Unit u;
   u.unit = unit;
-  u.b = unit / a.Hkv;
+  u.b = (uint32_t)unit / (uint32_t)a.Hkv;  // (32 bits: there are at most 2^30)
   u.h = unit - u.b * a.Hkv;
   u.n = (int)cached_rows(a.len, u.b);
   u.cut = u.n > a.budget;
@@ -314,10 +314,15 @@ __device__ inline Find find_after(const EvictArgs& a, const Unit& u, int turn, S
   const int parts = (u.E + PART - 1) / PART, d = BINS - 1 - 2 * (int)threadIdx.x;
   const uint32_t* hist = a.hist + ((int64_t)(turn - 1) * a.units + u.unit) * a.parts * BINS + d - 1;
   int c0 = 0, c1 = 0;
-  for (int i = 0; i < parts; ++i) {
-    const u32x2 c = *(const u32x2*)(hist + (int64_t)i * BINS);
-    c0 += (int)c.y;
-    c1 += (int)c.x;
+  for (int i = 0; i < parts; i += 8) {
+    u32x2 c[8];
+#pragma unroll
+    for (int v = 0; v < 8; ++v) c[v] = *(const u32x2*)(hist + (int64_t)(i + v < parts ? i + v : parts - 1) * BINS);
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+      c0 += i + v < parts ? (int)c[v].y : 0;
+      c1 += i + v < parts ? (int)c[v].x : 0;
+    }
   }
   next_digit(f, c0, c1, x);
   return f;
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(ST) void list_kernel(const EvictArgs a) {
 constexpr int SU = 8;
 __global__ __launch_bounds__(256) void save_kernel(const EvictArgs a, uint32_t per, int lanes) {
   const uint32_t at = blockIdx.x % per;
-  const int64_t x = blockIdx.x / per, unit = x >> 1, b = unit / a.Hkv, h = unit - b * a.Hkv;
+  const int64_t x = blockIdx.x / per, unit = x >> 1, b = (uint32_t)unit / (uint32_t)a.Hkv, h = unit - b * a.Hkv;
   const int step = 256 >> lanes, d0 = (int)at * step * SU + (int)(threadIdx.x >> lanes);
   const int c = 16 * (int)(threadIdx.x & ((1u << lanes) - 1)), row = a.D * a.esz;
   if (a.first[unit] >= a.budget) return;
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
   const uint32_t xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, slice = at8 % slices, y = at8 / slices * 8 + xcd;
   const int64_t x = y / segments, unit = x >> 1;
   if (unit >= a.units) return;
-  const int64_t b = unit / a.Hkv, h = unit - b * a.Hkv;
+  const int64_t b = (uint32_t)unit / (uint32_t)a.Hkv, h = unit - b * a.Hkv;
   // the places of this workgroup
   const int64_t s0 = (int64_t)(y - (uint32_t)x * segments) << a.segment, s1 = s0 + ((int64_t)1 << a.segment);
   const int first = a.first[unit] > s0 ? a.first[unit] : (int)s0, end = (int)(s1 < a.budget ? s1 : a.budget) - 1;
@@ -508,10 +513,11 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
 }
 
 // Whether a unit's weights are searched by a workgroup to each part of them: five
-// launches, which takes less time than one workgroup's turns from 7 parts on, while
-// the units leave CUs without one (8 units of 131072 rows: 45 us for 110; 64 of 32768:
-// the eviction 298 us, with one workgroup to each unit 268).
-bool by_parts(int64_t units, int64_t slots) { return units < 128 && slots > 6 * PART; }
+// launches, which take less time than one workgroup's turns where these are many and
+// the units leave CUs without one. The whole eviction with one workgroup to each unit
+// and by parts, us: 8 units of 24576 rows 52 and 56, of 32768 60 and 56, of 49152 71 and
+// 56; 32 of 49152 166 and 168; 64 of 65536 174 and 185, of 81920 196 and 197.
+bool by_parts(int64_t units, int64_t slots) { return units < 128 && slots > (3 + units / 10) * PART; }
 // log2 of the places of a segment, 31 where all are one. Segments for 512 workgroups,
 // none of less than 1024 places, where the chains of parts are too few to take the
 // memory's rate (64 with slices of 64 bytes) and long: copying rows aside is traffic
