@@ -267,3 +267,26 @@ def test_inference_mode(hip_backend):
     with pytest.raises(RuntimeError, match="[Ii]nference"):
         ts.paged_cache_append(c["k"] + 1, c["v"], c["kp"], c["vp"], c["table"], c["lengths"])
     assert torch.equal(c["kp"], kept)
+
+
+@pytest.mark.parametrize("host", [False, True])
+def test_public_refusal_of_gradients(hip_backend, host):
+    """Whichever operand asks for one, on the GPU or not; nothing is written."""
+    s = _state(17, F32, 2)
+    if host:
+        s = {n: t.cpu() if isinstance(t, torch.Tensor) else t for n, t in s.items()}
+    calls = {
+        "paged_attention": (lambda a: ts.paged_attention(a["q"], a["kp"], a["vp"], a["table"], a["lengths"], None, None, a["w"]),
+                            ("q", "kp", "vp", "w")),
+        "paged_cache_append": (lambda a: ts.paged_cache_append(a["k"], a["v"], a["kp"], a["vp"], a["table"], a["lengths"], None, a["w"]),
+                               ("k", "v", "kp", "vp", "w")),
+        "paged_cache_evict": (lambda a: ts.paged_cache_evict(a["kp"], a["vp"], a["w"], a["table"], a["lengths"], 20, 5),
+                              ("kp", "vp", "w")),
+    }
+    for name, (call, operands) in calls.items():
+        for n in operands:
+            a = {m: t.clone() if isinstance(t, torch.Tensor) else t for m, t in s.items()}
+            a[n].requires_grad_()
+            with pytest.raises(RuntimeError, match=f"{name} has no gradients"):
+                call(a)
+            assert all(torch.equal(a[m].detach(), s[m]) for m in ("kp", "vp", "w"))

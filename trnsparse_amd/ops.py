@@ -663,7 +663,22 @@ def shared_prefix_attention(
 # A key and value cache in pages: what the three operators share.
 
 
+_dispatch = None
+
+
+def _hip():
+    """hip.dispatch, imported by the first call that needs it (an import statement
+    costs every call about 0.5 us)."""
+    global _dispatch
+    if _dispatch is None:
+        from .hip import dispatch
+
+        _dispatch = dispatch
+    return _dispatch
+
+
 def _no_gradients(who: str, *tensors) -> None:
+    """The HIP operators refuse the same (csrc/torch_ops.cpp)."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{who} has no gradients: call it under torch.no_grad()")
 
@@ -749,11 +764,9 @@ def paged_attention(
     who = "paged_attention"
     if scale is None:
         scale = _default_scale(Q)
-    _no_gradients(who, Q, K_pages, V_pages, weights)
     if _use_hip():
-        from .hip.dispatch import hip_paged_attention
-
-        return hip_paged_attention(Q, K_pages, V_pages, block_table, lengths, new_lengths, scale, weights)
+        return _hip().hip_paged_attention(Q, K_pages, V_pages, block_table, lengths, new_lengths, scale, weights)
+    _no_gradients(who, Q, K_pages, V_pages, weights)
     _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights)
     B, cols = block_table.shape
     _, Hk, size, D = K_pages.shape
@@ -802,11 +815,9 @@ def paged_cache_append(
     K_pages and V_pages lie apart.
     """
     who = "paged_cache_append"
-    _no_gradients(who, K, V, K_pages, V_pages, weights)
     if _use_hip():
-        from .hip.dispatch import hip_paged_cache_append
-
-        return hip_paged_cache_append(K, V, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+        return _hip().hip_paged_cache_append(K, V, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+    _no_gradients(who, K, V, K_pages, V_pages, weights)
     _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights)
     B, cols = block_table.shape
     _, Hk, size, D = K_pages.shape
@@ -854,11 +865,9 @@ def paged_cache_evict(
     once in block_table, and K_pages and V_pages lie apart.
     """
     who = "paged_cache_evict"
-    _no_gradients(who, K_pages, V_pages, weights)
     if _use_hip():
-        from .hip.dispatch import hip_paged_cache_evict
-
-        return hip_paged_cache_evict(K_pages, V_pages, weights, block_table, lengths, budget, recent)
+        return _hip().hip_paged_cache_evict(K_pages, V_pages, weights, block_table, lengths, budget, recent)
+    _no_gradients(who, K_pages, V_pages, weights)
     _check_cache(who, K_pages, V_pages, block_table, lengths, None, weights)
     if not 0 <= recent <= budget:
         raise RuntimeError(f"{who}: recent {recent} is not in 0 .. budget {budget}")
