@@ -164,3 +164,27 @@ def test_evict_again_and_again(hip_backend):
 def test_evict_by_parts(hip_backend, size, kind):
     """Weights searched part by part, rows moved in one list or in segments."""
     test_evict_long(hip_backend, BF, size, kind)
+
+
+@pytest.mark.parametrize("cols", [64, 1000])
+@pytest.mark.parametrize("step", [1 << 23, 1 << 12, 5])
+@pytest.mark.parametrize("more", [-30, 0, 30])
+def test_evict_where_the_search_ends(hip_backend, cols, step, more):
+    """Two weights that differ in the first, the second or the last digit of the search; the
+    budget takes some of the larger ones, all of them, or some of the smaller too."""
+    _, kp, vp, table = make(2, 2, 2, 1, cols, 64, 16, BF)
+    L, recent = cols * 64, 100
+    g = torch.Generator(device="cuda").manual_seed(5)
+    large = torch.zeros(2, 2, L, dtype=torch.bool, device="cuda")
+    count = L // 5
+    for b in range(2):
+        for h in range(2):
+            large[b, h, torch.randperm(L - recent - 77 * b, device="cuda", generator=g)[:count]] = True
+    w = (torch.full((2, 2, L), 0x3F800000, dtype=torch.int32, device="cuda") + large.int() * step).view(torch.float32)
+    lengths = torch.tensor([L, L - 77], device="cuda")
+    k, v, x = kp.clone(), vp.clone(), w.clone()
+    ts.set_backend("pytorch")
+    want = ts.paged_cache_evict(k, v, x, table, lengths, count + more + recent, recent)
+    ts.set_backend("hip")
+    after = ts.paged_cache_evict(kp, vp, w, table, lengths, count + more + recent, recent)
+    same((kp, vp, w, after), (k, v, x, want))

@@ -10,9 +10,8 @@
 // rows with the digits so far stay), and lists the kept rows in order.
 //   select_kernel   one workgroup to a unit does it all; rows of up to one part
 //                   stay in its registers
-//   digit, count and list kernels (few units of many rows): a workgroup to a part
-//                   of 8192 rows, the histograms of a unit's parts added up by whoever
-//                   needs them
+//   digit and list kernels (few units of many rows): a workgroup to a part of 8192
+//                   rows, the histograms of a unit's parts added up by whoever needs them
 // move_kernel then moves the listed rows of K and V. A row goes to a place at or
 // before its own, and the list rises: a workgroup that takes the list in order, and
 // writes a part only once all of its rows are read, never writes over a row that is
@@ -42,9 +41,9 @@ struct EvictArgs {
   // few units of many rows
   int parts;       // of a unit's rows at most
   int segment;     // log2 of the places of a segment; 31: all are one
-  struct Find* state;  // [3][unit]: the search after the first, the second and the third digit
+  struct Find* state;  // [2][unit]: the search after the first and the second digit
   uint32_t* hist;  // [3][unit][part][BINS]
-  int32_t* count;  // [unit][part][2]: rows above the last key, rows equal to it
+  int32_t* count;  // [unit][part]: rows that stay whatever the last digit is
   float* kept;     // [unit][budget]: weights; null where they are in place
   char* saved;     // [unit][K, V][budget]: rows
 };
@@ -304,10 +303,12 @@ __global__ __launch_bounds__(ST) void select_kernel(const EvictArgs a) {
 
 // ------------------------------------------------- few units of many rows
 
-// The search after `turn` digits, from the one before and that digit's counts over the unit's parts.
-__device__ inline Find find_after(const EvictArgs& a, const Unit& u, int turn, Scratch& x) {
+// The search after `turn` digits, from the one before and that digit's counts over the unit's
+// parts; b0 and b1: the counts of this thread's two digits (next_digit) in the parts before `upto`.
+__device__ inline Find find_after(const EvictArgs& a, const Unit& u, int turn, Scratch& x, int upto, int& b0, int& b1) {
   Find f;
   f.start(u.keep);
+  b0 = b1 = 0;
   if (turn == 0) return f;
   if (turn > 1) f = a.state[(turn - 2) * a.units + u.unit];
   if (f.done) return f;
@@ -322,73 +323,88 @@ __device__ inline Find find_after(const EvictArgs& a, const Unit& u, int turn, S
     for (int v = 0; v < 8; ++v) {
       c0 += i + v < parts ? (int)c[v].y : 0;
       c1 += i + v < parts ? (int)c[v].x : 0;
+      b0 += i + v < parts && i + v < upto ? (int)c[v].y : 0;
+      b1 += i + v < parts && i + v < upto ? (int)c[v].x : 0;
     }
   }
   next_digit(f, c0, c1, x);
   return f;
 }
 
-// Counts of the next digit in one part of a unit; in the last turn, of the rows
-// above the last key and equal to it.
+// Counts of the next digit in one part of a unit; in the last turn, of the rows that stay
+// whatever the last digit is, too.
 __global__ __launch_bounds__(ST) void digit_kernel(const EvictArgs a, int turn) {
   __shared__ uint32_t hist[BINS];
   __shared__ Scratch x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x % (uint32_t)a.parts;
   const Unit u = unit_at(a, blockIdx.x / (uint32_t)a.parts);
   if (turn == 0 && part == 0) put_length(a, u);
-  const int end = turn < 3 ? u.E : u.n, j = part * PART + tid * SPT;
+  const int end = turn < 2 ? u.E : u.n, j = part * PART + tid * SPT;
   if (!u.cut || part * PART >= end) return;
   Part<SPT> p;
   p.load(u.w, j, u.n, u.aligned);
-  const Find f = find_after(a, u, turn, x);
+  int b0, b1;
+  const Find f = find_after(a, u, turn, x, 0, b0, b1);
   if (turn > 0 && part == 0 && tid == 0) a.state[(turn - 1) * a.units + u.unit] = f;
-  if (turn < 3) {
-    if (f.done) return;
-    for (int i = tid; i < BINS; i += ST) hist[i] = 0;
+  if (turn == 2) {
+    Find top = f;
+    if (!f.done) top.last = f.lo + (1u << 10) - 1;  // above all keys that are still in question
+    uint32_t above, same;
+    sort_out(u, top, p, j, above, same);
+    int total;
+    wave_scan(__builtin_popcount(above), total);
+    if (lane == 0) x.sums[1][wave] = total;
     __syncthreads();
-    add_digits(hist, f, p, j, u.E);
-    __syncthreads();
-    uint32_t* to = a.hist + (((int64_t)turn * a.units + u.unit) * a.parts + part) * BINS;
-    for (int i = tid; i < BINS; i += ST) to[i] = hist[i];
-    return;
+    if (tid == 0) {
+      int all = 0;
+      for (int i = 0; i < ST / 64; ++i) all += x.sums[1][i];
+      a.count[u.unit * a.parts + part] = all;
+    }
   }
-  uint32_t above, same;
-  sort_out(u, f, p, j, above, same);
-  int total;
-  wave_scan(__builtin_popcount(same) << 16 | __builtin_popcount(above), total);
-  if (lane == 0) x.sums[1][wave] = total;
+  if (f.done) return;
+  for (int i = tid; i < BINS; i += ST) hist[i] = 0;
   __syncthreads();
-  if (tid == 0) {
-    int all = 0;
-    for (int i = 0; i < ST / 64; ++i) all += x.sums[1][i];
-    int32_t* to = a.count + 2 * (u.unit * a.parts + part);
-    to[0] = all & 0xffff;
-    to[1] = all >> 16;
-  }
+  add_digits(hist, f, p, j, u.E);
+  __syncthreads();
+  uint32_t* to = a.hist + (((int64_t)turn * a.units + u.unit) * a.parts + part) * BINS;
+  for (int i = tid; i < BINS; i += ST) to[i] = hist[i];
 }
 __global__ __launch_bounds__(ST) void list_kernel(const EvictArgs a) {
   __shared__ Scratch x;
-  const int tid = threadIdx.x, lane = tid & 63, part = blockIdx.x % (uint32_t)a.parts;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x % (uint32_t)a.parts;
   const Unit u = unit_at(a, blockIdx.x / (uint32_t)a.parts);
   if (part == 0 && tid == 0) a.first[u.unit] = u.cut ? 0 : a.budget;
   const int j = part * PART + tid * SPT;
   if (!u.cut || part * PART >= u.n) return;
   Part<SPT> p;
   p.load(u.w, j, u.n, u.aligned);
-  const Find f = a.state[2 * a.units + u.unit];
-  const int32_t* count = a.count + 2 * u.unit * a.parts;
-  int above = 0, equal_base = 0;  // of the parts before
-  for (int i = lane; i < part; i += 64) {
-    above += count[2 * i];
-    equal_base += count[2 * i + 1];
+  const u32x2 spot = spot_of_row(a, u, j);
+  int above = 0;  // of the parts before: rows above the last key, and those that equal it
+  for (int i = tid; i < part; i += ST) above += a.count[u.unit * a.parts + i];
+  const bool done = a.state[a.units + u.unit].done;
+  int b0, b1;
+  const Find f = find_after(a, u, 3, x, part, b0, b1);
+  int equal = 0;
+  if (!done) {
+    const int d = BINS - 1 - 2 * tid, last = (int)(f.lo & 1023);
+    above += (d > last ? b0 : 0) + (d - 1 > last ? b1 : 0);
+    equal = (d == last ? b0 : 0) + (d - 1 == last ? b1 : 0);
+    if (f.equal == 0) above += equal, equal = 0;  // (all of them stay)
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    above += __shfl_xor(above, o, 64);
-    equal_base += __shfl_xor(equal_base, o, 64);
+  int above_w, equal_w;
+  wave_scan(above, above_w);
+  wave_scan(equal, equal_w);
+  __syncthreads();
+  if (lane == 0) x.sums[0][wave] = above_w, x.sums[1][wave] = equal_w;
+  __syncthreads();
+  int base = 0, equal_base = 0;
+  for (int i = 0; i < ST / 64; ++i) {
+    base += x.sums[0][i];
+    equal_base += x.sums[1][i];
   }
-  int base = above + (equal_base < f.equal ? equal_base : f.equal);
-  list_part(a, u, f, p, j, spot_of_row(a, u, j), a.kept + u.unit * a.budget, base, equal_base, 0, x);
+  base += equal_base < f.equal ? equal_base : f.equal;
+  __syncthreads();
+  list_part(a, u, f, p, j, spot, a.kept + u.unit * a.budget, base, equal_base, 0, x);
 }
 
 // Copies aside the rows that come from another segment's places, and puts the kept
@@ -512,7 +528,7 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
   }
 }
 
-// Whether a unit's weights are searched by a workgroup to each part of them: five
+// Whether a unit's weights are searched by a workgroup to each part of them: four
 // launches, which take less time than one workgroup's turns where these are many and
 // the units leave CUs without one. The whole eviction with one workgroup to each unit
 // and by parts, us: 8 units of 24576 rows 52 and 56, of 32768 60 and 56, of 49152 71 and
@@ -540,9 +556,9 @@ Space space_of(int64_t units, int64_t slots, int64_t budget, int64_t row) {
   s.list = s.first + up(4 * units);
   s.state = s.list + up(8 * units * budget);
   const int64_t parts = by_parts(units, slots) ? ceil_div(slots, PART) : 0;
-  s.hist = s.state + (parts ? up(3 * units * (int64_t)sizeof(Find)) : 0);
+  s.hist = s.state + (parts ? up(2 * units * (int64_t)sizeof(Find)) : 0);
   s.count = s.hist + 3 * units * parts * BINS * 4;
-  s.kept = s.count + up(8 * units * parts);
+  s.kept = s.count + up(4 * units * parts);
   s.saved = s.kept + (parts ? up(4 * units * budget) : 0);
   s.end = s.saved + (segment_of(units, budget, row) < 31 ? units * 2 * budget * row : 0);
   return s;
@@ -617,7 +633,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   if (grid > INT32_MAX || units * a.parts > INT32_MAX || units * 2 * per > INT32_MAX)
     return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
   if (parts) {
-    for (int turn = 0; turn < 4; ++turn)
+    for (int turn = 0; turn < 3; ++turn)
       hipLaunchKernelGGL(paged::digit_kernel, dim3((unsigned)(units * a.parts)), dim3(paged::ST), 0, st, a, turn);
     hipLaunchKernelGGL(paged::list_kernel, dim3((unsigned)(units * a.parts)), dim3(paged::ST), 0, st, a);
   } else {
