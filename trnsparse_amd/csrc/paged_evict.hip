@@ -617,9 +617,15 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   a.list = (u32x2*)(a.spare + sp.list);
   a.segment = paged::segment_of(units, budget, row);
   const uint32_t segments = a.segment < 31 ? (uint32_t)ceil_div(budget, int64_t(1) << a.segment) : 1;
-  // slices of 128 bytes, a line of the cache; of 64 where they leave CUs without one
+  // Slices of 256 bytes where these are no more bytes than slices of 128 (a line of the
+  // cache) and give 192 workgroups; of 64 where those of 128 leave CUs without one. (The
+  // eviction of units of 4096 rows to 2048, slices of 128 and 256 bytes, us: rows of 256
+  // bytes, 64 units 34.6 and 37.2, 96 units 46.6 and 44.1, 256 units 122 and 117; rows of
+  // 192 bytes, 256 units 119 and 97; of 384 bytes, 128 units 88 and 92. 32768 rows of 131072
+  // in segments, 8 units: 105 and 101.)
   const bool parts = paged::by_parts(units, slots), thin = segments == 1 && units * 2 * ceil_div(row, 128) < 256;
-  const int64_t slices = ceil_div(row, thin ? 64 : 128), lanes = row > 256 ? 5 : row > 128 ? 4 : 3,
+  const bool broad = ceil_div(row, 128) % 2 == 0 && units * 2 * segments * ceil_div(row, 256) >= 192;
+  const int64_t slices = ceil_div(row, broad ? 256 : thin ? 64 : 128), lanes = row > 256 ? 5 : row > 128 ? 4 : 3,
                 per = ceil_div(budget, (256 >> lanes) * paged::SU);
   if (parts) {
     a.parts = (int)ceil_div(slots, paged::PART);
@@ -648,11 +654,14 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
     hipLaunchKernelGGL(paged::save_kernel, dim3((unsigned)(units * 2 * per)), dim3(256), 0, st, a, (uint32_t)per, (int)lanes);
   if ((rc = check_launch("select launch"))) return rc;
   if (pages == 0 || budget == 0) return TSP_OK;
+  const auto move = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
+  };
   if (segments > 1)
-    hipLaunchKernelGGL((paged::move_kernel<8, true>), dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
-  else if (thin)
-    hipLaunchKernelGGL((paged::move_kernel<4, false>), dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
+    broad ? move(paged::move_kernel<16, true>) : move(paged::move_kernel<8, true>);
+  else if (broad)
+    move(paged::move_kernel<16, false>);
   else
-    hipLaunchKernelGGL((paged::move_kernel<8, false>), dim3((unsigned)grid), dim3(paged::MT), 0, st, a, (uint32_t)slices, segments);
+    thin ? move(paged::move_kernel<4, false>) : move(paged::move_kernel<8, false>);
   return check_launch("move launch");
 }
