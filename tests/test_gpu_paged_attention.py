@@ -297,3 +297,15 @@ def test_rows_of_scores_that_are_all_minus_infinity(hip_backend, dt, heads, N, c
     r["W"][:, 1 // (heads[0] // heads[1])] -= each  # head 1's key head
     far = (w.double().cpu() - r["W"]).abs() - wtol(64, L, heads[0] // heads[1] * N, r["smax"]) * r["W"]
     assert far.max() <= 1e-15, float(far.max())
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("size", [(1, 8, 1, 300, 20, 16, 64), (2, 4, 1, 1100, 72, 16, 128), (3, 16, 2, 513, 9, 64, 40), (1, 7, 1, 900, 57, 16, 80)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_weights_of_many_rows_and_few_keys(hip_backend, size, dt, mixed):
+    """The rows of a key head in parts, next to sequences of none, one and few rows."""
+    Q, kp, vp, table = make(*size, dt, seed=6)
+    B, N, L = size[0], size[3], size[4] * size[5]
+    lengths = torch.tensor([L, N - 7, L - 33], device="cuda")[:B]
+    new = torch.tensor([N - 5, 1, 0] if B < 3 else [1, N - 3, 0], device="cuda")[:B] if mixed else None
+    check(Q, kp, vp, table, lengths, new)

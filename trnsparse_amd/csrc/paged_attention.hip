@@ -64,6 +64,9 @@ struct Args {
   float scale_log2;
   float* W;
   int64_t wb, wh;
+  int wsplits;               // parts of a unit's rows in weights_kernel; their sums:
+  float* wpart;              // [part][unit][wkeys], where there are several
+  int wkeys;
 };
 
 constexpr int MOST_RANGES = 64;  // of a unit's keys where the host chooses them
@@ -638,7 +641,9 @@ __global__ __launch_bounds__(256) void weigh_kernel(const Args a, int cw, int kw
 //   RW 1  128 keys to a workgroup, whose four wavefronts share the stages
 //   RW 4  32 keys to a workgroup, every wavefront with every fourth stage of 32
 //         rows through LDS of its own, their sums added at the end: four times as
-//         many workgroups, each a quarter as long, for launches that have few
+//         many workgroups, each a quarter as long, for launches that have few; where
+//         these would still be few and long, a workgroup takes a part of the rows only,
+//         and add_kernel adds the parts' sums
 template <typename T, int RW>
 struct Weigh {
   static constexpr int NT = RW == 1 && T::ESZ == 2 ? 2 : 1, HR = 32 * NT, STAGE = HR * T::ROWB;
@@ -652,16 +657,25 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
   __shared__ __attribute__((aligned(256))) float lse[G::RINGS][2][64];  // of a stage's rows
   uint32_t unit, b, hk;
   int item;
-  if (!unit_of(a, blockIdx.x, per, unit, b, hk, item)) return;
+  if constexpr (RW == 1) {
+    if (!unit_of(a, blockIdx.x, per, unit, b, hk, item)) return;
+  } else {
+    // the few units' workgroups over all XCDs (one long sequence of two key heads next to
+    // three of one token, each head on an XCD of its own: 78 us, 30 over all)
+    const uint32_t p = blockIdx.x / (uint32_t)a.Hkv;
+    hk = blockIdx.x - p * (uint32_t)a.Hkv;
+    b = p / (uint32_t)per;
+    item = (int)(p - b * (uint32_t)per);
+  }
   b = longest_first(a, b);
   unit = b * (uint32_t)a.Hkv + hk;
   const Share s = share_of(a, (int64_t)b);  // (its lengths)
-  const int j0 = item * G::KEYS;
+  const int part = RW == 1 ? 0 : item % a.wsplits, j0 = (RW == 1 ? item : item / a.wsplits) * G::KEYS;
   if (j0 >= s.n || s.rows == 0) return;
   float* W = a.W + b * a.wb + hk * a.wh;
   if (s.rows <= a.sr) {
     const int k = j0 + (int)threadIdx.x;
-    if ((int)threadIdx.x < G::KEYS && k < s.n) W[k] += weight_of(a, s, unit, a.lse + (int64_t)unit * a.R, k);
+    if (part == 0 && (int)threadIdx.x < G::KEYS && k < s.n) W[k] += weight_of(a, s, unit, a.lse + (int64_t)unit * a.R, k);
     return;
   }
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
@@ -676,8 +690,13 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
     T::load(k, p, live && page != NO_PAGE, a.D, h);
   }
   const int before = s.n - s.m;  // token i sees keys up to before + i
-  const int first = j0 > before ? (j0 - before) * a.G / G::HR : 0;  // the first stage with a row that sees a key
-  const int stages = (s.rows + G::HR - 1) / G::HR;
+  int first = j0 > before ? (j0 - before) * a.G / G::HR : 0;  // the first stage with a row that sees a key
+  int stages = (s.rows + G::HR - 1) / G::HR;
+  if (RW > 1 && a.wsplits > 1) {
+    const int most = (stages - first + a.wsplits - 1) / a.wsplits;
+    first += part * most;
+    stages = stages < first + most ? stages : first + most;
+  }
   const int seen_by = (j > before ? j - before : 0) * a.G;          // the first row that sees this lane's key
   const int all_from = (k0 + 31 > before ? k0 + 31 - before : 0) * a.G;
   const char* Qh = a.Q.p + b * a.Q.b + hk * a.G * a.Q.h;
@@ -777,7 +796,23 @@ __global__ __launch_bounds__(256, (Weigh<T, RW>::LDS <= 72 * 1024 ? 2 : 1)) void
     const int l32 = lane & 31;
     total = (x[l32] + x[32 + l32]) + (x[64 + l32] + x[96 + l32]);
   }
-  if (live && h == 0) W[j] += total;
+  if (!live || h) return;
+  if (RW > 1 && a.wsplits > 1)
+    a.wpart[((int64_t)part * a.B * a.Hkv + unit) * a.wkeys + j] = total;
+  else
+    W[j] += total;
+}
+// The sums of the parts of the rows, `per` workgroups to a unit.
+__global__ __launch_bounds__(256) void add_kernel(const Args a, int per) {
+  const uint32_t unit = blockIdx.x / (uint32_t)per, at = blockIdx.x - unit * (uint32_t)per;
+  const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
+  const Share s = share_of(a, (int64_t)b);
+  const int j = (int)(at * 256 + threadIdx.x);
+  if (s.rows <= a.sr || j >= s.n) return;  // (up to sr rows have been added)
+  const float* p = a.wpart + (int64_t)unit * a.wkeys + j;
+  float sum = 0.f;
+  for (int i = 0; i < a.wsplits; ++i) sum += p[(int64_t)i * a.B * a.Hkv * a.wkeys];
+  a.W[b * a.wb + hk * a.wh + j] += sum;
 }
 
 // ------------------------------------------------------------------- host
@@ -786,7 +821,10 @@ struct Plan {
   bool narrow;
   int items, slots, least, step, slot_rows;
   int sr;
-  int64_t part, lse, scores;  // floats
+  bool again, few;  // weights from scores formed again, and by 32 keys to a workgroup
+  int wsplits;      // whose rows are taken in so many parts
+  int64_t part, lse, scores, wpart;  // floats
+  int64_t floats() const { return part + lse + scores + wpart; }
 };
 Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t keys, int64_t D, bool ragged, bool weights) {
   Plan p{};
@@ -821,6 +859,19 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   // sequences that have so few)
   p.sr = (int)(!weights || (p.narrow ? R > 16 : !ragged || (f32 && D > 64)) ? 0 : R < 16 ? R : 16);
   p.scores = units * ceil_div(keys, 32) * p.sr * 32;
+  p.again = weights && !(p.narrow && p.sr > 0);
+  // (9 units of 1008 keys and up to 399 rows in fp32: 28 us with 128 keys to a workgroup)
+  p.few = units * ceil_div(keys, 128) < 512;
+  p.wsplits = 1;
+  if (p.again && p.few) {
+    // 1024 workgroups, of which in a ragged batch most end at once, each with 32 stages of
+    // rows or more (4 sequences of two key heads, one of 10400 rows, 1300 keys: 96 us
+    // without parts, 30 and the addition's 5)
+    const int64_t n = ceil_div(ragged ? 4096 : 1024, units * ceil_div(keys > 0 ? keys : 1, 32)), most = ceil_div(R, 32) / 32;
+    p.wsplits = (int)(n < most ? n : most);
+    if (p.wsplits < 1) p.wsplits = 1;
+  }
+  p.wpart = p.wsplits > 1 ? p.wsplits * units * keys : 0;
   return p;
 }
 
@@ -835,7 +886,7 @@ extern "C" int64_t tsp_paged_attn_workspace_size(int dtype, int64_t B, int64_t H
   if (xat::check_sizes("tsp_paged_attn_workspace_size", dtype, B, Hq, Hkv, Sq, keys, D)) return -1;
   if (B * Hq * Sq == 0) return 0;
   const paged::Plan p = paged::plan_of(dtype, B, Hq, Hkv, Sq, keys, D, ragged != 0, weights != 0);
-  return 4 * (p.part + p.lse + p.scores);
+  return 4 * p.floats();
 }
 
 extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* K_pages, const int64_t* kps,
@@ -861,7 +912,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   if ((rc = paged::check_weights(who, weights, ws))) return rc;
   const bool weigh = weights && keys > 0;
   const paged::Plan p = paged::plan_of(dtype, B, Hq, Hkv, Sq, keys, D, new_lengths != nullptr, weigh);
-  const int64_t need = 4 * (p.part + p.lse + p.scores);
+  const int64_t need = 4 * p.floats();
   if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
   paged::Args a{};
   a.Q = xat::operand(Q, qs, Sq, D, dtype);
@@ -881,6 +932,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
     a.lse = (float*)workspace + p.part;
     a.scores = a.lse + p.lse;
     a.sr = p.sr;
+    a.wsplits = p.wsplits, a.wpart = a.scores + p.scores, a.wkeys = (int)keys;
     a.stages = (int)ceil_div(keys, 32);
     a.W = weights, a.wb = ws[0], a.wh = ws[1];
     // a stage of queries is read at 32-bit offsets from its first token
@@ -892,11 +944,8 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   // (where all workgroups start at once, dealing costs 1 us and gives nothing: 24
   // sequences of five tokens 34.7 and 36.7 us; 64 of one token 287 and 279)
   a.deal = B <= 64 && (new_lengths || units * p.items >= 512);
-  // (9 units of 1008 keys and up to 399 rows in fp32: 28 us with 128 keys to a workgroup)
-  const bool few = units * ceil_div(keys, 128) < 512;
-  const int64_t wper = ceil_div(keys, few ? 32 : 128);
-  const bool again = weigh && !(p.narrow && p.sr > 0);  // some scores are formed again
-  const int64_t wgrid = again ? head_grid(wper, units) : 0;
+  const int64_t wper = p.few ? ceil_div(keys, 32) * p.wsplits : ceil_div(keys, 128);
+  const int64_t wgrid = !p.again ? 0 : p.few ? wper * units : head_grid(wper, units), aper = ceil_div(keys, 256);
   const int64_t joined = p.narrow || (int64_t)(p.slots / 2) * paged::TILE > a.R ? a.R : (int64_t)(p.slots / 2) * paged::TILE;
   int64_t cper = p.slots > 1 ? ceil_div(joined, 8) : 0;
   if (!p.narrow && new_lengths && cper > ceil_div(2048, units)) cper = ceil_div(2048, units);  // (most have few rows)
@@ -904,7 +953,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   int64_t kper = ceil_div(2048, units);
   if (kper > ceil_div(keys, 1024)) kper = ceil_div(keys, 1024);
   if (kper < 1) kper = 1;
-  if (grid > INT32_MAX || wgrid > INT32_MAX || units * (cper + kper) > INT32_MAX)
+  if (grid > INT32_MAX || wgrid > INT32_MAX || units * (cper + kper) > INT32_MAX || units * aper > INT32_MAX)
     return fail(TSP_EUNSUPPORTED, "%s: too large a grid", who);
   return xat::with_tile(dtype, D, [&](auto tile) {
     typedef decltype(tile) T;
@@ -928,11 +977,13 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
       hipLaunchKernelGGL((paged::combine_kernel<T>), dim3((unsigned)(units * cper)), t, 0, st, a, (int)cper);
       if ((rc = check_launch("combine launch"))) return rc;
     }
-    if (again) {
-      if (few)
+    if (p.again) {
+      if (p.few)
         hipLaunchKernelGGL((paged::weights_kernel<T, 4>), dim3((unsigned)wgrid), t, 0, st, a, (int)wper);
       else
         hipLaunchKernelGGL((paged::weights_kernel<T, 1>), dim3((unsigned)wgrid), t, 0, st, a, (int)wper);
+      if ((rc = check_launch("weights launch")) || p.wsplits == 1) return rc;
+      hipLaunchKernelGGL(paged::add_kernel, dim3((unsigned)(units * aper)), t, 0, st, a, (int)aper);
       return check_launch("weights launch");
     }
     return TSP_OK;
