@@ -309,3 +309,19 @@ def test_weights_of_many_rows_and_few_keys(hip_backend, size, dt, mixed):
     lengths = torch.tensor([L, N - 7, L - 33], device="cuda")[:B]
     new = torch.tensor([N - 5, 1, 0] if B < 3 else [1, N - 3, 0], device="cuda")[:B] if mixed else None
     check(Q, kp, vp, table, lengths, new)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("size", [(4, 8, 1, 200, 80, 16, 64), (9, 4, 2, 130, 24, 64, 128), (33, 2, 1, 80, 40, 48, 40), (2, 12, 3, 70, 20, 128, 96)])
+def test_one_chunk_of_few_key_heads(hip_backend, size, dt):
+    """Its keys in as many ranges as fill the CUs; with several chunks, in fewer or none."""
+    Q, kp, vp, table = make(*size, dt, seed=7)
+    B, N, L = size[0], size[3], size[4] * size[5]
+    g = torch.Generator().manual_seed(8)
+    lengths = torch.randint(N, L + 1, (B,), generator=g).cuda()
+    lengths[B - 1] = L
+    for chunks in (1, (B + 1) // 2, B):
+        new = torch.ones(B, dtype=torch.int64, device="cuda")
+        new[B - chunks :] = N - torch.arange(chunks, device="cuda")
+        check(Q, kp, vp, table, lengths, new)
+        assert torch.equal(ts.paged_attention(Q, kp, vp, table, lengths, new), ts.paged_attention(Q, kp, vp, table, lengths, new))

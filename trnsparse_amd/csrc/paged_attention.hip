@@ -54,6 +54,8 @@ struct Args {
   int items;                 // workgroups of a unit at most
   int deal;                  // work goes to the launch's first workgroups, longest first (up to 64 sequences)
   int slots;                 // results of ranges that a unit has room for (0: keys stay whole)
+  int own;                   // of which it takes this many whatever the other sequences have
+  int places;                // and more as long as all units' tiles have this many workgroups (0: none)
   int least, step;           // a range's least keys, and what it is a multiple of
   int slot_rows;             // rows of one such result
   float *part, *plse;        // [unit][slot][row]: results, log-sum-exps (base 2)
@@ -74,8 +76,9 @@ constexpr int TILE = 128;  // rows of a wide workgroup (a narrow one has all of 
 struct Share {
   int n, m, rows, tiles, splits, chunk;
 };
-// What the workgroups of a unit of n cached and m new rows do.
-__device__ inline Share share_of(const Args& a, int n, int m) {
+// What the workgroups of a unit of n cached and m new rows do; its keys may be in `share` ranges
+// where there is room for them, and in more if a.own holds them.
+__device__ inline Share share_of(const Args& a, int n, int m, int share) {
   Share s;
   s.n = n;
   s.m = m;
@@ -83,7 +86,11 @@ __device__ inline Share share_of(const Args& a, int n, int m) {
   s.tiles = (s.rows + TILE - 1) / TILE;
   s.splits = 1;
   s.chunk = n > 0 ? n : 1;
-  int k = s.tiles && a.slots ? a.slots / s.tiles : 0;
+  int k = s.tiles ? a.own / s.tiles : 0;
+  if (share > 1 && s.tiles > 1) {
+    const int room = a.slots / s.tiles, more = share < room ? share : room;
+    k = k > more ? k : more;
+  }
   const int most = (n + a.least - 1) / a.least;
   k = k < most ? k : most;
   if (k > 1) {
@@ -92,8 +99,8 @@ __device__ inline Share share_of(const Args& a, int n, int m) {
   }
   return s;
 }
-__device__ inline Share share_of(const Args& a, int64_t b) {
-  return share_of(a, (int)cached_rows(a.len, b), (int)new_rows(a.len, b));
+__device__ inline Share share_of(const Args& a, int64_t b, int share = 1) {
+  return share_of(a, (int)cached_rows(a.len, b), (int)new_rows(a.len, b), share);
 }
 // A log-sum-exp (base 2) as the weights take it: of a row whose scores are all -inf,
 // whose result is zero, such that every weight 2^(score - it) is zero too.
@@ -128,6 +135,16 @@ __device__ inline Lane64 lane_lengths(const Args& a) {
   }
   return l;
 }
+// Ranges for the keys of every sequence such that all tiles have up to a.places workgroups
+// (of up to 64 sequences, each in a lane).
+__device__ inline int ranges_of(const Args& a, const Lane64& l) {
+  if (!a.places) return 1;
+  const int tiles = (l.m * a.G + TILE - 1) / TILE;
+  int total = 0;
+  for (int j = 0; j < a.B; ++j) total += __builtin_amdgcn_readlane(tiles, j);
+  const int64_t n = total > 0 ? a.places / ((int64_t)total * a.Hkv) : 1;
+  return n < 4 ? 1 : (int)n;  // (fewer cost more to join than they give: two of 54 tiles 69 us whole, 72)
+}
 // What a workgroup does: item `item` of the `wgs` that its unit has.
 struct Work {
   uint32_t unit, b, hk;
@@ -145,7 +162,8 @@ __device__ inline bool work_of(const Args& a, uint32_t block, Work& w) {
   // first of them takes. The longest go first.
   const int lane = threadIdx.x & 63;
   const Lane64 l = lane_lengths(a);
-  const Share v = share_of(a, l.n, l.m);
+  const int ranges = ranges_of(a, l);
+  const Share v = share_of(a, l.n, l.m, ranges);
   const int rest = (a.R - v.rows + 255) / 256;  // (rows to clear)
   int wgs = v.tiles * v.splits;
   wgs = lane < a.B ? (wgs > rest ? wgs : rest) : 0;
@@ -164,7 +182,7 @@ __device__ inline bool work_of(const Args& a, uint32_t block, Work& w) {
   w.unit = w.b * (uint32_t)a.Hkv + w.hk;
   w.item = p - __builtin_amdgcn_readlane(start, w.b);
   w.wgs = __builtin_amdgcn_readlane(wgs, w.b);
-  w.s = share_of(a, __builtin_amdgcn_readlane(l.n, w.b), __builtin_amdgcn_readlane(l.m, w.b));
+  w.s = share_of(a, __builtin_amdgcn_readlane(l.n, w.b), __builtin_amdgcn_readlane(l.m, w.b), ranges);
   return true;
 }
 // The sequence whose cache is the k-th longest (of up to 64, weighed with its new rows).
@@ -572,7 +590,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(const Args a, int per) {
   const uint32_t unit = blockIdx.x / (uint32_t)per, part = blockIdx.x - unit * (uint32_t)per;
   const uint32_t b = unit / (uint32_t)a.Hkv, hk = unit - b * (uint32_t)a.Hkv;
-  const Share s = share_of(a, (int64_t)b);
+  const Share s = share_of(a, (int64_t)b, a.places ? ranges_of(a, lane_lengths(a)) : 1);
   if (s.splits == 1) return;
   for (int r = (int)part * 8 + (int)(threadIdx.x >> 5); r < s.rows; r += 8 * per) {
     const float lse = combine_row<T>(a, s, unit, b, hk, r);
@@ -819,7 +837,7 @@ __global__ __launch_bounds__(256) void add_kernel(const Args a, int per) {
 
 struct Plan {
   bool narrow;
-  int items, slots, least, step, slot_rows;
+  int items, slots, own, places, least, step, slot_rows;
   int sr;
   bool again, few;  // weights from scores formed again, and by 32 keys to a workgroup
   int wsplits;      // whose rows are taken in so many parts
@@ -852,11 +870,27 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
     p.slots = (int)(p.items < more ? p.items : more);
     if (p.slots < 2) p.slots = 0;
   }
+  p.own = p.slots;
+  if (ragged && !p.narrow && B <= 64 && tiles > 1 && tiles * Hkv <= 64) {
+    // nor does a chunk of one sequence fill the CUs where key heads are few: as many ranges
+    // as do, as far as there is room for their results (one chunk of 512 tokens, 8 heads of
+    // one key head, next to 15 single tokens: 2048 keys 62 us and 40, 8192 keys 206 and 125;
+    // with up to 64 tiles of a sequence for all key heads, since finding the shares costs
+    // all workgroups: 16 sequences of 8 key heads and 16 tiles 187 us without, 190 with)
+    p.places = 512;
+    int64_t room = ceil_div(2048, units), use = tiles * (most < MOST_RANGES ? most : MOST_RANGES);
+    if (use > p.places / Hkv) use = p.places / Hkv;
+    if (room > use) room = use;
+    if (room > p.slots) p.slots = (int)room;
+    if (p.slots < 2) p.places = 0;
+  }
   auto pad = [](int64_t v) { return ceil_div(v, 64) * 64; };
   p.part = pad(p.slots * units * p.slot_rows * (D + 1));
   p.lse = weights ? pad(units * R) : 0;
   // scores of up to 16 rows are kept (with a chunk's workgroups, those of the
-  // sequences that have so few)
+  // sequences that have so few). 24 sequences of 4096 keys, 8 key heads of 128 in 16 bits:
+  // 20 rows 127 us kept and 129 formed again, 32 rows 170 and 130; fp32 is ahead up to
+  // 20 rows (16 sequences, head_dim 64: 80 and 92) and even at 32.
   p.sr = (int)(!weights || (p.narrow ? R > 16 : !ragged || (f32 && D > 64)) ? 0 : R < 16 ? R : 16);
   p.scores = units * ceil_div(keys, 32) * p.sr * 32;
   p.again = weights && !(p.narrow && p.sr > 0);
@@ -924,7 +958,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
   a.len = paged::Lengths{lengths, new_lengths, index_type == TSP_I64, keys, Sq};
   a.B = (int)B, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
-  a.items = p.items, a.slots = p.slots, a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
+  a.items = p.items, a.slots = p.slots, a.own = p.own, a.places = p.places, a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
   const int64_t units = B * Hkv;
   a.part = (float*)workspace;
   a.plse = a.part + p.slots * units * p.slot_rows * D;
@@ -940,7 +974,8 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
       return fail(TSP_EUNSUPPORTED, "%s: weights of query heads that lie 2 GiB apart", who);
   }
   a.scale_log2 = (float)(scale * 1.4426950408889634);
-  const int64_t grid = head_grid(p.items, units);
+  // (what the places are shared out to comes on top of a unit's own items)
+  const int64_t grid = p.places ? head_grid(B * p.items + p.places / Hkv, Hkv) : head_grid(p.items, units);
   // (where all workgroups start at once, dealing costs 1 us and gives nothing: 24
   // sequences of five tokens 34.7 and 36.7 us; 64 of one token 287 and 279)
   a.deal = B <= 64 && (new_lengths || units * p.items >= 512);
