@@ -538,7 +538,7 @@ bool by_parts(int64_t units, int64_t slots) { return units < 128 && slots > (3 +
 // none of less than 1024 places, where the chains of parts are too few to take the
 // memory's rate (64 with slices of 64 bytes) and long: copying rows aside is traffic
 // of its own. (8 units, head_dim 128 in 16 bits: 32768 places of 131072 rows 150 us,
-// in segments 57 and 24 to copy; 8192 of 16384: 47.6 us and 45.6 the whole eviction.
+// in segments 53 and 25 to copy; 8192 of 16384: 47.6 us and 45.6 the whole eviction.
 // 32 units, 8192 of 16384: 69 us, 104 in segments.)
 int segment_of(int64_t units, int64_t budget, int64_t row) {
   if (units * 2 * ceil_div(row, 64) > 64 || budget <= 8192) return 31;
