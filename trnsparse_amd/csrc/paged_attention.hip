@@ -181,7 +181,7 @@ __device__ inline bool work_of(const Args& a, uint32_t block, Work& w) {
     start += tj > time || (tj == time && j < lane) ? wj : 0;
   }
   int64_t hk, at;
-  if (!head_item(block, total, a.Hkv, hk, at)) return false;
+  if (!sorted_item(block, total, a.Hkv, hk, at)) return false;
   const int p = (int)at;
   w.b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__builtin_amdgcn_ballot_w64(start <= p && p < start + wgs)));
   w.hk = (uint32_t)hk;
