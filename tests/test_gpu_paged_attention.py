@@ -325,3 +325,18 @@ def test_one_chunk_of_few_key_heads(hip_backend, size, dt):
         new[B - chunks :] = N - torch.arange(chunks, device="cuda")
         check(Q, kp, vp, table, lengths, new)
         assert torch.equal(ts.paged_attention(Q, kp, vp, table, lengths, new), ts.paged_attention(Q, kp, vp, table, lengths, new))
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("B", [63, 64, 65, 130])
+@pytest.mark.parametrize("heads,N", [((4, 1), 70), ((6, 3), 12)])
+def test_batches_of_many_sequences(hip_backend, dt, B, heads, N):
+    """Chunks next to single tokens and to sequences of none, over caches in several ranges, on
+    both sides of the 64 sequences that a wavefront deals out (one to a lane)."""
+    Q, kp, vp, table = make(B, *heads, N, 70, 16, 64, dt, seed=15)
+    g = torch.Generator().manual_seed(16)
+    new = torch.ones(B, dtype=torch.int64)
+    new[::9], new[5::17], new[B - 1] = N, 0, N - 1
+    lengths = torch.randint(N, 1121, (B,), generator=g)
+    lengths[::9], lengths[3] = 1120 - torch.arange(len(lengths[::9])), 0
+    check(Q, kp, vp, table, lengths.cuda(), new.cuda())

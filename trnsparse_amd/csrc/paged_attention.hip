@@ -61,7 +61,7 @@ struct Args {
   int deal;                  // work goes to the launch's first workgroups, longest first (up to 64 sequences)
   int slots;                 // results of ranges that a unit has room for (0: keys stay whole)
   int own;                   // of which it takes this many whatever the other sequences have
-  int places;                // and more as long as all units' tiles have this many workgroups (0: none)
+  int places;                // and more as long as all tiles of a key head have this many workgroups (0: none)
   int least, step;           // a range's least keys, and what it is a multiple of
   int slot_rows;             // rows of one such result
   float *part, *plse;        // [unit][slot][row]: results, log-sum-exps (base 2)
@@ -145,10 +145,9 @@ __device__ inline Lane64 lane_lengths(const Args& a) {
 // (of up to 64 sequences, each in a lane).
 __device__ inline int ranges_of(const Args& a, const Lane64& l) {
   if (!a.places) return 1;
-  const int tiles = (l.m * a.G + TILE - 1) / TILE;
-  int total = 0;
-  for (int j = 0; j < a.B; ++j) total += __builtin_amdgcn_readlane(tiles, j);
-  const int64_t n = total > 0 ? a.places / ((int64_t)total * a.Hkv) : 1;
+  int total;
+  wave_scan((l.m * a.G + TILE - 1) / TILE, total);
+  const uint32_t n = total > 0 ? (uint32_t)a.places / (uint32_t)total : 1;
   return n < 4 ? 1 : (int)n;  // (fewer give less than joining them costs: 2 heads of 108 tiles 69 us whole, 72 in two)
 }
 // What a workgroup does: item `item` of the `wgs` that its unit has.
@@ -174,15 +173,18 @@ __device__ inline bool work_of(const Args& a, uint32_t block, Work& w) {
   int wgs = v.tiles * v.splits;
   wgs = lane < a.B ? (wgs > rest ? wgs : rest) : 0;
   const int keys = v.chunk < l.n ? v.chunk : l.n, time = v.rows > 32 ? 4 * keys : keys;
-  int total = 0, start = 0;
-  for (int j = 0; j < a.B; ++j) {
-    const int wj = __builtin_amdgcn_readlane(wgs, j), tj = __builtin_amdgcn_readlane(time, j);
-    total += wj;
-    start += tj > time || (tj == time && j < lane) ? wj : 0;
-  }
+  // Workgroups without work end before the places are found: they are most where a batch has
+  // many sequences and few chunks. (64 sequences, 4 chunks of 256 tokens, 16 heads over 4 of
+  // 128, up to 2048 keys: 105 us where all went through the loop over the sequences, 81 so.)
+  int total, start = 0;
+  wave_scan(wgs, total);
   int64_t hk, at;
   if (!sorted_item(block, total, a.Hkv, hk, at)) return false;
   const int p = (int)at;
+  for (int j = 0; j < a.B; ++j) {
+    const int wj = __builtin_amdgcn_readlane(wgs, j), tj = __builtin_amdgcn_readlane(time, j);
+    start += tj > time || (tj == time && j < lane) ? wj : 0;
+  }
   w.b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__builtin_amdgcn_ballot_w64(start <= p && p < start + wgs)));
   w.hk = (uint32_t)hk;
   w.unit = w.b * (uint32_t)a.Hkv + w.hk;
@@ -880,9 +882,10 @@ Plan plan_of(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t 
   if (ragged && !p.narrow && B <= 64 && tiles > 1 && tiles * Hkv <= 64) {
     // nor does a chunk of one sequence fill the CUs where key heads are few: as many ranges
     // as do, as far as there is room for their results (one chunk of 512 tokens, 8 heads of
-    // one key head, next to 15 single tokens: 2048 keys 62 us and 40, 8192 keys 206 and 125;
-    // with up to 64 tiles of a sequence for all key heads, since finding the shares costs
-    // all workgroups: 16 sequences of 8 key heads and 16 tiles 187 us without, 190 with)
+    // one key head, next to 15 single tokens: 2048 keys 59 us and 32, 8192 keys 197 and 70;
+    // with up to 64 tiles of a sequence for all key heads: 16 sequences of 8 key heads and 16
+    // tiles, four chunks, 142 us without and 144 with; 4 sequences of one key head, one chunk
+    // of 2000 tokens of 8 heads over 8192 keys, 144 without and 71 with)
     p.places = 512;
     int64_t room = ceil_div(2048, units), use = tiles * (most < MOST_RANGES ? most : MOST_RANGES);
     if (use > p.places / Hkv) use = p.places / Hkv;
@@ -964,7 +967,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
   a.len = paged::Lengths{lengths, new_lengths, index_type == TSP_I64, keys, Sq};
   a.B = (int)B, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
-  a.items = p.items, a.slots = p.slots, a.own = p.own, a.places = p.places, a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
+  a.items = p.items, a.slots = p.slots, a.own = p.own, a.places = (int)(p.places / Hkv), a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
   const int64_t units = B * Hkv;
   a.part = (float*)workspace;
   a.plse = a.part + p.slots * units * p.slot_rows * D;
@@ -982,8 +985,11 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   // (what the places are shared out to comes on top of a unit's own items)
   const int64_t grid = p.places ? head_grid(B * p.items + p.places / Hkv, Hkv) : head_grid(p.items, units);
-  // (where all workgroups start at once, dealing costs 1 us and gives nothing: 24
-  // sequences of five tokens 34.7 and 36.7 us; 64 of one token 287 and 279)
+  // (where all workgroups of tables that are filled alike start at once, dealing has no
+  // certain gain: one token, 32 heads over 8 of 128, not dealt and dealt, us: 4 sequences of
+  // up to 512 keys 9.0 and 9.5, 62 of 1024 36 and 40, of 4096 145 and 143, of 8192 286 and
+  // 275; 15 of 128 tokens over 2048 keys 68 and 62; 24 of five tokens, 32 heads over 4, 32
+  // and 33)
   a.deal = B <= 64 && (new_lengths || units * p.items >= 512);
   const int64_t wper = p.few ? ceil_div(keys, 32) * p.wsplits : ceil_div(keys, 128);
   const int64_t wgrid = !p.again ? 0 : p.few ? wper * units : head_grid(wper, units), aper = ceil_div(keys, 256);

@@ -1,5 +1,5 @@
 // A key and value cache in pages, as the kernels over it see it
-// (paged_attention.hip, paged_cache.hip).
+// (paged_attention.hip, paged_cache.hip, paged_evict.hip).
 //
 // K and V pages are (pages, kv_heads, page_size, head_dim); row j of sequence b
 // is row j % page_size of page table[b][j / page_size]. A table entry outside
@@ -76,6 +76,20 @@ __device__ inline uint32_t page_of_entry(const Table& t, u32x2 e) {
 }
 __device__ inline uint32_t page_of_lane(const Table& t, int64_t row, uint32_t col) {
   return page_of_entry(t, entry_of_lane(t, row, col));
+}
+
+// Sum over the lanes before this one, and the total of the wavefront: within rows of
+// 16 lanes by shifts, then the rows' totals to those behind them.
+__device__ inline int wave_scan(int v, int& total) {
+  int x = v;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row to the next row, rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+  total = __builtin_amdgcn_readlane(x, 63);
+  return x - v;
 }
 
 // ------------------------------------------------------------------- host

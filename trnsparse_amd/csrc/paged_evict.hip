@@ -57,20 +57,6 @@ __device__ inline uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the lanes before this one, and the total of the wavefront: within rows of
-// 16 lanes by shifts, then the rows' totals to those behind them.
-__device__ inline int wave_scan(int v, int& total) {
-  int x = v;
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row to the next row, rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
-  total = __builtin_amdgcn_readlane(x, 63);
-  return x - v;
-}
-
 // A thread's N rows of a part, consecutive ones of one page; rows from `end` on are not read.
 template <int N>
 struct Part {
