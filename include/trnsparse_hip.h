@@ -41,6 +41,7 @@ extern "C" {
 /* ---- index type codes (CSR) ------------------------------------------ */
 #define TSP_I32 0
 #define TSP_I64 1
+#define TSP_NEW_OTHER 2 /* a cache in pages: added where new_lengths are of the other type */
 
 /* Library version as 100*major + minor. */
 int tsp_version(void);
@@ -694,8 +695,9 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  * A page that is written (by an eviction: that holds rows of a cut sequence)
  * stands once in the table, and K_pages and V_pages do not overlap there: what
  * two writes to one row leave is not defined.
- * lengths and new_lengths (batch,) are of index_type and are taken into
- * [0, slots] and [0, queries or tokens]; new_lengths NULL: all. weights
+ * lengths and new_lengths (batch,) are of index_type (with TSP_NEW_OTHER added,
+ * new_lengths are of the other type) and are taken into [0, slots] and
+ * [0, queries or tokens]; new_lengths NULL: all. weights
  * (batch, kv_heads, slots) fp32, unit stride over slots; weight_strides: two
  * int64 in host memory, the strides of batch and head.
  * No counterpart in the reference, whose attention takes one sequence's K and

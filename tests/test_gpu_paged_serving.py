@@ -290,3 +290,33 @@ def test_public_refusal_of_gradients(hip_backend, host):
             with pytest.raises(RuntimeError, match=f"{name} has no gradients"):
                 call(a)
             assert all(torch.equal(a[m].detach(), s[m]) for m in ("kp", "vp", "w"))
+
+
+@pytest.mark.parametrize("types", [(torch.int32, torch.int64), (torch.int64, torch.int32), (torch.int64, torch.int64)])
+def test_lengths_past_32_bits(hip_backend, types):
+    """Lengths and numbers of new tokens are taken into their ranges as they are, whatever
+    the other's type: not by their low halves."""
+    far = [2**31, 2**32 + 1, 2**32, -(2**32) + 1, 2]
+    near = torch.tensor([3, 3, 3, 0, 2], device="cuda")
+    s = _state(18, F32, 3, cols=6, B=4)
+    g = torch.Generator(device="cuda").manual_seed(19)
+    q, k, v = rand(g, 5, H, 3, D), rand(g, 5, Hk, 3, D), rand(g, 5, Hk, 3, D)
+    table = torch.cat([s["table"][:3], s["table"][:2].flip(0)])
+    values = torch.tensor(far, device="cuda")
+    n = torch.tensor([70, 71, 72, 73, 74], device="cuda")
+    n64, n32 = (n, n.int())
+    lengths = n64 if types[0] == torch.int64 else n32
+    new = values if types[1] == torch.int64 else near.int()
+    want = ts.paged_attention(q, s["kp"], s["vp"], table, n64, near)
+    assert torch.equal(ts.paged_attention(q, s["kp"], s["vp"], table, lengths, new), want)
+    assert (want[3] == 0).all() and (want[4, :, 2] == 0).all() and (want[:3] != 0).any(-1).all()
+    table = s["table"][:, :5].reshape(5, 4)  # (every page once)
+    n = torch.tensor([40, 41, 42, 43, 44], device="cuda")
+    a, b = ([x.clone() for x in (s["kp"], s["vp"])] for _ in range(2))
+    after = ts.paged_cache_append(k, v, *a, table, n.to(types[0]), new)
+    assert after.dtype == types[0] and after.tolist() == [43, 44, 45, 43, 46]
+    ts.paged_cache_append(k, v, *b, table, n, near)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    if types[0] == torch.int64:  # lengths themselves past 32 bits: as many rows as there is room for, or none
+        n = torch.tensor([2**32 + 40, -(2**32) + 41, 42, 43, 44], device="cuda")
+        assert ts.paged_cache_append(k, v, *a, table, n, new).tolist() == [64, 3, 45, 43, 46]

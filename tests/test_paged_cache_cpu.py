@@ -265,3 +265,19 @@ def test_meta_shapes():
     for out in (ops.paged_append(m(2, 2, 5, 64), m(2, 2, 5, 64), kp, kp, t, n, None, None),
                 ops.paged_evict(kp, kp, m(2, 2, 64, dt=torch.float32), t, n, 8, 2)):
         assert out.shape == (2,) and out.dtype == torch.int32
+
+
+@built
+def test_c_abi_types_of_lengths():
+    """new_lengths may be of the other type than lengths; an eviction has none."""
+    import ctypes
+
+    lib, d, B = _lib.load(), 256, 0
+    s3, bf = (ctypes.c_int64 * 3)(2048, 1024, 64), _lib.TSP_BF16
+    for it, rc in ((0, 0), (1, 0), (2, 0), (3, 0), (4, -1), (9, -1), (-1, -1)):
+        assert lib.tsp_paged_attn_fwd(d, s3, d, s3, d, s3, bf, B, 2, 2, 1, 8, 16, 64, d, 1, 4, 4, d, d, it, 0.1, d, s3,
+                                      None, None, None, 0, None) == rc
+        assert lib.tsp_paged_append(d, s3, d, s3, d, s3, 4096, s3, bf, B, 2, 1, 8, 16, 64, d, 1, 4, 4, d, d, it, 512,
+                                    None, None, None) == rc
+        assert lib.tsp_paged_evict(d, s3, 4096, s3, bf, B, 2, 8, 16, 64, d, 1, 4, 4, d, it, d, s3, 8, 2, 512, None, 0,
+                                   None) == (rc if it < 2 else -1)

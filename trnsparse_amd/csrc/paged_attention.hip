@@ -133,11 +133,11 @@ __device__ inline Lane64 lane_lengths(const Args& a) {
   const int lane = threadIdx.x & 63;
   Lane64 l{0, 0};
   if (lane < a.B) {
-    const auto at = [&](const void* p) {
-      return a.len.wide ? ((const int64_t*)p)[lane] : (int64_t)((const int32_t*)p)[lane];
+    const auto at = [&](const void* p, int wide) {
+      return wide ? ((const int64_t*)p)[lane] : (int64_t)((const int32_t*)p)[lane];
     };
-    l.n = (int)clamped(at(a.len.p), a.len.slots);
-    l.m = (int)(a.len.fresh ? clamped(at(a.len.fresh), a.len.most) : a.len.most);
+    l.n = (int)clamped(at(a.len.p, a.len.wide), a.len.slots);
+    l.m = (int)(a.len.fresh ? clamped(at(a.len.fresh, a.len.fresh_wide), a.len.most) : a.len.most);
   }
   return l;
 }
@@ -945,7 +945,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   if (rc) return rc;
   const int64_t keys = cols * page_size;
   if ((rc = xat::check_sizes(who, dtype, B, Hq, Hkv, Sq, keys, D))) return rc;
-  if ((rc = paged::check_lengths(who, B, lengths, index_type))) return rc;
+  if ((rc = paged::check_lengths(who, B, lengths, index_type, true))) return rc;
   if (!(scale > 1e-30) || !(scale < 1e30)) return fail(TSP_EINVAL, "%s: scale must be positive", who);
   if (B * Hq * Sq == 0) return TSP_OK;
   if ((rc = xat::check_operand(who, "Q", Q, qs, Sq, D, dtype))) return rc;
@@ -965,7 +965,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   a.K = paged::pages_of(K_pages, kps, dtype);
   a.V = paged::pages_of(V_pages, vps, dtype);
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
-  a.len = paged::Lengths{lengths, new_lengths, index_type == TSP_I64, keys, Sq};
+  a.len = paged::lengths_of(lengths, new_lengths, index_type, keys, Sq);
   a.B = (int)B, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
   a.items = p.items, a.slots = p.slots, a.own = p.own, a.places = (int)(p.places / Hkv), a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
   const int64_t units = B * Hkv;

@@ -29,10 +29,11 @@ struct Pages {
   char* p;
   int64_t page, h, s;  // strides in bytes: page, head, row
 };
-// lengths of cached rows and of new ones (null: all of `most`) of each sequence
+// lengths of cached rows and of new ones (null: all of `most`) of each sequence, each of
+// int64 (`wide`) or int32
 struct Lengths {
   const void *p, *fresh;
-  int wide;
+  int wide, fresh_wide;
   int64_t slots, most;
 };
 
@@ -51,7 +52,7 @@ __device__ inline int64_t cached_rows(const Lengths& a, int64_t b) {
   return clamped(index_at(a.p, a.wide, b), a.slots);
 }
 __device__ inline int64_t new_rows(const Lengths& a, int64_t b) {
-  return a.fresh ? clamped(index_at(a.fresh, a.wide, b), a.most) : a.most;
+  return a.fresh ? clamped(index_at(a.fresh, a.fresh_wide, b), a.most) : a.most;
 }
 
 // The column of piece `i` (16 rows): i / (page_size / 16), by the reciprocal. Exact as
@@ -101,7 +102,7 @@ int check_cache(const char* who, int dtype, int64_t batch, int64_t kv_heads, int
                 int64_t head_dim, const void* table, int table_type, int64_t table_stride, int64_t columns);
 int check_pages(const char* who, const char* name, const void* p, const int64_t* strides, int dtype, int64_t pages,
                 int64_t head_dim);
-int check_lengths(const char* who, int64_t batch, const void* lengths, int index_type);
+int check_lengths(const char* who, int64_t batch, const void* lengths, int index_type, bool has_new);
 int check_weights(const char* who, const void* weights, const int64_t* strides);
 
 inline Table table_of(const void* table, int table_type, int64_t table_stride, int64_t columns, int64_t pages,
@@ -109,6 +110,10 @@ inline Table table_of(const void* table, int table_type, int64_t table_stride, i
   const uint64_t d = (uint64_t)(page_size / PIECE);
   return Table{table, table_stride, pages, table_type == TSP_I64, (int)columns, (int)page_size,
                ((uint64_t(1) << 32) + d - 1) / d};
+}
+inline Lengths lengths_of(const void* lengths, const void* fresh, int index_type, int64_t slots, int64_t most) {
+  const int wide = (index_type & ~TSP_NEW_OTHER) == TSP_I64;
+  return Lengths{lengths, fresh, wide, index_type & TSP_NEW_OTHER ? !wide : wide, slots, most};
 }
 inline Pages pages_of(const void* p, const int64_t* s, int dtype) {
   const int64_t e = esize(dtype);

@@ -41,8 +41,9 @@ int check_pages(const char* who, const char* name, const void* p, const int64_t*
   return TSP_OK;
 }
 
-int check_lengths(const char* who, int64_t B, const void* lengths, int index_type) {
-  if (index_type != TSP_I32 && index_type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
+int check_lengths(const char* who, int64_t B, const void* lengths, int index_type, bool has_new) {
+  const int type = has_new ? index_type & ~TSP_NEW_OTHER : index_type;
+  if (type != TSP_I32 && type != TSP_I64) return fail(TSP_EINVAL, "%s: bad index type", who);
   if (B > 0 && !lengths) return fail(TSP_EINVAL, "%s: null lengths", who);
   return TSP_OK;
 }
@@ -134,7 +135,7 @@ extern "C" int tsp_paged_append(const void* K, const int64_t* ks, const void* V,
   int rc = paged::check_cache(who, dtype, B, Hkv, pages, page_size, D, table, table_type, table_stride, cols);
   if (rc) return rc;
   if (N < 0 || N > (int64_t(1) << 30)) return fail(TSP_EINVAL, "%s: %lld tokens", who, (long long)N);
-  if ((rc = paged::check_lengths(who, B, lengths, index_type))) return rc;
+  if ((rc = paged::check_lengths(who, B, lengths, index_type, true))) return rc;
   if (B == 0) return TSP_OK;
   if (!lengths_out || lengths_out == lengths) return fail(TSP_EINVAL, "%s: lengths_out must be a place of its own", who);
   if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, D))) return rc;
@@ -157,7 +158,7 @@ extern "C" int tsp_paged_append(const void* K, const int64_t* ks, const void* V,
   a.Kp = paged::pages_of(K_pages, kps, dtype);
   a.Vp = paged::pages_of(V_pages, vps, dtype);
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
-  a.len = paged::Lengths{lengths, new_lengths, index_type == TSP_I64, cols * page_size, N};
+  a.len = paged::lengths_of(lengths, new_lengths, index_type, cols * page_size, N);
   a.out = lengths_out;
   a.W = weights;
   if (weights) a.wb = ws[0], a.wh = ws[1];

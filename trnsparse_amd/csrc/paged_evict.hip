@@ -575,7 +575,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   int rc = paged::check_cache(who, dtype, B, Hkv, pages, page_size, D, table, table_type, table_stride, cols);
   if (rc) return rc;
   if (recent < 0 || budget < recent) return fail(TSP_EINVAL, "%s: budget %lld, recent %lld", who, (long long)budget, (long long)recent);
-  if ((rc = paged::check_lengths(who, B, lengths, index_type))) return rc;
+  if ((rc = paged::check_lengths(who, B, lengths, index_type, false))) return rc;
   if (B == 0) return TSP_OK;
   const int64_t slots = cols * page_size;
   if (budget > slots) budget = slots;  // (nothing to evict: as for any budget that holds all)
@@ -593,7 +593,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   a.Kp = paged::pages_of(K_pages, kps, dtype);
   a.Vp = paged::pages_of(V_pages, vps, dtype);
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
-  a.len = paged::Lengths{lengths, nullptr, index_type == TSP_I64, slots, 0};
+  a.len = paged::lengths_of(lengths, nullptr, index_type, slots, 0);
   a.out = lengths_out;
   a.W = weights, a.wb = ws[0], a.wh = ws[1];
   a.units = units, a.Hkv = (int)Hkv, a.D = (int)D, a.esz = paged::esize(dtype);

@@ -749,9 +749,8 @@ struct PagedArgs {
     lens = lengths_of(lengths, "lengths", like, who, held[1]);
     icode = index_code(lengths.scalar_type());
     if (new_lengths.has_value()) {
-      index_code(new_lengths->scalar_type());
-      const bool one = new_lengths->scalar_type() == lengths.scalar_type();
-      fresh = lengths_of(one ? *new_lengths : new_lengths->to(lengths.scalar_type()), "new_lengths", like, who, held[2]);
+      fresh = lengths_of(*new_lengths, "new_lengths", like, who, held[2]);
+      if (index_code(new_lengths->scalar_type()) != icode) icode |= TSP_NEW_OTHER;
     }
   }
   const void* lengths_of(const at::Tensor& l, const char* name, const at::Tensor& like, const char* who, at::Tensor& kept) const {
