@@ -692,9 +692,10 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  * entries are of table_type (TSP_I32 or TSP_I64). slots = columns * page_size,
  * the rows a sequence may have, is at most 2^30, and slots * page_size below
  * 2^40. An entry outside [0, pages) is a page of zeros that cannot be written.
- * A page that is written (by an eviction: that holds rows of a cut sequence)
- * stands once in the table, and K_pages and V_pages do not overlap there: what
- * two writes to one row leave is not defined.
+ * Rows of what is written (K_pages, V_pages, weights) lie apart: strides under
+ * which they overlap are refused. A page that is written (by an eviction: that
+ * holds rows of a cut sequence) stands once in the table, and K_pages and
+ * V_pages do not overlap there: what two writes to one row leave is not defined.
  * lengths and new_lengths (batch,) are of index_type (with TSP_NEW_OTHER added,
  * new_lengths are of the other type) and are taken into [0, slots] and
  * [0, queries or tokens]; new_lengths NULL: all. weights

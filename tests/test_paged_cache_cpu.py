@@ -281,3 +281,93 @@ def test_c_abi_types_of_lengths():
                                     None, None, None) == rc
         assert lib.tsp_paged_evict(d, s3, 4096, s3, bf, B, 2, 8, 16, 64, d, 1, 4, 4, d, it, d, s3, 8, 2, 512, None, 0,
                                    None) == (rc if it < 2 else -1)
+
+
+def overlapping(dt=F64, dev="cpu"):
+    """Calls whose written pages or weights have rows that share memory, though no stride is zero."""
+    Q, K, V, kp, vp, t = (x.to(dev) for x in make(dt=dt))
+    n, w = torch.tensor([5, 6, 7], device=dev), torch.zeros(3, 2, 64, device=dev)
+    pool = torch.zeros(8192, dtype=dt, device=dev)
+    a, p, e = ts.paged_attention, ts.paged_cache_append, ts.paged_cache_evict
+    calls = []
+    for strides in ((256, 8, 8), (8, 128, 8), (128, 128, 8), (256, 120, 8), (256, 64, 16), (16, 8, 104)):
+        bad = pool.as_strided((13, 2, 16, 8), (*strides, 1))
+        calls += [(p, (K, V, bad, vp, t, n)), (p, (K, V, kp, bad, t, n)), (e, (bad, vp, w, t, n, 4)), (e, (kp, bad, w, t, n, 4))]
+    for strides in ((64, 64), (128, 1), (4, 128), (96, 64), (32, 64)):
+        bad = torch.zeros(512, device=dev).as_strided((3, 2, 64), (*strides, 1))
+        calls += [(a, (Q, kp, vp, t, n, None, 0.1, bad)), (p, (K, V, kp, vp, t, n, None, bad)), (e, (kp, vp, bad, t, n, 4))]
+    return calls
+
+
+@pytest.mark.parametrize("i", range(len(overlapping())))
+def test_written_rows_that_overlap_are_refused(pytorch_backend, i):
+    f, args = overlapping()[i]
+    with pytest.raises(RuntimeError, match="overlap"):
+        f(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(len(overlapping())))
+@pytest.mark.parametrize("dev", ["cuda", "cpu"])
+def test_written_rows_that_overlap_are_refused_on_the_gpu(hip_backend, i, dev):
+    f, args = overlapping(torch.float32, dev)[i]
+    # (the GPU's copy of a host view may have strides that are refused by another check)
+    with pytest.raises(RuntimeError, match="overlap|lie apart" if dev == "cuda" else "overlap|lie apart|unit stride"):
+        f(*args)
+
+
+def apart(dt=F64, dev="cpu"):
+    """Views of pages and weights whose rows lie apart, in any order of dimensions."""
+    _, _, _, kp, vp, _ = (x.to(dev) for x in make(dt=dt))
+    both, more = torch.stack([kp, vp], 1), torch.zeros(26, 4, 48, 24, dtype=dt, device=dev)
+    w = torch.zeros(3, 2, 64, device=dev)
+    turn = lambda x, *d: x.permute(*d).contiguous().permute(*(d.index(i) for i in range(len(d))))  # noqa: E731
+    pages = [(kp, vp), (turn(kp, 0, 2, 1, 3), turn(vp, 2, 0, 1, 3)), (turn(kp, 1, 2, 0, 3), turn(vp, 2, 1, 0, 3)),
+             (both[:, 0], both[:, 1]), (more[::2, 1::2, ::3, 8:16], more[1::2, ::2, 16:32, :8])]
+    weights = [w, turn(w, 1, 0, 2), torch.zeros(5, 4, 99, device=dev)[::2, 1::2, 5:69]]
+    return pages, weights
+
+
+def run_apart(dt, dev):
+    _, K, V, kp, vp, t = (x.to(dev) for x in make(dt=dt))
+    n, g = torch.tensor([5, 46, 61], device=dev), torch.Generator().manual_seed(4)
+    w0 = torch.rand(3, 2, 64, generator=g).to(dev)
+    first = layer.paged_append(K, V, kp, vp, t, n, None, w0)
+    want = layer.paged_evict(*first[:3], t, first[3], 20, 4)
+    pages, weights = apart(dt, dev)
+    for k, v in pages:
+        for w in weights:
+            k.copy_(kp), v.copy_(vp), w.copy_(w0)
+            after = ts.paged_cache_append(K, V, k, v, t, n, None, w)
+            assert all(torch.equal(x.cpu(), y) for x, y in zip((k, v, w, after), first))
+            after = ts.paged_cache_evict(k, v, w, t, after, 20, 4)
+            assert all(torch.equal(x.cpu(), y) for x, y in zip((k, v, w, after), want))
+
+
+def test_views_that_lie_apart(pytorch_backend):
+    run_apart(F64, "cpu")
+
+
+@pytest.mark.gpu
+def test_views_that_lie_apart_on_the_gpu(hip_backend):
+    run_apart(torch.float32, "cuda")
+
+
+@built
+def test_c_abi_written_rows_that_overlap():
+    import ctypes
+
+    lib = _lib.load()
+    st = lambda *v: (ctypes.c_int64 * len(v))(*v)  # noqa: E731
+    d, good, bf = 256, st(2048, 1024, 64), _lib.TSP_BF16
+    for bad in (st(2048, 64, 64), st(64, 1024, 64), st(2048, 1016, 64), st(1 << 62, 512, 64), st(2048, 512, 128)):
+        for k, v in ((bad, good), (good, bad)):
+            assert lib.tsp_paged_append(d, good, d, good, d, k, 4096, v, bf, 1, 2, 1, 8, 16, 64, d, 1, 4, 4, d, None, 1, 512,
+                                        None, None, None) == -1 and b"overlap" in lib.tsp_last_error()
+            assert lib.tsp_paged_evict(d, k, 4096, v, bf, 1, 2, 8, 16, 64, d, 1, 4, 4, d, 1, d, st(128, 64), 8, 2, 512, d,
+                                       1 << 40, None) == -1 and b"overlap" in lib.tsp_last_error()
+    for bad in (st(128, 63), st(64, 64), st(64, 1), st(1 << 62, 0)):
+        assert lib.tsp_paged_attn_fwd(d, good, d, good, d, good, bf, 2, 2, 2, 1, 8, 16, 64, d, 1, 4, 4, d, None, 1, 0.1, d,
+                                      good, d, bad, d, 1 << 40, None) == -1 and b"overlap" in lib.tsp_last_error()
+        assert lib.tsp_paged_evict(d, good, 4096, good, bf, 2, 2, 8, 16, 64, d, 1, 4, 4, d, 1, d, bad, 8, 2, 512, d, 1 << 40,
+                                   None) == -1 and b"overlap" in lib.tsp_last_error()

@@ -950,9 +950,9 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   if (B * Hq * Sq == 0) return TSP_OK;
   if ((rc = xat::check_operand(who, "Q", Q, qs, Sq, D, dtype))) return rc;
   if ((rc = xat::check_operand(who, "O", O, os, Sq, D, dtype))) return rc;
-  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, D))) return rc;
-  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, D))) return rc;
-  if ((rc = paged::check_weights(who, weights, ws))) return rc;
+  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, Hkv, page_size, D, false))) return rc;
+  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, Hkv, page_size, D, false))) return rc;
+  if ((rc = paged::check_weights(who, weights, ws, B, Hkv, keys))) return rc;
   const bool weigh = weights && keys > 0;
   const paged::Plan p = paged::plan_of(dtype, B, Hq, Hkv, Sq, keys, D, new_lengths != nullptr, weigh);
   const int64_t need = 4 * p.floats();

@@ -100,10 +100,12 @@ inline int esize(int dtype) { return dtype == TSP_F32 ? 4 : 2; }
 // Checks of a cache's sizes, pages and table; 0 or a status with a message.
 int check_cache(const char* who, int dtype, int64_t batch, int64_t kv_heads, int64_t pages, int64_t page_size,
                 int64_t head_dim, const void* table, int table_type, int64_t table_stride, int64_t columns);
+// (`written`: the kernels write them, so their rows may not overlap)
 int check_pages(const char* who, const char* name, const void* p, const int64_t* strides, int dtype, int64_t pages,
-                int64_t head_dim);
+                int64_t kv_heads, int64_t page_size, int64_t head_dim, bool written);
 int check_lengths(const char* who, int64_t batch, const void* lengths, int index_type, bool has_new);
-int check_weights(const char* who, const void* weights, const int64_t* strides);
+int check_weights(const char* who, const void* weights, const int64_t* strides, int64_t batch, int64_t kv_heads,
+                  int64_t slots);
 
 inline Table table_of(const void* table, int table_type, int64_t table_stride, int64_t columns, int64_t pages,
                       int64_t page_size) {

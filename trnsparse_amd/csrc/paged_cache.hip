@@ -28,7 +28,27 @@ int check_cache(const char* who, int dtype, int64_t B, int64_t Hkv, int64_t page
   return TSP_OK;
 }
 
-int check_pages(const char* who, const char* name, const void* p, const int64_t* s, int dtype, int64_t pages, int64_t D) {
+// Whether rows of `row` elements lie apart, `n` dimensions of them: each dimension's stride
+// passes the extent of those of smaller strides. (Rows that interleave in other ways without
+// an overlap are no views of a tensor by slices and transpositions.)
+static bool lie_apart(const int64_t* size, const int64_t* stride, int n, int64_t row) {
+  bool done[3] = {};
+  __int128 extent = row;
+  for (int k = 0; k < n; ++k) {
+    int at = -1;
+    for (int i = 0; i < n; ++i)
+      if (!done[i] && (at < 0 || stride[i] < stride[at])) at = i;
+    done[at] = true;
+    if (size[at] == 0) return true;
+    if (size[at] == 1) continue;
+    if (stride[at] < extent) return false;
+    extent += (__int128)stride[at] * (size[at] - 1);
+  }
+  return true;
+}
+
+int check_pages(const char* who, const char* name, const void* p, const int64_t* s, int dtype, int64_t pages, int64_t Hkv,
+                int64_t page_size, int64_t D, bool written) {
   if (!s) return fail(TSP_EINVAL, "%s: no strides of %s", who, name);
   if (pages == 0) return TSP_OK;
   if (!p) return fail(TSP_EINVAL, "%s: null %s", who, name);
@@ -38,6 +58,10 @@ int check_pages(const char* who, const char* name, const void* p, const int64_t*
   if (s[0] < 0 || s[1] < 0 || s[2] < D || s[2] * e >= (int64_t(1) << 24))
     return fail(TSP_EINVAL, "%s: strides of %s: %lld, %lld, %lld", who, name, (long long)s[0], (long long)s[1],
                 (long long)s[2]);
+  const int64_t size[3] = {pages, Hkv, page_size};
+  if (written && !lie_apart(size, s, 3, D))
+    return fail(TSP_EINVAL, "%s: rows of %s, which are written, overlap: strides %lld, %lld, %lld", who, name,
+                (long long)s[0], (long long)s[1], (long long)s[2]);
   return TSP_OK;
 }
 
@@ -48,10 +72,14 @@ int check_lengths(const char* who, int64_t B, const void* lengths, int index_typ
   return TSP_OK;
 }
 
-int check_weights(const char* who, const void* w, const int64_t* s) {
+int check_weights(const char* who, const void* w, const int64_t* s, int64_t B, int64_t Hkv, int64_t slots) {
   if (!w) return TSP_OK;
   if (!s) return fail(TSP_EINVAL, "%s: no strides of weights", who);
   if (((uintptr_t)w & 3) || s[0] < 0 || s[1] < 0) return fail(TSP_EINVAL, "%s: bad weights", who);
+  const int64_t size[2] = {B, Hkv};
+  if (!lie_apart(size, s, 2, slots))
+    return fail(TSP_EINVAL, "%s: rows of weights, which are written, overlap: strides %lld, %lld", who, (long long)s[0],
+                (long long)s[1]);
   return TSP_OK;
 }
 
@@ -138,9 +166,9 @@ extern "C" int tsp_paged_append(const void* K, const int64_t* ks, const void* V,
   if ((rc = paged::check_lengths(who, B, lengths, index_type, true))) return rc;
   if (B == 0) return TSP_OK;
   if (!lengths_out || lengths_out == lengths) return fail(TSP_EINVAL, "%s: lengths_out must be a place of its own", who);
-  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, D))) return rc;
-  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, D))) return rc;
-  if ((rc = paged::check_weights(who, weights, ws))) return rc;
+  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, Hkv, page_size, D, true))) return rc;
+  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, Hkv, page_size, D, true))) return rc;
+  if ((rc = paged::check_weights(who, weights, ws, B, Hkv, cols * page_size))) return rc;
   const int64_t e = paged::esize(dtype);
   const int64_t* st[2] = {ks, vs};
   const void* pt[2] = {K, V};

@@ -582,9 +582,9 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   if (recent > budget) recent = budget;
   if (!lengths_out || lengths_out == lengths) return fail(TSP_EINVAL, "%s: lengths_out must be a place of its own", who);
   if (!weights) return fail(TSP_EINVAL, "%s: null weights", who);
-  if ((rc = paged::check_weights(who, weights, ws))) return rc;
-  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, D))) return rc;
-  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, D))) return rc;
+  if ((rc = paged::check_weights(who, weights, ws, B, Hkv, slots))) return rc;
+  if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, Hkv, page_size, D, true))) return rc;
+  if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, Hkv, page_size, D, true))) return rc;
   if (pages > 0 && K_pages == V_pages) return fail(TSP_EINVAL, "%s: K_pages and V_pages are the same", who);
   const int64_t units = B * Hkv, row = D * paged::esize(dtype);
   const paged::Space sp = paged::space_of(units, slots, budget, row);

@@ -971,6 +971,10 @@ def hip_shared_prefix_attention(Q, prefix_K, prefix_V, K, V, lengths, scale: flo
 
 def _back(written, given):
     """Copies what was written on the GPU back to operands elsewhere."""
+    from ..ops import _apart
+
+    if not all(w is g or _apart(g) for w, g in zip(written, given)):
+        raise RuntimeError("rows of pages or weights, which are written, overlap")
     for w, g in zip(written, given):
         if w is not g:
             g.copy_(w)

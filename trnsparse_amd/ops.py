@@ -683,9 +683,21 @@ def _no_gradients(who: str, *tensors) -> None:
         raise RuntimeError(f"{who} has no gradients: call it under torch.no_grad()")
 
 
-def _check_cache(who: str, K_pages, V_pages, block_table, lengths, new_lengths, weights) -> None:
-    """Shapes and types of a paged cache. The HIP operators refuse the same
-    calls themselves (csrc/torch_ops.cpp)."""
+def _apart(t) -> bool:
+    """Whether no two elements of a view share memory: every dimension's stride passes the
+    extent of those of smaller strides."""
+    extent = 1
+    for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+        if stride < extent:
+            return False
+        extent += stride * (size - 1)
+    return True
+
+
+def _check_cache(who: str, K_pages, V_pages, block_table, lengths, new_lengths, weights, written=()) -> None:
+    """Shapes and types of a paged cache, and that the rows of what is `written` lie
+    apart. The HIP operators refuse the same calls themselves (csrc/torch_ops.cpp,
+    csrc/paged_cache.hip)."""
     k, dt = K_pages.shape, K_pages.dtype
     if len(k) != 4 or V_pages.shape != k or V_pages.dtype != dt or not dt.is_floating_point:
         raise RuntimeError(f"{who}: K_pages {tuple(k)} of {dt} and V_pages {tuple(V_pages.shape)} of {V_pages.dtype} must "
@@ -704,6 +716,8 @@ def _check_cache(who: str, K_pages, V_pages, block_table, lengths, new_lengths, 
     if weights is not None and (weights.shape != (B, k[1], cols * k[2]) or weights.dtype != torch.float32):
         raise RuntimeError(f"{who}: weights must be ({B}, {k[1]}, {cols * k[2]}) of float32, got {tuple(weights.shape)} of "
                            f"{weights.dtype}")
+    if any(t is not None and t.numel() and not _apart(t) for t in written):
+        raise RuntimeError(f"{who}: rows of pages or weights, which are written, overlap")
 
 
 def _page_rows(K_pages, block_table, slots):
@@ -767,7 +781,7 @@ def paged_attention(
     if _use_hip():
         return _hip().hip_paged_attention(Q, K_pages, V_pages, block_table, lengths, new_lengths, scale, weights)
     _no_gradients(who, Q, K_pages, V_pages, weights)
-    _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+    _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights, (weights,))
     B, cols = block_table.shape
     _, Hk, size, D = K_pages.shape
     if Q.dim() != 4 or Q.shape[0] != B or Q.shape[3] != D or Q.shape[1] % Hk or Q.dtype != K_pages.dtype:
@@ -818,7 +832,7 @@ def paged_cache_append(
     if _use_hip():
         return _hip().hip_paged_cache_append(K, V, K_pages, V_pages, block_table, lengths, new_lengths, weights)
     _no_gradients(who, K, V, K_pages, V_pages, weights)
-    _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights)
+    _check_cache(who, K_pages, V_pages, block_table, lengths, new_lengths, weights, (K_pages, V_pages, weights))
     B, cols = block_table.shape
     _, Hk, size, D = K_pages.shape
     if K.dim() != 4 or K.shape != V.shape or (K.shape[0], K.shape[1], K.shape[3]) != (B, Hk, D):
@@ -868,7 +882,7 @@ def paged_cache_evict(
     if _use_hip():
         return _hip().hip_paged_cache_evict(K_pages, V_pages, weights, block_table, lengths, budget, recent)
     _no_gradients(who, K_pages, V_pages, weights)
-    _check_cache(who, K_pages, V_pages, block_table, lengths, None, weights)
+    _check_cache(who, K_pages, V_pages, block_table, lengths, None, weights, (K_pages, V_pages, weights))
     if not 0 <= recent <= budget:
         raise RuntimeError(f"{who}: recent {recent} is not in 0 .. budget {budget}")
     if K_pages.numel() and K_pages.data_ptr() == V_pages.data_ptr():
