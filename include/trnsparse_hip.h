@@ -719,6 +719,7 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  *   head_dim), i < new_lengths[b], become row lengths[b] + i; rows past slots
  *   are left out. weights, where not NULL, is set to zero there. lengths_out
  *   (batch,), not lengths itself, receives min(lengths[b] + new_lengths[b], slots).
+ *   K and V do not overlap K_pages and V_pages.
  *
  * tsp_paged_evict: a sequence of more than `budget` rows keeps, for each key
  *   head, its last `recent` rows (0 <= recent <= budget) and of the others the

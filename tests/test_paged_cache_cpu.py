@@ -371,3 +371,35 @@ def test_c_abi_written_rows_that_overlap():
                                       good, d, bad, d, 1 << 40, None) == -1 and b"overlap" in lib.tsp_last_error()
         assert lib.tsp_paged_evict(d, good, 4096, good, bf, 2, 2, 8, 16, 64, d, 1, 4, 4, d, 1, d, bad, 8, 2, 512, d, 1 << 40,
                                    None) == -1 and b"overlap" in lib.tsp_last_error()
+
+
+def run_append_of_cached_rows(dt, dev):
+    """New rows that are views of the pages: of rows that other sequences, other heads or the
+    other cache's rows overwrite, and of the very rows that they move by one."""
+    _, _, _, kp, vp, t = make(B=3, N=1, cols=4, dt=dt, seed=21)
+    n = torch.tensor([3, 20, 33])
+    order = t[:, 0].tolist()
+    for new in (None, torch.tensor([9, 2, 0])):
+        for sources in (lambda k, v: (k[t[0, 0]][None], v[t[0, 0]][None]), lambda k, v: (v[t[1, 1]][None], k[t[0, 0]][None]),
+                        lambda k, v: (k[order[0]][None], k[order[0]][None])):
+            k, v, table = kp.clone().to(dev), vp.clone().to(dev), t.to(dev)
+            a, b = (x.expand(3, -1, -1, -1)[:, :, :12] for x in sources(k, v))
+            want = layer.paged_append(a.cpu().clone(), b.cpu().clone(), kp, vp, t, n, new)
+            after = ts.paged_cache_append(a, b, k, v, table, n.to(dev), None if new is None else new.to(dev))
+            assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1]) and torch.equal(after.cpu(), want[3])
+        k, v = kp.clone().to(dev), vp.clone().to(dev)  # one pool of pages, whose first one's rows go to another
+        pool = torch.stack([k, v], 1)
+        a, b = pool[:3, 0, :, 2:14], pool[:3, 1, :, 2:14]
+        want = layer.paged_append(a.cpu().clone(), b.cpu().clone(), kp, vp, t, n, new)
+        after = ts.paged_cache_append(a, b, pool[:, 0], pool[:, 1], t.to(dev), n.to(dev), None if new is None else new.to(dev))
+        assert torch.equal(pool[:, 0].cpu(), want[0]) and torch.equal(pool[:, 1].cpu(), want[1])
+
+
+def test_append_of_cached_rows(pytorch_backend):
+    run_append_of_cached_rows(F64, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dev", ["cuda", "cpu"])
+def test_append_of_cached_rows_on_the_gpu(hip_backend, dev):
+    run_append_of_cached_rows(torch.float32, dev)

@@ -813,6 +813,20 @@ at::Tensor paged_attn_fwd_meta(const at::Tensor& Q, const at::Tensor&, const at:
   return attn_like(Q, Q.size(3));
 }
 
+// t, or a copy of it where it may share bytes with a tensor that is written (by the spans of both).
+at::Tensor apart_from(const at::Tensor& t, std::initializer_list<const at::Tensor*> written) {
+  const auto end_of = [](const at::Tensor& x) {
+    int64_t last = 1;
+    for (int64_t i = 0; i < x.dim(); ++i) last += (x.size(i) - 1) * x.stride(i);
+    return (const char*)x.data_ptr() + last * x.element_size();
+  };
+  if (t.numel() == 0) return t;
+  for (const at::Tensor* w : written)
+    if (w->numel() > 0 && (const char*)t.data_ptr() < end_of(*w) && (const char*)w->data_ptr() < end_of(t))
+      return t.clone(at::MemoryFormat::Contiguous);
+  return t;
+}
+
 at::Tensor paged_append(const at::Tensor& K_, const at::Tensor& V_, const at::Tensor& Kp, const at::Tensor& Vp,
                         const at::Tensor& table, const at::Tensor& lengths, const c10::optional<at::Tensor>& new_lengths,
                         const c10::optional<at::Tensor>& weights) {
@@ -825,7 +839,8 @@ at::Tensor paged_append(const at::Tensor& K_, const at::Tensor& V_, const at::Te
               V_.sizes(), ", K_pages ", Kp.sizes(), " and block_table ", table.sizes(), " do not belong together");
   int64_t ws2[2];
   if (weights.has_value()) need_weights(*weights, p, Kp, who, ws2);
-  const auto K = attn_operand(K_), V = attn_operand(V_);
+  // (new rows that stand in the pages are read before any are written)
+  const auto K = apart_from(attn_operand(K_), {&Kp, &Vp}), V = apart_from(attn_operand(V_), {&Kp, &Vp});
   auto out = at::empty({p.B}, lengths.options());
   written({&Kp, &Vp});
   if (weights.has_value()) written({&*weights});

@@ -824,8 +824,9 @@ def paged_cache_append(
     K, V (batch, kv_heads, tokens, head_dim) in the pages' dtype, strided views
     allowed: row i < new_lengths[b] (None: all) becomes row lengths[b] + i of
     sequence b. Rows past the table's columns, or in a page that is not there,
-    are left out. `weights` (batch, kv_heads, slots), where given, is set to
-    zero at the new rows. A page that is written stands once in block_table, and
+    are left out. K and V may be rows of the pages themselves: they are read before
+    any is written. `weights` (batch, kv_heads, slots), where given, is set to zero at
+    the new rows. A page that is written stands once in block_table, and
     K_pages and V_pages lie apart.
     """
     who = "paged_cache_append"
@@ -844,6 +845,8 @@ def paged_cache_append(
     N, L, dev = K.shape[2], cols * size, K_pages.device
     n = lengths.to(dev).long().clamp(0, L)
     m = torch.full_like(n, N) if new_lengths is None else new_lengths.to(dev).long().clamp(0, N)
+    held = [p.untyped_storage().data_ptr() for p in (K_pages, V_pages)]
+    K, V = (t.clone() if t.untyped_storage().data_ptr() in held else t for t in (K, V))
     for b in range(B):
         new = min(int(m[b]), L - int(n[b]))
         if new <= 0:
