@@ -712,8 +712,8 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  *   are zero. With weights not NULL, weights[b,hk,j] += the softmax weight of
  *   key j, summed over the key head's query heads and the queries. Strides,
  *   alignment and scale of Q and O as in tsp_cross_attn_fwd. workspace:
- *   tsp_paged_attn_workspace_size bytes, `keys` being slots, `ragged` whether
- *   new_lengths is given and `weights` whether weights is.
+ *   tsp_paged_attn_workspace_size bytes, 16-byte aligned, `keys` being slots,
+ *   `ragged` whether new_lengths is given and `weights` whether weights is.
  *
  * tsp_paged_append: K[b, :, i] and V[b, :, i] of (batch, kv_heads, tokens,
  *   head_dim), i < new_lengths[b], become row lengths[b] + i; rows past slots

@@ -403,3 +403,18 @@ def test_append_of_cached_rows(pytorch_backend):
 @pytest.mark.parametrize("dev", ["cuda", "cpu"])
 def test_append_of_cached_rows_on_the_gpu(hip_backend, dev):
     run_append_of_cached_rows(torch.float32, dev)
+
+
+@built
+def test_c_abi_workspaces_are_aligned():
+    """Results of ranges and scores are read 16 bytes at a time."""
+    import ctypes
+
+    lib, d = _lib.load(), 256
+    s3, w2, bf = (ctypes.c_int64 * 3)(2048, 1024, 64), (ctypes.c_int64 * 2)(65536, 32768), _lib.TSP_BF16
+    for ws in (260, 264, 258):
+        for w in (None, d):
+            assert lib.tsp_paged_attn_fwd(d, s3, d, s3, d, s3, bf, 1, 2, 2, 1, 8, 16, 64, d, 1, 2048, 2048, d, None, 1, 0.1, d,
+                                          s3, w, w2, ws, 1 << 40, None) == -1 and b"aligned" in lib.tsp_last_error()
+        assert lib.tsp_paged_evict(d, s3, 4096, s3, bf, 1, 2, 8, 16, 64, d, 1, 2048, 2048, d, 1, d, w2, 8, 2, 512, ws, 1 << 40,
+                                   None) == -1 and b"aligned" in lib.tsp_last_error()

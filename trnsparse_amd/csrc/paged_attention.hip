@@ -956,7 +956,8 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   const bool weigh = weights && keys > 0;
   const paged::Plan p = paged::plan_of(dtype, B, Hq, Hkv, Sq, keys, D, new_lengths != nullptr, weigh);
   const int64_t need = 4 * p.floats();
-  if (need > 0 && (!workspace || workspace_bytes < need)) return fail(TSP_EINVAL, "%s: workspace too small", who);
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+    return fail(TSP_EINVAL, "%s: workspace too small or not 16-byte aligned", who);
   paged::Args a{};
   a.Q = xat::operand(Q, qs, Sq, D, dtype);
   const xat::Operand o = xat::operand(O, os, Sq, D, dtype);

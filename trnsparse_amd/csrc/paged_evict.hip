@@ -588,7 +588,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   if (pages > 0 && K_pages == V_pages) return fail(TSP_EINVAL, "%s: K_pages and V_pages are the same", who);
   const int64_t units = B * Hkv, row = D * paged::esize(dtype);
   const paged::Space sp = paged::space_of(units, slots, budget, row);
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < sp.end) return fail(TSP_EINVAL, "%s: workspace too small", who);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < sp.end) return fail(TSP_EINVAL, "%s: workspace too small or not 16-byte aligned", who);
   paged::EvictArgs a{};
   a.Kp = paged::pages_of(K_pages, kps, dtype);
   a.Vp = paged::pages_of(V_pages, vps, dtype);
