@@ -718,15 +718,16 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  * tsp_paged_append: K[b, :, i] and V[b, :, i] of (batch, kv_heads, tokens,
  *   head_dim), i < new_lengths[b], become row lengths[b] + i; rows past slots
  *   are left out. weights, where not NULL, is set to zero there. lengths_out
- *   (batch,), not lengths itself, receives min(lengths[b] + new_lengths[b], slots).
+ *   (batch,), of lengths' type and apart from lengths and new_lengths, receives
+ *   min(lengths[b] + new_lengths[b], slots).
  *   K and V do not overlap K_pages and V_pages.
  *
  * tsp_paged_evict: a sequence of more than `budget` rows keeps, for each key
  *   head, its last `recent` rows (0 <= recent <= budget) and of the others the
  *   budget - recent of the largest weights: of equal ones the first, NaN above
  *   all numbers. The kept rows of K, V and weights move to rows [0, budget) in
- *   their order; what stands behind is left as it was. lengths_out, not lengths
- *   itself, receives min(lengths[b], budget). workspace:
+ *   their order; what stands behind is left as it was. lengths_out, of lengths'
+ *   type and apart from them, receives min(lengths[b], budget). workspace:
  *   tsp_paged_evict_workspace_size bytes, 16-byte aligned.
  * ==================================================================== */
 int64_t tsp_paged_attn_workspace_size(int dtype, int64_t batch, int64_t heads,

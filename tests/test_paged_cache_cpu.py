@@ -418,3 +418,25 @@ def test_c_abi_workspaces_are_aligned():
                                           s3, w, w2, ws, 1 << 40, None) == -1 and b"aligned" in lib.tsp_last_error()
         assert lib.tsp_paged_evict(d, s3, 4096, s3, bf, 1, 2, 8, 16, 64, d, 1, 2048, 2048, d, 1, d, w2, 8, 2, 512, ws, 1 << 40,
                                    None) == -1 and b"aligned" in lib.tsp_last_error()
+
+
+@built
+@pytest.mark.parametrize("it", [0, 1, 2, 3])
+def test_c_abi_lengths_out_is_apart(it):
+    """It is written while other workgroups of the sequence still read lengths and new_lengths."""
+    import ctypes
+
+    lib, d, n, new, B = _lib.load(), 256, 4096, 8192, 3
+    s3, w2, bf = (ctypes.c_int64 * 3)(2048, 1024, 64), (ctypes.c_int64 * 2)(128, 64), _lib.TSP_BF16
+    out = 8 if it & 1 else 4
+    held = (out, 12 - out if it & 2 else out)
+    for p, size in ((n, held[0]), (new, held[1])):
+        for at in (p, p + size, p + (B - 1) * size, p + B * size - 4, p - (B - 1) * out, p - 4):
+            assert lib.tsp_paged_append(d, s3, d, s3, d, s3, 512, s3, bf, B, 2, 1, 8, 16, 64, d, 1, 4, 4, n, new, it, at,
+                                        None, None, None) == -1 and b"lengths_out" in lib.tsp_last_error(), (p, at)
+            if p == n and it < 2:
+                assert lib.tsp_paged_evict(d, s3, 512, s3, bf, B, 2, 8, 16, 64, d, 1, 4, 4, n, it, d, w2, 8, 2, at, d, 1 << 40,
+                                           None) == -1 and b"lengths_out" in lib.tsp_last_error(), at
+        for at in (p + B * size, p - B * out):  # (the next check's message)
+            assert lib.tsp_paged_append(d, s3, d, s3, None, s3, 512, s3, bf, B, 2, 1, 8, 16, 64, d, 1, 4, 4, n, new, it, at,
+                                        None, None, None) == -1 and b"null K_pages" in lib.tsp_last_error(), (p, at)

@@ -104,6 +104,7 @@ int check_cache(const char* who, int dtype, int64_t batch, int64_t kv_heads, int
 int check_pages(const char* who, const char* name, const void* p, const int64_t* strides, int dtype, int64_t pages,
                 int64_t kv_heads, int64_t page_size, int64_t head_dim, bool written);
 int check_lengths(const char* who, int64_t batch, const void* lengths, int index_type, bool has_new);
+int check_lengths_out(const char* who, int64_t batch, const void* out, const Lengths& l);
 int check_weights(const char* who, const void* weights, const int64_t* strides, int64_t batch, int64_t kv_heads,
                   int64_t slots);
 

@@ -72,6 +72,17 @@ int check_lengths(const char* who, int64_t B, const void* lengths, int index_typ
   return TSP_OK;
 }
 
+// Workgroups of a sequence read its lengths while another writes the one after.
+int check_lengths_out(const char* who, int64_t B, const void* out, const Lengths& l) {
+  const auto meets = [&](const void* p, int wide) {
+    const char *a = (const char*)out, *b = (const char*)p;
+    return p && a < b + B * (wide ? 8 : 4) && b < a + B * (l.wide ? 8 : 4);
+  };
+  if (!out || meets(l.p, l.wide) || meets(l.fresh, l.fresh_wide))
+    return fail(TSP_EINVAL, "%s: lengths_out must be a place of its own", who);
+  return TSP_OK;
+}
+
 int check_weights(const char* who, const void* w, const int64_t* s, int64_t B, int64_t Hkv, int64_t slots) {
   if (!w) return TSP_OK;
   if (!s) return fail(TSP_EINVAL, "%s: no strides of weights", who);
@@ -165,7 +176,8 @@ extern "C" int tsp_paged_append(const void* K, const int64_t* ks, const void* V,
   if (N < 0 || N > (int64_t(1) << 30)) return fail(TSP_EINVAL, "%s: %lld tokens", who, (long long)N);
   if ((rc = paged::check_lengths(who, B, lengths, index_type, true))) return rc;
   if (B == 0) return TSP_OK;
-  if (!lengths_out || lengths_out == lengths) return fail(TSP_EINVAL, "%s: lengths_out must be a place of its own", who);
+  const paged::Lengths len = paged::lengths_of(lengths, new_lengths, index_type, cols * page_size, N);
+  if ((rc = paged::check_lengths_out(who, B, lengths_out, len))) return rc;
   if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, Hkv, page_size, D, true))) return rc;
   if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, Hkv, page_size, D, true))) return rc;
   if ((rc = paged::check_weights(who, weights, ws, B, Hkv, cols * page_size))) return rc;
@@ -186,7 +198,7 @@ extern "C" int tsp_paged_append(const void* K, const int64_t* ks, const void* V,
   a.Kp = paged::pages_of(K_pages, kps, dtype);
   a.Vp = paged::pages_of(V_pages, vps, dtype);
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
-  a.len = paged::lengths_of(lengths, new_lengths, index_type, cols * page_size, N);
+  a.len = len;
   a.out = lengths_out;
   a.W = weights;
   if (weights) a.wb = ws[0], a.wh = ws[1];

@@ -580,7 +580,8 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   const int64_t slots = cols * page_size;
   if (budget > slots) budget = slots;  // (nothing to evict: as for any budget that holds all)
   if (recent > budget) recent = budget;
-  if (!lengths_out || lengths_out == lengths) return fail(TSP_EINVAL, "%s: lengths_out must be a place of its own", who);
+  const paged::Lengths len = paged::lengths_of(lengths, nullptr, index_type, slots, 0);
+  if ((rc = paged::check_lengths_out(who, B, lengths_out, len))) return rc;
   if (!weights) return fail(TSP_EINVAL, "%s: null weights", who);
   if ((rc = paged::check_weights(who, weights, ws, B, Hkv, slots))) return rc;
   if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, Hkv, page_size, D, true))) return rc;
@@ -593,7 +594,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   a.Kp = paged::pages_of(K_pages, kps, dtype);
   a.Vp = paged::pages_of(V_pages, vps, dtype);
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
-  a.len = paged::lengths_of(lengths, nullptr, index_type, slots, 0);
+  a.len = len;
   a.out = lengths_out;
   a.W = weights, a.wb = ws[0], a.wh = ws[1];
   a.units = units, a.Hkv = (int)Hkv, a.D = (int)D, a.esz = paged::esize(dtype);
