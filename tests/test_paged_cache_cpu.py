@@ -440,3 +440,37 @@ def test_c_abi_lengths_out_is_apart(it):
         for at in (p + B * size, p - B * out):  # (the next check's message)
             assert lib.tsp_paged_append(d, s3, d, s3, None, s3, 512, s3, bf, B, 2, 1, 8, 16, 64, d, 1, 4, 4, n, new, it, at,
                                         None, None, None) == -1 and b"null K_pages" in lib.tsp_last_error(), (p, at)
+
+
+def run_no_columns(dt, dev):
+    """Sequences without room for a row, weights of no elements included."""
+    Q, K, V, kp, vp, t = (x.to(dev) for x in make(dt=dt))
+    t, n, w = t[:, :0], torch.tensor([0, 5, -3], device=dev), torch.ones(3, 2, 0, device=dev)
+    before = kp.clone(), vp.clone()
+    for weights in (None, w):
+        assert ts.paged_cache_append(K, V, kp, vp, t, n, None, weights).tolist() == [0, 0, 0]
+        assert (ts.paged_attention(Q, kp, vp, t, n, None, None, weights) == 0).all()
+    for budget in (0, 7):
+        assert ts.paged_cache_evict(kp, vp, w, t, n, budget).tolist() == [0, 0, 0]
+    assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+
+
+def test_no_columns(pytorch_backend):
+    run_no_columns(F64, "cpu")
+
+
+@pytest.mark.gpu
+def test_no_columns_on_the_gpu(hip_backend):
+    run_no_columns(torch.float32, "cuda")
+
+
+@built
+def test_c_abi_null_weights_of_no_columns():
+    """A tensor without elements has no address; with columns, null weights are refused."""
+    import ctypes
+
+    lib, d = _lib.load(), 256
+    s3, w2 = (ctypes.c_int64 * 3)(2048, 1024, 64), (ctypes.c_int64 * 2)(0, 0)
+    for cols, message in ((0, b"null K_pages"), (4, b"null weights")):
+        assert lib.tsp_paged_evict(None, s3, 512, s3, _lib.TSP_BF16, 1, 2, 8, 16, 64, d, 1, cols, cols, 1024, 1, None, w2, 8,
+                                   2, 4096, d, 1 << 40, None) == -1 and message in lib.tsp_last_error()

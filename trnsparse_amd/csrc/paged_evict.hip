@@ -582,7 +582,7 @@ extern "C" int tsp_paged_evict(void* K_pages, const int64_t* kps, void* V_pages,
   if (recent > budget) recent = budget;
   const paged::Lengths len = paged::lengths_of(lengths, nullptr, index_type, slots, 0);
   if ((rc = paged::check_lengths_out(who, B, lengths_out, len))) return rc;
-  if (!weights) return fail(TSP_EINVAL, "%s: null weights", who);
+  if (!weights && slots > 0) return fail(TSP_EINVAL, "%s: null weights", who);
   if ((rc = paged::check_weights(who, weights, ws, B, Hkv, slots))) return rc;
   if ((rc = paged::check_pages(who, "K_pages", K_pages, kps, dtype, pages, Hkv, page_size, D, true))) return rc;
   if ((rc = paged::check_pages(who, "V_pages", V_pages, vps, dtype, pages, Hkv, page_size, D, true))) return rc;
