@@ -340,3 +340,17 @@ def test_batches_of_many_sequences(hip_backend, dt, B, heads, N):
     lengths = torch.randint(N, 1121, (B,), generator=g)
     lengths[::9], lengths[3] = 1120 - torch.arange(len(lengths[::9])), 0
     check(Q, kp, vp, table, lengths.cuda(), new.cuda())
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("G", [63, 64, 65, 96])
+@pytest.mark.parametrize("size", [(2, 1, 1, 7, 16, 64), (3, 2, 3, 9, 48, 40), (8, 1, 2, 64, 128, 64)])
+def test_weights_of_many_heads_to_a_key_head(hip_backend, dt, G, size):
+    """A token's rows fill whole stages of the weights' rows, or more; 32 keys to a workgroup
+    and (the last size) 128."""
+    B, Hk, N, cols, ps, D = size
+    Q, kp, vp, table = make(B, G * Hk, Hk, N, cols, ps, D, dt, seed=17)
+    L = cols * ps
+    lengths = torch.tensor([L, N, L - 31, L // 2, 0, L - 1, 77, 1][:B], device="cuda")
+    check(Q, kp, vp, table, lengths)
+    check(Q, kp, vp, table, lengths, torch.tensor([1, N, N, 0, 1, N, 1, N][:B], device="cuda"))

@@ -320,3 +320,27 @@ def test_lengths_past_32_bits(hip_backend, types):
     if types[0] == torch.int64:  # lengths themselves past 32 bits: as many rows as there is room for, or none
         n = torch.tensor([2**32 + 40, -(2**32) + 41, 42, 43, 44], device="cuda")
         assert ts.paged_cache_append(k, v, *a, table, n, new).tolist() == [64, 3, 45, 43, 46]
+
+
+@pytest.mark.parametrize("B,cols,budget", [(2, 1700, 9000), (3, 1700, 8000), (2, 2600, 40000)])
+def test_graph_of_long_evictions_of_several_sequences(hip_backend, B, cols, budget):
+    """Weights searched by parts, rows moved in segments and (8000) in one list, captured and
+    replayed on other weights and lengths, one of them below the budget."""
+    _, kp, vp, table = make(B, Hk, Hk, 1, cols, SIZE, 16, BF, seed=7)
+    L = cols * SIZE
+    w, lengths = torch.zeros(B, Hk, L, device="cuda"), torch.full((B,), L, device="cuda")
+    graph, (after,) = _capture(lambda: ts.paged_cache_evict(kp, vp, w, table, lengths, budget, 70))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    for i in range(5):
+        x = rand(g, *w.shape).exp()
+        w.copy_(x.round() if i % 2 else x)
+        lengths.copy_(torch.randint(budget, L + 1, (B,), device="cuda", generator=g))
+        lengths[i % B] = budget - i
+        k, v, y = kp.clone(), vp.clone(), w.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        ts.set_backend("pytorch")
+        n = ts.paged_cache_evict(k, v, y, table, lengths, budget, 70)
+        ts.set_backend("hip")
+        torch.cuda.synchronize()
+        assert torch.equal(kp, k) and torch.equal(vp, v) and torch.equal(w, y) and torch.equal(after, n)
