@@ -45,7 +45,6 @@ int check_sizes(const char* who, int dtype, int64_t B, int64_t Hq, int64_t Hkv, 
 namespace paged {
 namespace {
 
-using xat::LOG2E;
 using xat::Operand;
 using xat::OUT_OF_RANGE;
 
@@ -56,7 +55,7 @@ struct Args {
   Pages K, V;
   Table t;
   Lengths len;
-  int B, Hkv, G, Sq, R, D;   // R: rows of a unit, G Sq
+  int B, Hkv, G, R, D;       // R: rows of a unit
   int items;                 // workgroups of a unit at most
   int deal;                  // work goes to the launch's first workgroups, longest first (up to 64 sequences)
   int slots;                 // results of ranges that a unit has room for (0: keys stay whole)
@@ -967,7 +966,7 @@ extern "C" int tsp_paged_attn_fwd(const void* Q, const int64_t* qs, const void* 
   a.V = paged::pages_of(V_pages, vps, dtype);
   a.t = paged::table_of(table, table_type, table_stride, cols, pages, page_size);
   a.len = paged::lengths_of(lengths, new_lengths, index_type, keys, Sq);
-  a.B = (int)B, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.Sq = (int)Sq, a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
+  a.B = (int)B, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.R = (int)(Hq / Hkv * Sq), a.D = (int)D;
   a.items = p.items, a.slots = p.slots, a.own = p.own, a.places = (int)(p.places / Hkv), a.least = p.least, a.step = p.step, a.slot_rows = p.slot_rows;
   const int64_t units = B * Hkv;
   a.part = (float*)workspace;
