@@ -710,7 +710,9 @@ int tsp_prefix_attn_fwd(const void* Q, const int64_t* q_strides,
  *     O[b,h,i] = sum_j softmax_j(scale Q[b,h,i].K_j) V_j, j < lengths[b] - (m - 1 - i)
  *   with key head h / (heads / kv_heads); rows i >= m, and rows that see no key,
  *   are zero. With weights not NULL, weights[b,hk,j] += the softmax weight of
- *   key j, summed over the key head's query heads and the queries. Strides,
+ *   key j, summed over the key head's query heads and the queries. In 16 bits P
+ *   enters its product with V as the sum of two 16-bit numbers where a sequence
+ *   has up to 32 rows to a key head, as one where it has more. Strides,
  *   alignment and scale of Q and O as in tsp_cross_attn_fwd. workspace:
  *   tsp_paged_attn_workspace_size bytes, 16-byte aligned, `keys` being slots,
  *   `ragged` whether new_lengths is given and `weights` whether weights is.

@@ -30,10 +30,13 @@
 // way a key's sum is added up in a fixed order: no atomics.
 //
 // What bounds them: narrow, the reads of K and V (64 sequences of up to 8192 keys, 8 key
-// heads of 128 in bf16, one token each: 278 us, 5.8 TB/s); wide, the matrix instructions
-// with the softmax next to them rather than under them (2 x 2048 tokens over up to 10240
-// keys, 32 heads over 8 of 128: 464 us, 0.96 PFLOP/s); small calls, the launch and one
-// workgroup's chain of stages (4 sequences of up to 512 keys: 8 us).
+// heads of 128, one token each: bf16 278 to 291 us by the lengths, 5.6 to 5.8 TB/s, fp32 550
+// to 576, 5.7); wide, the matrix instructions with the softmax next to them rather than
+// under them (2 x 2048 tokens over up to 10240 keys, 32 heads over 8 of 128 in bf16: 430 to
+// 514 us, 1.01 to 1.03 PFLOP/s); small calls, the launch and one workgroup's chain of
+// stages (4 sequences of up to 512 keys: 8.6 us). Tiles have 64 or 128 elements of a row:
+// head_dim 16 to 32 reads as slowly as 64 (32 sequences of up to 8192 keys, 8 heads, one
+// token: 46 us at 16 and 83 at 64 in bf16, 128 and 166 in fp32).
 #include "lds_dma.h"
 #include "paged_cache.h"
 #include "xattn_fwd.h"
@@ -349,6 +352,10 @@ struct Wide {
       const int at = c0 + st * HK;
       const uint32_t stage = lds0 + (st & 1) * STAGE;
       const int lim = least < k1 ? least : k1;
+      // P as one 16-bit number, whose rounding is as large as the result's own: off by 2.3e-3
+      // of the norm in bf16 and 2.9e-4 in fp16, as the sum of two, which the narrow kernel has,
+      // 1.7e-3 and 2.1e-4. Two are half as many products again and registers that the
+      // stages need: 2 x 2048 tokens 447 us and 610.
       xat::softmax_stage<T, NT, false>(x, q, stage, stage + HBYTES, ln, h, a.scale_log2, at + HK > lim,
                                        xat::keys_from(sees, k1, at), [] {});
     }

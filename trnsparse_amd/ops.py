@@ -770,6 +770,10 @@ def paged_attention(
     row, summed over the key head's query heads and the new tokens, is added to
     it: what `paged_cache_evict` goes by.
 
+    The HIP kernels sum and normalise in float32; in 16 bits the softmax weights enter
+    the product with V as sums of two 16-bit numbers where a sequence has at most 32 rows
+    to a key head (new tokens times query heads over it), as one where it has more.
+
     Types, scale, strides of Q and the result's order as in `cross_attention`;
     pages and weights may be views with unit stride over the last dimension and
     (pages) other strides of whole 16-byte pieces. head_dim**-0.5 is the default
