@@ -188,3 +188,9 @@ def test_evict_where_the_search_ends(hip_backend, cols, step, more):
     ts.set_backend("hip")
     after = ts.paged_cache_evict(kp, vp, w, table, lengths, count + more + recent, recent)
     same((kp, vp, w, after), (k, v, x, want))
+
+
+@pytest.mark.parametrize("cols", [16384, 16385])
+def test_evict_at_the_most_parts(hip_backend, cols):
+    """The longest caches of 8 units that are searched by parts, and the shortest that are not."""
+    test_evict_long(hip_backend, BF, (2, 4, cols, 256, 8, 5000, 300), "ties")

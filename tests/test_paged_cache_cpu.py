@@ -474,3 +474,14 @@ def test_c_abi_null_weights_of_no_columns():
     for cols, message in ((0, b"null K_pages"), (4, b"null weights")):
         assert lib.tsp_paged_evict(None, s3, 512, s3, _lib.TSP_BF16, 1, 2, 8, 16, 64, d, 1, cols, cols, 1024, 1, None, w2, 8,
                                    2, 4096, d, 1 << 40, None) == -1 and message in lib.tsp_last_error()
+
+
+@built
+def test_evict_workspace_of_very_long_caches():
+    """Counts by parts, which every part reads, are kept only where the parts are few: the
+    workspace (and the work) of the longest caches does not grow with their square."""
+    lib = _lib.load()
+    for units, slots in ((1, 1 << 30), (8, 1 << 30), (100, 1 << 28), (8, (1 << 22) + 1), (32, (1 << 20) + 1)):
+        size = lib.tsp_paged_evict_workspace_size(_lib.TSP_BF16, units, 1, slots, 64, 5)
+        assert 0 < size < 1 << 16, (units, slots, size)
+    assert lib.tsp_paged_evict_workspace_size(_lib.TSP_BF16, 8, 1, 1 << 22, 64, 5) >= 4096 * 3 * 2048 * 4

@@ -518,8 +518,14 @@ __global__ __launch_bounds__(MT) void move_kernel(const EvictArgs a, uint32_t sl
 // launches, which take less time than one workgroup's turns where these are many and
 // the units leave CUs without one. The whole eviction with one workgroup to each unit
 // and by parts, us: 8 units of 24576 rows 52 and 56, of 32768 60 and 56, of 49152 71 and
-// 56; 32 of 49152 166 and 168; 64 of 65536 174 and 185, of 81920 196 and 197.
-bool by_parts(int64_t units, int64_t slots) { return units < 128 && slots > (3 + units / 10) * PART; }
+// 56; 32 of 49152 166 and 168; 64 of 65536 174 and 185, of 81920 196 and 197. Every part
+// reads all parts' counts, so that the work grows with their square: up to 4096 parts of
+// all units (one workgroup to a unit and by parts, a budget of 4096: 32 units of 2^19 rows
+// 399 us and 235, of 2^20 741 and 667; 8 units of 2^21 1412 and 661, of 2^22 2773 and 2435;
+// one of 2^23 5475 and 1445).
+bool by_parts(int64_t units, int64_t slots) {
+  return units < 128 && slots > (3 + units / 10) * PART && units * ceil_div(slots, PART) <= 4096;
+}
 // log2 of the places of a segment, 31 where all are one. Segments for 512 workgroups,
 // none of less than 1024 places, where the chains of parts are too few to take the
 // memory's rate (64 with slices of 64 bytes) and long: copying rows aside is traffic
