@@ -354,3 +354,26 @@ def test_weights_of_many_heads_to_a_key_head(hip_backend, dt, G, size):
     lengths = torch.tensor([L, N, L - 31, L // 2, 0, L - 1, 77, 1][:B], device="cuda")
     check(Q, kp, vp, table, lengths)
     check(Q, kp, vp, table, lengths, torch.tensor([1, N, N, 0, 1, N, 1, N][:B], device="cuda"))
+
+
+@pytest.mark.parametrize("dt,D", [(BF, 8), (HF, 24), (F32, 4), (F32, 12)])
+@pytest.mark.parametrize("N,heads", [(1, (4, 2)), (5, (8, 2)), (50, (6, 3))])
+def test_smallest_head_dims(hip_backend, dt, D, N, heads):
+    """A row of one 16-byte piece, and of three."""
+    Q, kp, vp, table = make(3, *heads, N, 9, 32, D, dt, seed=18)
+    lengths = torch.tensor([288, 51, N], device="cuda")
+    check(Q, kp, vp, table, lengths)
+    check(Q, kp, vp, table, lengths, torch.tensor([1, N, max(N - 2, 0)], device="cuda"))
+
+
+@pytest.mark.parametrize("N", [1, 40])
+def test_one_pool_for_both_and_one_page_for_all(hip_backend, N):
+    """Pages are only read here: K and V may be one tensor, and pages a view of stride zero."""
+    Q, kp, vp, table = make(3, 4, 2, N, 5, 32, 64, BF, seed=19)
+    lengths = torch.tensor([160, 40, 99], device="cuda")
+    check(Q, kp, kp, table, lengths)
+    one = kp[3:4].expand(len(kp), -1, -1, -1)
+    want = check(Q, one, vp, table, lengths)
+    assert torch.equal(ts.paged_attention(Q, one.contiguous(), vp, table, lengths), want)
+    same = table[:1].expand(3, -1)  # one row of the table for all sequences
+    check(Q, kp, vp, same, lengths)

@@ -344,3 +344,48 @@ def test_graph_of_long_evictions_of_several_sequences(hip_backend, B, cols, budg
         ts.set_backend("hip")
         torch.cuda.synchronize()
         assert torch.equal(kp, k) and torch.equal(vp, v) and torch.equal(w, y) and torch.equal(after, n)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_the_longest_cache(hip_backend, dt):
+    """2^30 rows of one sequence, of which three pages are there. All scores are zero, so that
+    every key weighs 1 / n and sums of them are exact: results tell which rows were read."""
+    cols, n, d = 1 << 26, 1 << 30, 16
+    table = torch.full((1, cols), -1, dtype=torch.int32, device="cuda")
+    table[0, 0], table[0, cols // 2 + 1], table[0, cols - 1] = 2, 0, 1
+    g = torch.Generator(device="cuda").manual_seed(20)
+    kp = torch.zeros(3, 1, SIZE, d, dtype=dt, device="cuda")
+    vp = torch.randint(-64, 65, (3, 1, SIZE, d), device="cuda", generator=g).to(dt)
+    lengths = torch.tensor([n - 3], device="cuda")
+    k, v = rand(g, 1, 1, 5, d, dt=dt), torch.ones(1, 1, 5, d, dtype=dt, device="cuda")
+    last = vp[1].clone()
+    lengths = ts.paged_cache_append(torch.zeros_like(k), v, kp, vp, table, lengths)
+    assert lengths.tolist() == [n] and torch.equal(vp[1, :, :13], last[:, :13]) and (vp[1, :, 13:] == 1).all()
+    q = rand(g, 1, 2, 40, d, dt=dt)
+    total = vp[:, 0].double().sum((0, 1))
+    O = ts.paged_attention(q[:, :, :1], kp, vp, table, lengths)
+    assert torch.equal(O[0, :, 0].double(), (total / n).to(dt).double().expand(2, -1))
+    # Query i of 40 does not see the last 39 - i rows, which lie in the last page and before it.
+    # e a rounding of float32: the ranges that have a page hold whole numbers over their number of
+    # keys (4 e), and are joined by weights 2^(lse - largest lse) over their sum. An lse is a log2
+    # of about 2^24, from 16 to 32, where half a step is 2^-20 = 16 e; logarithm and rounding
+    # make it 48 e at most, so that weights and their sum are off by 48 ln 2 < 34 e each.
+    O = ts.paged_attention(q, kp, vp, table, lengths)
+    pages = [vp[2, 0].double().sum(0), vp[0, 0].double().sum(0)]
+    for i in range(40):
+        parts = torch.stack([*pages, vp[1, 0, : 16 - min(39 - i, 16)].double().sum(0)]) / (n - 39 + i)
+        off = (O[0, :, i].double() - parts.sum(0)).abs()
+        far = off - (2 * 34 + 8) * 2.0**-24 * parts.abs().sum(0) - torch.finfo(dt).eps / 2 * parts.sum(0).abs()
+        assert far.max() <= 0, (i, float(far.max()))
+    w = torch.zeros(1, 1, n, device="cuda")
+    O = ts.paged_attention(q[:, :, :1], kp, vp, table, lengths, weights=w)
+    assert bool((w == 2.0 / n).all())
+    places = [3, 17, n // 2 + 20, n - 30, n - 12]
+    w.zero_()
+    w[0, 0, places] = torch.arange(1.0, 6.0, device="cuda")
+    kept = sorted(places + [j for j in range(20) if j not in places][:11]) + list(range(n - 4, n))
+    rows = {0: vp[2, 0].clone(), cols // 2 + 1: vp[0, 0].clone(), cols - 1: vp[1, 0].clone()}
+    want = torch.stack([rows[j // SIZE][j % SIZE] if j // SIZE in rows else torch.zeros_like(last[0, 0]) for j in kept[:SIZE]])
+    weights = w[0, 0, kept]
+    assert ts.paged_cache_evict(kp, vp, w, table, lengths, 20, 4).tolist() == [20]
+    assert torch.equal(vp[2, 0], want) and torch.equal(w[0, 0, :20], weights)
