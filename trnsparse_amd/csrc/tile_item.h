@@ -53,7 +53,8 @@ __host__ __device__ inline bool head_item(uint32_t g, int64_t P_, int64_t H_, in
 // with long items and end together. (paged_attention of four chunks of 512 tokens next
 // to 12 single ones, 8 or 4 heads of 128 to a key head in bf16, up to 4096 keys, by
 // eighths and by turns, us: 1 key head 115 and 95, 2 176 and 98, 3 156 and 97, 4 197
-// and 137, 9 249 and 221, 12 234 and 210; whole heads and by turns: 16 280 and 286.)
+// and 137, 9 249 and 221, 12 234 and 210; whole heads and by turns: 16 280 and 286, of two chunks of
+// 200 tokens next to 6 single ones 70 and 57.)
 __host__ __device__ inline bool sorted_item(uint32_t g, int64_t P, int64_t H, int64_t& head, int64_t& item) {
   if (H % 8 == 0) return head_item(g, P, H, head, item);
   item = g / (uint32_t)H;
